@@ -373,6 +373,118 @@ yuear_status yuear_nar_attention(const uint16_t *dev_q, const uint16_t *dev_k,
                                  int32_t head_dim, int32_t causal, int32_t query_chunk_size,
                                  void *dev_workspace, uint16_t *dev_out, void *stream,
                                  char **error_json);
+/* ---- pages of a key-value cache (no counterpart in the reference, whose
+ * cache is one array per request) ----
+ * A page holds `page_slots` slots (a power of two, at least 32) of every kv
+ * head of one layer: K [kv_heads][slots][128], V in the cache's 32-slot blocks
+ * [kv_heads][slots / 32][128][32], both bf16; a layer's pages are contiguous,
+ * dev_k_pages / dev_v_pages [pages] of them. A sequence is a row of `table`
+ * (int32 [batch], rows table_stride apart, table_width entries each): key t is
+ * in page table[t / page_slots], slot t % page_slots. An entry outside
+ * [0, pages) stands for keys that are not there: they are seen by nobody, and
+ * rows that would be appended to them are dropped. All device arrays are
+ * 16-byte aligned (tables, starts and positions: 4-byte), strides (in elements)
+ * are multiples of 8, heads / kv_heads is 1, 2, 3, 4, 6 or 8, head_dim 128.
+ * Invalid arguments return hipErrorInvalidValue (1) and launch nothing; empty
+ * calls (batch or rows 0) return 0. The entry points run on `stream` of the
+ * current device, allocate nothing and can be captured. A page that a call
+ * appends to may be in no other row's visible keys. */
+/* Prompt rows into pages. qkv [rows] of (heads + 2 kv_heads) * 128 (q | k | v);
+ * sequence b owns rows [starts[b], starts[b + 1]) (int32 [batch + 1], not
+ * decreasing), at positions pos0[b], pos0[b] + 1, ... Writes
+ * q_out[row] = bf16(rope(norm(q))), K[t] = bf16(rope(norm(k))), V[t] = v, with
+ * norm the per-head RMSNorm (skipped for a null gain) and rope by row t of the
+ * tables ([positions][64]): 32-bit arithmetic, one rounding each (the engine's
+ * own cache append keeps the reference's roundings in between). Rows of a
+ * sequence that starts outside [0, limit), and rows at or past limit =
+ * min(positions, table_width * page_slots), are left untouched. */
+int32_t yuear_op_paged_append(const uint16_t *dev_qkv, int64_t qkv_stride,
+                              const uint16_t *dev_q_norm, const uint16_t *dev_k_norm, float eps,
+                              const uint16_t *dev_rope_cos, const uint16_t *dev_rope_sin,
+                              int32_t positions, uint16_t *dev_k_pages, uint16_t *dev_v_pages,
+                              int32_t pages, int32_t page_slots, const int32_t *dev_table,
+                              int32_t table_width, int32_t table_stride,
+                              const int32_t *dev_starts, const int32_t *dev_pos0, int32_t batch,
+                              int32_t rows, int32_t heads, int32_t kv_heads, uint16_t *dev_q_out,
+                              int64_t q_stride, void *stream);
+/* Attention of the rows that yuear_op_paged_append left (or any q): row i of
+ * sequence b, at position p = pos0[b] + i, over the keys t <= p with
+ * p - t < window or t < sinks (window 0: every t <= p) that the table has;
+ * fp32 scores q . K / sqrt(128), softmax and sums, bf16 out [rows] of heads *
+ * 128. A row that sees no key gives zeros; rows that the append leaves out for
+ * their position in the table are left untouched here. workspace as below. */
+int32_t yuear_op_paged_attention_prefill(
+    const uint16_t *dev_q, int64_t q_stride, const uint16_t *dev_k_pages,
+    const uint16_t *dev_v_pages, int32_t pages, int32_t page_slots, const int32_t *dev_table,
+    int32_t table_width, int32_t table_stride, const int32_t *dev_starts, const int32_t *dev_pos0,
+    int32_t batch, int32_t rows, int32_t heads, int32_t kv_heads, int32_t window, int32_t sinks,
+    void *dev_workspace, int64_t workspace_bytes, uint16_t *dev_out, int64_t out_stride,
+    void *stream);
+/* The decode step's form: one new token per sequence at pos[b], its append and
+ * its attention in one launch. qkv [batch] rows; K and V of the token are
+ * stored as yuear_op_paged_append stores them, and the token's query (not
+ * rounded) attends to the stored keys t <= pos[b], with window and sinks as
+ * above. The token always sees itself, also where the table has no page to
+ * keep it. A sequence with pos outside [0, min(positions, table_width *
+ * page_slots)) is left untouched. */
+int32_t yuear_op_paged_attention_decode(
+    const uint16_t *dev_qkv, int64_t qkv_stride, const uint16_t *dev_q_norm,
+    const uint16_t *dev_k_norm, float eps, const uint16_t *dev_rope_cos,
+    const uint16_t *dev_rope_sin, int32_t positions, uint16_t *dev_k_pages, uint16_t *dev_v_pages,
+    int32_t pages, int32_t page_slots, const int32_t *dev_table, int32_t table_width,
+    int32_t table_stride, const int32_t *dev_pos, int32_t batch, int32_t heads, int32_t kv_heads,
+    int32_t window, int32_t sinks, void *dev_workspace, int64_t workspace_bytes,
+    uint16_t *dev_out, int64_t out_stride, void *stream);
+/* Bytes of the workspace of the two attention calls (rows 0: the decode form),
+ * 0 for invalid arguments. The caller zeroes it once; every call leaves it ready
+ * for the next, of any shape that it is large enough for. Calls that may
+ * overlap (other streams, graphs replayed at once) need one each. */
+int64_t yuear_op_paged_workspace_bytes(int32_t batch, int32_t heads, int32_t kv_heads,
+                                       int32_t rows);
+/* Page copies: page dst[i] = page src[i] of K and V in each of `layers` layers,
+ * whose pages are layer_stride elements apart. src and dst are host arrays of n
+ * pages; no page may be written twice or be both read and written (1). */
+int32_t yuear_op_pages_copy(uint16_t *dev_k_pages, uint16_t *dev_v_pages, int32_t layers,
+                            int64_t layer_stride, int32_t pages, int32_t kv_heads,
+                            int32_t page_slots, const int32_t *src, const int32_t *dst, int32_t n,
+                            void *stream);
+/* Which sequence holds which page (host only; the pages' memory is the
+ * caller's). Pages are handed out lowest first and shared by forks; a page goes
+ * back when its last holder lets go of it. Calls that give copies expect the
+ * caller to run them (yuear_op_pages_copy) before the cache is used again. */
+typedef struct yuear_pages yuear_pages;
+yuear_status yuear_pages_create(int32_t pages, int32_t page_slots, yuear_pages **out,
+                                char **error_json);
+void yuear_pages_destroy(yuear_pages *pool);
+/* A new empty sequence; a new one that shares all pages of another. */
+yuear_status yuear_pages_open(yuear_pages *pool, int32_t *sequence, char **error_json);
+yuear_status yuear_pages_fork(yuear_pages *pool, int32_t sequence, int32_t *fork,
+                              char **error_json);
+/* Room for `tokens` more. Where other sequences hold the partly filled last
+ * page, the sequence gets its own: *copy_src / *copy_dst is the copy to run
+ * (-1: none). MemoryError "out of pages" changes nothing. */
+yuear_status yuear_pages_extend(yuear_pages *pool, int32_t sequence, int32_t tokens,
+                                int32_t *copy_src, int32_t *copy_dst, char **error_json);
+/* Back to `length` tokens (not before the length of the last trim that gave
+ * pages back). */
+yuear_status yuear_pages_truncate(yuear_pages *pool, int32_t sequence, int32_t length,
+                                  char **error_json);
+/* Gives back the pages that the token at the sequence's length, and those after
+ * it, do not see through a window with sinks (so: before the room for that
+ * token is taken); their table entries become -1. */
+yuear_status yuear_pages_trim(yuear_pages *pool, int32_t sequence, int32_t window, int32_t sinks,
+                              char **error_json);
+yuear_status yuear_pages_close(yuear_pages *pool, int32_t sequence, char **error_json);
+/* Moves the held pages to the lowest numbers; copy_src / copy_dst (room for
+ * every page of the pool) receive the n copies to run. */
+yuear_status yuear_pages_compact(yuear_pages *pool, int32_t *copy_src, int32_t *copy_dst,
+                                 int32_t *n, char **error_json);
+/* Table rows of n sequences, `width` entries each, -1 past a sequence's pages. */
+yuear_status yuear_pages_table(yuear_pages *pool, const int32_t *sequences, int32_t n,
+                               int32_t width, int32_t *table, char **error_json);
+/* Tokens of a sequence (-1: no such sequence); pages that nobody holds. */
+int32_t yuear_pages_length(yuear_pages *pool, int32_t sequence);
+int32_t yuear_pages_unused(yuear_pages *pool);
 /* RoPE cos/sin tables exactly as the engine builds them (host). */
 void yuear_rope_table(int32_t positions, int32_t head_dim, double theta,
                       uint16_t *cos_out, uint16_t *sin_out);

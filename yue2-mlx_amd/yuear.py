@@ -148,6 +148,50 @@ _SIGS = {
     "yuear_op_attention_prefill": (C.c_int32, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_int32,
                                                C.c_int32, C.c_int32, C.c_int32, C.c_int32,
                                                C.c_void_p, C.c_void_p]),
+    "yuear_op_paged_append": (C.c_int32, [
+            C.c_void_p, C.c_int64, C.c_void_p, C.c_void_p, C.c_float, C.c_void_p, C.c_void_p,
+            C.c_int32, C.c_void_p, C.c_void_p, C.c_int32, C.c_int32, C.c_void_p, C.c_int32,
+            C.c_int32, C.c_void_p, C.c_void_p, C.c_int32, C.c_int32, C.c_int32, C.c_int32,
+            C.c_void_p, C.c_int64, C.c_void_p]),
+    "yuear_op_paged_attention_prefill": (C.c_int32, [
+            C.c_void_p, C.c_int64, C.c_void_p, C.c_void_p, C.c_int32, C.c_int32, C.c_void_p,
+            C.c_int32, C.c_int32, C.c_void_p, C.c_void_p, C.c_int32, C.c_int32, C.c_int32,
+            C.c_int32, C.c_int32, C.c_int32, C.c_void_p, C.c_int64, C.c_void_p, C.c_int64,
+            C.c_void_p]),
+    "yuear_op_paged_attention_decode": (C.c_int32, [
+            C.c_void_p, C.c_int64, C.c_void_p, C.c_void_p, C.c_float, C.c_void_p, C.c_void_p,
+            C.c_int32, C.c_void_p, C.c_void_p, C.c_int32, C.c_int32, C.c_void_p, C.c_int32,
+            C.c_int32, C.c_void_p, C.c_int32, C.c_int32, C.c_int32, C.c_int32, C.c_int32,
+            C.c_void_p, C.c_int64, C.c_void_p, C.c_int64, C.c_void_p]),
+    "yuear_op_paged_workspace_bytes": (C.c_int64, [
+            C.c_int32, C.c_int32, C.c_int32, C.c_int32]),
+    "yuear_op_pages_copy": (C.c_int32, [
+            C.c_void_p, C.c_void_p, C.c_int32, C.c_int64, C.c_int32, C.c_int32, C.c_int32, i32p,
+            i32p, C.c_int32, C.c_void_p]),
+    "yuear_pages_create": (C.c_int, [
+            C.c_int32, C.c_int32, _P(C.c_void_p), _P(C.c_void_p)]),
+    "yuear_pages_destroy": (None, [
+            C.c_void_p]),
+    "yuear_pages_open": (C.c_int, [
+            C.c_void_p, i32p, _P(C.c_void_p)]),
+    "yuear_pages_fork": (C.c_int, [
+            C.c_void_p, C.c_int32, i32p, _P(C.c_void_p)]),
+    "yuear_pages_extend": (C.c_int, [
+            C.c_void_p, C.c_int32, C.c_int32, i32p, i32p, _P(C.c_void_p)]),
+    "yuear_pages_truncate": (C.c_int, [
+            C.c_void_p, C.c_int32, C.c_int32, _P(C.c_void_p)]),
+    "yuear_pages_trim": (C.c_int, [
+            C.c_void_p, C.c_int32, C.c_int32, C.c_int32, _P(C.c_void_p)]),
+    "yuear_pages_close": (C.c_int, [
+            C.c_void_p, C.c_int32, _P(C.c_void_p)]),
+    "yuear_pages_compact": (C.c_int, [
+            C.c_void_p, i32p, i32p, i32p, _P(C.c_void_p)]),
+    "yuear_pages_table": (C.c_int, [
+            C.c_void_p, i32p, C.c_int32, C.c_int32, i32p, _P(C.c_void_p)]),
+    "yuear_pages_length": (C.c_int32, [
+            C.c_void_p, C.c_int32]),
+    "yuear_pages_unused": (C.c_int32, [
+            C.c_void_p]),
     "yuear_tokenizer_load": (C.c_int, [C.c_char_p, _P(C.c_void_p), _P(C.c_void_p)]),
     "yuear_tokenizer_destroy": (None, [C.c_void_p]),
     "yuear_tokenizer_encode": (C.c_int, [C.c_void_p, C.c_char_p, C.c_int64, _P(i32p),
@@ -330,6 +374,318 @@ def v_unblocked(vb):
     *lead, n, d = vb.shape
     return np.ascontiguousarray(
         vb.reshape(*lead, n // V_BLOCK, d, V_BLOCK).swapaxes(-1, -2)).reshape(*lead, n, d)
+
+
+# ---- pages of a key-value cache ----
+
+class PagePool:
+    """Which sequence holds which page of a cache (host bookkeeping of
+    yuear_pages_*; the pages' tensors are the caller's). `extend` and `compact`
+    return (src, dst) page lists for `pages_copy`, to be run before the cache is
+    used again."""
+
+    def __init__(self, pages, page_slots):
+        h, err = C.c_void_p(), C.c_void_p()
+        _check(lib.yuear_pages_create(pages, page_slots, C.byref(h), C.byref(err)), err)
+        self._handle, self.pages, self.page_slots = h, pages, page_slots
+
+    def close(self, _destroy=lib.yuear_pages_destroy):
+        if getattr(self, "_handle", None):
+            _destroy(self._handle)
+            self._handle = None
+
+    def __del__(self):
+        self.close()
+
+    def _call(self, name, *args):
+        err = C.c_void_p()
+        _check(getattr(lib, "yuear_pages_" + name)(self._handle, *args, C.byref(err)), err)
+
+    def open(self):
+        """A new empty sequence."""
+        out = C.c_int32()
+        self._call("open", C.byref(out))
+        return out.value
+
+    def fork(self, sequence):
+        """A new sequence that shares all pages of `sequence`."""
+        out = C.c_int32()
+        self._call("fork", sequence, C.byref(out))
+        return out.value
+
+    def extend(self, sequence, tokens):
+        """Room for `tokens` more; the copies to run (at most one page)."""
+        src, dst = C.c_int32(), C.c_int32()
+        self._call("extend", sequence, tokens, C.byref(src), C.byref(dst))
+        return ([], []) if src.value < 0 else ([src.value], [dst.value])
+
+    def truncate(self, sequence, length):
+        self._call("truncate", sequence, length)
+
+    def trim(self, sequence, window, sinks=0):
+        """Gives back the pages that no later token sees."""
+        self._call("trim", sequence, window, sinks)
+
+    def close_sequence(self, sequence):
+        self._call("close", sequence)
+
+    def compact(self):
+        """Moves the held pages to the lowest numbers; the copies to run."""
+        src, dst = (C.c_int32 * self.pages)(), (C.c_int32 * self.pages)()
+        n = C.c_int32()
+        self._call("compact", src, dst, C.byref(n))
+        return list(src[:n.value]), list(dst[:n.value])
+
+    def table(self, sequences, width):
+        """int32 [sequences, width] page table, -1 past a sequence's pages."""
+        ids = np.ascontiguousarray(sequences, dtype=np.int32).reshape(-1)
+        out = np.full((ids.size, width), -1, dtype=np.int32)
+        self._call("table", ids.ctypes.data_as(i32p), ids.size, width, out.ctypes.data_as(i32p))
+        return out
+
+    def length(self, sequence):
+        n = lib.yuear_pages_length(self._handle, sequence)
+        if n < 0:
+            raise ValueError("no such sequence")
+        return n
+
+    @property
+    def unused(self):
+        return lib.yuear_pages_unused(self._handle)
+
+
+def _hip_check(status, name):
+    if status == 1:
+        raise ValueError(f"{name}: invalid arguments")
+    if status:
+        raise RuntimeError(f"{name}: HIP error {status}")
+
+
+def _require(ok, message):
+    if not ok:
+        raise ValueError(message)
+
+
+def _check_pages(k_pages, v_pages, device):
+    """(pages, kv heads, slots) of one layer's contiguous bf16 pages."""
+    import torch
+    bf16 = torch.bfloat16
+    _require(k_pages.dim() == 4 and v_pages.dim() == 5, "pages are k [pages, kv heads, slots, 128] and "
+             "v [pages, kv heads, slots / 32, 128, 32]")
+    n, hkv, slots, d = k_pages.shape
+    _require(d == 128 and tuple(v_pages.shape) == (n, hkv, slots // 32, 128, 32),
+             "pages are k [pages, kv heads, slots, 128] and v [pages, kv heads, slots / 32, 128, 32]")
+    _require(k_pages.dtype is bf16 and v_pages.dtype is bf16 and k_pages.is_contiguous()
+             and v_pages.is_contiguous(), "pages are contiguous bfloat16")
+    _require(k_pages.device == device and v_pages.device == device, "all tensors are on one device")
+    return n, hkv, slots
+
+
+def _check_ints(t, shape, device, name):
+    import torch
+    _require(t.dtype is torch.int32 and tuple(t.shape) == shape and t.device == device
+             and t.is_contiguous(), f"{name} is a contiguous int32 tensor {list(shape)} on the pages' device")
+
+
+def _check_table(table, device):
+    import torch
+    _require(table.dtype is torch.int32 and table.dim() == 2 and table.device == device
+             and (table.stride(1) == 1 or table.shape[1] == 1) and table.shape[1] >= 1,
+             "table is int32 [sequences, pages] with whole rows")
+    return table.shape[1], max(table.stride(0), table.shape[1])
+
+
+def _check_rope(cos, sin, device):
+    import torch
+    for t in (cos, sin):
+        _require(t.dtype is torch.bfloat16 and t.dim() == 2 and t.shape[1] == 64 and t.is_contiguous()
+                 and t.device == device, "cos and sin are contiguous bfloat16 [positions, 64]")
+    _require(cos.shape == sin.shape, "cos and sin have one shape")
+
+
+def _gain(t, device):
+    import torch
+    if t is None:
+        return None
+    _require(t.dtype is torch.bfloat16 and tuple(t.shape) == (128,) and t.is_contiguous() and t.device == device,
+             "norm gains are contiguous bfloat16 [128]")
+    return t.data_ptr()
+
+
+def _row_view(t, heads, device, name):
+    """Row stride of bf16 rows [n, heads, 128] (or [n, heads * 128])."""
+    import torch
+    flat = t.dim() == 2
+    _require(t.dtype is torch.bfloat16 and t.device == device and t.dim() in (2, 3)
+             and t.shape[1] * (1 if flat else t.shape[-1]) == heads * 128 and (flat or t.shape[2] == 128),
+             f"{name} is bfloat16 [rows, heads, 128] on the pages' device")
+    _require(t.stride(-1) == 1 and (flat or t.stride(1) == 128), f"{name} has contiguous rows")
+    return t.stride(0) if t.shape[0] > 1 else heads * 128
+
+
+class _On:
+    """The device of a call's tensors as the current one."""
+
+    def __init__(self, device):
+        import torch
+        self._guard = None if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+
+    def __enter__(self):
+        if self._guard:
+            self._guard.__enter__()
+
+    def __exit__(self, *exc):
+        if self._guard:
+            self._guard.__exit__(*exc)
+
+
+def _stream(stream, device, *given):
+    """The stream to run on: torch's current one, or the given one, for which
+    the call allocates nothing (`given`: the caller's out and workspace)."""
+    import torch
+    current = torch.cuda.current_stream(device).cuda_stream
+    if stream is None or stream == current:
+        return current
+    _require(all(t is not None for t in given), "a call on another stream than the current one needs out "
+             "and workspace tensors")
+    return stream
+
+
+def _on_gpu(t):
+    _require(t.is_cuda, "tensors are on the GPU")
+    return t.device
+
+
+def pages_copy(k_pages, v_pages, src, dst, stream=None):
+    """Page dst[i] = page src[i] of the keys and values, in every layer: k_pages
+    [layers, pages, kv heads, slots, 128] and v_pages [layers, pages, kv heads,
+    slots / 32, 128, 32] (or one layer's, without the first dimension), src and
+    dst lists of pages on the host."""
+    k, v = (k_pages, v_pages) if k_pages.dim() == 5 else (k_pages[None], v_pages[None])
+    device = _on_gpu(k)
+    _require(k.dim() == 5 and v.dim() == 6 and k.shape[0] == v.shape[0] and k.shape[0] >= 1,
+             "pages are k [layers, pages, kv heads, slots, 128] and v [layers, pages, kv heads, slots / 32, 128, 32]")
+    n, hkv, slots = _check_pages(k[0], v[0], device)
+    _require(k.shape[0] == 1 or k.stride(0) == v.stride(0), "keys and values have one layer stride")
+    _require(len(src) == len(dst), "src and dst have one length")
+    s, d = ((C.c_int32 * len(src))(*src), (C.c_int32 * len(dst))(*dst))
+    with _On(device):
+        _hip_check(lib.yuear_op_pages_copy(k.data_ptr(), v.data_ptr(), k.shape[0], k.stride(0), n, hkv, slots,
+                                           s, d, len(src), _stream(stream, device)), "pages_copy")
+
+
+def paged_workspace(batch, heads, kv_heads, rows=0, device=None):
+    """A zeroed workspace for the paged attention of up to these sizes (rows 0:
+    decode steps only). Calls that may overlap need one each."""
+    import torch
+    n = lib.yuear_op_paged_workspace_bytes(batch, heads, kv_heads, rows)
+    _require(n > 0, "paged_workspace: invalid arguments")
+    return torch.zeros(n // 4, dtype=torch.int32, device="cuda" if device is None else device)
+
+
+def _workspace(workspace, batch, heads, kv_heads, rows, device):
+    import torch
+    if workspace is None:
+        return paged_workspace(batch, heads, kv_heads, rows, device)
+    _require(workspace.dtype is torch.int32 and workspace.is_contiguous() and workspace.device == device,
+             "workspace comes from paged_workspace")
+    return workspace
+
+
+def paged_append(qkv, k_pages, v_pages, table, starts, pos0, cos, sin, q_norm=None, k_norm=None, eps=1e-5, out=None,
+                 stream=None):
+    """Rows of qkv [rows, (heads + 2 kv heads) * 128] into pages; the rotated
+    queries [rows, heads, 128]. Sequence b (row b of the page table) owns rows
+    starts[b] to starts[b + 1], at positions from pos0[b]; cos / sin [positions,
+    64]. See yuear_op_paged_append."""
+    import torch
+    device = _on_gpu(qkv)
+    n, hkv, slots = _check_pages(k_pages, v_pages, device)
+    _require(qkv.dim() == 2 and qkv.shape[1] % 128 == 0 and qkv.shape[1] // 128 > 2 * hkv,
+             "qkv is bfloat16 [rows, (heads + 2 kv heads) * 128]")
+    stream = _stream(stream, device, out)
+    rows, heads = qkv.shape[0], qkv.shape[1] // 128 - 2 * hkv
+    stride = _row_view(qkv, heads + 2 * hkv, device, "qkv")
+    width, table_stride = _check_table(table, device)
+    batch = table.shape[0]
+    _check_ints(starts, (batch + 1,), device, "starts")
+    _check_ints(pos0, (batch,), device, "pos0")
+    _check_rope(cos, sin, device)
+    if out is None:
+        out = torch.empty(rows, heads, 128, dtype=torch.bfloat16, device=device)
+    _require(out.shape[0] == rows, "out has a row for each of qkv's")
+    out_stride = _row_view(out, heads, device, "out")
+    with _On(device):
+        _hip_check(lib.yuear_op_paged_append(
+            qkv.data_ptr(), stride, _gain(q_norm, device), _gain(k_norm, device), eps, cos.data_ptr(),
+            sin.data_ptr(), cos.shape[0], k_pages.data_ptr(), v_pages.data_ptr(), n, slots, table.data_ptr(),
+            width, table_stride, starts.data_ptr(), pos0.data_ptr(), batch, rows, heads, hkv, out.data_ptr(),
+            out_stride, stream), "paged_append")
+    return out
+
+
+def paged_attention_prefill(q, k_pages, v_pages, table, starts, pos0, window=0, sinks=0, workspace=None, out=None,
+                            stream=None):
+    """Causal attention of rows q [rows, heads, 128] over pages: sequence b owns
+    rows starts[b] to starts[b + 1], at positions from pos0[b]; a row at p sees
+    the keys t <= p with p - t < window or t < sinks (window 0: all). See
+    yuear_op_paged_attention_prefill."""
+    import torch
+    device = _on_gpu(q)
+    n, hkv, slots = _check_pages(k_pages, v_pages, device)
+    _require(q.dim() == 3, "q is bfloat16 [rows, heads, 128]")
+    stream = _stream(stream, device, out, workspace)
+    rows, heads = q.shape[0], q.shape[1]
+    stride = _row_view(q, heads, device, "q")
+    width, table_stride = _check_table(table, device)
+    batch = table.shape[0]
+    _check_ints(starts, (batch + 1,), device, "starts")
+    _check_ints(pos0, (batch,), device, "pos0")
+    if out is None:
+        out = torch.empty(rows, heads, 128, dtype=torch.bfloat16, device=device)
+    _require(out.shape[0] == rows, "out has a row for each of q's")
+    out_stride = _row_view(out, heads, device, "out")
+    with _On(device):
+        workspace = _workspace(workspace, batch, heads, hkv, rows, device)
+        _hip_check(lib.yuear_op_paged_attention_prefill(
+            q.data_ptr(), stride, k_pages.data_ptr(), v_pages.data_ptr(), n, slots, table.data_ptr(), width,
+            table_stride, starts.data_ptr(), pos0.data_ptr(), batch, rows, heads, hkv, window, sinks,
+            workspace.data_ptr(), workspace.numel() * 4, out.data_ptr(), out_stride, stream),
+            "paged_attention_prefill")
+    return out
+
+
+def paged_attention_decode(qkv, k_pages, v_pages, table, pos, cos, sin, q_norm=None, k_norm=None, eps=1e-5, window=0,
+                           sinks=0, workspace=None, out=None, stream=None):
+    """One new token per sequence: its keys and values into its page, and its
+    attention [sequences, heads, 128] over the table's pages. qkv [sequences,
+    (heads + 2 kv heads) * 128], pos [sequences]. See
+    yuear_op_paged_attention_decode."""
+    import torch
+    device = _on_gpu(qkv)
+    n, hkv, slots = _check_pages(k_pages, v_pages, device)
+    _require(qkv.dim() == 2 and qkv.shape[1] % 128 == 0 and qkv.shape[1] // 128 > 2 * hkv,
+             "qkv is bfloat16 [sequences, (heads + 2 kv heads) * 128]")
+    stream = _stream(stream, device, out, workspace)
+    batch, heads = qkv.shape[0], qkv.shape[1] // 128 - 2 * hkv
+    stride = _row_view(qkv, heads + 2 * hkv, device, "qkv")
+    width, table_stride = _check_table(table, device)
+    _require(table.shape[0] == batch, "table has a row for each of qkv's")
+    _check_ints(pos, (batch,), device, "pos")
+    _check_rope(cos, sin, device)
+    if out is None:
+        out = torch.empty(batch, heads, 128, dtype=torch.bfloat16, device=device)
+    _require(out.shape[0] == batch, "out has a row for each of qkv's")
+    out_stride = _row_view(out, heads, device, "out")
+    with _On(device):
+        workspace = _workspace(workspace, batch, heads, hkv, 0, device)
+        _hip_check(lib.yuear_op_paged_attention_decode(
+            qkv.data_ptr(), stride, _gain(q_norm, device), _gain(k_norm, device), eps, cos.data_ptr(),
+            sin.data_ptr(), cos.shape[0], k_pages.data_ptr(), v_pages.data_ptr(), n, slots, table.data_ptr(),
+            width, table_stride, pos.data_ptr(), batch, heads, hkv, window, sinks, workspace.data_ptr(),
+            workspace.numel() * 4, out.data_ptr(), out_stride, stream),
+            "paged_attention_decode")
+    return out
 
 
 def rope_table(positions, head_dim, theta):
