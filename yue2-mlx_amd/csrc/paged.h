@@ -30,6 +30,18 @@ struct Cache {
   }
 };
 
+// Inclusive sums over the lanes of a wave (DPP: shifts inside the 16-lane rows,
+// then the last lane of each row into the rows after it).
+__device__ __forceinline__ int wave_scan(int v) {
+  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, true);  // row_shr 1, 2, 4, 8
+  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, true);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, true);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, true);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);  // row_bcast 15: rows 1, 3
+  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);  // row_bcast 31: rows 2, 3
+  return v;
+}
+
 // Item `target` of items numbered through the sequences, count(b) of them for
 // sequence b: its sequence and place there; false past the last item. Every
 // wave walks 64 sequences at a time, one per lane.
@@ -39,12 +51,7 @@ __device__ __forceinline__ bool find_item(int batch, int target, F &&count, int 
   int before = 0;
   for (int b0 = 0; b0 < batch; b0 += 64) {
     const int n = b0 + lane < batch ? count(b0 + lane) : 0;
-    int incl = n;
-#pragma unroll
-    for (int s = 1; s < 64; s <<= 1) {
-      const int up = __shfl_up(incl, s);
-      incl += lane >= s ? up : 0;
-    }
+    const int incl = wave_scan(n);
     const int total = __builtin_amdgcn_readlane(incl, 63);
     if (target < before + total) {
       const int at = __builtin_popcountll(__ballot(before + incl <= target));

@@ -6,16 +6,30 @@
 //
 // over t <= pos with pos - t < window or t < sinks (window 0: all t), in pages
 // that the table has. The bytes of the visible K and V bound it; the arithmetic
-// is 2 G multiply-adds a byte.
+// is G multiply-adds a byte.
 //
-// The work of a launch is the list of (sequence, kv head, pass), a pass being
-// the next 4 visible 32-key blocks, one a wave. It is cut into equal runs, one
-// per workgroup, whatever the lengths of the sequences: the positions are read
-// on the device, so a captured launch serves every length. A workgroup walks the
-// (sequence, kv head) items of its run one by one. An item that lies in one
-// run is finished there; of one that several runs share, each workgroup leaves
-// its running maximum, sum and weighted values in its slots of the workspace,
-// and the one that arrives last joins them in order of the keys.
+// The work of a launch is the list of the visible 32-key blocks of every
+// (sequence, kv head) item. The positions are read on the device, so one captured
+// launch serves every length. Two ways to cut the list into workgroups:
+//
+// - up to 512 items and 24 blocks a workgroup: each item into equal chunks, one
+//   workgroup each, as many as 512 workgroups and 64 parts an item allow (one
+//   sequence of 4096 keys: 12.9 us, 15.9 cut the other way; one kv head of
+//   20000: 20.7 and 65);
+// - else into equal runs, whatever the lengths of the sequences, and a workgroup
+//   walks the items of its run (45 sequences of 150 to 24500 keys: 160 us, 189 in
+//   chunks). To begin an item (positions, page, q, the joining of the waves) costs
+//   a workgroup about as much as 8 blocks, which the runs count (2: 172 us).
+//
+// A part that is a whole item is finished there; else the workgroup leaves its
+// running maximum, sum and weighted values in its slots of the workspace, and
+// the one that arrives last joins the item's parts in order of the keys.
+//
+// A wave takes every fourth block of its workgroup's. The block's K and V go to
+// an LDS stage of the wave's own in whole KiB (buffer_load lds) and from there to
+// registers, when the next block's loads are issued: 16 KiB a wave are always in
+// flight, 32 MB over the chip. The loads are non-temporal: caches larger than the
+// last-level cache pass through it 10% slower otherwise (45 sequences 176 us).
 //
 // Both products run on v_mfma_f32_16x16x32_bf16 as in attn_core.h (S^T = K q,
 // O^T = V^T P^T, K rows permuted so that a lane's scores are its operand of the
@@ -40,8 +54,13 @@ using attn::f32x4;
 using paged::Cache;
 using paged::D;
 using paged::kBlock;
+using paged::wave_scan;
 
 constexpr int kWaves = 4;
+constexpr int kChunks = 512, kChunkBlocks = 24 * kChunks, kParts = 64;
+typedef __attribute__((address_space(3))) void *lds_ptr_t;
+constexpr int kLoadAux = 2;  // nt
+constexpr int kItemCost = 8;  // blocks
 
 struct DecodeParams {
   const uint16_t *qkv = nullptr;
@@ -72,23 +91,104 @@ __device__ __forceinline__ Span span_of(int pos, int window, int sinks) {
   s.blocks = s.lead + pos / kBlock - s.first + 1;
   return s;
 }
-__device__ __forceinline__ int passes_of(const DecodeParams &p, int b) {
+__device__ __forceinline__ int blocks_of(const DecodeParams &p, int b) {
   const int pos = p.pos[b];
-  if (pos < 0 || pos >= p.limit)
-    return 0;
-  return (span_of(pos, p.window, p.sinks).blocks + kWaves - 1) / kWaves;
+  return pos < 0 || pos >= p.limit ? 0 : span_of(pos, p.window, p.sinks).blocks;
 }
 
+// m (running maximum of the raw scores), l, and o of one head of a
+// workgroup's part of an item.
+constexpr int kPartFloats = D + 2;
+// parts that a joining thread has in flight (more heads: more of its registers are taken)
+template <int G> constexpr int kRoundOf = G > 4 ? 16 : 32;
+
 template <int G> struct Shared {
+  union {
+    u32x4 stage[kWaves][2][512];  // a wave's 32 keys: K, V; then its o over K
+    float w[2][G][paged::kDecodeGroups];  // joining parts: m then weights, l
+  };
   float q[G][D];
   uint16_t kv_new[2][D];
-  float m[kWaves][G], l[kWaves][G], o[kWaves][G][D];
+  float m[kWaves][G], l[kWaves][G];
   int is_last;
 };
 
-// m (running maximum, in units of qscale * score), l, and o of one head of a
-// workgroup's part of an item.
-constexpr int kPartFloats = D + 2;
+// Parts of an item that runs r0 .. r1 share, joined in order into the output of
+// its G heads. Every load that a thread needs is issued before the first is
+// used, kRound parts at a time: one after the other, 32 parts took 20 us.
+template <int G>
+__device__ __forceinline__ void join_parts(const DecodeParams &p, float qscale, int r0, int r1,
+                                           int step, uint16_t *out, Shared<G> &sh) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int n = (r1 - r0) / step + 1;
+  constexpr int kRound = kRoundOf<G>, kPairs = G * D / 2, kThreads = 64 * kWaves;
+  // slot 2 r0 + 1, then 2 g: kSlot floats apart but for the first
+  const int kSlot = 2 * G * kPartFloats * step;
+  const float *first = p.part + size_t(2 * r0 + 1) * (G * kPartFloats);
+  const float *rest = p.part + size_t(2 * r0) * (G * kPartFloats);
+  const auto part = [&](int t) { return (t ? rest + size_t(t) * kSlot : first); };
+  typedef float f32x2 __attribute__((ext_vector_type(2)));
+  const auto load2 = [&](const float *at) {
+    const unsigned long long v =
+        __hip_atomic_load(reinterpret_cast<const unsigned long long *>(at), __ATOMIC_RELAXED,
+                          __HIP_MEMORY_SCOPE_AGENT);
+    return f32x2{__builtin_bit_cast(float, uint32_t(v)), __builtin_bit_cast(float, uint32_t(v >> 32))};
+  };
+  f32x2 o[kRound];
+  auto load_round = [&](int q, int t0) {
+    const int h = q / (D / 2), d = 2 * (q % (D / 2));
+#pragma unroll
+    for (int j = 0; j < kRound; ++j)  // (past the last part: that one, with weight 0)
+      o[j] = load2(part(min(t0 + j, n - 1)) + h * kPartFloats + d);
+  };
+  const int q0 = min(int(threadIdx.x), kPairs - 1);
+  const auto load_ml = [&](int at) { return load2(part(at / G) + (at % G) * kPartFloats + D); };
+  const auto keep_ml = [&](int at, f32x2 ml) {
+    sh.w[0][at % G][at / G] = ml.x;
+    sh.w[1][at % G][at / G] = ml.y;
+  };
+  const f32x2 ml0 = load_ml(min(int(threadIdx.x), G * n - 1));
+  load_round(q0, 0);
+  if (int(threadIdx.x) < G * n)
+    keep_ml(threadIdx.x, ml0);
+  for (int at = threadIdx.x + kThreads; at < G * n; at += kThreads)
+    keep_ml(at, load_ml(at));
+  __syncthreads();
+  for (int h = wave; h < G; h += kWaves) {
+    float M = -__builtin_inff();
+    for (int t = lane; t < n; t += 64)
+      M = fmaxf(M, sh.w[0][h][t]);
+    M = wave_max(M);
+    float den = 0.f;
+    for (int t = lane; t < n; t += 64) {
+      const float m = sh.w[0][h][t];
+      const float f = m == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f((m - M) * qscale);
+      den += f * sh.w[1][h][t];
+      sh.w[0][h][t] = f;
+    }
+    const float inv = 1.f / wave_sum(den);
+    for (int t = lane; t < (n + kRound - 1) / kRound * kRound; t += 64)
+      sh.w[0][h][t] = t < n ? sh.w[0][h][t] * inv : 0.f;
+  }
+  __syncthreads();
+  for (int q = threadIdx.x; q < kPairs; q += kThreads) {
+    if (q != q0)
+      load_round(q, 0);
+    const int h = q / (D / 2);
+    float a0 = 0.f, a1 = 0.f;
+    for (int t0 = 0; t0 < n; t0 += kRound) {
+      if (t0)
+        load_round(q, t0);
+#pragma unroll
+      for (int j = 0; j < kRound; ++j) {
+        const float w = sh.w[0][h][t0 + j];
+        a0 = fmaf(w, o[j].x, a0);
+        a1 = fmaf(w, o[j].y, a1);
+      }
+    }
+    reinterpret_cast<uint32_t *>(out)[q] = uint32_t(f2bf(a0)) | (uint32_t(f2bf(a1)) << 16);
+  }
+}
 
 template <int G>
 __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2, 2))) void
@@ -99,74 +199,163 @@ paged_decode_kernel(DecodeParams p, float qscale) {
   const int r = lane >> 4, i = lane & 15;
   const int hkv = p.cache.kv_heads;
 
-  // this workgroup's run [u0, u1) of the passes of all (sequence, kv head)
-  int total = 0;
+  // ---- which blocks are this workgroup's ----
+  int total = 0, sequences = 0;
   for (int b0 = 0; b0 < p.batch; b0 += 64) {
-    int n = b0 + lane < p.batch ? passes_of(p, b0 + lane) : 0;
-#pragma unroll
-    for (int s = 1; s < 64; s <<= 1)
-      n += __shfl_xor(n, s);
-    total += __builtin_amdgcn_readfirstlane(n);
+    const int n = b0 + lane < p.batch ? blocks_of(p, b0 + lane) : 0;
+    total += __builtin_amdgcn_readlane(wave_scan(n), 63);
+    sequences += __builtin_popcountll(__ballot(n > 0));
   }
+  const int items = sequences * hkv;
   total *= hkv;
-  const int each = total / p.groups, more = total % p.groups;  // the first `more` take one more
+  // dispatch goes round the 8 XCDs: each takes neighbouring runs
+  int run = int(blockIdx.x % 8) * (p.groups / 8) + int(blockIdx.x / 8);
+  int b, place, nb, kvh, x, u, u1, each = 0, more = 0, r0 = 0, r1 = 0, step = 1;
+  const bool chunks = p.batch <= 64 && total <= kChunkBlocks && items <= kChunks;
   auto run_begin = [&](int g) { return g * each + min(g, more); };
-  auto run_of = [&](int u) {
-    return u < more * (each + 1) ? u / (each + 1) : more + (u - more * (each + 1)) / each;
+  auto run_of = [&](int v) {
+    return v < more * (each + 1) ? v / (each + 1) : more + (v - more * (each + 1)) / each;
   };
-  const int run = blockIdx.x;
-  int u = run_begin(run);
-  const int u1 = run_begin(run + 1);
-  if (u >= u1)
-    return;
-  int b, place;
-  paged::find_item(p.batch, u, [&](int s) { return passes_of(p, s) * hkv; }, b, place);
-  int np = passes_of(p, b), kvh = place / np, x = place - kvh * np;
+  if (chunks) {
+    const int n = lane < p.batch ? blocks_of(p, lane) : 0;
+    // blocks of a chunk, at most: one a wave, kChunks chunks, kParts of a sequence
+    const int longest = int(wave_max(float(n)));
+    int size = max(max(kWaves, (longest + kParts - 1) / kParts), (total + kChunks - 1) / kChunks);
+    auto cut = [&](int blocks) { return (blocks + size - 1) / size; };
+    int count;
+    while ((count = __builtin_amdgcn_readlane(wave_scan(cut(n)), 63) * hkv) > kChunks)
+      ++size;
+    const int per = (count + 7) / 8;
+    run = int(blockIdx.x % 8) * per + int(blockIdx.x / 8);
+    if (int(blockIdx.x / 8) >= per ||
+        !paged::find_item(p.batch, run, [&](int) { return cut(n) * hkv; }, b, place))
+      return;
+    nb = __builtin_amdgcn_readlane(n, b);
+    const int of = cut(nb), j = place / hkv;
+    kvh = place % hkv;
+    step = hkv;
+    r0 = run - j * hkv;
+    r1 = r0 + (of - 1) * hkv;
+    x = j * nb / of;
+    u = x;
+    u1 = (j + 1) * nb / of;
+  } else {
+    // units: an item's first kItemCost stand for what it takes to begin one
+    total += items * kItemCost;
+    each = total / p.groups;
+    more = total % p.groups;  // the first `more` runs take one more
+    u = run_begin(run);
+    u1 = run_begin(run + 1);
+    if (u >= u1)
+      return;
+    paged::find_item(
+        p.batch, u,
+        [&](int s) {
+          const int n = blocks_of(p, s);
+          return n ? (n + kItemCost) * hkv : 0;
+        },
+        b, place);
+    nb = blocks_of(p, b);
+    kvh = place / (nb + kItemCost);
+    x = place - kvh * (nb + kItemCost) - kItemCost;  // (negative: begins an item)
+  }
 
   while (true) {
-    const int x1 = min(np, x + u1 - u);  // passes [x, x1) of item (b, kvh)
+    const int first = u - x, x1 = min(nb, x + u1 - u);  // blocks [x, x1) of item (b, kvh)
+    if (x1 <= 0)
+      return;  // not one block of the run's last item
+    x = max(x, 0);
     const int pos = p.pos[b];
     const Span span = span_of(pos, p.window, p.sinks);
-    const int item = u - x;  // first unit of the item
-    const bool whole = x == 0 && x1 == np;
+    const bool whole = x == 0 && x1 == nb;
+    if (!chunks) {  // the runs that share the item
+      r0 = run_of(first);
+      r1 = run_of(first + nb - 1);
+    }
+    const int low = p.window > 0 ? pos - p.window : -1;  // visible: t > low or t < sinks
 
-    // pages of this wave's blocks: lane j the one of pass x + j
+    // pages of this wave's blocks: lane j the one of block base + 4 j
     const int32_t *table = p.cache.table + size_t(b) * p.cache.table_stride;
-    int pages = 0, page_base = x;
-    auto load_pages = [&](int x0) {
-      const int v = min(kWaves * (x0 + lane) + wave, span.blocks - 1);
-      pages = table[(span.block(v) * kBlock) >> p.cache.shift];
-      page_base = x0;
+    int v = x + wave, pages = 0, page_base = v;
+    auto load_pages = [&](int v0) {
+      const int vb = min(v0 + kWaves * lane, span.blocks - 1);
+      pages = table[(span.block(vb) * kBlock) >> p.cache.shift];
+      page_base = v0;
     };
-    load_pages(x);
+    load_pages(v);
 
-    // ---- the token's heads: h < G query head, G key, G + 1 value ----
+    // ---- the token's heads h = wave + 4 j: h < G query, G key, G + 1 value;
+    // their inputs are on the way before K and V ----
+    constexpr int kHeads = (G + 2 + kWaves - 1) / kWaves;
     const uint16_t *row = p.qkv + size_t(b) * p.qkv_stride;
-    for (int h = wave; h < G + 2; h += kWaves) {
+    uint32_t pair[kHeads], gain2[kHeads];
+    NormRope nr;
+    load_rope(nr, p.cos + size_t(pos) * (D / 2), p.sin + size_t(pos) * (D / 2), lane);
+#pragma unroll
+    for (int j = 0; j < kHeads; ++j) {
+      const int h = min(wave + kWaves * j, G + 1);
       const size_t col = h < G ? size_t(kvh * G + h) * D : size_t(p.heads + (h - G) * hkv + kvh) * D;
-      const uint32_t pair = reinterpret_cast<const uint32_t *>(row + col)[lane];
-      if (h == G + 1) {
-        reinterpret_cast<uint32_t *>(sh.kv_new[1])[lane] = pair;
-        continue;
-      }
-      NormRope nr;
-      load_rope(nr, p.cos + size_t(pos) * (D / 2), p.sin + size_t(pos) * (D / 2), lane);
+      pair[j] = reinterpret_cast<const uint32_t *>(row + col)[lane];
       const uint16_t *gain = h < G ? p.q_norm : p.k_norm;
-      float x0 = bflo(pair), x1 = bfhi(pair);
-      if (gain) {
-        load_gain(nr, gain, lane);
-        const float scale = 1.0f / __builtin_sqrtf(wave_sum(x0 * x0 + x1 * x1) / float(D) + p.eps);
-        x0 = x0 * scale * nr.g0;
-        x1 = x1 * scale * nr.g1;
-      }
-      const float sgn = lane < 32 ? -1.f : 1.f;
-      const float y0 = fmaf(sgn * xor32(x0, lane), nr.s0, x0 * nr.c0);
-      const float y1 = fmaf(sgn * xor32(x1, lane), nr.s1, x1 * nr.c1);
+      gain2[j] = reinterpret_cast<const uint32_t *>(gain ? gain : row + col)[lane];
+    }
+    __builtin_amdgcn_sched_barrier(0);
+
+    // A block's K and V go straight to LDS in whole KiB, into the wave's own
+    // stage: K's 16-byte chunk c of key R to slot c ^ (4 (R / 8) + R % 4) of its
+    // 256 bytes, V's chunk c of dim d to slot c ^ (d / 4 % 4) of its 64 (the
+    // operand reads below then meet no bank twice, attn_tile.h).
+    u32x4 *ks = sh.stage[wave][0], *vs = sh.stage[wave][1];
+    int t0 = 0;
+    bool held = false;
+    auto fetch = [&](int vb) {
+      if (vb - page_base >= 64 * kWaves)
+        load_pages(vb);
+      const int page = __builtin_amdgcn_readlane(pages, (vb - page_base) / kWaves);
+      t0 = span.block(vb) * kBlock;
+      held = p.cache.has(page);
+      const size_t at = p.cache.at(held ? page : 0, kvh, t0 & ((1 << p.cache.shift) - 1));
+      const auto rk = __builtin_amdgcn_make_buffer_rsrc(p.cache.k + at, 0, kBlock * D * 2, 0x00020000);
+      const auto rv = __builtin_amdgcn_make_buffer_rsrc(p.cache.v + at, 0, kBlock * D * 2, 0x00020000);
+#pragma unroll
+      for (int q = 0; q < 8; ++q)
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(
+            rk, (lds_ptr_t)(ks + 64 * q), 16,
+            uint32_t((4 * q + r) * (D * 2) + (i ^ (4 * (q >> 1) + r)) * 16), 0, 0, kLoadAux);
+#pragma unroll
+      for (int q = 0; q < 8; ++q)
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(rv, (lds_ptr_t)(vs + 64 * q), 16,
+                                                 uint32_t(q * 1024 + (lane >> 2) * 64 +
+                                                          ((lane & 3) ^ (lane >> 4)) * 16),
+                                                 0, 0, kLoadAux);
+    };
+    if (v < x1)
+      fetch(v);
+
+    // every head's chain side by side; the value's is not used
+    float y0[kHeads], y1[kHeads];
+#pragma unroll
+    for (int j = 0; j < kHeads; ++j) {
+      y0[j] = bflo(pair[j]);
+      y1[j] = bfhi(pair[j]);
+      const bool normed = wave + kWaves * j < G ? p.q_norm : p.k_norm;
+      const float scale =
+          __builtin_amdgcn_rsqf(wave_sum(y0[j] * y0[j] + y1[j] * y1[j]) * (1.f / D) + p.eps);
+      y0[j] *= normed ? scale * bflo(gain2[j]) : 1.f;
+      y1[j] *= normed ? scale * bfhi(gain2[j]) : 1.f;
+    }
+    const float sgn = lane < 32 ? -1.f : 1.f;
+#pragma unroll
+    for (int j = 0; j < kHeads; ++j) {
+      const float a = sgn * xor32(y0[j], lane), c = sgn * xor32(y1[j], lane);
+      y0[j] = fmaf(a, nr.s0, y0[j] * nr.c0);
+      y1[j] = fmaf(c, nr.s1, y1[j] * nr.c1);
+      const int h = wave + kWaves * j;
       if (h < G)
-        reinterpret_cast<float2 *>(sh.q[h])[lane] = float2{y0, y1};
-      else
-        reinterpret_cast<uint32_t *>(sh.kv_new[0])[lane] =
-            uint32_t(f2bf(y0)) | (uint32_t(f2bf(y1)) << 16);
+        reinterpret_cast<float2 *>(sh.q[h])[lane] = float2{y0[j], y1[j]};
+      else if (h < G + 2)
+        reinterpret_cast<uint32_t *>(sh.kv_new[h - G])[lane] =
+            h == G ? uint32_t(f2bf(y0[j])) | (uint32_t(f2bf(y1[j])) << 16) : pair[j];
     }
     __syncthreads();
     // q operands: columns 0-7 the leading pieces of the heads, 8-15 the rests
@@ -187,54 +376,45 @@ paged_decode_kernel(DecodeParams p, float qscale) {
       qb[s] = u32x4{w[0], w[1], w[2], w[3]};
     }
 
-    // ---- passes ----
+    // ---- the wave's blocks: one in registers, the next on its way to LDS ----
     float m_run = -__builtin_inff(), l_run = 0.f;
     f32x4 o[8];
 #pragma unroll
     for (int dt = 0; dt < 8; ++dt)
       o[dt] = f32x4{0.f, 0.f, 0.f, 0.f};
-    for (; x < x1; ++x, ++u) {
-      const int v = kWaves * x + wave;
-      if (v >= span.blocks)  // uniform in the wave
-        continue;
-      if (x - page_base >= 64)
-        load_pages(x);
-      const int page = __builtin_amdgcn_readlane(pages, x - page_base);
-      const bool held = p.cache.has(page);
-      const int t0 = span.block(v) * kBlock;
-      const size_t at = p.cache.at(held ? page : 0, kvh, t0 & ((1 << p.cache.shift) - 1));
-      const u32x4 *kc = reinterpret_cast<const u32x4 *>(p.cache.k + at);
-      const u32x4 *vc = reinterpret_cast<const u32x4 *>(p.cache.v + at);
+    for (; v < x1; v += kWaves) {
+      wait_vmem();  // the block has landed
+      __builtin_amdgcn_sched_barrier(0);
       u32x4 kr[8], vr[8];
 #pragma unroll
-      for (int T = 0; T < 2; ++T)
-#pragma unroll
-        for (int s = 0; s < 4; ++s)
-          kr[4 * T + s] = kc[attn::key_ofs(T, i) * (D / 8) + 4 * s + r];
+      for (int j = 0; j < 8; ++j)
+        kr[j] = ks[attn::key_ofs(j >> 2, i) * 16 + ((4 * (j & 3) + r) ^ i)];
 #pragma unroll
       for (int dt = 0; dt < 8; ++dt)
-        vr[dt] = vc[(16 * dt + i) * (kBlock / 8) + r];
+        vr[dt] = vs[64 * dt + 4 * i + (r ^ (i >> 2))];
+      __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0): it is in registers
+      __builtin_amdgcn_sched_barrier(0);
+      const int key0 = t0;
       // a block that holds the token's own slot, keys it does not see, or no page
-      const int low = p.window > 0 ? pos - p.window : -1;  // visible: t > low or t < sinks
-      const bool part = !held || t0 + kBlock > pos || (t0 <= low && t0 + kBlock > p.sinks);
-      uint32_t seen = 0xffu;  // bit e: key t0 + 8 r + e
+      const bool part = !held || key0 + kBlock > pos || (key0 <= low && key0 + kBlock > p.sinks);
+      uint32_t seen = 0xffu;  // bit e: key key0 + 8 r + e
       if (part) {
         seen = 0u;
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          const int t = t0 + 8 * r + e;
+          const int t = key0 + 8 * r + e;
           if (t == pos || (held && t < pos && (t > low || t < p.sinks)))
             seen |= 1u << e;
         }
 #pragma unroll
         for (int T = 0; T < 2; ++T)
-          if (t0 + attn::key_ofs(T, i) == pos)
+          if (key0 + attn::key_ofs(T, i) == pos)
 #pragma unroll
             for (int s = 0; s < 4; ++s)
               kr[4 * T + s] = reinterpret_cast<const u32x4 *>(sh.kv_new[0])[4 * s + r];
         // values of keys that are not seen become zeros (their weights are: but
         // 0 times an infinity or NaN would count), the token's own come from LDS
-        const int ep = pos - (t0 + 8 * r);
+        const int ep = pos - (key0 + 8 * r);
         uint32_t keep[4];
 #pragma unroll
         for (int w = 0; w < 4; ++w)
@@ -248,14 +428,17 @@ paged_decode_kernel(DecodeParams p, float qscale) {
             vr[dt] = attn::with_elem(vr[dt], ep, sh.kv_new[1][16 * dt + i]);
         }
       }
+      if (v + kWaves < x1)
+        fetch(v + kWaves);
       f32x4 st[2];
 #pragma unroll
-      for (int T = 0; T < 2; ++T) {
+      for (int T = 0; T < 2; ++T)
         st[T] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int s = 0; s < 4; ++s)
+      for (int s = 0; s < 4; ++s)
+#pragma unroll
+        for (int T = 0; T < 2; ++T)
           st[T] = attn::mfma(kr[4 * T + s], qb[s], st[T]);
-      }
       float sc[8], mx = -__builtin_inff();
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
@@ -290,8 +473,9 @@ paged_decode_kernel(DecodeParams p, float qscale) {
         o[dt] = attn::mfma(vr[dt], u32x4{pw[0], pw[1], pw[2], pw[3]}, o[dt]);
       }
     }
+    u = first + x1;
 
-    // ---- join the waves ----
+    // ---- join the waves: each leaves its result in its own stage ----
     const float l_all = sum_halves(sum_row_pairs(l_run));
 #pragma unroll
     for (int dt = 0; dt < 8; ++dt) {
@@ -300,47 +484,54 @@ paged_decode_kernel(DecodeParams p, float qscale) {
       for (int e = 0; e < 4; ++e)
         s[e] = o[dt][e] + paged::xor8(o[dt][e]);  // the pieces of P
       if (i < G)
-        *reinterpret_cast<f32x4 *>(&sh.o[wave][i][16 * dt + 4 * r]) = s;
+        reinterpret_cast<f32x4 *>(ks)[i * (D / 4) + 4 * dt + r] = s;
     }
     if (i < G && r == 0) {
       sh.m[wave][i] = m_run;
       sh.l[wave][i] = l_all;
     }
     __syncthreads();
+    uint16_t *out = p.out + size_t(b) * p.out_stride + size_t(kvh * G) * D;
     // slot 2 run + 1: the item begins in this run (its last one); 2 run: before it
-    float *part = p.part + size_t(2 * run + (item >= run_begin(run))) * (G * kPartFloats);
-    for (int e = threadIdx.x; e < G * D; e += 64 * kWaves) {
-      const int h = e / D;
+    float *part = p.part + size_t(2 * run + (run == r0)) * (G * kPartFloats);
+    if (threadIdx.x < G * D / 4) {  // one thread per head and 4 dims
+      const int h = threadIdx.x / (D / 4), d = 4 * (threadIdx.x % (D / 4));
       float M = sh.m[0][h];
 #pragma unroll
       for (int w = 1; w < kWaves; ++w)
         M = fmaxf(M, sh.m[w][h]);
-      float acc = 0.f, l = 0.f;
+      f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+      float l = 0.f;
 #pragma unroll
       for (int w = 0; w < kWaves; ++w) {
         const float f = sh.m[w][h] == -__builtin_inff()
                             ? 0.f
                             : __builtin_amdgcn_exp2f((sh.m[w][h] - M) * qscale);
-        acc = fmaf(f, sh.o[w][h][e % D], acc);
+        acc += f * *reinterpret_cast<const f32x4 *>(
+                       reinterpret_cast<const float *>(sh.stage[w][0]) + h * D + d);
         l = fmaf(f, sh.l[w][h], l);
       }
       if (whole) {
-        p.out[size_t(b) * p.out_stride + size_t(kvh * G) * D + e] = f2bf(acc / l);
-        continue;
-      }
-      // write-through (agent-scope) stores: visible to every XCD once complete
-      __hip_atomic_store(&part[h * kPartFloats + e % D], acc, __ATOMIC_RELAXED,
-                         __HIP_MEMORY_SCOPE_AGENT);
-      if (e % D == 0) {
-        __hip_atomic_store(&part[h * kPartFloats + D], M, __ATOMIC_RELAXED,
-                           __HIP_MEMORY_SCOPE_AGENT);
-        __hip_atomic_store(&part[h * kPartFloats + D + 1], l, __ATOMIC_RELAXED,
-                           __HIP_MEMORY_SCOPE_AGENT);
+        acc *= 1.f / l;
+        *reinterpret_cast<uint2 *>(out + h * D + d) =
+            uint2{uint32_t(f2bf(acc[0])) | (uint32_t(f2bf(acc[1])) << 16),
+                  uint32_t(f2bf(acc[2])) | (uint32_t(f2bf(acc[3])) << 16)};
+      } else {
+        // write-through (agent-scope) stores: visible to every XCD once complete
+        const auto put = [&](int at, float lo, float hi) {
+          __hip_atomic_store(reinterpret_cast<unsigned long long *>(part + h * kPartFloats + at),
+                             (unsigned long long)f32_bits(hi) << 32 | f32_bits(lo),
+                             __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        };
+        put(d, acc[0], acc[1]);
+        put(d + 2, acc[2], acc[3]);
+        if (d == 0)
+          put(D, M, l);
       }
     }
     // ---- append, by the workgroup that holds the last pass (the one that read
     // the block) ----
-    if (x1 == np) {
+    if (x1 == nb) {
       const int page = table[pos >> p.cache.shift];
       const int slot = pos & ((1 << p.cache.shift) - 1);
       if (p.cache.has(page) && threadIdx.x < D / 8 + D) {
@@ -358,37 +549,16 @@ paged_decode_kernel(DecodeParams p, float qscale) {
       // Arrival: every wave's stores have completed, then one increment. The
       // counter is the one of the run that holds the item's first pass; no other
       // shared item begins in that run. The last workgroup joins the parts.
-      const int r0 = run_of(item), r1 = run_of(item + np - 1);
       wait_vmem();
       __syncthreads();
       if (threadIdx.x == 0) {
         const int prev = __hip_atomic_fetch_add(&p.counters[r0 * kCounterStride], 1,
                                                 __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        sh.is_last = prev == r1 - r0;
+        sh.is_last = prev == (r1 - r0) / step;
       }
       __syncthreads();
       if (sh.is_last) {
-        const auto slot_of = [&](int g) { return size_t(2 * g + (g == r0)) * (G * kPartFloats); };
-        for (int e = threadIdx.x; e < G * D; e += 64 * kWaves) {
-          const int h = e / D;
-          const auto load = [&](int g, int f) {
-            return __hip_atomic_load(&p.part[slot_of(g) + h * kPartFloats + f], __ATOMIC_RELAXED,
-                                     __HIP_MEMORY_SCOPE_AGENT);
-          };
-          float M = -__builtin_inff(), acc = 0.f, l = 0.f;
-          for (int g = r0; g <= r1; ++g) {
-            const float m = load(g, D), lg = load(g, D + 1), og = load(g, e % D);
-            if (m == -__builtin_inff())
-              continue;
-            const float top = fmaxf(M, m);
-            const float f0 = M == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f((M - top) * qscale);
-            const float f1 = __builtin_amdgcn_exp2f((m - top) * qscale);
-            acc = fmaf(f1, og, acc * f0);
-            l = fmaf(f1, lg, l * f0);
-            M = top;
-          }
-          p.out[size_t(b) * p.out_stride + size_t(kvh * G) * D + e] = f2bf(acc / l);
-        }
+        join_parts<G>(p, qscale, r0, r1, step, out, sh);
         if (threadIdx.x == 0)
           __hip_atomic_store(&p.counters[r0 * kCounterStride], 0, __ATOMIC_RELAXED,
                              __HIP_MEMORY_SCOPE_AGENT);
@@ -396,13 +566,13 @@ paged_decode_kernel(DecodeParams p, float qscale) {
     }
     if (u >= u1)
       return;
-    __syncthreads();  // the join has read what the next item writes
-    x = 0;
+    __syncthreads();  // what the join read is written by the next item
+    x = -kItemCost;
     if (++kvh == hkv) {
       kvh = 0;
       do
-        np = passes_of(p, ++b);
-      while (np == 0);
+        nb = blocks_of(p, ++b);
+      while (nb == 0);
     }
   }
 }
@@ -438,8 +608,8 @@ extern "C" int32_t yuear_op_paged_attention_decode(
       workspace_bytes < yuear_op_paged_workspace_bytes(batch, heads, kv_heads, 0))
     return int32_t(hipErrorInvalidValue);
   p.limit = std::min(p.cache.capacity, positions);
-  // passes are counted in 31 bits
-  if ((long long)batch * kv_heads * (p.limit / (paged::kBlock * kWaves) + 1) > 0x3fffffffLL)
+  // blocks, and what begins items, are counted in 31 bits
+  if ((long long)batch * kv_heads * (p.limit / paged::kBlock + 1 + kItemCost) > 0x3fffffffLL)
     return int32_t(hipErrorInvalidValue);
   p.qkv = qkv;
   p.qkv_stride = qkv_stride;

@@ -454,106 +454,126 @@ class PagePool:
         return lib.yuear_pages_unused(self._handle)
 
 
+# The calls below cost a decode step's host time per layer, so each check reads
+# an attribute once and builds its message only where it fails (paged_attention_decode
+# of one sequence, host time: 21.8 -> HOST us).
+
+def _refuse(name, message):
+    raise ValueError(f"{name}: {message}")
+
+
 def _hip_check(status, name):
     if status == 1:
-        raise ValueError(f"{name}: invalid arguments")
-    if status:
-        raise RuntimeError(f"{name}: HIP error {status}")
+        _refuse(name, "invalid arguments")
+    raise RuntimeError(f"{name}: HIP error {status}")
 
 
-def _require(ok, message):
-    if not ok:
-        raise ValueError(message)
+def _torch():
+    """torch, and its types that the checks compare with."""
+    global _T
+    if _T is None:
+        import torch
+        _T = (torch, torch.bfloat16, torch.int32)
+    return _T
 
 
-def _check_pages(k_pages, v_pages, device):
-    """(pages, kv heads, slots) of one layer's contiguous bf16 pages."""
-    import torch
-    bf16 = torch.bfloat16
-    _require(k_pages.dim() == 4 and v_pages.dim() == 5, "pages are k [pages, kv heads, slots, 128] and "
-             "v [pages, kv heads, slots / 32, 128, 32]")
-    n, hkv, slots, d = k_pages.shape
-    _require(d == 128 and tuple(v_pages.shape) == (n, hkv, slots // 32, 128, 32),
-             "pages are k [pages, kv heads, slots, 128] and v [pages, kv heads, slots / 32, 128, 32]")
-    _require(k_pages.dtype is bf16 and v_pages.dtype is bf16 and k_pages.is_contiguous()
-             and v_pages.is_contiguous(), "pages are contiguous bfloat16")
-    _require(k_pages.device == device and v_pages.device == device, "all tensors are on one device")
+_T = None
+_LAYOUT = ("pages are contiguous bfloat16 tensors on one device: k [pages, kv heads, slots, 128] and "
+           "v [pages, kv heads, slots / 32, 128, 32]")
+
+
+def _check_pages(k_pages, v_pages, index, name):
+    """(pages, kv heads, slots) of one layer's pages."""
+    bf16 = _torch()[1]
+    shape = k_pages.shape
+    if len(shape) != 4:
+        _refuse(name, _LAYOUT)
+    n, hkv, slots, d = shape
+    if not (d == 128 and v_pages.shape == (n, hkv, slots // 32, 128, 32) and k_pages.dtype is bf16
+            and v_pages.dtype is bf16 and k_pages.get_device() == index and v_pages.get_device() == index
+            and k_pages.is_contiguous() and v_pages.is_contiguous()):
+        _refuse(name, _LAYOUT)
     return n, hkv, slots
 
 
-def _check_ints(t, shape, device, name):
-    import torch
-    _require(t.dtype is torch.int32 and tuple(t.shape) == shape and t.device == device
-             and t.is_contiguous(), f"{name} is a contiguous int32 tensor {list(shape)} on the pages' device")
+def _check_ints(t, n, index, name, what):
+    if not (t.dtype is _torch()[2] and t.shape == (n,) and t.get_device() == index and t.is_contiguous()):
+        _refuse(name, f"{what} is a contiguous int32 tensor [{n}] on the pages' device")
 
 
-def _check_table(table, device):
-    import torch
-    _require(table.dtype is torch.int32 and table.dim() == 2 and table.device == device
-             and (table.stride(1) == 1 or table.shape[1] == 1) and table.shape[1] >= 1,
-             "table is int32 [sequences, pages] with whole rows")
-    return table.shape[1], max(table.stride(0), table.shape[1])
+def _check_table(table, index, name):
+    """(sequences, entries of a row, row stride) of a page table."""
+    shape = table.shape
+    if table.dtype is _torch()[2] and len(shape) == 2 and table.get_device() == index and shape[1] >= 1:
+        if table.is_contiguous():
+            return shape[0], shape[1], shape[1]
+        stride = table.stride()
+        if stride[1] == 1 and stride[0] >= shape[1]:
+            return shape[0], shape[1], stride[0]
+    _refuse(name, "table is int32 [sequences, pages] with whole rows on the pages' device")
 
 
-def _check_rope(cos, sin, device):
-    import torch
-    for t in (cos, sin):
-        _require(t.dtype is torch.bfloat16 and t.dim() == 2 and t.shape[1] == 64 and t.is_contiguous()
-                 and t.device == device, "cos and sin are contiguous bfloat16 [positions, 64]")
-    _require(cos.shape == sin.shape, "cos and sin have one shape")
+def _check_rope(cos, sin, index, name):
+    """Rows of the rotation tables."""
+    bf16, shape = _torch()[1], cos.shape
+    if not (len(shape) == 2 and shape[1] == 64 and sin.shape == shape and cos.dtype is bf16 and sin.dtype is bf16
+            and cos.get_device() == index and sin.get_device() == index and cos.is_contiguous()
+            and sin.is_contiguous()):
+        _refuse(name, "cos and sin are contiguous bfloat16 [positions, 64] on the pages' device")
+    return shape[0]
 
 
-def _gain(t, device):
-    import torch
+def _gain(t, index, name):
     if t is None:
         return None
-    _require(t.dtype is torch.bfloat16 and tuple(t.shape) == (128,) and t.is_contiguous() and t.device == device,
-             "norm gains are contiguous bfloat16 [128]")
+    if not (t.dtype is _torch()[1] and t.shape == (128,) and t.get_device() == index and t.is_contiguous()):
+        _refuse(name, "norm gains are contiguous bfloat16 [128] on the pages' device")
     return t.data_ptr()
 
 
-def _row_view(t, heads, device, name):
-    """Row stride of bf16 rows [n, heads, 128] (or [n, heads * 128])."""
-    import torch
-    flat = t.dim() == 2
-    _require(t.dtype is torch.bfloat16 and t.device == device and t.dim() in (2, 3)
-             and t.shape[1] * (1 if flat else t.shape[-1]) == heads * 128 and (flat or t.shape[2] == 128),
-             f"{name} is bfloat16 [rows, heads, 128] on the pages' device")
-    _require(t.stride(-1) == 1 and (flat or t.stride(1) == 128), f"{name} has contiguous rows")
-    return t.stride(0) if t.shape[0] > 1 else heads * 128
+def _qkv(qkv, hkv, index, name):
+    """(rows, query heads, row stride) of rows q | k | v."""
+    shape = qkv.shape
+    if len(shape) == 2 and qkv.dtype is _torch()[1] and not shape[1] % 128 and shape[1] // 128 > 2 * hkv:
+        stride = qkv.stride()
+        if stride[1] == 1:
+            return shape[0], shape[1] // 128 - 2 * hkv, stride[0] if shape[0] > 1 else shape[1]
+    _refuse(name, "qkv is bfloat16 [rows, (heads + 2 kv heads) * 128] with whole rows")
 
 
-class _On:
-    """The device of a call's tensors as the current one."""
-
-    def __init__(self, device):
-        import torch
-        self._guard = None if device.index == torch.cuda.current_device() else torch.cuda.device(device)
-
-    def __enter__(self):
-        if self._guard:
-            self._guard.__enter__()
-
-    def __exit__(self, *exc):
-        if self._guard:
-            self._guard.__exit__(*exc)
+def _rows(t, rows, heads, index, name, what):
+    """Row stride of [rows, heads, 128]."""
+    if t.dtype is _torch()[1] and t.shape == (rows, heads, 128) and t.get_device() == index:
+        stride = t.stride()
+        if stride[2] == 1 and (stride[1] == 128 or heads == 1):
+            return stride[0] if rows > 1 else heads * 128
+    _refuse(name, f"{what} is bfloat16 [{rows}, {heads}, 128] with whole rows on the pages' device")
 
 
-def _stream(stream, device, *given):
+def _stream(stream, index, name, *given):
     """The stream to run on: torch's current one, or the given one, for which
     the call allocates nothing (`given`: the caller's out and workspace)."""
-    import torch
-    current = torch.cuda.current_stream(device).cuda_stream
+    torch = _torch()[0]
+    if index < 0:
+        _refuse(name, "tensors are on the GPU")
+    current = torch._C._cuda_getCurrentRawStream(index)
     if stream is None or stream == current:
         return current
-    _require(all(t is not None for t in given), "a call on another stream than the current one needs out "
-             "and workspace tensors")
+    if any(t is None for t in given):
+        _refuse(name, "a call on another stream than the current one needs out and workspace tensors")
     return stream
 
 
-def _on_gpu(t):
-    _require(t.is_cuda, "tensors are on the GPU")
-    return t.device
+def _call(fn, name, index, *args):
+    """The library's call, with the tensors' device as the current one."""
+    cuda = _torch()[0].cuda
+    if index == cuda.current_device():
+        status = fn(*args)
+    else:
+        with cuda.device(index):
+            status = fn(*args)
+    if status:
+        _hip_check(status, name)
 
 
 def pages_copy(k_pages, v_pages, src, dst, stream=None):
@@ -561,35 +581,39 @@ def pages_copy(k_pages, v_pages, src, dst, stream=None):
     [layers, pages, kv heads, slots, 128] and v_pages [layers, pages, kv heads,
     slots / 32, 128, 32] (or one layer's, without the first dimension), src and
     dst lists of pages on the host."""
+    name, bf16 = "pages_copy", _torch()[1]
     k, v = (k_pages, v_pages) if k_pages.dim() == 5 else (k_pages[None], v_pages[None])
-    device = _on_gpu(k)
-    _require(k.dim() == 5 and v.dim() == 6 and k.shape[0] == v.shape[0] and k.shape[0] >= 1,
-             "pages are k [layers, pages, kv heads, slots, 128] and v [layers, pages, kv heads, slots / 32, 128, 32]")
-    n, hkv, slots = _check_pages(k[0], v[0], device)
-    _require(k.shape[0] == 1 or k.stride(0) == v.stride(0), "keys and values have one layer stride")
-    _require(len(src) == len(dst), "src and dst have one length")
-    s, d = ((C.c_int32 * len(src))(*src), (C.c_int32 * len(dst))(*dst))
-    with _On(device):
-        _hip_check(lib.yuear_op_pages_copy(k.data_ptr(), v.data_ptr(), k.shape[0], k.stride(0), n, hkv, slots,
-                                           s, d, len(src), _stream(stream, device)), "pages_copy")
+    index = k.get_device()
+    shape = k.shape
+    layers, n, hkv, slots, d = shape if len(shape) == 5 else (0,) * 5
+    ks, vs = k.stride(), v.stride()
+    row = hkv * slots * 128
+    if not (layers >= 1 and d == 128 and v.shape == (layers, n, hkv, slots // 32, 128, 32) and k.dtype is bf16
+            and v.dtype is bf16 and v.get_device() == index and ks[1:] == (row, slots * 128, 128, 1)
+            and vs[1:] == (row, slots * 128, 4096, 32, 1) and (layers == 1 or ks[0] == vs[0])):
+        _refuse(name, _LAYOUT + ", with one layer stride")
+    if len(src) != len(dst):
+        _refuse(name, "src and dst have one length")
+    pairs = C.c_int32 * len(src)
+    _call(lib.yuear_op_pages_copy, name, index, k.data_ptr(), v.data_ptr(), layers, ks[0], n, hkv, slots,
+          pairs(*src), pairs(*dst), len(src), _stream(stream, index, name))
 
 
 def paged_workspace(batch, heads, kv_heads, rows=0, device=None):
     """A zeroed workspace for the paged attention of up to these sizes (rows 0:
     decode steps only). Calls that may overlap need one each."""
-    import torch
+    torch = _torch()[0]
     n = lib.yuear_op_paged_workspace_bytes(batch, heads, kv_heads, rows)
-    _require(n > 0, "paged_workspace: invalid arguments")
+    if n <= 0:
+        _refuse("paged_workspace", "invalid arguments")
     return torch.zeros(n // 4, dtype=torch.int32, device="cuda" if device is None else device)
 
 
-def _workspace(workspace, batch, heads, kv_heads, rows, device):
-    import torch
-    if workspace is None:
-        return paged_workspace(batch, heads, kv_heads, rows, device)
-    _require(workspace.dtype is torch.int32 and workspace.is_contiguous() and workspace.device == device,
-             "workspace comes from paged_workspace")
-    return workspace
+def _workspace(workspace, index, name):
+    """Bytes of a caller's workspace."""
+    if not (workspace.dtype is _torch()[2] and workspace.get_device() == index and workspace.is_contiguous()):
+        _refuse(name, "workspace comes from paged_workspace")
+    return workspace.numel() * 4
 
 
 def paged_append(qkv, k_pages, v_pages, table, starts, pos0, cos, sin, q_norm=None, k_norm=None, eps=1e-5, out=None,
@@ -598,29 +622,22 @@ def paged_append(qkv, k_pages, v_pages, table, starts, pos0, cos, sin, q_norm=No
     queries [rows, heads, 128]. Sequence b (row b of the page table) owns rows
     starts[b] to starts[b + 1], at positions from pos0[b]; cos / sin [positions,
     64]. See yuear_op_paged_append."""
-    import torch
-    device = _on_gpu(qkv)
-    n, hkv, slots = _check_pages(k_pages, v_pages, device)
-    _require(qkv.dim() == 2 and qkv.shape[1] % 128 == 0 and qkv.shape[1] // 128 > 2 * hkv,
-             "qkv is bfloat16 [rows, (heads + 2 kv heads) * 128]")
-    stream = _stream(stream, device, out)
-    rows, heads = qkv.shape[0], qkv.shape[1] // 128 - 2 * hkv
-    stride = _row_view(qkv, heads + 2 * hkv, device, "qkv")
-    width, table_stride = _check_table(table, device)
-    batch = table.shape[0]
-    _check_ints(starts, (batch + 1,), device, "starts")
-    _check_ints(pos0, (batch,), device, "pos0")
-    _check_rope(cos, sin, device)
+    name, index = "paged_append", qkv.get_device()
+    stream = _stream(stream, index, name, out)
+    n, hkv, slots = _check_pages(k_pages, v_pages, index, name)
+    rows, heads, stride = _qkv(qkv, hkv, index, name)
+    batch, width, table_stride = _check_table(table, index, name)
+    _check_ints(starts, batch + 1, index, name, "starts")
+    _check_ints(pos0, batch, index, name, "pos0")
+    positions = _check_rope(cos, sin, index, name)
+    q_gain, k_gain = _gain(q_norm, index, name), _gain(k_norm, index, name)
     if out is None:
-        out = torch.empty(rows, heads, 128, dtype=torch.bfloat16, device=device)
-    _require(out.shape[0] == rows, "out has a row for each of qkv's")
-    out_stride = _row_view(out, heads, device, "out")
-    with _On(device):
-        _hip_check(lib.yuear_op_paged_append(
-            qkv.data_ptr(), stride, _gain(q_norm, device), _gain(k_norm, device), eps, cos.data_ptr(),
-            sin.data_ptr(), cos.shape[0], k_pages.data_ptr(), v_pages.data_ptr(), n, slots, table.data_ptr(),
-            width, table_stride, starts.data_ptr(), pos0.data_ptr(), batch, rows, heads, hkv, out.data_ptr(),
-            out_stride, stream), "paged_append")
+        torch, bf16, _ = _torch()
+        out = torch.empty((rows, heads, 128), dtype=bf16, device=qkv.device)
+    out_stride = _rows(out, rows, heads, index, name, "out")
+    _call(lib.yuear_op_paged_append, name, index, qkv.data_ptr(), stride, q_gain, k_gain, eps, cos.data_ptr(),
+          sin.data_ptr(), positions, k_pages.data_ptr(), v_pages.data_ptr(), n, slots, table.data_ptr(), width,
+          table_stride, starts.data_ptr(), pos0.data_ptr(), batch, rows, heads, hkv, out.data_ptr(), out_stride, stream)
     return out
 
 
@@ -630,28 +647,25 @@ def paged_attention_prefill(q, k_pages, v_pages, table, starts, pos0, window=0, 
     rows starts[b] to starts[b + 1], at positions from pos0[b]; a row at p sees
     the keys t <= p with p - t < window or t < sinks (window 0: all). See
     yuear_op_paged_attention_prefill."""
-    import torch
-    device = _on_gpu(q)
-    n, hkv, slots = _check_pages(k_pages, v_pages, device)
-    _require(q.dim() == 3, "q is bfloat16 [rows, heads, 128]")
-    stream = _stream(stream, device, out, workspace)
-    rows, heads = q.shape[0], q.shape[1]
-    stride = _row_view(q, heads, device, "q")
-    width, table_stride = _check_table(table, device)
-    batch = table.shape[0]
-    _check_ints(starts, (batch + 1,), device, "starts")
-    _check_ints(pos0, (batch,), device, "pos0")
+    name, index = "paged_attention_prefill", q.get_device()
+    stream = _stream(stream, index, name, out, workspace)
+    n, hkv, slots = _check_pages(k_pages, v_pages, index, name)
+    shape = q.shape
+    rows, heads = shape[0], shape[1] if len(shape) == 3 else 0
+    stride = _rows(q, rows, heads, index, name, "q")
+    batch, width, table_stride = _check_table(table, index, name)
+    _check_ints(starts, batch + 1, index, name, "starts")
+    _check_ints(pos0, batch, index, name, "pos0")
     if out is None:
-        out = torch.empty(rows, heads, 128, dtype=torch.bfloat16, device=device)
-    _require(out.shape[0] == rows, "out has a row for each of q's")
-    out_stride = _row_view(out, heads, device, "out")
-    with _On(device):
-        workspace = _workspace(workspace, batch, heads, hkv, rows, device)
-        _hip_check(lib.yuear_op_paged_attention_prefill(
-            q.data_ptr(), stride, k_pages.data_ptr(), v_pages.data_ptr(), n, slots, table.data_ptr(), width,
-            table_stride, starts.data_ptr(), pos0.data_ptr(), batch, rows, heads, hkv, window, sinks,
-            workspace.data_ptr(), workspace.numel() * 4, out.data_ptr(), out_stride, stream),
-            "paged_attention_prefill")
+        torch, bf16, _ = _torch()
+        out = torch.empty((rows, heads, 128), dtype=bf16, device=q.device)
+    out_stride = _rows(out, rows, heads, index, name, "out")
+    if workspace is None:
+        workspace = paged_workspace(batch, heads, hkv, rows, q.device)
+    _call(lib.yuear_op_paged_attention_prefill, name, index, q.data_ptr(), stride, k_pages.data_ptr(),
+          v_pages.data_ptr(), n, slots, table.data_ptr(), width, table_stride, starts.data_ptr(), pos0.data_ptr(),
+          batch, rows, heads, hkv, window, sinks, workspace.data_ptr(), _workspace(workspace, index, name),
+          out.data_ptr(), out_stride, stream)
     return out
 
 
@@ -661,30 +675,26 @@ def paged_attention_decode(qkv, k_pages, v_pages, table, pos, cos, sin, q_norm=N
     attention [sequences, heads, 128] over the table's pages. qkv [sequences,
     (heads + 2 kv heads) * 128], pos [sequences]. See
     yuear_op_paged_attention_decode."""
-    import torch
-    device = _on_gpu(qkv)
-    n, hkv, slots = _check_pages(k_pages, v_pages, device)
-    _require(qkv.dim() == 2 and qkv.shape[1] % 128 == 0 and qkv.shape[1] // 128 > 2 * hkv,
-             "qkv is bfloat16 [sequences, (heads + 2 kv heads) * 128]")
-    stream = _stream(stream, device, out, workspace)
-    batch, heads = qkv.shape[0], qkv.shape[1] // 128 - 2 * hkv
-    stride = _row_view(qkv, heads + 2 * hkv, device, "qkv")
-    width, table_stride = _check_table(table, device)
-    _require(table.shape[0] == batch, "table has a row for each of qkv's")
-    _check_ints(pos, (batch,), device, "pos")
-    _check_rope(cos, sin, device)
+    name, index = "paged_attention_decode", qkv.get_device()
+    stream = _stream(stream, index, name, out, workspace)
+    n, hkv, slots = _check_pages(k_pages, v_pages, index, name)
+    batch, heads, stride = _qkv(qkv, hkv, index, name)
+    sequences, width, table_stride = _check_table(table, index, name)
+    if sequences != batch:
+        _refuse(name, "table has a row for each of qkv's")
+    _check_ints(pos, batch, index, name, "pos")
+    positions = _check_rope(cos, sin, index, name)
+    q_gain, k_gain = _gain(q_norm, index, name), _gain(k_norm, index, name)
     if out is None:
-        out = torch.empty(batch, heads, 128, dtype=torch.bfloat16, device=device)
-    _require(out.shape[0] == batch, "out has a row for each of qkv's")
-    out_stride = _row_view(out, heads, device, "out")
-    with _On(device):
-        workspace = _workspace(workspace, batch, heads, hkv, 0, device)
-        _hip_check(lib.yuear_op_paged_attention_decode(
-            qkv.data_ptr(), stride, _gain(q_norm, device), _gain(k_norm, device), eps, cos.data_ptr(),
-            sin.data_ptr(), cos.shape[0], k_pages.data_ptr(), v_pages.data_ptr(), n, slots, table.data_ptr(),
-            width, table_stride, pos.data_ptr(), batch, heads, hkv, window, sinks, workspace.data_ptr(),
-            workspace.numel() * 4, out.data_ptr(), out_stride, stream),
-            "paged_attention_decode")
+        torch, bf16, _ = _torch()
+        out = torch.empty((batch, heads, 128), dtype=bf16, device=qkv.device)
+    out_stride = _rows(out, batch, heads, index, name, "out")
+    if workspace is None:
+        workspace = paged_workspace(batch, heads, hkv, 0, qkv.device)
+    _call(lib.yuear_op_paged_attention_decode, name, index, qkv.data_ptr(), stride, q_gain, k_gain, eps,
+          cos.data_ptr(), sin.data_ptr(), positions, k_pages.data_ptr(), v_pages.data_ptr(), n, slots,
+          table.data_ptr(), width, table_stride, pos.data_ptr(), batch, heads, hkv, window, sinks,
+          workspace.data_ptr(), _workspace(workspace, index, name), out.data_ptr(), out_stride, stream)
     return out
 
 
