@@ -366,6 +366,29 @@ def test_prefill(torch, yuear_lib, heads, kv, slots, lens, pos0, window, sinks):
     check_prefill(torch, s, prefill(torch, yuear_lib, s, window, sinks), window, sinks, 40 if len(lens) < 20 else 1)
 
 
+@pytest.mark.parametrize("heads,kv,slots,lens,pos0,window,sinks", [
+    (24, 8, 64, [1], [0], 0, 0),
+    (24, 8, 64, [97], [4000], 0, 0),
+    (24, 8, 64, [43, 42], [41, 4000], 0, 0),
+    (16, 8, 32, [5, 0, 33, 64, 1, 200], [0, 7, 31, 32, 63, 95], 0, 0),
+    (1, 1, 32, [500], [77], 0, 0),
+    (4, 4, 128, [31, 32, 65], [1, 127, 96], 0, 0),
+    (6, 1, 256, [300], [255], 0, 0),
+    (8, 1, 64, [130, 41], [20, 3000], 0, 0),
+    (16, 8, 32, [400, 1, 300], [0, 3000, 350], 1000, 33),
+    (3, 1, 64, [1000], [100], 700, 130),
+    (2, 1, 32, [200], [1500], 30, 5000),
+    (2, 1, 32, [77], [700], 2 ** 31 - 1, 3),
+    (3, 1, 32, [1 + i % 3 for i in range(16)], [i % 70 for i in range(16)], 0, 0),
+    (3, 1, 32, [1 + i % 3 for i in range(17)], [i % 70 for i in range(17)], 0, 0),
+])
+def test_prefill_in_a_table_with_room(torch, yuear_lib, heads, kv, slots, lens, pos0, window, sinks):
+    """A table of 16384 slots, where steps are dealt out however few keys there are."""
+    rng = np.random.default_rng(heads + kv + len(lens) + window % 997)
+    s = prefill_inputs(torch, rng, heads, kv, slots, lens, pos0, 500, width=16384 // slots)
+    check_prefill(torch, s, prefill(torch, yuear_lib, s, window, sinks), window, sinks)
+
+
 def test_prefill_of_large_scores(torch, yuear_lib):
     """Rows whose largest score grows by hundreds along the keys, and rows whose
     scores all lie far below zero."""

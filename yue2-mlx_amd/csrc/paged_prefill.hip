@@ -8,28 +8,42 @@
 // the table has; a row that sees nothing gives zeros. Bound by the two matrix
 // products (4 * 128 operations a query head, row and visible key).
 //
-// A workgroup takes a tile of 32 rows a wave of one kv head: its "rows" are
-// the (token, query head) pairs of the kv head's group, token by token, so all
-// heads of a group share the K and V that the workgroup stages, and a tile spans
-// few tokens, so little of its causal edge is computed for nothing. It walks the
-// 64-key blocks that any of its rows sees. Both products run on
+// A workgroup of 4 waves takes a tile of 128 rows of one kv head, 32 a wave: its
+// "rows" are the (token, query head) pairs of the kv head's group, token by token,
+// so all heads of a group share the K and V that the workgroup stages, and a tile
+// spans few tokens, so little of its causal edge is computed for nothing. It
+// walks the 64-key steps that any of its rows sees. Both products run on
 // v_mfma_f32_32x32x16_bf16:
 //
 //   S^T[key][row] = K[key][:] . q[row][:]      O^T[dim][row] += V^T[dim][key] . P^T[key][row]
 //
 // A lane holds one row's scores (column lane % 32), so the softmax needs one
-// exchange with lane ^ 32 a block, and a rescale multiplies its own sums. The rows
+// exchange with lane ^ 32 a step, and a rescale multiplies its own sums. The rows
 // of the K operand are permuted (key_of) so that the scores a lane ends up with
-// are its operand of the second product.
+// are its operand of the second product: P never passes through LDS.
 //
-// The running maximum m of a row enters S as the accumulator's start (-m), so
-// the difference is taken before the scale. It is raised only when a block's
-// score passes it by more than kSlack (weights up to 2^8, exact in 32 bits as
-// smaller ones are), which saves almost every rescale of the 64 sums. P is
-// rounded to bf16, 2^-9 of each weight at most, as the output is: one MFMA per
-// operand instead of two or three; the denominator sums the rounded weights.
+// K and V go from HBM to LDS without registers, two steps of each in 64 KiB, so
+// two workgroups share a CU and one's products run beside the other's barriers.
+// A step computes S of the step after it beside its own exponentials, and P V
+// beside the scaling of those scores; K is therefore loaded a step ahead of V.
+// Measured, 24 heads of 8 at 3000 rows / two prompts and a window of 1024, 5
+// sequences of 1500 (us): this form 72 / 115 (775 / 620 TFLOP/s); 8 waves and four
+// steps of LDS, one workgroup a CU: 88 / 130; S and P V of the same step one
+// after the other: 103 / 155.
+//
+// The running maximum m of a row is taken off its scores as they are scaled. It
+// is raised only when a score passes it by more than kSlack (the weights, up to
+// 2^20, are as exact in 32 bits and in bf16 as smaller ones), so almost no step
+// rescales the 64 sums. P is rounded to bf16, half a step of 2^-8 of each weight,
+// as the output is: one product per operand instead of two; the denominator sums
+// the rounded weights.
+//
+// A prompt piece of few rows behind many keys has fewer tiles than CUs
+// (worth_dealing): there 256 workgroups take equal runs of all tiles' steps, leave
+// the sums of tiles that they share, and a second kernel joins them.
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 #include "../../include/yuear.h"
 #include "attn_core.h"
@@ -41,13 +55,17 @@ namespace yuear {
 namespace {
 
 using attn::as_bf16x8;
+using attn::f32x4;
 using paged::Cache;
 using paged::D;
 using paged::kBlock;
+using paged::wave_scan;
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef __attribute__((address_space(3))) void *lds_ptr_t;
 
-constexpr int kKeys = 64;  // keys of a step
+constexpr int kKeys = 64;                 // keys of a step
+constexpr int kWaves = 4, kRows = 32 * kWaves;  // of a tile
+constexpr float kSlack = 20.f;  // log2 of the largest weight
 
 struct PrefillParams {
   const uint16_t *q = nullptr;
@@ -57,14 +75,25 @@ struct PrefillParams {
   int batch = 0, rows = 0, heads = 0, window = 0, sinks = 0;
   uint16_t *out = nullptr;
   long long out_stride = 0;
+  int tiles = 0;  // of a kv head, at most
+  // dealt launches: records of the tiles (head: their number) and partials
+  int32_t *info = nullptr;
+  float *part = nullptr;
 };
 
-// [stage][32-key half][K | V][16-byte pieces]: 8 KiB each. K: the chunk c of
-// key R in slot c ^ (R % 16) of its 256 bytes. V: chunk c (8 keys) of dim d in
-// slot c ^ (d / 4 % 4) of its 64. Either way the 16 lanes that a ds_read_b128
-// serves at once read 16 different 16-byte slots (gemm.hip).
-struct Stage {
-  u32x4 kv[2][2][512];
+constexpr int kRuns = 256;                      // workgroups of a dealt launch, one a CU
+constexpr int kTileCost = 3;                    // steps that beginning a tile costs
+constexpr int kDealSequences = 16;              // of a dealt launch, at most
+// A piece's sums as the lanes hold them, then its rows' maxima and denominators.
+constexpr size_t kPartFloats = size_t(kRows) * D + 2 * kRows;
+constexpr int kInfo = 8;  // words of a tile's record: first and last run, rows
+
+// A step's K or V: [32-key half][16-byte pieces], 16 KiB. K: the chunk c of key
+// R in slot c ^ (R % 16) of its 256 bytes. V: chunk c (8 keys) of dim d in slot
+// c ^ (d / 4 % 4) of its 64. Either way the 16 lanes that a ds_read_b128 serves
+// at once read 16 different 16-byte slots (gemm.hip).
+struct Ring {
+  u32x4 k[2][2][512], v[2][2][512];  // [step % 2]
 };
 
 // Key of a 32-key block in row r of the K operand: lane l of the result then
@@ -73,156 +102,272 @@ __device__ __forceinline__ int key_of(int r) {
   return 16 * (r >> 4) + 8 * ((r >> 2) & 1) + 4 * ((r >> 3) & 1) + (r & 3);
 }
 
+__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
+  typedef float f32x2 __attribute__((ext_vector_type(2)));
+  return __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{lo, hi}, bf16x2_t));
+}
 __device__ __forceinline__ f32x16 mfma32(u32x4 a, u32x4 b, f32x16 c) {
   return __builtin_amdgcn_mfma_f32_32x32x16_bf16(as_bf16x8(a), as_bf16x8(b), c, 0, 0, 0);
 }
 
-template <int G, int W>
-__global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(2, 2))) void
-paged_prefill_kernel(PrefillParams p, float qscale, int max_tiles) {
-  constexpr int kRows = 32 * W;
-  __shared__ Stage ring[2];
+// A tile of kRows rows of one kv head: its sequence's rows, its own, and the
+// 64-key blocks that it walks, [0, lead) and [first, ...).
+struct Tile {
+  paged::Rows rows;
+  int seq, index;               // index: in the sequence
+  int first_row, end_row;       // of the sequence's packed rows
+  int p0, p1;                   // positions of the first and the last
+  int first, lead, steps;
+  __device__ __forceinline__ int block(int x) const { return x < lead ? x : first + x - lead; }
+};
+template <int G> __device__ __forceinline__ int tiles_of(const paged::Rows &r) {
+  return (r.n * G + kRows - 1) / kRows;
+}
+template <int G>
+__device__ __forceinline__ Tile tile_of(const PrefillParams &p, const paged::Rows &rows, int seq,
+                                        int index) {
+  Tile t;
+  t.rows = rows;
+  t.seq = seq;
+  t.index = index;
+  t.first_row = index * kRows;
+  t.end_row = min(rows.n * G, t.first_row + kRows);
+  t.p0 = rows.pos0 + t.first_row / G;
+  t.p1 = rows.pos0 + (t.end_row - 1) / G;
+  t.first = t.lead = 0;
+  if (p.window > 0) {
+    t.first = max(0, t.p0 - p.window + 1) / kKeys;
+    t.lead = min((p.sinks - 1) / kKeys + (p.sinks > 0), t.first);
+  }
+  t.steps = t.lead + t.p1 / kKeys - t.first + 1;
+  return t;
+}
+
+// The work of a dealt launch in units, a step each and kTileCost for beginning a
+// tile: the units of a kv head are those of its tiles, sequence by sequence. Every
+// wave holds the (at most 64) sequences, one a lane, and walks their tiles 64 at
+// a time.
+template <int G> struct Deal {
+  const PrefillParams &p;
+  paged::Rows mine;  // of the lane's sequence
+  int total = 0, tiles = 0;
+  __device__ __forceinline__ explicit Deal(const PrefillParams &params) : p(params) {
+    const int lane = threadIdx.x & 63;
+    mine = paged::Rows{0, 0, 0};
+    if (lane < p.batch)
+      mine = paged::sequence_rows(p.starts, p.pos0, lane, p.rows, p.cache.capacity);
+    for (int b = 0; b < p.batch; ++b) {
+      const paged::Rows r = rows(b);
+      const int n = tiles_of<G>(r);
+      for (int t0 = 0; t0 < n; t0 += 64)
+        total += __builtin_amdgcn_readlane(wave_scan(units(r, b, t0 + lane, n)), 63);
+      tiles += n;
+    }
+  }
+  __device__ __forceinline__ paged::Rows rows(int b) const {
+    return paged::Rows{__builtin_amdgcn_readlane(mine.first, b), __builtin_amdgcn_readlane(mine.n, b),
+                       __builtin_amdgcn_readlane(mine.pos0, b)};
+  }
+  __device__ __forceinline__ int units(const paged::Rows &r, int b, int t, int n) const {
+    return t < n ? tile_of<G>(p, r, b, t).steps + kTileCost : 0;
+  }
+  // The tile of unit u < total, its number among a head's tiles, and the unit's
+  // place in it.
+  __device__ __forceinline__ Tile find(int u, int &number, int &place) const {
+    const int lane = threadIdx.x & 63;
+    number = 0;
+    for (int b = 0;; ++b) {
+      const paged::Rows r = rows(b);
+      const int n = tiles_of<G>(r);
+      for (int t0 = 0; t0 < n; t0 += 64) {
+        const int mine_ = units(r, b, t0 + lane, n), incl = wave_scan(mine_);
+        const int all = __builtin_amdgcn_readlane(incl, 63);
+        if (u < all) {
+          const int at = __builtin_popcountll(__ballot(incl <= u));
+          place = u - __builtin_amdgcn_readlane(incl - mine_, at);
+          number += t0 + at;
+          return tile_of<G>(p, r, b, t0 + at);
+        }
+        u -= all;
+      }
+      number += n;
+    }
+  }
+  // The tile after t of the same head; false past its last.
+  __device__ __forceinline__ bool next(Tile &t) const {
+    if (t.index + 1 < tiles_of<G>(t.rows)) {
+      t = tile_of<G>(p, t.rows, t.seq, t.index + 1);
+      return true;
+    }
+    for (int b = t.seq + 1; b < p.batch; ++b) {
+      const paged::Rows r = rows(b);
+      if (r.n) {
+        t = tile_of<G>(p, r, b, 0);
+        return true;
+      }
+    }
+    return false;
+  }
+};
+
+// Steps [x_begin, x_end) of a tile of kv head kvh; part: where a piece of the
+// tile leaves its sums (null: the whole tile).
+template <int G>
+__device__ __forceinline__ void walk_tile(const PrefillParams &p, float qscale, const Tile &tl, int kvh,
+                                          int x_begin, int x_end, float *part_of,
+                                          Ring &ring) {
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int col = lane & 31, half = lane >> 5;
-  const int kvh = blockIdx.x;
+  // the packed row of this lane
+  const int my_row = tl.first_row + 32 * wave + col;
+  const bool valid = my_row < tl.end_row;
+  const int token = min(my_row, tl.end_row - 1) / G, head = min(my_row, tl.end_row - 1) % G;
+  const int my_pos = tl.rows.pos0 + token;
 
-  // the tile: the last ones, which see the most keys, first
-  auto rows_of = [&](int b) {
-    return paged::sequence_rows(p.starts, p.pos0, b, p.rows, p.cache.capacity);
-  };
-  int b, tile;
-  if (!paged::find_item(p.batch, max_tiles - 1 - int(blockIdx.y),
-                        [&](int s) { return (rows_of(s).n * G + kRows - 1) / kRows; }, b, tile))
-    return;
-  const paged::Rows rs = rows_of(b);
-  const int pos0 = rs.pos0;
-  // packed rows of this tile, and of this wave's lane
-  const int first_row = tile * kRows, end_row = min(rs.n * G, first_row + kRows);
-  const int p0 = pos0 + first_row / G, p1 = pos0 + (end_row - 1) / G;
-  const int my_row = first_row + 32 * wave + col;
-  const bool valid = my_row < end_row;
-  const int token = min(my_row, end_row - 1) / G, head = min(my_row, end_row - 1) % G;
-  const int my_pos = pos0 + token;
+  const int low = p.window > 0 ? my_pos - p.window : -1;  // visible: t > low or t < sinks
+  const int x_last = x_end - 1;
 
-  // 64-key blocks [0, lead) and [first, p1 / 64]
-  int first = 0, lead = 0;
-  if (p.window > 0) {
-    first = max(0, p0 - p.window + 1) / kKeys;
-    lead = min((p.sinks - 1) / kKeys + (p.sinks > 0), first);
-  }
-  const int steps = lead + p1 / kKeys - first + 1;
-  auto block_of = [&](int x) { return x < lead ? x : first + x - lead; };
+  // ---- what the steps of [base, base + 32) need, lane 2 j + h for half h of
+  // step base + j: its page's element (of this kv head; page 0 where the table
+  // has none) and which steps have no page (absent), keys that some row of the
+  // wave does not see (partial) or that no row of the tile sees (dead) ----
+  const int32_t *table = p.cache.table + size_t(tl.seq) * p.cache.table_stride;
+  int base = 0;
+  uint32_t at_lo = 0, at_hi = 0;
+  unsigned long long absent = 0, partial = 0, dead = 0;
+  const int w0 = tl.rows.pos0 + min(tl.first_row + 32 * wave, tl.end_row - 1) / G;
+  const int w1 = tl.rows.pos0 + min(tl.first_row + 32 * wave + 31, tl.end_row - 1) / G;
+  auto load_steps = [&](int x0) __attribute__((always_inline)) {
+    const int t0 = tl.block(min(x0 + (lane >> 1), x_last)) * kKeys, t = t0 + kBlock * (lane & 1);
+    const int page = t < p.cache.capacity ? table[t >> p.cache.shift] : -1;
+    const bool has = p.cache.has(page);
+    const size_t at = p.cache.at(has ? page : 0, kvh, t & ((1 << p.cache.shift) - 1));
+    at_lo = uint32_t(at);
+    at_hi = uint32_t(at >> 32);
+    absent = __ballot(!has);
+    auto unseen = [&](int last, int first) {  // by rows at first .. last
+      return t0 + kKeys - 1 > first ||
+             (p.window > 0 && t0 <= last - p.window && t0 + kKeys > p.sinks);
+    };
+    partial = absent | __ballot(unseen(w1, w0));
+    dead = absent | __ballot(unseen(tl.p0, tl.p1));
+    base = x0;
+  };
+  auto bits = [&](unsigned long long of, int x) __attribute__((always_inline)) { return int(of >> (2 * (x - base))) & 3; };
 
-  // pages of the 32-key halves: lane 2 j + h the one of step base + j, half h
-  const int32_t *table = p.cache.table + size_t(b) * p.cache.table_stride;
-  int pages = 0, page_base = 0;
-  auto load_pages = [&](int x0) {
-    const int t = block_of(min(x0 + (lane >> 1), steps - 1)) * kKeys + kBlock * (lane & 1);
-    pages = t < p.cache.capacity ? table[t >> p.cache.shift] : -1;
-    page_base = x0;
-  };
-  load_pages(0);
-  auto page_at = [&](int x, int h) {
-    return __builtin_amdgcn_readlane(pages, 2 * (x - page_base) + h);
-  };
-  // this wave's part of step x: pieces of 1 KiB, 8 a half of K or V
-  auto fetch = [&](int x, int stage) {
-    if (x - page_base >= 32)
-      load_pages(x);
-    const int t0 = block_of(x) * kKeys;
+  // ---- loads: a wave's part of a step's K and V is 4 pieces of 1 KiB of
+  // one half. Past the last step it is taken again (nobody reads it), so every
+  // step issues as many loads and the waits count them. ----
+  constexpr int kPieces = 16 / kWaves;
+  const int my_half = wave >> 1, piece0 = (wave & 1) * kPieces;
+  uint32_t k_off[kPieces];
 #pragma unroll
-    for (int j = 0; j < 32 / W; ++j) {
-      const int piece = wave * (32 / W) + j;  // [half][K | V][8]
-      const int h = piece >> 4, is_v = (piece >> 3) & 1, q = piece & 7;
-      const int page = page_at(x, h);
-      const size_t at = p.cache.at(p.cache.has(page) ? page : 0, kvh,
-                                   (t0 + kBlock * h) & ((1 << p.cache.shift) - 1));
-      const auto rsrc = __builtin_amdgcn_make_buffer_rsrc(
-          (is_v ? p.cache.v : p.cache.k) + at, 0, kBlock * D * 2, 0x00020000);
-      const uint32_t off =
-          is_v ? uint32_t(q * 1024 + (lane >> 2) * 64 + ((lane & 3) ^ (lane >> 4)) * 16)
-               : uint32_t(q * 1024 + (lane >> 4) * 256 +
-                          ((lane & 15) ^ ((4 * q + (lane >> 4)) & 15)) * 16);
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (lds_ptr_t)&ring[stage].kv[h][is_v][64 * q],
-                                               16, off, 0, 0, 0);
-    }
+  for (int j = 0; j < kPieces; ++j)
+    k_off[j] = uint32_t((piece0 + j) * 1024 + (lane >> 4) * 256 +
+                        ((lane & 15) ^ ((4 * (piece0 + j) + (lane >> 4)) & 15)) * 16);
+  const uint32_t v_off = uint32_t(piece0 * 1024 + (lane >> 2) * 64 + ((lane & 3) ^ (lane >> 4)) * 16);
+  auto at_of = [&](int x) __attribute__((always_inline)) {
+    const int from = 2 * (min(x, x_last) - base) + my_half;
+    return (unsigned long long)(uint32_t(__builtin_amdgcn_readlane(at_hi, from))) << 32 |
+           uint32_t(__builtin_amdgcn_readlane(at_lo, from));
   };
-  fetch(0, 0);
+  auto load = [&](const uint16_t *from, size_t at, u32x4 *to, uint32_t off, int piece) __attribute__((always_inline)) {
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(
+        __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t *>(from) + at, 0, kBlock * D * 2,
+                                          0x00020000),
+        (lds_ptr_t)(to + 64 * piece), 16, off, 0, 0, 0);
+  };
+  auto load_k = [&](size_t at, int x, int j) __attribute__((always_inline)) {
+    load(p.cache.k, at, ring.k[x & 1][my_half], k_off[j], piece0 + j);
+  };
+  auto load_v = [&](size_t at, int x, int j) __attribute__((always_inline)) {
+    load(p.cache.v, at, ring.v[x & 1][my_half], v_off + 1024 * j, piece0 + j);
+  };
 
   // q operands: row `col`, dims 16 s + 8 half + [0, 8)
   u32x4 qb[8];
   {
     const u32x4 *src = reinterpret_cast<const u32x4 *>(
-        p.q + (size_t(rs.first) + token) * p.q_stride + size_t(kvh * G + head) * D);
+        p.q + (size_t(tl.rows.first) + token) * p.q_stride + size_t(kvh * G + head) * D);
 #pragma unroll
     for (int s = 0; s < 8; ++s)
       qb[s] = src[2 * s + half];
   }
-  const float slack = 8.f / qscale;
-  f32x16 start;  // -m in every element
+  load_steps(x_begin);
+  size_t v_at = at_of(x_begin);  // of the step whose V is loaded next
 #pragma unroll
-  for (int j = 0; j < 16; ++j)
-    start[j] = 0.f;
-  bool set = false;  // m is a score of this row
-  float l_run = 0.f;
-  f32x16 o[4];
+  for (int j = 0; j < kPieces; ++j)
+    load_k(v_at, x_begin, j);
+  const size_t second_at = at_of(x_begin + 1);
+#pragma unroll
+  for (int j = 0; j < kPieces; ++j)
+    load_v(v_at, x_begin, j);
+#pragma unroll
+  for (int j = 0; j < kPieces; ++j)
+    load_k(second_at, x_begin + 1, j);
+  v_at = second_at;
+
+  float m_run = 0.f;  // what is taken off the row's qscale * score
+  bool set = false;   // m_run is from a score of this row
+  float l_run[2] = {0.f, 0.f};
+  f32x16 o[4], e[2];
 #pragma unroll
   for (int dt = 0; dt < 4; ++dt)
 #pragma unroll
     for (int j = 0; j < 16; ++j)
       o[dt][j] = 0.f;
   const int key_row = key_of(col);
+  const int k_read = key_row * 16, k_xor = (key_row & 15) ^ half;  // chunk 2 s + half: 2 s ^ k_xor
+  const int v_read = col * 4, v_xor = ((col >> 2) & 3) ^ half;
+  auto k_operand = [&](int x, int n) __attribute__((always_inline)) {  // of product n: half n % 2, dims 16 (n / 2)
+    return ring.k[x & 1][n & 1][k_read + ((n & ~1) ^ k_xor)];
+  };
 
-  for (int x = 0; x < steps; ++x) {
-    const int stage = x & 1, t0 = block_of(x) * kKeys;
-    const bool held[2] = {p.cache.has(page_at(x, 0)), p.cache.has(page_at(x, 1))};
-    __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0): this wave's part has landed
-    __syncthreads();                     // ... and everyone's; the other stage is free
-    if (x + 1 < steps)
-      fetch(x + 1, stage ^ 1);
-    const int low = p.window > 0 ? my_pos - p.window : -1;  // visible: t > low or t < sinks
-    // keys that some row of the tile does not see
-    const bool part = !held[0] || !held[1] || t0 + kKeys - 1 > p0 ||
-                      (p.window > 0 && t0 <= p1 - p.window && t0 + kKeys > p.sinks);
-    f32x16 st[2];
+  // What a step needs before its weights are formed, where its keys are not all
+  // seen or its largest score passed the running maximum by kSlack: the scores
+  // of keys that the lane's row does not see, and a raised maximum.
+  auto settle = [&](int x) __attribute__((always_inline)) {
+    const int t0 = tl.block(x) * kKeys;
+    if (bits(partial, x)) {
+      const bool cut = p.window > 0 && t0 <= w1 - p.window;  // (uniform)
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      st[h] = start;
-      const u32x4 *ks = ring[stage].kv[h][0] + key_row * 16;
+      for (int h = 0; h < 2; ++h) {
+        // element j is the key at + 16 (j / 8) + j % 8; unseen: past `last`, or
+        // `many` keys from `from` on
+        const int at = t0 + kBlock * h + 8 * half, from = p.sinks - at;
+        const int last = (bits(absent, x) >> h) & 1 ? -1 : my_pos - at;
+        const uint32_t many = uint32_t(max(low - p.sinks + 1, 0));
 #pragma unroll
-      for (int s = 0; s < 8; ++s)
-        st[h] = mfma32(ks[(2 * s + half) ^ (key_row & 15)], qb[s], st[h]);
+        for (int j = 0; j < 16; ++j)
+          if (16 * (j >> 3) + (j & 7) > last)
+            e[h][j] = -__builtin_inff();
+        if (cut)
+#pragma unroll
+          for (int j = 0; j < 16; ++j)
+            if (uint32_t(16 * (j >> 3) + (j & 7) - from) < many)
+              e[h][j] = -__builtin_inff();
+      }
     }
-    if (part) {
-#pragma unroll
-      for (int h = 0; h < 2; ++h)
-#pragma unroll
-        for (int j = 0; j < 16; ++j) {
-          const int t = t0 + kBlock * h + 16 * (j >> 3) + 8 * half + (j & 7);
-          if (!held[h] || t > my_pos || (t <= low && t >= p.sinks))
-            st[h][j] = -__builtin_inff();
-        }
-    }
-    float mx = st[0][0];
+    float mx = e[0][0];
 #pragma unroll
     for (int h = 0; h < 2; ++h)
 #pragma unroll
       for (int j = 0; j < 16; ++j)
-        mx = fmaxf(mx, st[h][j]);
+        mx = fmaxf(mx, e[h][j]);
     mx = max_halves(mx);
-    const bool raise = mx > slack || (!set && mx > -__builtin_inff());
+    const bool raise = set ? mx > kSlack : mx > -__builtin_inff();
     if (__any(raise)) {
       const float d = raise ? mx : 0.f;
-      const float corr = __builtin_amdgcn_exp2f(-d * qscale);
-      const float f = set ? corr : 1.f;  // (all sums are zero before the first score)
-      l_run *= f;
+      const float f = set ? __builtin_amdgcn_exp2f(-d) : 1.f;  // (no sums before the first score)
+      l_run[0] *= f;
+      l_run[1] *= f;
+      m_run += d;
       set = set || raise;
 #pragma unroll
       for (int j = 0; j < 16; ++j) {
-        start[j] -= d;
-        st[0][j] -= d;
-        st[1][j] -= d;
+        e[0][j] -= d;
+        e[1][j] -= d;
       }
 #pragma unroll
       for (int dt = 0; dt < 4; ++dt)
@@ -230,72 +375,359 @@ paged_prefill_kernel(PrefillParams p, float qscale, int max_tiles) {
         for (int j = 0; j < 16; ++j)
           o[dt][j] *= f;
     }
+  };
+  // what every wave does at the start of a step
+  auto begin_step = [&](int x) __attribute__((always_inline)) {
+    __builtin_amdgcn_s_waitcnt(0x0F70);  // V of step x and K of step x + 1
+    __syncthreads();  // everyone's part; V's slot of step x - 1 and K's of x are free
+    if (__builtin_expect(x + 2 - base >= 32, 0))
+      load_steps(x);
+  };
+  // Values of a step's keys that no row of the tile sees become zeros: their
+  // weights are, but 0 times an infinity or NaN would count. A wave takes 8 keys
+  // of all dims at a time, a lane two dims.
+  auto bury = [&](int x) __attribute__((always_inline)) {
+    const int t0 = tl.block(x) * kKeys;
+    for (int n = wave; n < kKeys / 8; n += kWaves) {
+      const int h = n >> 2, c = n & 3, t = t0 + 8 * n;
+      uint32_t keep[4] = {0u, 0u, 0u, 0u};
+      if (!((bits(absent, x) >> h) & 1)) {
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      uint32_t pw[8];
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const float a = __builtin_amdgcn_exp2f(st[h][2 * j] * qscale);
-        const float c = __builtin_amdgcn_exp2f(st[h][2 * j + 1] * qscale);
-        pw[j] = uint32_t(f2bf(a)) | (uint32_t(f2bf(c)) << 16);
-        l_run = __builtin_amdgcn_fdot2_f32_bf16(as_bf16x2(pw[j]), as_bf16x2(0x3f803f80u), l_run,
-                                                false);
+        for (int k = 0; k < 8; ++k)
+          if (t + k <= tl.p1 && (p.window <= 0 || t + k > tl.p0 - p.window || t + k < p.sinks))
+            keep[k >> 1] |= 0xffffu << (16 * (k & 1));
       }
-      uint32_t keep[8];  // values of keys that no row of the tile sees become zeros
-      if (part) {
+      if ((keep[0] & keep[1] & keep[2] & keep[3]) == 0xffffffffu)
+        continue;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          keep[j] = 0u;
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const int t = t0 + kBlock * h + 16 * (j >> 2) + 8 * half + 2 * (j & 3) + e;
-            if (held[h] && t <= p1 && (p.window <= 0 || t > p0 - p.window || t < p.sinks))
-              keep[j] |= 0xffffu << (16 * e);
-          }
-        }
-      }
-#pragma unroll
-      for (int s = 0; s < 2; ++s) {
-        const u32x4 pb = u32x4{pw[4 * s], pw[4 * s + 1], pw[4 * s + 2], pw[4 * s + 3]};
-#pragma unroll
-        for (int dt = 0; dt < 4; ++dt) {
-          u32x4 v = ring[stage].kv[h][1][(32 * dt + col) * 4 + ((2 * s + half) ^ ((col >> 2) & 3))];
-          if (part)
-            v = u32x4{v.x & keep[4 * s], v.y & keep[4 * s + 1], v.z & keep[4 * s + 2],
-                      v.w & keep[4 * s + 3]};
-          o[dt] = mfma32(v, pb, o[dt]);
-        }
+      for (int d = lane; d < D; d += 64) {
+        u32x4 &v = ring.v[x & 1][h][d * (kBlock / 8) + (c ^ ((d >> 2) & 3))];
+        v = u32x4{v.x & keep[0], v.y & keep[1], v.z & keep[2], v.w & keep[3]};
       }
     }
+    __syncthreads();  // (the same for all waves: the tile's keys and pages are)
+  };
+
+  __builtin_amdgcn_s_waitcnt(0x0F70 | 2 * kPieces);  // Q and K of the first step
+  __syncthreads();
+  {
+    f32x16 st[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int j = 0; j < 16; ++j)
+        st[h][j] = 0.f;
+#pragma unroll
+    for (int n = 0; n < 16; ++n)
+      st[n & 1] = mfma32(k_operand(x_begin, n), qb[n >> 1], st[n & 1]);
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int j = 0; j < 16; ++j)
+        e[h][j] = st[h][j] * qscale;
   }
-  const float l = sum_halves(l_run);
+
+  if (tl.first_row + 32 * wave >= tl.end_row) {  // no row of the wave's: it only loads
+    for (int x = x_begin; x < x_end; ++x) {
+      begin_step(x);
+      if (bits(dead, x))
+        bury(x);
+      const size_t k_at = at_of(x + 2);
+#pragma unroll
+      for (int j = 0; j < kPieces; ++j)
+        load_v(v_at, x + 1, j);
+#pragma unroll
+      for (int j = 0; j < kPieces; ++j)
+        load_k(k_at, x + 2, j);
+      v_at = k_at;
+    }
+    return;
+  }
+  bool due = true;  // settle() is
+  auto step = [&](int x, auto more_tag) __attribute__((always_inline)) {
+    constexpr bool more = decltype(more_tag)::value;  // not the last one
+    begin_step(x);
+    if (__builtin_expect(bits(dead, x), 0))
+      bury(x);
+    if (__builtin_expect(due, 0))
+      settle(x);
+    u32x4(&vs)[2][512] = ring.v[x & 1];
+    uint32_t pw[2][8];
+    auto weights = [&](int w) __attribute__((always_inline)) {  // words 2 w, 2 w + 1 of P's 16, rounded, and their sum
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        const int h = w >> 2, j = (2 * w + k) & 7;
+        pw[h][j] = pack_bf16(__builtin_amdgcn_exp2f(e[h][2 * j]),
+                             __builtin_amdgcn_exp2f(e[h][2 * j + 1]));
+        l_run[k] = __builtin_amdgcn_fdot2_f32_bf16(as_bf16x2(pw[h][j]), as_bf16x2(0x3f803f80u),
+                                                   l_run[k], false);
+      }
+    };
+    auto values = [&](int n) __attribute__((always_inline)) {  // the 16 products of P and V
+      const int h = n >> 3, s = (n >> 2) & 1, dt = n & 3;
+      o[dt] = mfma32(vs[h][v_read + 128 * dt + ((2 * s) ^ v_xor)],
+                     u32x4{pw[h][4 * s], pw[h][4 * s + 1], pw[h][4 * s + 2], pw[h][4 * s + 3]},
+                     o[dt]);
+    };
+    if constexpr (more) {
+      const size_t k_at = at_of(x + 2);
+      f32x16 st[2];
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int j = 0; j < 16; ++j)
+          st[h][j] = 0.f;
+      // S of the next step beside P of this one
+#pragma unroll
+      for (int n = 0; n < 16; ++n) {
+        st[n & 1] = mfma32(k_operand(x + 1, n), qb[n >> 1], st[n & 1]);
+        if (n % (16 / kPieces) == 0)
+          load_v(v_at, x + 1, n / (16 / kPieces));
+        if (n & 1)
+          weights(n >> 1);
+      }
+      // P V beside the scaling of the next step's scores
+      float mx[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        mx[k] = -__builtin_inff();
+#pragma unroll
+      for (int n = 0; n < 16; ++n) {
+        values(n);
+        if (n % (16 / kPieces) == 0)
+          load_k(k_at, x + 2, n / (16 / kPieces));
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          const int h = n >> 3, j = (2 * n + k) & 15;
+          e[h][j] = fmaf(st[h][j], qscale, -m_run);
+          mx[n & 3] = fmaxf(mx[n & 3], e[h][j]);
+        }
+      }
+      v_at = k_at;
+      // LDS reads a few products ahead of their use
+      constexpr int kAhead = 4;
+      __builtin_amdgcn_sched_group_barrier(0x100, kAhead, 0);
+#pragma unroll
+      for (int n = 0; n < 32 - kAhead; ++n) {
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+      }
+      __builtin_amdgcn_sched_group_barrier(0x008, kAhead, 0);
+      due = bool(int(bits(partial, x + 1) != 0) |
+                 int(__ballot(!set | (fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) > kSlack)) != 0));
+    } else {
+#pragma unroll
+      for (int w = 0; w < 8; ++w)
+        weights(w);
+#pragma unroll
+      for (int n = 0; n < 16; ++n)
+        values(n);
+    }
+  };
+  for (int x = x_begin; x < x_last; ++x)
+    step(x, std::true_type{});
+  step(x_last, std::false_type{});
+  const float l = sum_halves(l_run[0] + l_run[1]);
+  if (part_of) {
+    f32x4 *to = reinterpret_cast<f32x4 *>(part_of) + wave * (16 * 64) + lane;
+#pragma unroll
+    for (int dt = 0; dt < 4; ++dt)
+#pragma unroll
+      for (int a = 0; a < 4; ++a)
+        to[(4 * dt + a) * 64] =
+            f32x4{o[dt][4 * a], o[dt][4 * a + 1], o[dt][4 * a + 2], o[dt][4 * a + 3]};
+    if (half == 0)
+      reinterpret_cast<float2 *>(part_of + kRows * D)[32 * wave + col] =
+          float2{set ? m_run : -__builtin_inff(), l};
+    return;
+  }
   if (!valid)
     return;
   const float inv = set ? 1.f / l : 0.f;
   // element j of tile dt: dim 32 dt + 8 (j / 4) + 4 half + j % 4
-  uint16_t *dst = p.out + (size_t(rs.first) + token) * p.out_stride + size_t(kvh * G + head) * D;
+  uint16_t *dst = p.out + (size_t(tl.rows.first) + token) * p.out_stride + size_t(kvh * G + head) * D;
 #pragma unroll
   for (int dt = 0; dt < 4; ++dt)
 #pragma unroll
     for (int a = 0; a < 4; ++a) {
-      const uint32_t lo = uint32_t(f2bf(o[dt][4 * a] * inv)) |
-                          (uint32_t(f2bf(o[dt][4 * a + 1] * inv)) << 16);
-      const uint32_t hi = uint32_t(f2bf(o[dt][4 * a + 2] * inv)) |
-                          (uint32_t(f2bf(o[dt][4 * a + 3] * inv)) << 16);
+      const uint32_t lo = pack_bf16(o[dt][4 * a] * inv, o[dt][4 * a + 1] * inv);
+      const uint32_t hi = pack_bf16(o[dt][4 * a + 2] * inv, o[dt][4 * a + 3] * inv);
       *reinterpret_cast<uint2 *>(dst + 32 * dt + 8 * a + 4 * half) = uint2{lo, hi};
     }
 }
 
-template <int G> hipError_t launch_g(const PrefillParams &p, hipStream_t s) {
-  constexpr int W = 4;
+// One tile a workgroup, those of a sequence's end, which see the most keys, first
+// (several sequences: the last one's).
+template <int G>
+__global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2, 2))) void
+paged_prefill_kernel(PrefillParams p, float qscale) {
+  __shared__ Ring ring;
+  int seq, index;
+  auto rows_of = [&](int b) {
+    return paged::sequence_rows(p.starts, p.pos0, b, p.rows, p.cache.capacity);
+  };
+  if (!paged::find_item(
+          p.batch, p.tiles - 1 - int(blockIdx.y), [&](int b) { return tiles_of<G>(rows_of(b)); },
+          seq, index))
+    return;
+  const Tile t = tile_of<G>(p, rows_of(seq), seq, index);
+  walk_tile<G>(p, qscale, t, blockIdx.x, 0, t.steps, nullptr, ring);
+}
+
+// Dealt: every workgroup takes an equal run of the units of all heads.
+template <int G>
+__global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2, 2))) void
+paged_prefill_deal_kernel(PrefillParams p, float qscale) {
+  __shared__ Ring ring;
+  const Deal<G> deal(p);
+  const int total = deal.total * p.cache.kv_heads, each = total / kRuns, more = total % kRuns;
+  auto run_begin = [&](int g) { return g * each + min(g, more); };
+  auto run_of = [&](int u) {
+    return u < more * (each + 1) ? u / (each + 1) : more + (u - more * (each + 1)) / each;
+  };
+  // dispatch goes round the 8 XCDs: each takes neighbouring runs, whose tiles
+  // share K and V in its L2
+  const int run = int(blockIdx.x % 8) * (kRuns / 8) + int(blockIdx.x / 8);
+  if (run == 0 && threadIdx.x == 0)
+    p.info[0] = deal.tiles;
+  int u = run_begin(run);
+  const int u1 = run_begin(run + 1);
+  if (u >= u1)
+    return;
+  int kvh = u / deal.total, number, place;
+  Tile t = deal.find(u - kvh * deal.total, number, place);
+  while (true) {
+    const int first = u - place + kTileCost;  // unit of the tile's first step
+    const int x0 = max(place - kTileCost, 0), x1 = min(t.steps, u1 - first);
+    if (x1 <= 0)
+      return;  // not one step of the run's last tile
+    const int r0 = run_of(first), r1 = run_of(first + t.steps - 1);
+    if (x0 == 0 && threadIdx.x == 0) {
+      int32_t *info = p.info + kInfo * (1 + size_t(kvh) * p.tiles + number);
+      info[0] = r0;
+      info[1] = r1;
+      info[2] = t.rows.first;
+      info[3] = t.first_row;
+      info[4] = t.end_row;
+    }
+    // slot 2 run + 1: the tile begins in this run (its last one); 2 run: before it
+    walk_tile<G>(p, qscale, t, kvh, x0, x1,
+                 r0 == r1 ? nullptr : p.part + size_t(2 * run + (run == r0)) * kPartFloats, ring);
+    u = first + x1;
+    if (u >= u1)
+      return;
+    __syncthreads();  // the ring is free
+    place = 0;
+    ++number;
+    if (!deal.next(t)) {
+      ++kvh;
+      t = deal.find(0, number, place);
+    }
+  }
+}
+
+// Rows of tiles that several runs hold, joined in order of the keys: a wave per
+// 32 rows and 32 dims, its lanes as the tile's held them. Every load of a round
+// of pieces is issued before the first is used.
+template <int G>
+__global__ __launch_bounds__(256) void paged_prefill_join_kernel(PrefillParams p) {
+  const int lane = threadIdx.x & 63, dt = threadIdx.x >> 6;
+  const int col = lane & 31, half = lane >> 5, kvh = blockIdx.x, group = blockIdx.y;
+  if (int(blockIdx.z) >= p.info[0])
+    return;
+  const int32_t *info = p.info + kInfo * (1 + size_t(kvh) * p.tiles + blockIdx.z);
+  const int r0 = info[0], r1 = info[1], first = info[2], first_row = info[3], end_row = info[4];
+  if (r0 == r1 || first_row + 32 * group >= end_row)
+    return;
+  const int pieces = r1 - r0 + 1, row = first_row + 32 * group + col;
+  constexpr int kRound = 4;
+  float M = -__builtin_inff(), l = 0.f;
+  f32x4 o[4] = {};
+  for (int j0 = 0; j0 < pieces; j0 += kRound) {
+    float2 ml[kRound];
+    f32x4 v[kRound][4];
+#pragma unroll
+    for (int j = 0; j < kRound; ++j) {  // (past the last piece: that one, with weight 0)
+      const int g = min(j0 + j, pieces - 1);
+      const float *from = p.part + size_t(2 * (r0 + g) + (g == 0)) * kPartFloats;
+      ml[j] = reinterpret_cast<const float2 *>(from + kRows * D)[32 * group + col];
+#pragma unroll
+      for (int a = 0; a < 4; ++a)
+        v[j][a] = reinterpret_cast<const f32x4 *>(from)[group * (16 * 64) + (4 * dt + a) * 64 + lane];
+    }
+    float top = M;
+#pragma unroll
+    for (int j = 0; j < kRound; ++j)
+      top = fmaxf(top, ml[j].x);
+    const float f = M == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(M - top);
+    l *= f;
+#pragma unroll
+    for (int a = 0; a < 4; ++a)
+      o[a] *= f;
+#pragma unroll
+    for (int j = 0; j < kRound; ++j) {
+      const bool out = j0 + j >= pieces || ml[j].x == -__builtin_inff();
+      const float w = out ? 0.f : __builtin_amdgcn_exp2f(ml[j].x - top);
+      l += out ? 0.f : w * ml[j].y;
+#pragma unroll
+      for (int a = 0; a < 4; ++a)
+        o[a] += out ? f32x4{0.f, 0.f, 0.f, 0.f} : w * v[j][a];
+    }
+    M = top;
+  }
+  if (row >= end_row)
+    return;
+  const float inv = M == -__builtin_inff() ? 0.f : 1.f / l;
+  uint16_t *dst = p.out + (size_t(first) + row / G) * p.out_stride +
+                  size_t(kvh * G + row % G) * D + 32 * dt + 4 * half;
+#pragma unroll
+  for (int a = 0; a < 4; ++a)
+    *reinterpret_cast<uint2 *>(dst + 8 * a) =
+        uint2{pack_bf16(o[a][0] * inv, o[a][1] * inv), pack_bf16(o[a][2] * inv, o[a][3] * inv)};
+}
+
+// Tiles of a kv head that `rows` rows of `batch` sequences take at most.
+long long tiles_at_most(int batch, int rows, int group) {
+  return (long long)rows * group / kRows + std::min(batch, rows);
+}
+
+// Whether to deal the steps out: where the tiles would leave compute units idle
+// for longer than dealing costs. A launch of whole tiles takes as long as one
+// that sees all the keys that the tables hold, at most; dealt, its steps are
+// spread over all units, but begin every piece anew and need a second kernel,
+// about six steps' time. 24 heads of 8, time of whole tiles and dealt (us):
+//   200 rows after 0 keys 11.3 / 15.8    700 rows after 0     18.6 / 24.2
+//   97 after 4000         64.8 / 26.7    700 after 3000       63.8 / 59.5
+//   400 after 3000        57.1 / 41.9    1000 after 3000      71.6 / 79.2
+bool worth_dealing(const PrefillParams &p, long long tiles) {
+  constexpr int kDealTiles = 192, kDealSteps = 6;
+  if (p.batch > kDealSequences || tiles >= kDealTiles)
+    return false;
+  long long keys = p.cache.capacity;
+  if (p.window > 0)
+    keys = std::min(keys, (long long)p.window + p.sinks + 2 * kKeys);
+  const long long steps = keys / kKeys;
+  return steps < (1 << 21) && steps * (kDealTiles - tiles) > kDealSteps * kDealTiles;
+}
+
+template <int G> hipError_t launch_g(PrefillParams p, hipStream_t s) {
   const float qscale = float(std::pow(double(D), -0.5)) * attn::kLog2e;
-  // sequences of n rows take at most n G / 128 + 1 tiles each
-  const long long tiles =
-      (long long)p.rows * G / (32 * W) + std::min(p.batch, p.rows);
+  const int kv_heads = p.cache.kv_heads;
+  const long long tiles = tiles_at_most(p.batch, p.rows, G);
   if (tiles > 65535)
     return hipErrorInvalidValue;
-  hipLaunchKernelGGL((paged_prefill_kernel<G, W>), dim3(p.cache.kv_heads, unsigned(tiles)),
-                     dim3(64 * W), 0, s, p, qscale, int(tiles));
+  p.tiles = int(tiles);
+  if (!worth_dealing(p, tiles * kv_heads)) {
+    hipLaunchKernelGGL(paged_prefill_kernel<G>, dim3(kv_heads, p.tiles), dim3(64 * kWaves), 0, s, p,
+                       qscale);
+    return hipGetLastError();
+  }
+  hipLaunchKernelGGL(paged_prefill_deal_kernel<G>, dim3(kRuns), dim3(64 * kWaves), 0, s, p, qscale);
+  const hipError_t e = hipGetLastError();
+  if (e != hipSuccess)
+    return e;
+  hipLaunchKernelGGL(paged_prefill_join_kernel<G>, dim3(kv_heads, kWaves, p.tiles), dim3(256), 0, s,
+                     p);
   return hipGetLastError();
 }
 
@@ -309,8 +741,12 @@ int64_t yuear_op_paged_workspace_bytes(int32_t batch, int32_t heads, int32_t kv_
   using namespace yuear;
   if (batch < 0 || rows < 0 || !paged::group_ok(heads, kv_heads))
     return 0;
-  const int64_t group = heads / kv_heads;
-  return int64_t(paged::kCounterBytes) + int64_t(2 * paged::kDecodeGroups) * group * (paged::D + 2) * 4;
+  // enough for every call of no more sequences, rows and heads
+  const int64_t decode = int64_t(2 * paged::kDecodeGroups) * paged::kMaxGroup * (paged::D + 2) * 4;
+  const int64_t tiles = tiles_at_most(batch, rows, paged::kMaxGroup) * kv_heads;
+  const int64_t prefill =
+      rows ? (1 + tiles) * int64_t(kInfo * 4) + 2 * kRuns * int64_t(kPartFloats * 4) : 0;
+  return int64_t(paged::kCounterBytes) + std::max(decode, prefill);
 }
 
 int32_t yuear_op_paged_attention_prefill(
@@ -344,6 +780,8 @@ int32_t yuear_op_paged_attention_prefill(
   p.sinks = sinks;
   p.out = out;
   p.out_stride = out_stride;
+  p.part = reinterpret_cast<float *>(static_cast<uint8_t *>(workspace) + paged::kCounterBytes);
+  p.info = reinterpret_cast<int32_t *>(p.part + 2 * kRuns * kPartFloats);
   const hipStream_t s = static_cast<hipStream_t>(stream);
   switch (heads / kv_heads) {
   case 1: return int32_t(launch_g<1>(p, s));
