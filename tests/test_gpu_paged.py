@@ -413,6 +413,39 @@ def test_prefill_sees_no_key_of_a_page_that_is_not_there(torch, yuear_lib, bad):
     assert not out[200:240].any() and not out[240:252].any() and out[252:].any()
 
 
+@pytest.mark.parametrize("width", [8, 128])
+@pytest.mark.parametrize("window,sinks", [(0, 0), (100, 3)])
+def test_prefill_keeps_infinities_from_rows_that_do_not_see_them(torch, yuear_lib, width, window, sinks):
+    """Values of some keys are infinities and NaNs: rows that see them give those,
+    the rows beside them in a tile what they give with zeros there."""
+    rng = np.random.default_rng(23)
+    heads, kv, n, before = 24, 8, 150, 130
+    s = prefill_inputs(torch, rng, heads, kv, 64, [n], [before], 30, width=width)
+    inf = float("inf")
+    marks = {131: inf, 170: float("nan"), 171: -inf, 200: inf, 201: -inf, 279: inf}
+    v = normal(torch, rng, kv, before + n, 128)
+    odd = torch.zeros_like(v)
+    for t, x in marks.items():
+        odd[:, t, 5:100:7] = x
+        if t in (170, 201):
+            odd[:, t] = x
+    k = normal(torch, rng, kv, before + n, 128)
+    s["pages"].put(s["table"][0], 0, k, torch.where(odd == 0, v, torch.zeros_like(v)))
+    clean = prefill(torch, yuear_lib, s, window, sinks)
+    check_prefill(torch, s, clean, window, sinks)
+    s["pages"].put(s["table"][0], 0, k, torch.where(odd == 0, v, odd))
+    out = prefill(torch, yuear_lib, s, window, sinks).float()
+    want = clean.float()
+    for i in range(n):
+        for t in marks:
+            if ref.visible(before + i, before + n, window, sinks)[t]:
+                want[i] += odd[:, t].float().repeat_interleave(heads // kv, 0)
+    finite = torch.isfinite(want)
+    assert torch.equal(torch.isnan(out), torch.isnan(want)) and torch.equal(out[~finite].nan_to_num(), want[~finite].nan_to_num())
+    s["pages"].put(s["table"][0], 0, k, torch.where(odd == 0, v, torch.zeros_like(v)))
+    check_prefill(torch, s, torch.where(finite, out, want.nan_to_num(0, 0, 0) + clean), window, sinks, some=150)
+
+
 def test_prefill_leaves_other_rows_as_they_are(torch, yuear_lib):
     rng = np.random.default_rng(17)
     s = prefill_inputs(torch, rng, 3, 1, 32, [40, 10, 10, 40], [40, 0, 3, 0], 30, width=3)

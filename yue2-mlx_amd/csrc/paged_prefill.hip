@@ -210,10 +210,11 @@ template <int G> struct Deal {
   }
 };
 
-// Steps [x_begin, x_end) of a tile of kv head kvh; part: where a piece of the
-// tile leaves its sums (null: the whole tile).
+// Steps [x_begin, x_end) of a tile of kv head kvh; part_of: where a piece of the
+// tile leaves its sums (null: the whole tile). False, with nothing written, where
+// walk_odd() has to do it.
 template <int G>
-__device__ __forceinline__ void walk_tile(const PrefillParams &p, float qscale, const Tile &tl, int kvh,
+__device__ __forceinline__ bool walk_tile(const PrefillParams &p, float qscale, const Tile &tl, int kvh,
                                           int x_begin, int x_end, float *part_of,
                                           Ring &ring) {
   const int lane = threadIdx.x & 63;
@@ -231,11 +232,12 @@ __device__ __forceinline__ void walk_tile(const PrefillParams &p, float qscale, 
   // ---- what the steps of [base, base + 32) need, lane 2 j + h for half h of
   // step base + j: its page's element (of this kv head; page 0 where the table
   // has none) and which steps have no page (absent), keys that some row of the
-  // wave does not see (partial) or that no row of the tile sees (dead) ----
+  // wave does not see (partial), some row
+  // of the tile does not see (edge) or no row of the tile sees (dead) ----
   const int32_t *table = p.cache.table + size_t(tl.seq) * p.cache.table_stride;
   int base = 0;
   uint32_t at_lo = 0, at_hi = 0;
-  unsigned long long absent = 0, partial = 0, dead = 0;
+  unsigned long long absent = 0, partial = 0, edge = 0, dead = 0;
   const int w0 = tl.rows.pos0 + min(tl.first_row + 32 * wave, tl.end_row - 1) / G;
   const int w1 = tl.rows.pos0 + min(tl.first_row + 32 * wave + 31, tl.end_row - 1) / G;
   auto load_steps = [&](int x0) __attribute__((always_inline)) {
@@ -251,6 +253,7 @@ __device__ __forceinline__ void walk_tile(const PrefillParams &p, float qscale, 
              (p.window > 0 && t0 <= last - p.window && t0 + kKeys > p.sinks);
     };
     partial = absent | __ballot(unseen(w1, w0));
+    edge = absent | __ballot(unseen(tl.p1, tl.p0));
     dead = absent | __ballot(unseen(tl.p0, tl.p1));
     base = x0;
   };
@@ -383,29 +386,61 @@ __device__ __forceinline__ void walk_tile(const PrefillParams &p, float qscale, 
     if (__builtin_expect(x + 2 - base >= 32, 0))
       load_steps(x);
   };
-  // Values of a step's keys that no row of the tile sees become zeros: their
-  // weights are, but 0 times an infinity or NaN would count. A wave takes 8 keys
-  // of all dims at a time, a lane two dims.
+  // An unseen key weighs 0, but 0 times an infinity or a NaN would count. So in a
+  // step with keys that not all rows of the tile see, the values of those that
+  // none sees become zeros here (a wave takes 8 keys of all dims at a time, a lane
+  // two dims), and infinities or NaNs that remain are noticed: walk_odd() then does
+  // the tile again.
+  uint32_t odd = 0;
+  auto odd_halves = [&](uint32_t w) __attribute__((always_inline)) {
+    return ((w & 0x7f807f80u) + 0x00800080u) & 0x80008000u;
+  };
+  // (the lane's number anew, so that what this computes from it stays here)
+  auto rare = [&](int v) __attribute__((always_inline)) {
+    asm volatile("" : "+v"(v));
+    return v;
+  };
   auto bury = [&](int x) __attribute__((always_inline)) {
-    const int t0 = tl.block(x) * kKeys;
-    for (int n = wave; n < kKeys / 8; n += kWaves) {
-      const int h = n >> 2, c = n & 3, t = t0 + 8 * n;
-      uint32_t keep[4] = {0u, 0u, 0u, 0u};
-      if (!((bits(absent, x) >> h) & 1)) {
+    const int me = rare(lane);
+    if (bits(dead, x)) {
+      const int t0 = tl.block(x) * kKeys;
+      for (int n = wave; n < kKeys / 8; n += kWaves) {
+        const int t = t0 + 8 * n;
+        uint32_t keep[4] = {0u, 0u, 0u, 0u};
+        if (!((bits(absent, x) >> (n >> 2)) & 1)) {
 #pragma unroll
-        for (int k = 0; k < 8; ++k)
-          if (t + k <= tl.p1 && (p.window <= 0 || t + k > tl.p0 - p.window || t + k < p.sinks))
-            keep[k >> 1] |= 0xffffu << (16 * (k & 1));
-      }
-      if ((keep[0] & keep[1] & keep[2] & keep[3]) == 0xffffffffu)
-        continue;
+          for (int k = 0; k < 8; ++k)
+            if (t + k <= tl.p1 && (p.window <= 0 || t + k > tl.p0 - p.window || t + k < p.sinks))
+              keep[k >> 1] |= 0xffffu << (16 * (k & 1));
+        }
+        if ((keep[0] & keep[1] & keep[2] & keep[3]) == 0xffffffffu)
+          continue;
 #pragma unroll
-      for (int d = lane; d < D; d += 64) {
-        u32x4 &v = ring.v[x & 1][h][d * (kBlock / 8) + (c ^ ((d >> 2) & 3))];
-        v = u32x4{v.x & keep[0], v.y & keep[1], v.z & keep[2], v.w & keep[3]};
+        for (int d0 = 0; d0 < D; d0 += 64) {
+          const int d = d0 + me;
+          u32x4 &v = ring.v[x & 1][n >> 2][d * (kBlock / 8) + ((n & 3) ^ ((d >> 2) & 3))];
+          v = u32x4{v.x & keep[0], v.y & keep[1], v.z & keep[2], v.w & keep[3]};
+        }
       }
+      __syncthreads();  // (all waves agree: the tile's keys and pages are the same)
     }
-    __syncthreads();  // (the same for all waves: the tile's keys and pages are)
+    const u32x4 *v = ring.v[x & 1][0] + 256 * wave + me;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const u32x4 w = v[64 * i];
+      odd |= odd_halves(w.x) | odd_halves(w.y) | odd_halves(w.z) | odd_halves(w.w);
+    }
+  };
+  // At the tile's end: whether any wave noticed some. Through K's slot of the last
+  // step, which nothing is loaded into any more.
+  auto any_odd = [&]() __attribute__((always_inline)) {
+    const uint32_t mine = __any(odd != 0);
+    u32x4 &slot = ring.k[x_last & 1][0][0];
+    if (lane == 0)
+      reinterpret_cast<uint32_t *>(&slot)[wave] = mine;
+    __syncthreads();
+    const u32x4 all = slot;
+    return __builtin_amdgcn_readfirstlane(all.x | all.y | all.z | all.w) != 0;
   };
 
   __builtin_amdgcn_s_waitcnt(0x0F70 | 2 * kPieces);  // Q and K of the first step
@@ -430,8 +465,10 @@ __device__ __forceinline__ void walk_tile(const PrefillParams &p, float qscale, 
   if (tl.first_row + 32 * wave >= tl.end_row) {  // no row of the wave's: it only loads
     for (int x = x_begin; x < x_end; ++x) {
       begin_step(x);
-      if (bits(dead, x))
+      if (bits(edge, x))
         bury(x);
+      if (x == x_last)
+        break;
       const size_t k_at = at_of(x + 2);
 #pragma unroll
       for (int j = 0; j < kPieces; ++j)
@@ -441,13 +478,13 @@ __device__ __forceinline__ void walk_tile(const PrefillParams &p, float qscale, 
         load_k(k_at, x + 2, j);
       v_at = k_at;
     }
-    return;
+    return !any_odd();
   }
   bool due = true;  // settle() is
   auto step = [&](int x, auto more_tag) __attribute__((always_inline)) {
     constexpr bool more = decltype(more_tag)::value;  // not the last one
     begin_step(x);
-    if (__builtin_expect(bits(dead, x), 0))
+    if (__builtin_expect(bits(edge, x), 0))
       bury(x);
     if (__builtin_expect(due, 0))
       settle(x);
@@ -527,6 +564,8 @@ __device__ __forceinline__ void walk_tile(const PrefillParams &p, float qscale, 
   for (int x = x_begin; x < x_last; ++x)
     step(x, std::true_type{});
   step(x_last, std::false_type{});
+  if (any_odd())
+    return false;
   const float l = sum_halves(l_run[0] + l_run[1]);
   if (part_of) {
     f32x4 *to = reinterpret_cast<f32x4 *>(part_of) + wave * (16 * 64) + lane;
@@ -539,10 +578,10 @@ __device__ __forceinline__ void walk_tile(const PrefillParams &p, float qscale, 
     if (half == 0)
       reinterpret_cast<float2 *>(part_of + kRows * D)[32 * wave + col] =
           float2{set ? m_run : -__builtin_inff(), l};
-    return;
+    return true;
   }
   if (!valid)
-    return;
+    return true;
   const float inv = set ? 1.f / l : 0.f;
   // element j of tile dt: dim 32 dt + 8 (j / 4) + 4 half + j % 4
   uint16_t *dst = p.out + (size_t(tl.rows.first) + token) * p.out_stride + size_t(kvh * G + head) * D;
@@ -554,6 +593,75 @@ __device__ __forceinline__ void walk_tile(const PrefillParams &p, float qscale, 
       const uint32_t hi = pack_bf16(o[dt][4 * a + 2] * inv, o[dt][4 * a + 3] * inv);
       *reinterpret_cast<uint2 *>(dst + 32 * dt + 8 * a + 4 * half) = uint2{lo, hi};
     }
+  return true;
+}
+
+// walk_tile() where a value that some rows of the tile see and others do not is
+// not finite: row by row, a lane per key for the scores and per two dims for the
+// sums, over the keys that the row sees alone. Rare, so plain.
+template <int G>
+__device__ __forceinline__ void walk_odd(const PrefillParams &p, float qscale, const Tile &tl, int kvh,
+                                         int x_begin, int x_end, float *part_of) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int32_t *table = p.cache.table + size_t(tl.seq) * p.cache.table_stride;
+  const int last = min(tl.first_row + 32 * (wave + 1), tl.end_row);
+#pragma unroll 1
+  for (int r = tl.first_row + 32 * wave; r < last; ++r) {
+    const int token = r / G, head = kvh * G + r % G, pos = tl.rows.pos0 + token;
+    const uint32_t *q = reinterpret_cast<const uint32_t *>(
+        p.q + (size_t(tl.rows.first) + token) * p.q_stride + size_t(head) * D);
+    float M = -__builtin_inff(), l = 0.f, o[2] = {0.f, 0.f};  // of dims lane and lane + 64
+#pragma unroll 1
+    for (int x = x_begin; x < x_end; ++x) {
+      const int t0 = tl.block(x) * kKeys, t = t0 + lane;
+      const int page = t < p.cache.capacity ? table[t >> p.cache.shift] : -1;
+      const bool sees = p.cache.has(page) && t <= pos &&
+                        (p.window <= 0 || t > pos - p.window || t < p.sinks);
+      const size_t at = p.cache.at(p.cache.has(page) ? page : 0, kvh,
+                                   (t & ~(kBlock - 1)) & ((1 << p.cache.shift) - 1));
+      const uint32_t *k = reinterpret_cast<const uint32_t *>(p.cache.k + at) + (lane & 31) * (D / 2);
+      float score = 0.f;
+#pragma unroll 8
+      for (int d = 0; d < D / 2; ++d)
+        score = __builtin_amdgcn_fdot2_f32_bf16(as_bf16x2(k[d]), as_bf16x2(q[d]), score, false);
+      score = sees ? score * qscale : -__builtin_inff();
+      float top = score;
+#pragma unroll
+      for (int b = 1; b < 64; b <<= 1)
+        top = fmaxf(top, __shfl_xor(top, b));
+      top = fmaxf(M, top);
+      unsigned long long left = __ballot(sees);
+      if (!left || top == -__builtin_inff())
+        continue;
+      const float f = M == -__builtin_inff() ? 1.f : __builtin_amdgcn_exp2f(M - top);
+      const float w = sees ? __builtin_amdgcn_exp2f(score - top) : 0.f;
+      M = top;
+      l *= f;
+      o[0] *= f;
+      o[1] *= f;
+      for (; left; left &= left - 1) {
+        const int n = __builtin_ctzll(left);
+        const float wn = __shfl(w, n);
+        const uint16_t *v = p.cache.v + __shfl((long long)at, n) + (n & 31);
+        l += wn;
+        o[0] += wn * __uint_as_float(uint32_t(v[lane * kBlock]) << 16);
+        o[1] += wn * __uint_as_float(uint32_t(v[(lane + 64) * kBlock]) << 16);
+      }
+    }
+    if (part_of) {  // as walk_tile() leaves it
+      const int col = r - tl.first_row - 32 * wave;
+      for (int k = 0; k < 2; ++k) {
+        const int d = lane + 64 * k;
+        part_of[4 * (wave * (16 * 64) + (d >> 3) * 64 + (d >> 2 & 1) * 32 + col) + (d & 3)] = o[k];
+      }
+      if (lane == 0)
+        reinterpret_cast<float2 *>(part_of + kRows * D)[32 * wave + col] = float2{M, l};
+      continue;
+    }
+    uint16_t *dst = p.out + (size_t(tl.rows.first) + token) * p.out_stride + size_t(head) * D;
+    for (int k = 0; k < 2; ++k)
+      dst[lane + 64 * k] = uint16_t(pack_bf16(M == -__builtin_inff() ? 0.f : o[k] / l, 0.f));
+  }
 }
 
 // One tile a workgroup, those of a sequence's end, which see the most keys, first
@@ -571,7 +679,8 @@ paged_prefill_kernel(PrefillParams p, float qscale) {
           seq, index))
     return;
   const Tile t = tile_of<G>(p, rows_of(seq), seq, index);
-  walk_tile<G>(p, qscale, t, blockIdx.x, 0, t.steps, nullptr, ring);
+  if (!walk_tile<G>(p, qscale, t, blockIdx.x, 0, t.steps, nullptr, ring))
+    walk_odd<G>(p, qscale, t, blockIdx.x, 0, t.steps, nullptr);
 }
 
 // Dealt: every workgroup takes an equal run of the units of all heads.
@@ -611,8 +720,9 @@ paged_prefill_deal_kernel(PrefillParams p, float qscale) {
       info[4] = t.end_row;
     }
     // slot 2 run + 1: the tile begins in this run (its last one); 2 run: before it
-    walk_tile<G>(p, qscale, t, kvh, x0, x1,
-                 r0 == r1 ? nullptr : p.part + size_t(2 * run + (run == r0)) * kPartFloats, ring);
+    float *part_of = r0 == r1 ? nullptr : p.part + size_t(2 * run + (run == r0)) * kPartFloats;
+    if (!walk_tile<G>(p, qscale, t, kvh, x0, x1, part_of, ring))
+      walk_odd<G>(p, qscale, t, kvh, x0, x1, part_of);
     u = first + x1;
     if (u >= u1)
       return;
