@@ -437,9 +437,11 @@ int32_t yuear_op_paged_attention_decode(
     int32_t window, int32_t sinks, void *dev_workspace, int64_t workspace_bytes,
     uint16_t *dev_out, int64_t out_stride, void *stream);
 /* Bytes of the workspace of the two attention calls (rows 0: the decode form),
- * 0 for invalid arguments. The caller zeroes it once; every call leaves it ready
- * for the next, of any shape that it is large enough for. Calls that may
- * overlap (other streams, graphs replayed at once) need one each. */
+ * 0 for invalid arguments. The caller zeroes its first
+ * YUEAR_PAGED_COUNTER_BYTES once; every call leaves it ready for the next, of
+ * any shape that it is large enough for. Calls that may overlap (other streams,
+ * graphs replayed at once) need one each. */
+#define YUEAR_PAGED_COUNTER_BYTES 131072
 int64_t yuear_op_paged_workspace_bytes(int32_t batch, int32_t heads, int32_t kv_heads,
                                        int32_t rows);
 /* Page copies: page dst[i] = page src[i] of K and V in each of `layers` layers,

@@ -34,7 +34,7 @@ struct AppendParams {
   long long q_stride = 0;
 };
 
-constexpr int kHeadsPerGroup = 8;
+constexpr int kHeadsPerGroup = 3;
 
 __device__ __forceinline__ void unpack8(u32x4 w, float (&x)[8]) {
   const uint32_t v[4] = {w.x, w.y, w.z, w.w};
@@ -45,19 +45,24 @@ __device__ __forceinline__ void unpack8(u32x4 w, float (&x)[8]) {
   }
 }
 __device__ __forceinline__ u32x4 pack8(const float (&x)[8]) {
+  typedef float f32x2 __attribute__((ext_vector_type(2)));
   uint32_t v[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i)
-    v[i] = uint32_t(f2bf(x[2 * i])) | (uint32_t(f2bf(x[2 * i + 1])) << 16);
+    v[i] = __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{x[2 * i], x[2 * i + 1]}, bf16x2_t));
   return u32x4{v[0], v[1], v[2], v[3]};
 }
 
 // q/k RMSNorm + RoPE of prompt rows, q out, K and V into their pages. A
-// workgroup takes one 32-slot block of one sequence and 8 of the qkv heads; a
+// workgroup takes one 32-slot block of one sequence and 3 of the qkv heads; a
 // wave takes 8 of the block's rows, 16 lanes a row with 8 dims each (dims 8 c of
 // chunk c, whose rotation partner 8 c +- 64 lies in lane ^ 8). All arithmetic is
 // in 32 bits and each value is rounded to bf16 once, where it is stored. The 8
-// keys of a wave are one 16-byte piece of V per dim, turned through LDS.
+// keys of a wave are one 16-byte piece of V per dim, turned through LDS. Bound by
+// latency where there are few rows and by HBM where there are many. Rows of 40
+// heads, 3000 of them / 7 sequences of 150 on average with 20 heads (us): 2 heads a
+// workgroup 17.5 / 7.3, 3 heads 15.3 / 7.9 (62 MB at 4.1 TB/s), 4 heads 15.8 / 8.6;
+// 8 heads, each loaded after the one before it, 17.4 / 12.5.
 __global__ __launch_bounds__(256) void paged_append_kernel(AppendParams p) {
   __shared__ uint32_t turn[4][8][D / 2 + 1];
   const int lane = threadIdx.x & 63;
@@ -79,19 +84,23 @@ __global__ __launch_bounds__(256) void paged_append_kernel(AppendParams p) {
   const int first = block * kBlock + 8 * wave;
   if (first >= hi || first + 8 <= lo)
     return;  // (no barrier below)
-  const int page = p.cache.table[size_t(b) * p.cache.table_stride +
-                                 ((block * kBlock) >> p.cache.shift)];
-  const bool held = p.cache.has(page);
+  const int kv = p.cache.kv_heads, h0 = blockIdx.y * kHeadsPerGroup;
+  const int h1 = min(h0 + kHeadsPerGroup, p.heads + 2 * kv);
   const int slot = (block * kBlock) & ((1 << p.cache.shift) - 1);
   const int chunk = lane & 15;
+  u32x4 all[kHeadsPerGroup][2];  // every load is on its way before the first use
   int pos[2];
-  const uint16_t *row[2];
   float c[2][8], s[2][8];
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
     pos[i] = first + 4 * i + (lane >> 4);
     const int in = min(max(pos[i], lo), hi - 1);
-    row[i] = p.qkv + (size_t(r.first) + (in - r.pos0)) * p.qkv_stride + 8 * chunk;
+    const uint16_t *row =
+        p.qkv + (size_t(r.first) + (in - r.pos0)) * p.qkv_stride + size_t(h0) * D + 8 * chunk;
+#pragma unroll
+    for (int h = 0; h < kHeadsPerGroup; ++h)
+      if (h0 + h < h1)
+        all[h][i] = *reinterpret_cast<const u32x4 *>(row + h * D);
     unpack8(*reinterpret_cast<const u32x4 *>(p.cos + size_t(in) * (D / 2) + 8 * (chunk & 7)), c[i]);
     unpack8(*reinterpret_cast<const u32x4 *>(p.sin + size_t(in) * (D / 2) + 8 * (chunk & 7)), s[i]);
     if (chunk < 8)  // first half: x c - partner s; second half: x c + partner s
@@ -99,13 +108,15 @@ __global__ __launch_bounds__(256) void paged_append_kernel(AppendParams p) {
       for (int e = 0; e < 8; ++e)
         s[i][e] = -s[i][e];
   }
-  const int kv = p.cache.kv_heads, h0 = blockIdx.y * kHeadsPerGroup;
-  const int h1 = min(h0 + kHeadsPerGroup, p.heads + 2 * kv);
-  for (int h = h0; h < h1; ++h) {
-    u32x4 w[2];
+  const int page = p.cache.table[size_t(b) * p.cache.table_stride +
+                                 ((block * kBlock) >> p.cache.shift)];
+  const bool held = p.cache.has(page);
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
-      w[i] = *reinterpret_cast<const u32x4 *>(row[i] + size_t(h) * D);
+  for (int n = 0; n < kHeadsPerGroup; ++n) {
+    const int h = h0 + n;
+    if (h >= h1)
+      break;
+    const u32x4(&w)[2] = all[n];
     if (h < p.heads + kv) {
       const bool is_q = h < p.heads;
       const uint16_t *gain = is_q ? p.q_norm : p.k_norm;
@@ -121,7 +132,7 @@ __global__ __launch_bounds__(256) void paged_append_kernel(AppendParams p) {
 #pragma unroll
           for (int e = 0; e < 8; ++e)
             ss += x[e] * x[e];
-          const float scale = 1.0f / __builtin_sqrtf(row_sum16(ss) / float(D) + p.eps);
+          const float scale = __builtin_amdgcn_rsqf(row_sum16(ss) * (1.f / D) + p.eps);
 #pragma unroll
           for (int e = 0; e < 8; ++e)
             x[e] = x[e] * scale * g[e];

