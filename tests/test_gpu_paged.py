@@ -446,6 +446,38 @@ def test_prefill_keeps_infinities_from_rows_that_do_not_see_them(torch, yuear_li
     check_prefill(torch, s, torch.where(finite, out, want.nan_to_num(0, 0, 0) + clean), window, sinks, some=150)
 
 
+@pytest.mark.parametrize("width", [8, 128])
+def test_prefill_gives_nan_for_a_row_whose_query_is_nan(torch, yuear_lib, width):
+    rng = np.random.default_rng(24)
+    s = prefill_inputs(torch, rng, 24, 8, 64, [150], [130], 30, width=width)
+    s["pages"].v[int(s["table"][0, 4]), 3, 0, 5, 20] = float("inf")  # key 276 of kv head 3: a tile with an odd value
+    clean = prefill(torch, yuear_lib, s)
+    s["q"][70, 4] = float("nan")
+    s["q"][148, 9:12] = float("nan")
+    out = prefill(torch, yuear_lib, s)
+    nan = torch.isnan(s["q"])
+    assert torch.isnan(out[nan]).all() and same_bits(torch, out[~nan], clean[~nan])
+
+
+@pytest.mark.parametrize("width", [8, 128])
+def test_prefill_with_decreasing_starts_stays_in_its_workspace(torch, yuear_lib, width):
+    rng = np.random.default_rng(25)
+    lens, n = [20] * 16, 320
+    s = prefill_inputs(torch, rng, 8, 8, 64, lens, [3] * 16, 300, width=width)
+    s["starts"] = np.array([0, n] * 8 + [0])  # every second sequence takes all rows
+    need = yuear_lib.lib.yuear_op_paged_workspace_bytes(16, 8, 8, n)
+    ws = yuear_lib.paged_workspace(16, 8, 8, n)
+    assert ws.numel() * 4 == need
+    guarded = torch.full((need // 4 + 4096,), 7, dtype=torch.int32, device="cuda")
+    guarded[:need // 4] = 0
+    prefill(torch, yuear_lib, s, workspace=guarded)
+    torch.cuda.synchronize()
+    assert (guarded[need // 4:] == 7).all() and not guarded[:131072 // 4].any()
+    # the workspace is fit for the next call
+    t = prefill_inputs(torch, rng, 8, 8, 64, lens, [3] * 16, 300, width=width)
+    check_prefill(torch, t, prefill(torch, yuear_lib, t, workspace=guarded))
+
+
 def test_prefill_leaves_other_rows_as_they_are(torch, yuear_lib):
     rng = np.random.default_rng(17)
     s = prefill_inputs(torch, rng, 3, 1, 32, [40, 10, 10, 40], [40, 0, 3, 0], 30, width=3)

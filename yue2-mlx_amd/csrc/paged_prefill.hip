@@ -577,12 +577,12 @@ __device__ __forceinline__ bool walk_tile(const PrefillParams &p, float qscale, 
             f32x4{o[dt][4 * a], o[dt][4 * a + 1], o[dt][4 * a + 2], o[dt][4 * a + 3]};
     if (half == 0)
       reinterpret_cast<float2 *>(part_of + kRows * D)[32 * wave + col] =
-          float2{set ? m_run : -__builtin_inff(), l};
+          float2{l == 0.f ? -__builtin_inff() : m_run, l};
     return true;
   }
   if (!valid)
     return true;
-  const float inv = set ? 1.f / l : 0.f;
+  const float inv = l == 0.f ? 0.f : 1.f / l;  // (0: the row sees nothing)
   // element j of tile dt: dim 32 dt + 8 (j / 4) + 4 half + j % 4
   uint16_t *dst = p.out + (size_t(tl.rows.first) + token) * p.out_stride + size_t(kvh * G + head) * D;
 #pragma unroll
@@ -631,8 +631,11 @@ __device__ __forceinline__ void walk_odd(const PrefillParams &p, float qscale, c
         top = fmaxf(top, __shfl_xor(top, b));
       top = fmaxf(M, top);
       unsigned long long left = __ballot(sees);
-      if (!left || top == -__builtin_inff())
-        continue;
+      if (top == -__builtin_inff()) {
+        if (!__any(sees && score != score))
+          continue;
+        top = 0.f;
+      }
       const float f = M == -__builtin_inff() ? 1.f : __builtin_amdgcn_exp2f(M - top);
       const float w = sees ? __builtin_amdgcn_exp2f(score - top) : 0.f;
       M = top;
@@ -670,17 +673,18 @@ template <int G>
 __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2, 2))) void
 paged_prefill_kernel(PrefillParams p, float qscale) {
   __shared__ Ring ring;
+  const int kv_heads = p.cache.kv_heads, kvh = int(blockIdx.x) % kv_heads;
   int seq, index;
   auto rows_of = [&](int b) {
     return paged::sequence_rows(p.starts, p.pos0, b, p.rows, p.cache.capacity);
   };
   if (!paged::find_item(
-          p.batch, p.tiles - 1 - int(blockIdx.y), [&](int b) { return tiles_of<G>(rows_of(b)); },
+          p.batch, p.tiles - 1 - int(blockIdx.x) / kv_heads, [&](int b) { return tiles_of<G>(rows_of(b)); },
           seq, index))
     return;
   const Tile t = tile_of<G>(p, rows_of(seq), seq, index);
-  if (!walk_tile<G>(p, qscale, t, blockIdx.x, 0, t.steps, nullptr, ring))
-    walk_odd<G>(p, qscale, t, blockIdx.x, 0, t.steps, nullptr);
+  if (!walk_tile<G>(p, qscale, t, kvh, 0, t.steps, nullptr, ring))
+    walk_odd<G>(p, qscale, t, kvh, 0, t.steps, nullptr);
 }
 
 // Dealt: every workgroup takes an equal run of the units of all heads.
@@ -697,8 +701,12 @@ paged_prefill_deal_kernel(PrefillParams p, float qscale) {
   // dispatch goes round the 8 XCDs: each takes neighbouring runs, whose tiles
   // share K and V in its L2
   const int run = int(blockIdx.x % 8) * (kRuns / 8) + int(blockIdx.x / 8);
+  // (more tiles than rows: `starts` decreases, and the workspace has no records for them)
+  const bool valid = deal.tiles <= p.tiles;
   if (run == 0 && threadIdx.x == 0)
-    p.info[0] = deal.tiles;
+    p.info[0] = valid ? deal.tiles : 0;
+  if (!valid)
+    return;
   int u = run_begin(run);
   const int u1 = run_begin(run + 1);
   if (u >= u1)
@@ -824,12 +832,12 @@ template <int G> hipError_t launch_g(PrefillParams p, hipStream_t s) {
   const float qscale = float(std::pow(double(D), -0.5)) * attn::kLog2e;
   const int kv_heads = p.cache.kv_heads;
   const long long tiles = tiles_at_most(p.batch, p.rows, G);
-  if (tiles > 65535)
+  if (tiles * kv_heads > 0xffffff)  // workgroups of a launch
     return hipErrorInvalidValue;
   p.tiles = int(tiles);
   if (!worth_dealing(p, tiles * kv_heads)) {
-    hipLaunchKernelGGL(paged_prefill_kernel<G>, dim3(kv_heads, p.tiles), dim3(64 * kWaves), 0, s, p,
-                       qscale);
+    hipLaunchKernelGGL(paged_prefill_kernel<G>, dim3(unsigned(p.tiles * kv_heads)), dim3(64 * kWaves), 0, s,
+                       p, qscale);
     return hipGetLastError();
   }
   hipLaunchKernelGGL(paged_prefill_deal_kernel<G>, dim3(kRuns), dim3(64 * kWaves), 0, s, p, qscale);
