@@ -744,13 +744,18 @@ paged_prefill_deal_kernel(PrefillParams p, float qscale) {
   }
 }
 
-// Rows of tiles that several runs hold, joined in order of the keys: a wave per
-// 32 rows and 32 dims, its lanes as the tile's held them. Every load of a round
-// of pieces is issued before the first is used.
+// Rows of tiles that several runs hold, joined in order of the keys: a workgroup
+// per 32 rows and 32 dims, a wave per quarter of the pieces, its lanes as the
+// tile's held them. Every load of a round of pieces is issued before the first is
+// used: what costs here is the latency of one round after the other (a wave for
+// all pieces: one row after 4000 keys 22.8 us in all, else 17.6).
 template <int G>
 __global__ __launch_bounds__(256) void paged_prefill_join_kernel(PrefillParams p) {
-  const int lane = threadIdx.x & 63, dt = threadIdx.x >> 6;
-  const int col = lane & 31, half = lane >> 5, kvh = blockIdx.x, group = blockIdx.y;
+  __shared__ f32x4 sums[kWaves][4][64];
+  __shared__ float2 tops[kWaves][32];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int col = lane & 31, half = lane >> 5, kvh = blockIdx.x;
+  const int group = blockIdx.y >> 2, dt = blockIdx.y & 3;
   if (int(blockIdx.z) >= p.info[0])
     return;
   const int32_t *info = p.info + kInfo * (1 + size_t(kvh) * p.tiles + blockIdx.z);
@@ -758,15 +763,15 @@ __global__ __launch_bounds__(256) void paged_prefill_join_kernel(PrefillParams p
   if (r0 == r1 || first_row + 32 * group >= end_row)
     return;
   const int pieces = r1 - r0 + 1, row = first_row + 32 * group + col;
-  constexpr int kRound = 4;
+  constexpr int kRound = 2;
   float M = -__builtin_inff(), l = 0.f;
   f32x4 o[4] = {};
-  for (int j0 = 0; j0 < pieces; j0 += kRound) {
+  for (int j0 = wave; j0 < pieces; j0 += kRound * kWaves) {
     float2 ml[kRound];
     f32x4 v[kRound][4];
 #pragma unroll
     for (int j = 0; j < kRound; ++j) {  // (past the last piece: that one, with weight 0)
-      const int g = min(j0 + j, pieces - 1);
+      const int g = min(j0 + kWaves * j, pieces - 1);
       const float *from = p.part + size_t(2 * (r0 + g) + (g == 0)) * kPartFloats;
       ml[j] = reinterpret_cast<const float2 *>(from + kRows * D)[32 * group + col];
 #pragma unroll
@@ -784,7 +789,7 @@ __global__ __launch_bounds__(256) void paged_prefill_join_kernel(PrefillParams p
       o[a] *= f;
 #pragma unroll
     for (int j = 0; j < kRound; ++j) {
-      const bool out = j0 + j >= pieces || ml[j].x == -__builtin_inff();
+      const bool out = j0 + kWaves * j >= pieces || ml[j].x == -__builtin_inff();
       const float w = out ? 0.f : __builtin_amdgcn_exp2f(ml[j].x - top);
       l += out ? 0.f : w * ml[j].y;
 #pragma unroll
@@ -793,15 +798,34 @@ __global__ __launch_bounds__(256) void paged_prefill_join_kernel(PrefillParams p
     }
     M = top;
   }
-  if (row >= end_row)
-    return;
-  const float inv = M == -__builtin_inff() ? 0.f : 1.f / l;
-  uint16_t *dst = p.out + (size_t(first) + row / G) * p.out_stride +
-                  size_t(kvh * G + row % G) * D + 32 * dt + 4 * half;
 #pragma unroll
   for (int a = 0; a < 4; ++a)
-    *reinterpret_cast<uint2 *>(dst + 8 * a) =
-        uint2{pack_bf16(o[a][0] * inv, o[a][1] * inv), pack_bf16(o[a][2] * inv, o[a][3] * inv)};
+    sums[wave][a][lane] = o[a];
+  if (half == 0)
+    tops[wave][col] = float2{M, l};
+  __syncthreads();
+  if (row >= end_row)
+    return;
+  // wave a: dims 8 a + [0, 8) of the 32
+  M = tops[0][col].x;
+#pragma unroll
+  for (int w = 1; w < kWaves; ++w)
+    M = fmaxf(M, tops[w][col].x);
+  f32x4 all = {};
+  l = 0.f;
+#pragma unroll
+  for (int w = 0; w < kWaves; ++w) {
+    const float2 ml = tops[w][col];
+    if (ml.x == -__builtin_inff())
+      continue;
+    const float f = __builtin_amdgcn_exp2f(ml.x - M);
+    l += f * ml.y;
+    all += f * sums[w][wave][lane];
+  }
+  all *= M == -__builtin_inff() ? 0.f : 1.f / l;
+  uint16_t *dst = p.out + (size_t(first) + row / G) * p.out_stride +
+                  size_t(kvh * G + row % G) * D + 32 * dt + 8 * wave + 4 * half;
+  *reinterpret_cast<uint2 *>(dst) = uint2{pack_bf16(all[0], all[1]), pack_bf16(all[2], all[3])};
 }
 
 // Tiles of a kv head that `rows` rows of `batch` sequences take at most.
@@ -844,7 +868,7 @@ template <int G> hipError_t launch_g(PrefillParams p, hipStream_t s) {
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess)
     return e;
-  hipLaunchKernelGGL(paged_prefill_join_kernel<G>, dim3(kv_heads, kWaves, p.tiles), dim3(256), 0, s,
+  hipLaunchKernelGGL(paged_prefill_join_kernel<G>, dim3(kv_heads, 4 * kWaves, p.tiles), dim3(256), 0, s,
                      p);
   return hipGetLastError();
 }

@@ -455,8 +455,8 @@ class PagePool:
 
 
 # The calls below cost a decode step's host time per layer, so each check reads
-# an attribute once and builds its message only where it fails (paged_attention_decode
-# of one sequence, host time: 21.8 -> 14.7 us).
+# an attribute once and builds its message only where it fails (host time of
+# paged_attention_decode: 11.2 us, 4 of them the launch; 18 with checks that did not).
 
 def _refuse(name, message):
     raise ValueError(f"{name}: {message}")
