@@ -38,9 +38,9 @@
 // as the output is: one product per operand instead of two; the denominator sums
 // the rounded weights.
 //
-// A prompt piece of few rows behind many keys has fewer tiles than CUs
-// (worth_dealing): there 256 workgroups take equal runs of all tiles' steps, leave
-// the sums of tiles that they share, and a second kernel joins them.
+// A prompt piece of few rows behind many keys has fewer tiles than CUs (runs_of):
+// there the workgroups take equal runs of all tiles' steps, leave the sums of tiles
+// that they share, and a second kernel joins them.
 #include <algorithm>
 #include <cmath>
 #include <type_traits>
@@ -76,12 +76,13 @@ struct PrefillParams {
   uint16_t *out = nullptr;
   long long out_stride = 0;
   int tiles = 0;  // of a kv head, at most
+  int runs = 0;   // workgroups of a dealt launch
   // dealt launches: records of the tiles (head: their number) and partials
   int32_t *info = nullptr;
   float *part = nullptr;
 };
 
-constexpr int kRuns = 256;                      // workgroups of a dealt launch, one a CU
+constexpr int kRuns = 512;                      // workgroups of a dealt launch, at most
 constexpr int kTileCost = 3;                    // steps that beginning a tile costs
 constexpr int kDealSequences = 16;              // of a dealt launch, at most
 // A piece's sums as the lanes hold them, then its rows' maxima and denominators.
@@ -693,14 +694,14 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2, 
 paged_prefill_deal_kernel(PrefillParams p, float qscale) {
   __shared__ Ring ring;
   const Deal<G> deal(p);
-  const int total = deal.total * p.cache.kv_heads, each = total / kRuns, more = total % kRuns;
+  const int total = deal.total * p.cache.kv_heads, each = total / p.runs, more = total % p.runs;
   auto run_begin = [&](int g) { return g * each + min(g, more); };
   auto run_of = [&](int u) {
     return u < more * (each + 1) ? u / (each + 1) : more + (u - more * (each + 1)) / each;
   };
   // dispatch goes round the 8 XCDs: each takes neighbouring runs, whose tiles
   // share K and V in its L2
-  const int run = int(blockIdx.x % 8) * (kRuns / 8) + int(blockIdx.x / 8);
+  const int run = int(blockIdx.x % 8) * (p.runs / 8) + int(blockIdx.x / 8);
   // (more tiles than rows: `starts` decreases, and the workspace has no records for them)
   const bool valid = deal.tiles <= p.tiles;
   if (run == 0 && threadIdx.x == 0)
@@ -833,23 +834,28 @@ long long tiles_at_most(int batch, int rows, int group) {
   return (long long)rows * group / kRows + std::min(batch, rows);
 }
 
-// Whether to deal the steps out: where the tiles would leave compute units idle
-// for longer than dealing costs. A launch of whole tiles takes as long as one
-// that sees all the keys that the tables hold, at most; dealt, its steps are
-// spread over all units, but begin every piece anew and need a second kernel,
-// about six steps' time. 24 heads of 8, time of whole tiles and dealt (us):
-//   200 rows after 0 keys 11.3 / 15.8    700 rows after 0     18.6 / 24.2
-//   97 after 4000         64.8 / 26.7    700 after 3000       63.8 / 59.5
-//   400 after 3000        57.1 / 41.9    1000 after 3000      71.6 / 79.2
-bool worth_dealing(const PrefillParams &p, long long tiles) {
-  constexpr int kDealTiles = 192, kDealSteps = 6;
+// Workgroups to deal the steps out over; 0: one tile a workgroup. To deal them
+// costs about 8 steps' time (every piece begins anew, and a second kernel joins
+// them), and is worth it where whole tiles would leave compute units idle for
+// longer: a launch of them takes as long as one that sees all the keys that the
+// tables hold, at most. A workgroup that shares its CU does a step in two thirds of
+// the time, but shares more tiles: two a CU from 8 steps a workgroup on. 24 heads of
+// 8, time of whole tiles / dealt over 256 / over 512 (us):
+//   200 rows after 0 keys 11.3 / 15.8 / 17.8    97 after 4000   64.8 / 26.7 / 28.7
+//   700 after 0           18.6 / 24.2 / 26.3    400 after 3000  57.1 / 41.9 / 38.3
+//   1000 after 0          24.4 / 31.9 / 29.9    1000 after 3000 71.6 / 79.2 / 66.5
+int runs_of(const PrefillParams &p, long long tiles) {
+  constexpr int kDealTiles = 256, kDealSteps = 8;
   if (p.batch > kDealSequences || tiles >= kDealTiles)
-    return false;
+    return 0;
   long long keys = p.cache.capacity;
   if (p.window > 0)
     keys = std::min(keys, (long long)p.window + p.sinks + 2 * kKeys);
   const long long steps = keys / kKeys;
-  return steps < (1 << 21) && steps * (kDealTiles - tiles) > kDealSteps * kDealTiles;
+  // (steps are counted in 31 bits)
+  if (steps >= (1 << 20) || steps * (kDealTiles - tiles) <= kDealSteps * kDealTiles)
+    return 0;
+  return steps * tiles < 8 * kRuns ? kRuns / 2 : kRuns;
 }
 
 template <int G> hipError_t launch_g(PrefillParams p, hipStream_t s) {
@@ -859,12 +865,13 @@ template <int G> hipError_t launch_g(PrefillParams p, hipStream_t s) {
   if (tiles * kv_heads > 0xffffff)  // workgroups of a launch
     return hipErrorInvalidValue;
   p.tiles = int(tiles);
-  if (!worth_dealing(p, tiles * kv_heads)) {
+  p.runs = runs_of(p, tiles * kv_heads);
+  if (!p.runs) {
     hipLaunchKernelGGL(paged_prefill_kernel<G>, dim3(unsigned(p.tiles * kv_heads)), dim3(64 * kWaves), 0, s,
                        p, qscale);
     return hipGetLastError();
   }
-  hipLaunchKernelGGL(paged_prefill_deal_kernel<G>, dim3(kRuns), dim3(64 * kWaves), 0, s, p, qscale);
+  hipLaunchKernelGGL(paged_prefill_deal_kernel<G>, dim3(p.runs), dim3(64 * kWaves), 0, s, p, qscale);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess)
     return e;
