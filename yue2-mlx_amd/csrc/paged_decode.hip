@@ -91,9 +91,16 @@ __device__ __forceinline__ Span span_of(int pos, int window, int sinks) {
   s.blocks = s.lead + pos / kBlock - s.first + 1;
   return s;
 }
-__device__ __forceinline__ int blocks_of(const DecodeParams &p, int b) {
-  const int pos = p.pos[b];
+__device__ __forceinline__ int blocks_at(const DecodeParams &p, int pos) {
   return pos < 0 || pos >= p.limit ? 0 : span_of(pos, p.window, p.sinks).blocks;
+}
+__device__ __forceinline__ int blocks_of(const DecodeParams &p, int b) {
+  return blocks_at(p, p.pos[b]);
+}
+
+__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
+  typedef float f32x2 __attribute__((ext_vector_type(2)));
+  return __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{lo, hi}, bf16x2_t));
 }
 
 // m (running maximum of the raw scores), l, and o of one head of a
@@ -186,7 +193,7 @@ __device__ __forceinline__ void join_parts(const DecodeParams &p, float qscale, 
         a1 = fmaf(w, o[j].y, a1);
       }
     }
-    reinterpret_cast<uint32_t *>(out)[q] = uint32_t(f2bf(a0)) | (uint32_t(f2bf(a1)) << 16);
+    reinterpret_cast<uint32_t *>(out)[q] = pack_bf16(a0, a1);
   }
 }
 
@@ -200,8 +207,11 @@ paged_decode_kernel(DecodeParams p, float qscale) {
   const int hkv = p.cache.kv_heads;
 
   // ---- which blocks are this workgroup's ----
-  int total = 0, sequences = 0;
-  for (int b0 = 0; b0 < p.batch; b0 += 64) {
+  const int my_pos = lane < p.batch ? p.pos[lane] : -1;  // of the first 64 sequences
+  const int my_blocks = blocks_at(p, my_pos);
+  int total = __builtin_amdgcn_readlane(wave_scan(my_blocks), 63);
+  int sequences = __builtin_popcountll(__ballot(my_blocks > 0));
+  for (int b0 = 64; b0 < p.batch; b0 += 64) {
     const int n = b0 + lane < p.batch ? blocks_of(p, b0 + lane) : 0;
     total += __builtin_amdgcn_readlane(wave_scan(n), 63);
     sequences += __builtin_popcountll(__ballot(n > 0));
@@ -217,7 +227,7 @@ paged_decode_kernel(DecodeParams p, float qscale) {
     return v < more * (each + 1) ? v / (each + 1) : more + (v - more * (each + 1)) / each;
   };
   if (chunks) {
-    const int n = lane < p.batch ? blocks_of(p, lane) : 0;
+    const int n = my_blocks;
     // blocks of a chunk, at most: one a wave, kChunks chunks, kParts of a sequence
     const int longest = int(wave_max(float(n)));
     int size = max(max(kWaves, (longest + kParts - 1) / kParts), (total + kChunks - 1) / kChunks);
@@ -265,7 +275,7 @@ paged_decode_kernel(DecodeParams p, float qscale) {
     if (x1 <= 0)
       return;  // not one block of the run's last item
     x = max(x, 0);
-    const int pos = p.pos[b];
+    const int pos = b < 64 ? __builtin_amdgcn_readlane(my_pos, b) : p.pos[b];
     const Span span = span_of(pos, p.window, p.sinks);
     const bool whole = x == 0 && x1 == nb;
     if (!chunks) {  // the runs that share the item
@@ -355,7 +365,7 @@ paged_decode_kernel(DecodeParams p, float qscale) {
         reinterpret_cast<float2 *>(sh.q[h])[lane] = float2{y0[j], y1[j]};
       else if (h < G + 2)
         reinterpret_cast<uint32_t *>(sh.kv_new[h - G])[lane] =
-            h == G ? uint32_t(f2bf(y0[j])) | (uint32_t(f2bf(y1[j])) << 16) : pair[j];
+            h == G ? pack_bf16(y0[j], y1[j]) : pair[j];
     }
     __syncthreads();
     // q operands: columns 0-7 the leading pieces of the heads, 8-15 the rests
@@ -366,12 +376,9 @@ paged_decode_kernel(DecodeParams p, float qscale) {
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const float2 q2 = reinterpret_cast<const float2 *>(sh.q[min(i & 7, G - 1)])[16 * s + 4 * r + e];
-        uint16_t a = f2bf(q2.x), c = f2bf(q2.y);
-        if (i >= 8) {
-          a = f2bf(q2.x - bf2f(a));
-          c = f2bf(q2.y - bf2f(c));
-        }
-        w[e] = (i & 7) < G ? uint32_t(a) | (uint32_t(c) << 16) : 0u;
+        const uint32_t lead = pack_bf16(q2.x, q2.y);
+        const uint32_t rest = pack_bf16(q2.x - bflo(lead), q2.y - bfhi(lead));
+        w[e] = (i & 7) < G ? (i < 8 ? lead : rest) : 0u;
       }
       qb[s] = u32x4{w[0], w[1], w[2], w[3]};
     }
@@ -458,12 +465,8 @@ paged_decode_kernel(DecodeParams p, float qscale) {
         const float p1 = __builtin_amdgcn_exp2f((sc[2 * q + 1] - m_use) * qscale);
         ps += p0;
         ps += p1;
-        uint16_t a = f2bf(p0), c = f2bf(p1);
-        if (i >= 8) {
-          a = f2bf(p0 - bf2f(a));
-          c = f2bf(p1 - bf2f(c));
-        }
-        pw[q] = uint32_t(a) | (uint32_t(c) << 16);
+        const uint32_t lead = pack_bf16(p0, p1);
+        pw[q] = i < 8 ? lead : pack_bf16(p0 - bflo(lead), p1 - bfhi(lead));
       }
       l_run = l_run * corr + ps;
       m_run = m_new;
@@ -514,8 +517,7 @@ paged_decode_kernel(DecodeParams p, float qscale) {
       if (whole) {
         acc *= 1.f / l;
         *reinterpret_cast<uint2 *>(out + h * D + d) =
-            uint2{uint32_t(f2bf(acc[0])) | (uint32_t(f2bf(acc[1])) << 16),
-                  uint32_t(f2bf(acc[2])) | (uint32_t(f2bf(acc[3])) << 16)};
+            uint2{pack_bf16(acc[0], acc[1]), pack_bf16(acc[2], acc[3])};
       } else {
         // write-through (agent-scope) stores: visible to every XCD once complete
         const auto put = [&](int at, float lo, float hi) {
