@@ -13,13 +13,17 @@
 // launch serves every length. Two ways to cut the list into workgroups:
 //
 // - up to 512 items and 24 blocks a workgroup: each item into equal chunks, one
-//   workgroup each, as many as 512 workgroups and 64 parts an item allow (one
-//   sequence of 4096 keys: 12.9 us, 15.9 cut the other way; one kv head of
-//   20000: 20.7 and 65);
+//   workgroup each, as many as 512 workgroups and 64 parts an item allow, of at
+//   least a block a wave (one sequence of 4096 keys: 12.5 us, 15.9 cut the other
+//   way, 14 with two blocks a wave; one kv head of 20000: 21 and 65);
 // - else into equal runs, whatever the lengths of the sequences, and a workgroup
-//   walks the items of its run (45 sequences of 150 to 24500 keys: 160 us, 189 in
+//   walks the items of its run (45 sequences of 150 to 24500 keys: 158 us, 189 in
 //   chunks). To begin an item (positions, page, q, the joining of the waves) costs
 //   a workgroup about as much as 8 blocks, which the runs count (2: 172 us).
+//
+// Short caches are bound by a chain of dependent loads, 8.2 us for one block a
+// wave: positions, page numbers, K and V, each in turn, then what the waves leave in
+// LDS; the joining of parts adds 2.8 us (333 keys: 11.0).
 //
 // A part that is a whole item is finished there; else the workgroup leaves its
 // running maximum, sum and weighted values in its slots of the workspace, and
