@@ -60,7 +60,7 @@ __device__ __forceinline__ u32x4 pack8(const float (&x)[8]) {
 // in 32 bits and each value is rounded to bf16 once, where it is stored. The 8
 // keys of a wave are one 16-byte piece of V per dim, turned through LDS. Bound by
 // latency where there are few rows and by HBM where there are many. Rows of 40
-// heads, 3000 of them / 7 sequences of 150 on average with 20 heads (us): 2 heads a
+// heads, 3000 of them / 7 sequences of 19 to 301 with 32 heads (us): 2 heads a
 // workgroup 17.5 / 7.3, 3 heads 15.3 / 7.9 (62 MB at 4.1 TB/s), 4 heads 15.8 / 8.6;
 // 8 heads, each loaded after the one before it, 17.4 / 12.5.
 __global__ __launch_bounds__(256) void paged_append_kernel(AppendParams p) {
@@ -193,8 +193,12 @@ __global__ __launch_bounds__(256) void paged_append_kernel(AppendParams p) {
 }
 
 // ---- page copies ----
-constexpr int kPairs = 240;       // (source, destination) pairs of a launch, in its arguments
-constexpr int kCopyChunks = 1024;  // 16-byte chunks of a workgroup
+// A thread copies one 16-byte chunk of a page of one layer's K or V. Bound by HBM;
+// what hides its latency is many short workgroups, and stores that do not stay in
+// L2. One page of 128 KiB to 7 others / 90 pages to 90, in 28 layers (59 MB / 1.3 GB;
+// us): 9.8 / 215 (6.1 TB/s); with ordinary stores 12.8 / 222, with those and four
+// chunks a thread 13.7 / 256.
+constexpr int kPairs = 240;  // (source, destination) pairs of a launch, in its arguments
 struct CopyParams {
   uint16_t *k = nullptr, *v = nullptr;
   long long layer_stride = 0, page_elems = 0;
@@ -205,16 +209,9 @@ __global__ __launch_bounds__(256) void pages_copy_kernel(CopyParams p) {
   const u32x4 *from =
       reinterpret_cast<const u32x4 *>(base + size_t(p.src[blockIdx.y]) * p.page_elems);
   u32x4 *to = reinterpret_cast<u32x4 *>(base + size_t(p.dst[blockIdx.y]) * p.page_elems);
-  const long long n = p.page_elems / 8, c0 = (long long)blockIdx.x * kCopyChunks + threadIdx.x;
-  u32x4 x[kCopyChunks / 256];
-#pragma unroll
-  for (int i = 0; i < kCopyChunks / 256; ++i)
-    if (c0 + 256 * i < n)
-      x[i] = from[c0 + 256 * i];
-#pragma unroll
-  for (int i = 0; i < kCopyChunks / 256; ++i)
-    if (c0 + 256 * i < n)
-      to[c0 + 256 * i] = x[i];
+  const long long c = (long long)blockIdx.x * 256 + threadIdx.x;
+  if (c < p.page_elems / 8)
+    __builtin_nontemporal_store(from[c], to + c);
 }
 
 hipError_t copy_pages(uint16_t *k, uint16_t *v, int layers, long long layer_stride, int pages,
@@ -242,7 +239,7 @@ hipError_t copy_pages(uint16_t *k, uint16_t *v, int layers, long long layer_stri
   p.v = v;
   p.layer_stride = layer_stride;
   p.page_elems = page_elems;
-  const long long chunks = (page_elems / 8 + kCopyChunks - 1) / kCopyChunks;
+  const long long chunks = (page_elems / 8 + 255) / 256;
   if (chunks > 0x7fffffffLL)
     return hipErrorInvalidValue;
   for (int i = 0; i < n; i += kPairs) {
