@@ -693,3 +693,16 @@ def test_binding_refuses_tensors_that_do_not_fit(torch, yuear_lib):
     empty = yuear_lib.paged_attention_decode(s["qkv"][:0], s["pages"].k, s["pages"].v, good["table"][:0],
                                              good["pos"][:0], *s["rope"])
     assert empty.shape == (0, 3, 128)
+
+
+def test_binding_refuses_numbers_past_32_bits(torch, yuear_lib):
+    """Such a number is refused, not cut to its low bits."""
+    rng = np.random.default_rng(26)
+    s = prefill_inputs(torch, rng, 3, 1, 32, [40], [0], 30)
+    for kw in (dict(window=2 ** 32 + 1), dict(window=1, sinks=2 ** 32 + 1), dict(window=2 ** 31)):
+        with pytest.raises(ValueError):
+            prefill(torch, yuear_lib, s, **kw)
+    for src, dst in (([2 ** 32], [1]), ([0], [2 ** 32 + 1]), ([0], [30]), ([-1], [1]), ([0, 1], [2])):
+        with pytest.raises(ValueError):
+            yuear_lib.pages_copy(s["pages"].k, s["pages"].v, src, dst)
+    yuear_lib.pages_copy(s["pages"].k, s["pages"].v, [], [])

@@ -183,3 +183,17 @@ def test_workspace_size(yuear_lib):
     assert size(1, 24, 8, 5000) >= size(1, 24, 8, 0)
     for bad in ((-1, 24, 8, 0), (1, 24, 0, 0), (1, 20, 8, 0), (1, 24, 8, -1), (1, 0, 1, 0)):
         assert size(*bad) == 0
+
+
+def test_pool_refuses_numbers_past_32_bits_and_calls_after_close(yuear_lib):
+    pool = yuear_lib.PagePool(8, 32)
+    a = pool.open()
+    for call in (lambda: pool.extend(a, 2 ** 32 + 1), lambda: pool.fork(a + 2 ** 32), lambda: pool.trim(a, 2 ** 32, 0)):
+        with pytest.raises(ValueError):
+            call()
+    with pytest.raises(ValueError):
+        yuear_lib.PagePool(2 ** 32 + 8, 32)
+    assert pool.length(a) == 0 and pool.unused == 8
+    pool.close()
+    with pytest.raises(ValueError):
+        pool.open()

@@ -384,7 +384,14 @@ class PagePool:
     return (src, dst) page lists for `pages_copy`, to be run before the cache is
     used again."""
 
+    @staticmethod
+    def _fit(*args):
+        for a in args:  # (a C argument would keep its low 32 bits)
+            if isinstance(a, (int, np.integer)) and not -2**31 <= a < 2**31:
+                raise ValueError("pages, sequences and lengths are 32-bit integers")
+
     def __init__(self, pages, page_slots):
+        self._fit(pages, page_slots)
         h, err = C.c_void_p(), C.c_void_p()
         _check(lib.yuear_pages_create(pages, page_slots, C.byref(h), C.byref(err)), err)
         self._handle, self.pages, self.page_slots = h, pages, page_slots
@@ -398,6 +405,7 @@ class PagePool:
         self.close()
 
     def _call(self, name, *args):
+        self._fit(*args)
         err = C.c_void_p()
         _check(getattr(lib, "yuear_pages_" + name)(self._handle, *args, C.byref(err)), err)
 
@@ -541,6 +549,11 @@ def _qkv(qkv, hkv, index, name):
     _refuse(name, "qkv is bfloat16 [rows, (heads + 2 kv heads) * 128] with whole rows")
 
 
+def _check_window(window, sinks, name):
+    if not (0 <= window < 2**31 and 0 <= sinks < 2**31):
+        _refuse(name, "window and sinks are counts of keys")
+
+
 def _rows(t, rows, heads, index, name, what):
     """Row stride of [rows, heads, 128]."""
     if t.dtype is _torch()[1] and t.shape == (rows, heads, 128) and t.get_device() == index:
@@ -592,8 +605,8 @@ def pages_copy(k_pages, v_pages, src, dst, stream=None):
             and v.dtype is bf16 and v.get_device() == index and ks[1:] == (row, slots * 128, 128, 1)
             and vs[1:] == (row, slots * 128, 4096, 32, 1) and (layers == 1 or ks[0] == vs[0])):
         _refuse(name, _LAYOUT + ", with one layer stride")
-    if len(src) != len(dst):
-        _refuse(name, "src and dst have one length")
+    if len(src) != len(dst) or any(not 0 <= page < n for page in (*src, *dst)):
+        _refuse(name, "src and dst are lists of pages of one length")
     pairs = C.c_int32 * len(src)
     _call(lib.yuear_op_pages_copy, name, index, k.data_ptr(), v.data_ptr(), layers, ks[0], n, hkv, slots,
           pairs(*src), pairs(*dst), len(src), _stream(stream, index, name))
@@ -656,6 +669,7 @@ def paged_attention_prefill(q, k_pages, v_pages, table, starts, pos0, window=0, 
     stream = _stream(stream, index, name, out, workspace)
     n, hkv, slots = _check_pages(k_pages, v_pages, index, name)
     shape = q.shape
+    _check_window(window, sinks, name)
     rows, heads = shape[0], shape[1] if len(shape) == 3 else 0
     stride = _rows(q, rows, heads, index, name, "q")
     batch, width, table_stride = _check_table(table, index, name)
@@ -687,6 +701,7 @@ def paged_attention_decode(qkv, k_pages, v_pages, table, pos, cos, sin, q_norm=N
     sequences, width, table_stride = _check_table(table, index, name)
     if sequences != batch:
         _refuse(name, "table has a row for each of qkv's")
+    _check_window(window, sinks, name)
     _check_ints(pos, batch, index, name, "pos")
     positions = _check_rope(cos, sin, index, name)
     q_gain, k_gain = _gain(q_norm, index, name), _gain(k_norm, index, name)
