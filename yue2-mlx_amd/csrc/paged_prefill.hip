@@ -581,18 +581,22 @@ __device__ __forceinline__ bool walk_tile(const PrefillParams &p, float qscale, 
           float2{l == 0.f ? -__builtin_inff() : m_run, l};
     return true;
   }
-  if (!valid)
-    return true;
   const float inv = l == 0.f ? 0.f : 1.f / l;  // (0: the row sees nothing)
   // element j of tile dt: dim 32 dt + 8 (j / 4) + 4 half + j % 4
   uint16_t *dst = p.out + (size_t(tl.rows.first) + token) * p.out_stride + size_t(kvh * G + head) * D;
 #pragma unroll
   for (int dt = 0; dt < 4; ++dt)
 #pragma unroll
-    for (int a = 0; a < 4; ++a) {
-      const uint32_t lo = pack_bf16(o[dt][4 * a] * inv, o[dt][4 * a + 1] * inv);
-      const uint32_t hi = pack_bf16(o[dt][4 * a + 2] * inv, o[dt][4 * a + 3] * inv);
-      *reinterpret_cast<uint2 *>(dst + 32 * dt + 8 * a + 4 * half) = uint2{lo, hi};
+    for (int a = 0; a < 4; a += 2) {  // the halves trade pieces: 16 bytes a lane
+      uint32_t w[4];
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        w[k] = pack_bf16(o[dt][4 * a + 2 * k] * inv, o[dt][4 * a + 2 * k + 1] * inv);
+        w[k + 2] = pack_bf16(o[dt][4 * a + 2 * k + 4] * inv, o[dt][4 * a + 2 * k + 5] * inv);
+        permlane32_swap(w[k], w[k + 2]);
+      }
+      if (valid)
+        *reinterpret_cast<u32x4 *>(dst + 32 * dt + 8 * (a + half)) = u32x4{w[0], w[1], w[2], w[3]};
     }
   return true;
 }
