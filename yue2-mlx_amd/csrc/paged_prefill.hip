@@ -26,10 +26,10 @@
 // two workgroups share a CU and one's products run beside the other's barriers.
 // A step computes S of the step after it beside its own exponentials, and P V
 // beside the scaling of those scores; K is therefore loaded a step ahead of V.
-// Measured, 24 heads of 8 at 3000 rows / two prompts and a window of 1024, 5
-// sequences of 1500 (us): this form 72 / 115 (775 / 620 TFLOP/s); 8 waves and four
-// steps of LDS, one workgroup a CU: 88 / 130; S and P V of the same step one
-// after the other: 103 / 155.
+// Measured, 24 heads of 8 at 3000 rows / 16 of 8 and a window of 1024, 5 sequences of
+// 411 to 5003 (us): this form 72 / 109 (770 / 650 TFLOP/s; 12000 rows 1080); 64 rows a
+// wave, one wave a SIMD, 106 / 155; 8 waves and four steps of LDS, one workgroup a CU,
+// 88 / 130; S and P V of the same step one after the other 103 / 155.
 //
 // The running maximum m of a row is taken off its scores as they are scaled. It
 // is raised only when a score passes it by more than kSlack (the weights, up to
