@@ -381,6 +381,8 @@ def test_prefill(torch, yuear_lib, heads, kv, slots, lens, pos0, window, sinks):
     (2, 1, 32, [77], [700], 2 ** 31 - 1, 3),
     (3, 1, 32, [1 + i % 3 for i in range(16)], [i % 70 for i in range(16)], 0, 0),
     (3, 1, 32, [1 + i % 3 for i in range(17)], [i % 70 for i in range(17)], 0, 0),
+    (3, 1, 32, [i % 4 for i in range(32)], [i % 70 for i in range(32)], 0, 0),
+    (3, 1, 32, [i % 4 for i in range(33)], [i % 70 for i in range(33)], 0, 0),
 ])
 def test_prefill_in_a_table_with_room(torch, yuear_lib, heads, kv, slots, lens, pos0, window, sinks):
     """A table of 16384 slots, where steps are dealt out however few keys there are."""

@@ -82,9 +82,13 @@ struct PrefillParams {
   float *part = nullptr;
 };
 
-constexpr int kRuns = 512;                      // workgroups of a dealt launch, at most
-constexpr int kTileCost = 3;                    // steps that beginning a tile costs
-constexpr int kDealSequences = 16;              // of a dealt launch, at most
+constexpr int kRuns = 512;  // workgroups of a dealt launch, at most
+// Steps that beginning a tile costs (97 rows after 4000 keys 27.8 us; 1: 29.5, 5: 27.4).
+constexpr int kTileCost = 3;
+// Sequences of a dealt launch, at most: every workgroup walks them all. Short pieces
+// after 2000 and 3000 keys (us), dealt / whole tiles: 32 sequences 30.7 / 35.0 and
+// 46.5 / 60.3, 60 sequences 46.6 / 35.3 and 70.8 / 66.0.
+constexpr int kDealSequences = 32;
 // A piece's sums as the lanes hold them, then its rows' maxima and denominators.
 constexpr size_t kPartFloats = size_t(kRows) * D + 2 * kRows;
 constexpr int kInfo = 8;  // words of a tile's record: first and last run, rows
