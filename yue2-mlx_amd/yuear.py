@@ -464,7 +464,7 @@ class PagePool:
 
 # The calls below cost a decode step's host time per layer, so each check reads
 # an attribute once and builds its message only where it fails (host time of
-# paged_attention_decode: 11.2 us, 4 of them the launch; 18 with checks that did not).
+# paged_attention_decode: 10.8 us, 4 of them the launch; 18 with checks that did not).
 
 def _refuse(name, message):
     raise ValueError(f"{name}: {message}")
@@ -477,42 +477,41 @@ def _hip_check(status, name):
 
 
 def _torch():
-    """torch, and its types that the checks compare with."""
-    global _T
+    """torch; the first call sets its types that the checks compare with."""
+    global _T, _BF16, _INT32
     if _T is None:
         import torch
-        _T = (torch, torch.bfloat16, torch.int32)
+        _T, _BF16, _INT32 = torch, torch.bfloat16, torch.int32
     return _T
 
 
-_T = None
+_T = _BF16 = _INT32 = None
 _LAYOUT = ("pages are contiguous bfloat16 tensors on one device: k [pages, kv heads, slots, 128] and "
            "v [pages, kv heads, slots / 32, 128, 32]")
 
 
 def _check_pages(k_pages, v_pages, index, name):
     """(pages, kv heads, slots) of one layer's pages."""
-    bf16 = _torch()[1]
     shape = k_pages.shape
     if len(shape) != 4:
         _refuse(name, _LAYOUT)
     n, hkv, slots, d = shape
-    if not (d == 128 and v_pages.shape == (n, hkv, slots // 32, 128, 32) and k_pages.dtype is bf16
-            and v_pages.dtype is bf16 and k_pages.get_device() == index and v_pages.get_device() == index
+    if not (d == 128 and v_pages.shape == (n, hkv, slots // 32, 128, 32) and k_pages.dtype is _BF16
+            and v_pages.dtype is _BF16 and k_pages.get_device() == index and v_pages.get_device() == index
             and k_pages.is_contiguous() and v_pages.is_contiguous()):
         _refuse(name, _LAYOUT)
     return n, hkv, slots
 
 
 def _check_ints(t, n, index, name, what):
-    if not (t.dtype is _torch()[2] and t.shape == (n,) and t.get_device() == index and t.is_contiguous()):
+    if not (t.dtype is _INT32 and t.shape == (n,) and t.get_device() == index and t.is_contiguous()):
         _refuse(name, f"{what} is a contiguous int32 tensor [{n}] on the pages' device")
 
 
 def _check_table(table, index, name):
     """(sequences, entries of a row, row stride) of a page table."""
     shape = table.shape
-    if table.dtype is _torch()[2] and len(shape) == 2 and table.get_device() == index and shape[1] >= 1:
+    if table.dtype is _INT32 and len(shape) == 2 and table.get_device() == index and shape[1] >= 1:
         if table.is_contiguous():
             return shape[0], shape[1], shape[1]
         stride = table.stride()
@@ -523,8 +522,8 @@ def _check_table(table, index, name):
 
 def _check_rope(cos, sin, index, name):
     """Rows of the rotation tables."""
-    bf16, shape = _torch()[1], cos.shape
-    if not (len(shape) == 2 and shape[1] == 64 and sin.shape == shape and cos.dtype is bf16 and sin.dtype is bf16
+    shape = cos.shape
+    if not (len(shape) == 2 and shape[1] == 64 and sin.shape == shape and cos.dtype is _BF16 and sin.dtype is _BF16
             and cos.get_device() == index and sin.get_device() == index and cos.is_contiguous()
             and sin.is_contiguous()):
         _refuse(name, "cos and sin are contiguous bfloat16 [positions, 64] on the pages' device")
@@ -534,7 +533,7 @@ def _check_rope(cos, sin, index, name):
 def _gain(t, index, name):
     if t is None:
         return None
-    if not (t.dtype is _torch()[1] and t.shape == (128,) and t.get_device() == index and t.is_contiguous()):
+    if not (t.dtype is _BF16 and t.shape == (128,) and t.get_device() == index and t.is_contiguous()):
         _refuse(name, "norm gains are contiguous bfloat16 [128] on the pages' device")
     return t.data_ptr()
 
@@ -542,7 +541,7 @@ def _gain(t, index, name):
 def _qkv(qkv, hkv, index, name):
     """(rows, query heads, row stride) of rows q | k | v."""
     shape = qkv.shape
-    if len(shape) == 2 and qkv.dtype is _torch()[1] and not shape[1] % 128 and shape[1] // 128 > 2 * hkv:
+    if len(shape) == 2 and qkv.dtype is _BF16 and not shape[1] % 128 and shape[1] // 128 > 2 * hkv:
         stride = qkv.stride()
         if stride[1] == 1:
             return shape[0], shape[1] // 128 - 2 * hkv, stride[0] if shape[0] > 1 else shape[1]
@@ -556,7 +555,7 @@ def _check_window(window, sinks, name):
 
 def _rows(t, rows, heads, index, name, what):
     """Row stride of [rows, heads, 128]."""
-    if t.dtype is _torch()[1] and t.shape == (rows, heads, 128) and t.get_device() == index:
+    if t.dtype is _BF16 and t.shape == (rows, heads, 128) and t.get_device() == index:
         stride = t.stride()
         if stride[2] == 1 and (stride[1] == 128 or heads == 1):
             return stride[0] if rows > 1 else heads * 128
@@ -566,7 +565,7 @@ def _rows(t, rows, heads, index, name, what):
 def _stream(stream, index, name, *given):
     """The stream to run on: torch's current one, or the given one, for which
     the call allocates nothing (`given`: the caller's out and workspace)."""
-    torch = _torch()[0]
+    torch = _T or _torch()
     if index < 0:
         _refuse(name, "tensors are on the GPU")
     current = torch._C._cuda_getCurrentRawStream(index)
@@ -579,11 +578,10 @@ def _stream(stream, index, name, *given):
 
 def _call(fn, name, index, *args):
     """The library's call, with the tensors' device as the current one."""
-    cuda = _torch()[0].cuda
-    if index == cuda.current_device():
+    if index == _T._C._cuda_getDevice():
         status = fn(*args)
     else:
-        with cuda.device(index):
+        with _T.cuda.device(index):
             status = fn(*args)
     if status:
         _hip_check(status, name)
@@ -594,15 +592,16 @@ def pages_copy(k_pages, v_pages, src, dst, stream=None):
     [layers, pages, kv heads, slots, 128] and v_pages [layers, pages, kv heads,
     slots / 32, 128, 32] (or one layer's, without the first dimension), src and
     dst lists of pages on the host."""
-    name, bf16 = "pages_copy", _torch()[1]
+    name = "pages_copy"
+    _torch()
     k, v = (k_pages, v_pages) if k_pages.dim() == 5 else (k_pages[None], v_pages[None])
     index = k.get_device()
     shape = k.shape
     layers, n, hkv, slots, d = shape if len(shape) == 5 else (0,) * 5
     ks, vs = k.stride(), v.stride()
     row = hkv * slots * 128
-    if not (layers >= 1 and d == 128 and v.shape == (layers, n, hkv, slots // 32, 128, 32) and k.dtype is bf16
-            and v.dtype is bf16 and v.get_device() == index and ks[1:] == (row, slots * 128, 128, 1)
+    if not (layers >= 1 and d == 128 and v.shape == (layers, n, hkv, slots // 32, 128, 32) and k.dtype is _BF16
+            and v.dtype is _BF16 and v.get_device() == index and ks[1:] == (row, slots * 128, 128, 1)
             and vs[1:] == (row, slots * 128, 4096, 32, 1) and (layers == 1 or ks[0] == vs[0])):
         _refuse(name, _LAYOUT + ", with one layer stride")
     if len(src) != len(dst) or any(not 0 <= page < n for page in (*src, *dst)):
@@ -618,7 +617,7 @@ PAGED_COUNTER_BYTES = 131072  # of a workspace, zero between calls
 def paged_workspace(batch, heads, kv_heads, rows=0, device=None):
     """A workspace, its counters zeroed, for the paged attention of up to these sizes (rows 0:
     decode steps only). Calls that may overlap need one each."""
-    torch = _torch()[0]
+    torch = _torch()
     n = lib.yuear_op_paged_workspace_bytes(batch, heads, kv_heads, rows)
     if n <= 0:
         _refuse("paged_workspace", "invalid arguments")
@@ -629,7 +628,7 @@ def paged_workspace(batch, heads, kv_heads, rows=0, device=None):
 
 def _workspace(workspace, index, name):
     """Bytes of a caller's workspace."""
-    if not (workspace.dtype is _torch()[2] and workspace.get_device() == index and workspace.is_contiguous()):
+    if not (workspace.dtype is _INT32 and workspace.get_device() == index and workspace.is_contiguous()):
         _refuse(name, "workspace comes from paged_workspace")
     return workspace.numel() * 4
 
@@ -650,8 +649,7 @@ def paged_append(qkv, k_pages, v_pages, table, starts, pos0, cos, sin, q_norm=No
     positions = _check_rope(cos, sin, index, name)
     q_gain, k_gain = _gain(q_norm, index, name), _gain(k_norm, index, name)
     if out is None:
-        torch, bf16, _ = _torch()
-        out = torch.empty((rows, heads, 128), dtype=bf16, device=qkv.device)
+        out = qkv.new_empty((rows, heads, 128))
     out_stride = _rows(out, rows, heads, index, name, "out")
     _call(lib.yuear_op_paged_append, name, index, qkv.data_ptr(), stride, q_gain, k_gain, eps, cos.data_ptr(),
           sin.data_ptr(), positions, k_pages.data_ptr(), v_pages.data_ptr(), n, slots, table.data_ptr(), width,
@@ -676,8 +674,7 @@ def paged_attention_prefill(q, k_pages, v_pages, table, starts, pos0, window=0, 
     _check_ints(starts, batch + 1, index, name, "starts")
     _check_ints(pos0, batch, index, name, "pos0")
     if out is None:
-        torch, bf16, _ = _torch()
-        out = torch.empty((rows, heads, 128), dtype=bf16, device=q.device)
+        out = q.new_empty((rows, heads, 128))
     out_stride = _rows(out, rows, heads, index, name, "out")
     if workspace is None:
         workspace = paged_workspace(batch, heads, hkv, rows, q.device)
@@ -706,8 +703,7 @@ def paged_attention_decode(qkv, k_pages, v_pages, table, pos, cos, sin, q_norm=N
     positions = _check_rope(cos, sin, index, name)
     q_gain, k_gain = _gain(q_norm, index, name), _gain(k_norm, index, name)
     if out is None:
-        torch, bf16, _ = _torch()
-        out = torch.empty((batch, heads, 128), dtype=bf16, device=qkv.device)
+        out = qkv.new_empty((batch, heads, 128))
     out_stride = _rows(out, batch, heads, index, name, "out")
     if workspace is None:
         workspace = paged_workspace(batch, heads, hkv, 0, qkv.device)
