@@ -78,6 +78,26 @@ __device__ __forceinline__ Rows sequence_rows(const int32_t *starts, const int32
   return Rows{s0, in ? min(s1 - s0, limit - p) : 0, in ? p : 0};
 }
 
+// find_item() of items that each sequence's rows count: with the rows of the one found.
+template <class F>
+__device__ __forceinline__ bool find_rows(const int32_t *starts, const int32_t *pos0, int batch,
+                                          int rows, int limit, int target, F &&count, int &seq,
+                                          int &place, Rows &of) {
+  Rows mine{0, 0, 0};  // of the lane's sequence of the last 64 looked at
+  if (!find_item(
+          batch, target,
+          [&](int b) {
+            mine = sequence_rows(starts, pos0, b, rows, limit);
+            return count(mine);
+          },
+          seq, place))
+    return false;
+  const int lane = seq & 63;
+  of = Rows{__builtin_amdgcn_readlane(mine.first, lane), __builtin_amdgcn_readlane(mine.n, lane),
+            __builtin_amdgcn_readlane(mine.pos0, lane)};
+  return true;
+}
+
 // Value of lane ^ 8 (lanes of a 16-lane row turned by half a row).
 __device__ __forceinline__ float xor8(float v) { return dpp<0x128>(v); }
 

@@ -61,23 +61,21 @@ __device__ __forceinline__ u32x4 pack8(const float (&x)[8]) {
 // keys of a wave are one 16-byte piece of V per dim, turned through LDS. Bound by
 // latency where there are few rows and by HBM where there are many. Rows of 40
 // heads, 3000 of them / 7 sequences of 19 to 301 with 32 heads (us): 2 heads a
-// workgroup 17.5 / 7.3, 3 heads 15.3 / 7.9 (62 MB at 4.1 TB/s), 4 heads 15.8 / 8.6;
+// workgroup 17.5 / 7.3, 3 heads 15.3 / 7.6 (62 MB at 4.1 TB/s), 4 heads 15.8 / 8.6;
 // 8 heads, each loaded after the one before it, 17.4 / 12.5.
 __global__ __launch_bounds__(256) void paged_append_kernel(AppendParams p) {
   __shared__ uint32_t turn[4][8][D / 2 + 1];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  auto rows_of = [&](int b) { return paged::sequence_rows(p.starts, p.pos0, b, p.rows, p.limit); };
   int b, place;
-  if (!paged::find_item(
-          p.batch, blockIdx.x,
-          [&](int s) {
-            const paged::Rows r = rows_of(s);
-            return r.n ? (r.pos0 + r.n - 1) / kBlock - r.pos0 / kBlock + 1 : 0;
+  paged::Rows r;
+  if (!paged::find_rows(
+          p.starts, p.pos0, p.batch, p.rows, p.limit, blockIdx.x,
+          [](const paged::Rows &of) {
+            return of.n ? (of.pos0 + of.n - 1) / kBlock - of.pos0 / kBlock + 1 : 0;
           },
-          b, place))
+          b, place, r))
     return;
-  const paged::Rows r = rows_of(b);
   const int block = r.pos0 / kBlock + place;
   const int lo = max(block * kBlock, r.pos0);
   const int hi = min(block * kBlock + kBlock, r.pos0 + r.n);  // positions [lo, hi)

@@ -684,14 +684,13 @@ paged_prefill_kernel(PrefillParams p, float qscale) {
   __shared__ Ring ring;
   const int kv_heads = p.cache.kv_heads, kvh = int(blockIdx.x) % kv_heads;
   int seq, index;
-  auto rows_of = [&](int b) {
-    return paged::sequence_rows(p.starts, p.pos0, b, p.rows, p.cache.capacity);
-  };
-  if (!paged::find_item(
-          p.batch, p.tiles - 1 - int(blockIdx.x) / kv_heads, [&](int b) { return tiles_of<G>(rows_of(b)); },
-          seq, index))
+  paged::Rows rows;
+  if (!paged::find_rows(
+          p.starts, p.pos0, p.batch, p.rows, p.cache.capacity,
+          p.tiles - 1 - int(blockIdx.x) / kv_heads,
+          [](const paged::Rows &of) { return tiles_of<G>(of); }, seq, index, rows))
     return;
-  const Tile t = tile_of<G>(p, rows_of(seq), seq, index);
+  const Tile t = tile_of<G>(p, rows, seq, index);
   if (!walk_tile<G>(p, qscale, t, kvh, 0, t.steps, nullptr, ring))
     walk_odd<G>(p, qscale, t, kvh, 0, t.steps, nullptr);
 }
