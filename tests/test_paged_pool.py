@@ -197,3 +197,26 @@ def test_pool_refuses_numbers_past_32_bits_and_calls_after_close(yuear_lib):
     pool.close()
     with pytest.raises(ValueError):
         pool.open()
+
+
+@pytest.mark.parametrize("past", [2 ** 32, -2 ** 32, 2 ** 31, 2 ** 40])
+def test_pool_reads_name_no_other_sequence(yuear_lib, past):
+    """Sequence numbers whose low 32 bits are a sequence's are not that sequence."""
+    pool = yuear_lib.PagePool(8, 32)
+    a, b = pool.open(), pool.open()
+    pool.extend(b, 40)
+    with pytest.raises(ValueError):
+        pool.length(b + past)
+    for ids in ([b + past], np.array([b + past], np.int64), np.array([[a], [b + past]], np.int64),
+                np.array([b + past], np.float64), np.array([b + 0.5])):
+        with pytest.raises(ValueError):
+            pool.table(ids, 4)
+    if past > 0:
+        with pytest.raises(ValueError):
+            pool.table(np.array([b + past], np.uint64), 4)
+    with pytest.raises(ValueError):
+        pool.table([b], 2 ** 32 + 2)
+    for ids in ([b], np.array([b], np.int64), np.array([[b]], np.uint8), (np.int32(b),)):
+        assert pool.table(ids, 3).tolist() == [[0, 1, -1]]
+    assert pool.length(np.int64(b)) == 40
+    assert pool.table([], 4).shape == (0, 4) and pool.table(np.empty(0), 4).shape == (0, 4)

@@ -446,12 +446,19 @@ class PagePool:
 
     def table(self, sequences, width):
         """int32 [sequences, width] page table, -1 past a sequence's pages."""
-        ids = np.ascontiguousarray(sequences, dtype=np.int32).reshape(-1)
+        self._fit(width)
+        given = np.asarray(sequences).reshape(-1)
+        if given.size and given.dtype.kind not in "iu":
+            raise ValueError("sequences are integers")
+        if given.size:
+            self._fit(int(given.min()), int(given.max()))
+        ids = np.ascontiguousarray(given, dtype=np.int32)
         out = np.full((ids.size, width), -1, dtype=np.int32)
         self._call("table", ids.ctypes.data_as(i32p), ids.size, width, out.ctypes.data_as(i32p))
         return out
 
     def length(self, sequence):
+        self._fit(sequence)
         n = lib.yuear_pages_length(self._handle, sequence)
         if n < 0:
             raise ValueError("no such sequence")
