@@ -220,3 +220,11 @@ def test_pool_reads_name_no_other_sequence(yuear_lib, past):
         assert pool.table(ids, 3).tolist() == [[0, 1, -1]]
     assert pool.length(np.int64(b)) == 40
     assert pool.table([], 4).shape == (0, 4) and pool.table(np.empty(0), 4).shape == (0, 4)
+
+
+@pytest.mark.parametrize("sizes", [(2 ** 32 + 1, 24, 8, 0), (1, 2 ** 32 + 24, 8, 0), (1, 24, 2 ** 32 + 8, 0),
+                                   (1, 24, 8, 2 ** 32 + 100), (2 ** 31, 24, 8, 0), (1 - 2 ** 32, 24, 8, 0)])
+def test_workspace_sizes_past_32_bits_are_refused(yuear_lib, sizes):
+    """Not answered with the workspace of their low 32 bits."""
+    with pytest.raises(ValueError, match="paged_workspace"):
+        yuear_lib.paged_workspace(*sizes)

@@ -625,7 +625,8 @@ def paged_workspace(batch, heads, kv_heads, rows=0, device=None):
     """A workspace, its counters zeroed, for the paged attention of up to these sizes (rows 0:
     decode steps only). Calls that may overlap need one each."""
     torch = _torch()
-    n = lib.yuear_op_paged_workspace_bytes(batch, heads, kv_heads, rows)
+    fits = max(batch, heads, kv_heads, rows) < 2**31 and min(batch, heads, kv_heads, rows) >= 0
+    n = lib.yuear_op_paged_workspace_bytes(batch, heads, kv_heads, rows) if fits else 0
     if n <= 0:
         _refuse("paged_workspace", "invalid arguments")
     workspace = torch.empty(n // 4, dtype=torch.int32, device="cuda" if device is None else device)
