@@ -1,0 +1,79 @@
+"""Paged cache operators on the GPU where their plans and their arithmetic meet an
+edge. Bounds are paged_ref.py's."""
+import numpy as np
+import pytest
+
+import paged_ref as ref
+from test_gpu_paged import check_decode, decode, decode_inputs, torch  # noqa: F401 (torch: the fixture)
+
+pytestmark = pytest.mark.gpu
+INF = float("inf")
+
+
+def put_v(s, b, t, head, dims, x):
+    page, slot = int(s["table"][b][t // s["pages"].slots]), t % s["pages"].slots
+    s["pages"].v[page, head, slot // 32, dims, slot % 32] = x
+
+
+def put_k(s, b, t, head, dims, x):
+    page, slot = int(s["table"][b][t // s["pages"].slots]), t % s["pages"].slots
+    s["pages"].k[page, head, slot, dims] = x
+
+
+# ---- infinities that a row sees ----
+
+@pytest.mark.parametrize("pos", [[40], [500, 40, 31, 700], [5000], [20 + 9 * i for i in range(70)]])
+def test_decode_gives_the_infinities_that_it_sees(torch, yuear_lib, pos):
+    """An infinite value gives an infinity of its sign whatever its key's weight is."""
+    rng = np.random.default_rng(len(pos))
+    heads, kv = 6, 2
+    s = decode_inputs(torch, yuear_lib, rng, heads, kv, 64, pos, 200 if len(pos) < 9 else 500)
+    first, middle, own, last = slice(0, 30, 7), slice(31, 60, 7), slice(61, 90, 7), slice(91, 120, 7)
+    rows = s["qkv"].view(len(pos), heads + 2 * kv, 128)
+
+    def marks(scale):
+        for b, p in enumerate(pos):
+            put_v(s, b, 0, 0, first, INF * scale if scale else 0.0)
+            put_v(s, b, p // 2, 1, middle, -INF * scale if scale else 0.0)
+            rows[b, heads + kv, own] = INF if scale else 0.0
+            put_v(s, b, p - 1, 1, last, INF if scale else 0.0)
+    marks(0)
+    check_decode(torch, s, decode(torch, yuear_lib, s))
+    marks(1)
+    out = decode(torch, yuear_lib, s)
+    want = torch.zeros(len(pos), kv, heads // kv, 128, device="cuda")
+    want[:, 0, :, first], want[:, 1, :, middle], want[:, 0, :, own], want[:, 1, :, last] = INF, -INF, INF, INF
+    want = want.view(len(pos), heads, 128)
+    odd = want != 0
+    assert torch.equal(out[odd].float(), want[odd])
+    marks(0)
+    plain = decode(torch, yuear_lib, s)
+    check_decode(torch, s, torch.where(odd, plain, out))
+
+
+@pytest.mark.parametrize("pos", [[40], [500, 40, 31, 700], [5000]])
+def test_decode_weighs_keys_with_an_infinity(torch, yuear_lib, pos):
+    """A key whose score is -inf weighs nothing; one of +inf makes its rows NaN."""
+    rng = np.random.default_rng(40 + len(pos))
+    heads, kv = 6, 2
+    s = decode_inputs(torch, yuear_lib, rng, heads, kv, 64, pos, 200)
+    for b, p in enumerate(pos):
+        x = s["qkv"][b].reshape(-1, 128)
+        q, _ = ref.turn(x[:heads], s["gains"][0], s["rope"][0][p], s["rope"][1][p], 1e-5)
+        d = int(q.abs().amin(0).argmax())  # no head's query is near zero there
+        at = {0: p // 3, 1: p - 1}
+        for h, t in at.items():
+            put_k(s, b, t, h, d, INF if h else -INF)
+        out = decode(torch, yuear_lib, s)[b]
+        for h, t in at.items():
+            put_k(s, b, t, h, d, 0.0)
+        k, v, present = ref.gather(s["pages"].k, s["pages"].v, s["table"][b], p + 1)
+        for n in range(heads):
+            h = n // (heads // kv)
+            if (float(q[n, d]) > 0) == (h == 1):
+                assert torch.isnan(out[n]).all(), (b, n)
+                continue
+            seen = present.copy()
+            seen[at[h]] = False
+            want, bound = ref.attend(q[n:n + 1], k[h:h + 1], v[h:h + 1], seen, 2.0 ** -16)
+            ref.check(out[n:n + 1], want, bound, f"sequence {b}, head {n}")

@@ -197,7 +197,82 @@ __device__ __forceinline__ void join_parts(const DecodeParams &p, float qscale, 
         a1 = fmaf(w, o[j].y, a1);
       }
     }
+    if (__builtin_expect(fmaf(a0, 0.f, a1 * 0.f) != 0.f, 0)) {
+      // not finite: maybe only by 0 times an infinity of what is past the last part
+      const int d = 2 * (q % (D / 2));
+      a0 = a1 = 0.f;
+#pragma unroll 1
+      for (int t = 0; t < n; ++t) {
+        const f32x2 v = load2(part(t) + h * kPartFloats + d);
+        a0 = fmaf(sh.w[0][h][t], v.x, a0);
+        a1 = fmaf(sh.w[0][h][t], v.y, a1);
+      }
+    }
     reinterpret_cast<uint32_t *>(out)[q] = pack_bf16(a0, a1);
+  }
+}
+
+// A wave's blocks x, x + kWaves, ... < x1 of an item once more, where its sums are
+// not finite: of an infinity the pieces of P and q can make a NaN (a second piece
+// of 0 or of the other sign), so here q and the weights keep their 32 bits. Head by
+// head, lanes n and n + 32 half a key each for the scores, a lane two dims for the
+// sums. Rare, so plain.
+template <int G>
+__device__ __forceinline__ void walk_odd(const DecodeParams &p, float qscale, const Span &span,
+                                         const int32_t *table, int kvh, int pos, int x, int x1,
+                                         int wave, Shared<G> &sh) {
+  const int lane = threadIdx.x & 63, low = p.window > 0 ? pos - p.window : -1;
+  float *to = reinterpret_cast<float *>(sh.stage[wave][0]);
+#pragma unroll 1
+  for (int h = 0; h < G; ++h) {
+    float M = -__builtin_inff(), l = 0.f, o[2] = {0.f, 0.f};  // of dims lane and lane + 64
+    const float2 *q = reinterpret_cast<const float2 *>(sh.q[h]) + (lane >> 5) * (D / 4);
+#pragma unroll 1
+    for (int v = x; v < x1; v += kWaves) {
+      const int t0 = span.block(v) * kBlock, t = t0 + (lane & 31);
+      const int page = table[t0 >> p.cache.shift];
+      const bool held = p.cache.has(page);
+      const size_t at = p.cache.at(held ? page : 0, kvh, t0 & ((1 << p.cache.shift) - 1));
+      const bool sees = t == pos || (held && t < pos && (t > low || t < p.sinks));
+      const uint32_t *k = reinterpret_cast<const uint32_t *>(p.cache.k + at) + lane % 32 * (D / 2) +
+                          (lane >> 5) * (D / 4);
+      const uint32_t *own = reinterpret_cast<const uint32_t *>(sh.kv_new[0]) + (lane >> 5) * (D / 4);
+      float score = 0.f;
+#pragma unroll 4
+      for (int d = 0; d < D / 4; ++d) {
+        const uint32_t w = t == pos ? own[d] : k[d];
+        score = fmaf(q[d].x, bflo(w), score);
+        score = fmaf(q[d].y, bfhi(w), score);
+      }
+      score += xor32(score, lane);
+      if (!sees)
+        score = -__builtin_inff();
+      const float top = fmaxf(M, wave_max(score));
+      const float m_use = top == -__builtin_inff() ? 0.f : top;
+      const float f = M == -__builtin_inff() ? 1.f : __builtin_amdgcn_exp2f((M - m_use) * qscale);
+      const float weight = sees ? __builtin_amdgcn_exp2f((score - m_use) * qscale) : 0.f;
+      M = top;
+      l *= f;
+      o[0] *= f;
+      o[1] *= f;
+      for (uint32_t left = uint32_t(__ballot(sees)); left; left &= left - 1) {
+        const int n = __builtin_ctz(left);
+        const float w = __shfl(weight, n);
+        l += w;
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const int d = lane + 64 * j;
+          const uint16_t value = t0 + n == pos ? sh.kv_new[1][d] : p.cache.v[at + d * kBlock + n];
+          o[j] = fmaf(w, bflo(value), o[j]);
+        }
+      }
+    }
+    to[h * D + lane] = o[0];
+    to[h * D + lane + 64] = o[1];
+    if (lane == 0) {
+      sh.m[wave][h] = M;
+      sh.l[wave][h] = l;
+    }
   }
 }
 
@@ -484,12 +559,15 @@ paged_decode_kernel(DecodeParams p, float qscale) {
 
     // ---- join the waves: each leaves its result in its own stage ----
     const float l_all = sum_halves(sum_row_pairs(l_run));
+    f32x4 finite = {l_all * 0.f, 0.f, 0.f, 0.f};  // a NaN where some sum is not
 #pragma unroll
     for (int dt = 0; dt < 8; ++dt) {
       f32x4 s;
 #pragma unroll
-      for (int e = 0; e < 4; ++e)
+      for (int e = 0; e < 4; ++e) {
         s[e] = o[dt][e] + paged::xor8(o[dt][e]);  // the pieces of P
+        finite[e] = fmaf(s[e], 0.f, finite[e]);
+      }
       if (i < G)
         reinterpret_cast<f32x4 *>(ks)[i * (D / 4) + 4 * dt + r] = s;
     }
@@ -497,6 +575,8 @@ paged_decode_kernel(DecodeParams p, float qscale) {
       sh.m[wave][i] = m_run;
       sh.l[wave][i] = l_all;
     }
+    if (__builtin_expect(__any(i < G && finite[0] + finite[1] + (finite[2] + finite[3]) != 0.f), 0))
+      walk_odd<G>(p, qscale, span, table, kvh, pos, x + wave, x1, wave, sh);
     __syncthreads();
     uint16_t *out = p.out + size_t(b) * p.out_stride + size_t(kvh * G) * D;
     // slot 2 run + 1: the item begins in this run (its last one); 2 run: before it
