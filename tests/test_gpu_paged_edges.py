@@ -4,7 +4,8 @@ import numpy as np
 import pytest
 
 import paged_ref as ref
-from test_gpu_paged import check_decode, decode, decode_inputs, torch  # noqa: F401 (torch: the fixture)
+from test_gpu_paged import (check_decode, decode, decode_inputs, prefill, prefill_inputs,
+                            torch)  # noqa: F401 (torch: the fixture)
 
 pytestmark = pytest.mark.gpu
 INF = float("inf")
@@ -77,3 +78,55 @@ def test_decode_weighs_keys_with_an_infinity(torch, yuear_lib, pos):
             seen[at[h]] = False
             want, bound = ref.attend(q[n:n + 1], k[h:h + 1], v[h:h + 1], seen, 2.0 ** -16)
             ref.check(out[n:n + 1], want, bound, f"sequence {b}, head {n}")
+
+
+# ---- scores far past the fp32 integers ----
+
+@pytest.mark.parametrize("size", [2.0 ** 8, 3.0e7, 1.0e12, 1.0e25])
+@pytest.mark.parametrize("width", [5, 128])
+@pytest.mark.parametrize("odd", [False, True])
+def test_prefill_gives_equal_keys_equal_weights(torch, yuear_lib, size, width, odd):
+    """Equal keys in different steps, behind smaller ones, weigh the same whatever
+    their score is. Every weight is 1, so what is rounded is the output (half a
+    step) and a few fp32 sums."""
+    rng = np.random.default_rng(43)
+    heads, kv, n, before = 3, 1, 90, 200
+    s = prefill_inputs(torch, rng, heads, kv, 64, [n], [before], 20, width=width)
+    s["q"][:] = torch.tensor([1.0, 1.171875, 2.96875], device="cuda")[None, :, None]  # of a head, all dims
+    s["pages"].k[:] = 0
+    small, big = [3, 66, 130], [70, 133, 190, 201, 250]
+    for t in small:
+        put_k(s, 0, t, 0, slice(None), size * 0.4453125)
+    for t in big:
+        put_k(s, 0, t, 0, slice(None), size)
+    if odd:
+        put_v(s, 0, 280, 0, 0, INF)  # of weight 0: a NaN, in this dim of rows that see it
+    out = prefill(torch, yuear_lib, s)
+    v = ref.gather(s["pages"].k, s["pages"].v, s["table"][0], before + n)[1][0]
+    for i in range(0, n, 5):
+        at = [t for t in big if t <= before + i]
+        want = v[at].mean(0)
+        bound = ref.HALF * want.abs() + ref.FINE * v[at].abs().mean(0)
+        dims = slice(1, None) if odd else slice(None)
+        for h in range(heads):
+            ref.check(out[i, h, dims], want[dims], bound[dims], f"row {i}, head {h}")
+
+
+@pytest.mark.parametrize("size", [2.0 ** 8, 3.0e7, 1.0e12, 1.0e25])
+@pytest.mark.parametrize("pos", [[290], [3000, 290]])
+def test_decode_gives_equal_keys_equal_weights(torch, yuear_lib, size, pos):
+    rng = np.random.default_rng(44)
+    heads = kv = 2
+    s = decode_inputs(torch, yuear_lib, rng, heads, kv, 64, pos, 100, gain=False)
+    s["pages"].k[:] = 0
+    s["qkv"].view(len(pos), -1, 128)[:, heads:heads + kv] = 0
+    small, big = [3, 66, 130], [70, 133, 190, 201, 250]
+    for b, p in enumerate(pos):
+        q, _ = ref.turn(s["qkv"][b].view(-1, 128)[:heads], None, s["rope"][0][p], s["rope"][1][p], 1e-5)
+        for t in small + big:
+            put_k(s, b, t, slice(None), slice(None), q.sign().to(torch.bfloat16) * (size * (0.4453125 if t in small else 1)))
+    out = decode(torch, yuear_lib, s)
+    for b, p in enumerate(pos):
+        v = ref.gather(s["pages"].k, s["pages"].v, s["table"][b], p + 1)[1]
+        want = v[:, big].mean(1)
+        ref.check(out[b], want, ref.HALF * want.abs() + ref.FINE * v[:, big].abs().mean(1), f"sequence {b}")

@@ -31,10 +31,12 @@
 // wave, one wave a SIMD, 106 / 155; 8 waves and four steps of LDS, one workgroup a CU,
 // 88 / 130; S and P V of the same step one after the other 103 / 155.
 //
-// The running maximum m of a row is taken off its scores as they are scaled. It
-// is raised only when a score passes it by more than kSlack (the weights, up to
-// 2^20, are as exact in 32 bits and in bf16 as smaller ones), so almost no step
-// rescales the 64 sums. P is rounded to bf16, half a step of 2^-8 of each weight,
+// The running maximum m of a row is a raw score, taken off the others before the
+// scale: equal keys weigh the same in every step, whatever their score is (off as
+// they are scaled, fma(score, scale, -m), weights of scores past 2^24 are wrong; as
+// fast). It is raised only when a score passes it by more than kSlack (the weights,
+// up to 2^20, are as exact in 32 bits and in bf16 as smaller ones), so almost no
+// step rescales the 64 sums. P is rounded to bf16, half a step of 2^-8 of each weight,
 // as the output is: one product per operand instead of two; the denominator sums
 // the rounded weights.
 //
@@ -316,7 +318,7 @@ __device__ __forceinline__ bool walk_tile(const PrefillParams &p, float qscale, 
     load_k(second_at, x_begin + 1, j);
   v_at = second_at;
 
-  float m_run = 0.f;  // what is taken off the row's qscale * score
+  float m_run = 0.f;  // what is taken off the row's scores: the largest at some step
   bool set = false;   // m_run is from a score of this row
   float l_run[2] = {0.f, 0.f};
   f32x16 o[4], e[2];
@@ -332,9 +334,10 @@ __device__ __forceinline__ bool walk_tile(const PrefillParams &p, float qscale, 
     return ring.k[x & 1][n & 1][k_read + ((n & ~1) ^ k_xor)];
   };
 
-  // What a step needs before its weights are formed, where its keys are not all
-  // seen or its largest score passed the running maximum by kSlack: the scores
-  // of keys that the lane's row does not see, and a raised maximum.
+  // The exponents of a step's weights from its scores st, where its keys are not all
+  // seen or its largest score passed the running maximum by kSlack: -inf for keys
+  // that the lane's row does not see, and a raised maximum.
+  f32x16 st[2];
   auto settle = [&](int x) __attribute__((always_inline)) {
     const int t0 = tl.block(x) * kKeys;
     if (bits(partial, x)) {
@@ -349,39 +352,39 @@ __device__ __forceinline__ bool walk_tile(const PrefillParams &p, float qscale, 
 #pragma unroll
         for (int j = 0; j < 16; ++j)
           if (16 * (j >> 3) + (j & 7) > last)
-            e[h][j] = -__builtin_inff();
+            st[h][j] = -__builtin_inff();
         if (cut)
 #pragma unroll
           for (int j = 0; j < 16; ++j)
             if (uint32_t(16 * (j >> 3) + (j & 7) - from) < many)
-              e[h][j] = -__builtin_inff();
+            st[h][j] = -__builtin_inff();
       }
     }
-    float mx = e[0][0];
+    float mx = st[0][0];
 #pragma unroll
     for (int h = 0; h < 2; ++h)
 #pragma unroll
       for (int j = 0; j < 16; ++j)
-        mx = fmaxf(mx, e[h][j]);
+        mx = fmaxf(mx, st[h][j]);
     mx = max_halves(mx);
-    const bool raise = set ? mx > kSlack : mx > -__builtin_inff();
+    const bool raise = set ? (mx - m_run) * qscale > kSlack : mx > -__builtin_inff();
     if (__any(raise)) {
-      const float d = raise ? mx : 0.f;
-      const float f = set ? __builtin_amdgcn_exp2f(-d) : 1.f;  // (no sums before the first score)
+      const float m_new = raise ? mx : m_run;
+      const float f = set ? __builtin_amdgcn_exp2f((m_run - m_new) * qscale) : 1.f;  // (no sums before the first score)
       l_run[0] *= f;
       l_run[1] *= f;
-      m_run += d;
+      m_run = m_new;
       set = set || raise;
-#pragma unroll
-      for (int j = 0; j < 16; ++j) {
-        e[0][j] -= d;
-        e[1][j] -= d;
-      }
 #pragma unroll
       for (int dt = 0; dt < 4; ++dt)
 #pragma unroll
         for (int j = 0; j < 16; ++j)
           o[dt][j] *= f;
+    }
+#pragma unroll
+    for (int j = 0; j < 16; ++j) {
+      e[0][j] = (st[0][j] - m_run) * qscale;
+      e[1][j] = (st[1][j] - m_run) * qscale;
     }
   };
   // what every wave does at the start of a step
@@ -450,22 +453,14 @@ __device__ __forceinline__ bool walk_tile(const PrefillParams &p, float qscale, 
 
   __builtin_amdgcn_s_waitcnt(0x0F70 | 2 * kPieces);  // Q and K of the first step
   __syncthreads();
-  {
-    f32x16 st[2];
 #pragma unroll
-    for (int h = 0; h < 2; ++h)
+  for (int h = 0; h < 2; ++h)
 #pragma unroll
-      for (int j = 0; j < 16; ++j)
-        st[h][j] = 0.f;
+    for (int j = 0; j < 16; ++j)
+      st[h][j] = 0.f;
 #pragma unroll
-    for (int n = 0; n < 16; ++n)
-      st[n & 1] = mfma32(k_operand(x_begin, n), qb[n >> 1], st[n & 1]);
-#pragma unroll
-    for (int h = 0; h < 2; ++h)
-#pragma unroll
-      for (int j = 0; j < 16; ++j)
-        e[h][j] = st[h][j] * qscale;
-  }
+  for (int n = 0; n < 16; ++n)
+    st[n & 1] = mfma32(k_operand(x_begin, n), qb[n >> 1], st[n & 1]);
 
   if (tl.first_row + 32 * wave >= tl.end_row) {  // no row of the wave's: it only loads
     for (int x = x_begin; x < x_end; ++x) {
@@ -485,14 +480,12 @@ __device__ __forceinline__ bool walk_tile(const PrefillParams &p, float qscale, 
     }
     return !any_odd();
   }
-  bool due = true;  // settle() is
+  settle(x_begin);
   auto step = [&](int x, auto more_tag) __attribute__((always_inline)) {
     constexpr bool more = decltype(more_tag)::value;  // not the last one
     begin_step(x);
     if (__builtin_expect(bits(edge, x), 0))
       bury(x);
-    if (__builtin_expect(due, 0))
-      settle(x);
     u32x4(&vs)[2][512] = ring.v[x & 1];
     uint32_t pw[2][8];
     auto weights = [&](int w) __attribute__((always_inline)) {  // words 2 w, 2 w + 1 of P's 16, rounded, and their sum
@@ -513,7 +506,6 @@ __device__ __forceinline__ bool walk_tile(const PrefillParams &p, float qscale, 
     };
     if constexpr (more) {
       const size_t k_at = at_of(x + 2);
-      f32x16 st[2];
 #pragma unroll
       for (int h = 0; h < 2; ++h)
 #pragma unroll
@@ -541,7 +533,7 @@ __device__ __forceinline__ bool walk_tile(const PrefillParams &p, float qscale, 
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
           const int h = n >> 3, j = (2 * n + k) & 15;
-          e[h][j] = fmaf(st[h][j], qscale, -m_run);
+          e[h][j] = (st[h][j] - m_run) * qscale;
           mx[n & 3] = fmaxf(mx[n & 3], e[h][j]);
         }
       }
@@ -555,8 +547,11 @@ __device__ __forceinline__ bool walk_tile(const PrefillParams &p, float qscale, 
         __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
       }
       __builtin_amdgcn_sched_group_barrier(0x008, kAhead, 0);
-      due = bool(int(bits(partial, x + 1) != 0) |
-                 int(__ballot(!set | (fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) > kSlack)) != 0));
+      const bool due = bool(
+          int(bits(partial, x + 1) != 0) |
+          int(__ballot(!set | (fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) > kSlack)) != 0));
+      if (__builtin_expect(due, 0))
+        settle(x + 1);
     } else {
 #pragma unroll
       for (int w = 0; w < 8; ++w)
@@ -633,7 +628,7 @@ __device__ __forceinline__ void walk_odd(const PrefillParams &p, float qscale, c
 #pragma unroll 8
       for (int d = 0; d < D / 2; ++d)
         score = __builtin_amdgcn_fdot2_f32_bf16(as_bf16x2(k[d]), as_bf16x2(q[d]), score, false);
-      score = sees ? score * qscale : -__builtin_inff();
+      score = sees ? score : -__builtin_inff();
       float top = score;
 #pragma unroll
       for (int b = 1; b < 64; b <<= 1)
@@ -645,8 +640,8 @@ __device__ __forceinline__ void walk_odd(const PrefillParams &p, float qscale, c
           continue;
         top = 0.f;
       }
-      const float f = M == -__builtin_inff() ? 1.f : __builtin_amdgcn_exp2f(M - top);
-      const float w = sees ? __builtin_amdgcn_exp2f(score - top) : 0.f;
+      const float f = M == -__builtin_inff() ? 1.f : __builtin_amdgcn_exp2f((M - top) * qscale);
+      const float w = sees ? __builtin_amdgcn_exp2f((score - top) * qscale) : 0.f;
       M = top;
       l *= f;
       o[0] *= f;
@@ -758,7 +753,7 @@ paged_prefill_deal_kernel(PrefillParams p, float qscale) {
 // used: what costs here is the latency of one round after the other (a wave for
 // all pieces: one row after 4000 keys 22.8 us in all, else 17.6).
 template <int G>
-__global__ __launch_bounds__(256) void paged_prefill_join_kernel(PrefillParams p) {
+__global__ __launch_bounds__(256) void paged_prefill_join_kernel(PrefillParams p, float qscale) {
   __shared__ f32x4 sums[kWaves][4][64];
   __shared__ float2 tops[kWaves][32];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -790,7 +785,7 @@ __global__ __launch_bounds__(256) void paged_prefill_join_kernel(PrefillParams p
 #pragma unroll
     for (int j = 0; j < kRound; ++j)
       top = fmaxf(top, ml[j].x);
-    const float f = M == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(M - top);
+    const float f = M == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f((M - top) * qscale);
     l *= f;
 #pragma unroll
     for (int a = 0; a < 4; ++a)
@@ -798,7 +793,7 @@ __global__ __launch_bounds__(256) void paged_prefill_join_kernel(PrefillParams p
 #pragma unroll
     for (int j = 0; j < kRound; ++j) {
       const bool out = j0 + kWaves * j >= pieces || ml[j].x == -__builtin_inff();
-      const float w = out ? 0.f : __builtin_amdgcn_exp2f(ml[j].x - top);
+      const float w = out ? 0.f : __builtin_amdgcn_exp2f((ml[j].x - top) * qscale);
       l += out ? 0.f : w * ml[j].y;
 #pragma unroll
       for (int a = 0; a < 4; ++a)
@@ -826,7 +821,7 @@ __global__ __launch_bounds__(256) void paged_prefill_join_kernel(PrefillParams p
     const float2 ml = tops[w][col];
     if (ml.x == -__builtin_inff())
       continue;
-    const float f = __builtin_amdgcn_exp2f(ml.x - M);
+    const float f = __builtin_amdgcn_exp2f((ml.x - M) * qscale);
     l += f * ml.y;
     all += f * sums[w][wave][lane];
   }
@@ -883,7 +878,7 @@ template <int G> hipError_t launch_g(PrefillParams p, hipStream_t s) {
   if (e != hipSuccess)
     return e;
   hipLaunchKernelGGL(paged_prefill_join_kernel<G>, dim3(kv_heads, 4 * kWaves, p.tiles), dim3(256), 0, s,
-                     p);
+                     p, qscale);
   return hipGetLastError();
 }
 
