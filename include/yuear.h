@@ -412,7 +412,7 @@ int32_t yuear_op_paged_append(const uint16_t *dev_qkv, int64_t qkv_stride,
  * p - t < window or t < sinks (window 0: every t <= p) that the table has;
  * fp32 scores q . K / sqrt(128), softmax and sums, bf16 out [rows] of heads *
  * 128. Infinities and NaNs reach the rows that see their keys, no others. A row
- * that sees no key gives zeros; rows that the append leaves out for
+ * that sees no key gives zeros, one that sees scores of -inf alone NaNs; rows that the append leaves out for
  * their position in the table are left untouched here. workspace as below. */
 int32_t yuear_op_paged_attention_prefill(
     const uint16_t *dev_q, int64_t q_stride, const uint16_t *dev_k_pages,

@@ -80,6 +80,55 @@ def test_decode_weighs_keys_with_an_infinity(torch, yuear_lib, pos):
             ref.check(out[n:n + 1], want, bound, f"sequence {b}, head {n}")
 
 
+@pytest.mark.parametrize("width", [8, 256])
+@pytest.mark.parametrize("odd", [False, True])
+def test_prefill_weighs_keys_with_an_infinity(torch, yuear_lib, width, odd):
+    """Keys 0 to 200 have an infinity, so their scores are infinite: rows that see
+    -inf scores alone have no softmax (NaN, as for +inf), rows that see others too
+    do not count those keys. odd: with an infinite value at the causal edge, too."""
+    rng = np.random.default_rng(41)
+    heads, kv, n, last = 6, 2, 330, 200
+    s = prefill_inputs(torch, rng, heads, kv, 64, [n], [0], 30, width=width)
+    for t in range(last + 1):
+        put_k(s, 0, t, slice(None), 9, INF)
+    s["q"][:, :, 9] = -s["q"][:, :, 9].abs() - 0.125
+    up = {5: 1, 210: 4, 300: 2}  # rows of a head whose query has the other sign
+    for i, h in up.items():
+        s["q"][i, h, 9] *= -1
+    if odd:
+        put_v(s, 0, 290, 0, 100, INF)
+    out = prefill(torch, yuear_lib, s)
+    for t in range(last + 1):
+        put_k(s, 0, t, slice(None), 9, 0.0)
+    if odd:
+        put_v(s, 0, 290, 0, 100, 0.0)
+        assert (out[290:300, :3, 100] == INF).all() and torch.isfinite(out[201:290, :, 100]).sum() == 89 * 6 - 1
+    k, v, present = ref.gather(s["pages"].k, s["pages"].v, s["table"][0], n)
+    assert torch.isnan(out[:last + 1]).all()
+    for i in [201, 202, 255, 256, 289, 290, n - 1] + [i for i in up if i > last]:
+        seen = ref.visible(i, n, 0, 0) & (np.arange(n) > last)
+        want, bound = ref.attend(s["q"][i].double(), k, v, seen, ref.HALF)
+        bad = up.get(i)
+        for h in range(heads):
+            if h == bad:
+                assert torch.isnan(out[i, h]).all()
+                continue
+            dims = [d for d in range(128) if not (odd and d == 100 and i >= 290 and h < 3)]
+            ref.check(out[i, h, dims], want[h, dims], bound[h, dims], f"row {i}, head {h}")
+
+
+@pytest.mark.parametrize("width", [6, 128])
+def test_prefill_rows_that_see_no_page_stay_zeros_beside_ones_without_a_softmax(torch, yuear_lib, width):
+    rng = np.random.default_rng(42)
+    s = prefill_inputs(torch, rng, 3, 1, 64, [200], [40], 30, width=width)
+    s["table"][0, 0] = -1              # rows at 40 to 63 see nothing
+    for t in range(64, 128):
+        put_k(s, 0, t, 0, 3, -INF)
+    s["q"][:, :, 3] = s["q"][:, :, 3].abs() + 0.125  # rows at 64 to 127 see scores of -inf alone
+    out = prefill(torch, yuear_lib, s)
+    assert not out[:24].any() and torch.isnan(out[24:88]).all() and torch.isfinite(out[88:]).all()
+
+
 # ---- scores far past the fp32 integers ----
 
 @pytest.mark.parametrize("size", [2.0 ** 8, 3.0e7, 1.0e12, 1.0e25])

@@ -217,6 +217,18 @@ template <int G> struct Deal {
   }
 };
 
+// Whether the row at pos sees a key of steps [x_begin, x_end).
+__device__ __forceinline__ bool sees_any(const PrefillParams &p, const Tile &tl, const int32_t *table,
+                                         int pos, int low, int x_begin, int x_end) {
+#pragma unroll 1
+  for (int x = 2 * x_begin; x < 2 * x_end; ++x) {  // 32-key halves
+    const int t = tl.block(x >> 1) * kKeys + kBlock * (x & 1);
+    if (t <= pos && (min(t + kBlock - 1, pos) > low || t < p.sinks) && p.cache.has(table[t >> p.cache.shift]))
+      return true;
+  }
+  return false;
+}
+
 // Steps [x_begin, x_end) of a tile of kv head kvh; part_of: where a piece of the
 // tile leaves its sums (null: the whole tile). False, with nothing written, where
 // walk_odd() has to do it.
@@ -566,7 +578,12 @@ __device__ __forceinline__ bool walk_tile(const PrefillParams &p, float qscale, 
   step(x_last, std::false_type{});
   if (any_odd())
     return false;
-  const float l = sum_halves(l_run[0] + l_run[1]);
+  float l = sum_halves(l_run[0] + l_run[1]);
+  // No weight: the lane's row sees no key, or scores of -inf alone (rare: not a
+  // number, but in a piece only where the others have none either).
+  const bool none = l == 0.f;
+  if (__builtin_expect(__any(none), 0))
+    l = none && sees_any(p, tl, table, my_pos, low, x_begin, x_end) ? __builtin_nanf("") : l;
   if (part_of) {
     f32x4 *to = reinterpret_cast<f32x4 *>(part_of) + wave * (16 * 64) + lane;
 #pragma unroll
@@ -577,7 +594,7 @@ __device__ __forceinline__ bool walk_tile(const PrefillParams &p, float qscale, 
             f32x4{o[dt][4 * a], o[dt][4 * a + 1], o[dt][4 * a + 2], o[dt][4 * a + 3]};
     if (half == 0)
       reinterpret_cast<float2 *>(part_of + kRows * D)[32 * wave + col] =
-          float2{l == 0.f ? -__builtin_inff() : m_run, l};
+          float2{none ? -__builtin_inff() : m_run, l};
     return true;
   }
   const float inv = l == 0.f ? 0.f : 1.f / l;  // (0: the row sees nothing)
@@ -615,6 +632,7 @@ __device__ __forceinline__ void walk_odd(const PrefillParams &p, float qscale, c
     const uint32_t *q = reinterpret_cast<const uint32_t *>(
         p.q + (size_t(tl.rows.first) + token) * p.q_stride + size_t(head) * D);
     float M = -__builtin_inff(), l = 0.f, o[2] = {0.f, 0.f};  // of dims lane and lane + 64
+    bool any = false;  // a key is seen
 #pragma unroll 1
     for (int x = x_begin; x < x_end; ++x) {
       const int t0 = tl.block(x) * kKeys, t = t0 + lane;
@@ -635,6 +653,7 @@ __device__ __forceinline__ void walk_odd(const PrefillParams &p, float qscale, c
         top = fmaxf(top, __shfl_xor(top, b));
       top = fmaxf(M, top);
       unsigned long long left = __ballot(sees);
+      any = any || left;
       if (top == -__builtin_inff()) {
         if (!__any(sees && score != score))
           continue;
@@ -655,6 +674,8 @@ __device__ __forceinline__ void walk_odd(const PrefillParams &p, float qscale, c
         o[1] += wn * __uint_as_float(uint32_t(v[(lane + 64) * kBlock]) << 16);
       }
     }
+    if (M == -__builtin_inff() && any)
+      l = __builtin_nanf("");
     if (part_of) {  // as walk_tile() leaves it
       const int col = r - tl.first_row - 32 * wave;
       for (int k = 0; k < 2; ++k) {
@@ -667,7 +688,7 @@ __device__ __forceinline__ void walk_odd(const PrefillParams &p, float qscale, c
     }
     uint16_t *dst = p.out + (size_t(tl.rows.first) + token) * p.out_stride + size_t(head) * D;
     for (int k = 0; k < 2; ++k)
-      dst[lane + 64 * k] = uint16_t(pack_bf16(M == -__builtin_inff() ? 0.f : o[k] / l, 0.f));
+      dst[lane + 64 * k] = uint16_t(pack_bf16(M == -__builtin_inff() ? l : o[k] / l, 0.f));
   }
 }
 
@@ -767,7 +788,7 @@ __global__ __launch_bounds__(256) void paged_prefill_join_kernel(PrefillParams p
     return;
   const int pieces = r1 - r0 + 1, row = first_row + 32 * group + col;
   constexpr int kRound = 2;
-  float M = -__builtin_inff(), l = 0.f;
+  float M = -__builtin_inff(), l = 0.f, none = 0.f;  // none: of pieces without a weight, 0 or a NaN
   f32x4 o[4] = {};
   for (int j0 = wave; j0 < pieces; j0 += kRound * kWaves) {
     float2 ml[kRound];
@@ -793,6 +814,7 @@ __global__ __launch_bounds__(256) void paged_prefill_join_kernel(PrefillParams p
 #pragma unroll
     for (int j = 0; j < kRound; ++j) {
       const bool out = j0 + kWaves * j >= pieces || ml[j].x == -__builtin_inff();
+      none += ml[j].x == -__builtin_inff() ? ml[j].y : 0.f;
       const float w = out ? 0.f : __builtin_amdgcn_exp2f((ml[j].x - top) * qscale);
       l += out ? 0.f : w * ml[j].y;
 #pragma unroll
@@ -805,7 +827,7 @@ __global__ __launch_bounds__(256) void paged_prefill_join_kernel(PrefillParams p
   for (int a = 0; a < 4; ++a)
     sums[wave][a][lane] = o[a];
   if (half == 0)
-    tops[wave][col] = float2{M, l};
+    tops[wave][col] = float2{M, M == -__builtin_inff() ? none : l};
   __syncthreads();
   if (row >= end_row)
     return;
@@ -815,17 +837,22 @@ __global__ __launch_bounds__(256) void paged_prefill_join_kernel(PrefillParams p
   for (int w = 1; w < kWaves; ++w)
     M = fmaxf(M, tops[w][col].x);
   f32x4 all = {};
-  l = 0.f;
+  l = none = 0.f;
 #pragma unroll
   for (int w = 0; w < kWaves; ++w) {
     const float2 ml = tops[w][col];
-    if (ml.x == -__builtin_inff())
+    if (ml.x == -__builtin_inff()) {
+      none += ml.y;
       continue;
+    }
     const float f = __builtin_amdgcn_exp2f((ml.x - M) * qscale);
     l += f * ml.y;
     all += f * sums[w][wave][lane];
   }
-  all *= M == -__builtin_inff() ? 0.f : 1.f / l;
+  if (M == -__builtin_inff())
+    all = f32x4{none, none, none, none};
+  else
+    all *= 1.f / l;
   uint16_t *dst = p.out + (size_t(first) + row / G) * p.out_stride +
                   size_t(kvh * G + row % G) * D + 32 * dt + 8 * wave + 4 * half;
   *reinterpret_cast<uint2 *>(dst) = uint2{pack_bf16(all[0], all[1]), pack_bf16(all[2], all[3])};
