@@ -4,11 +4,13 @@ import numpy as np
 import pytest
 
 import paged_ref as ref
-from test_gpu_paged import (check_decode, decode, decode_inputs, prefill, prefill_inputs,
+from test_gpu_paged import (check_decode, decode, decode_inputs, normal, prefill, prefill_inputs, rope, same_bits,
                             torch)  # noqa: F401 (torch: the fixture)
 
 pytestmark = pytest.mark.gpu
 INF = float("inf")
+COUNTERS = 131072 // 4  # int32 words of a workspace before its partial sums
+UNSET = 0x7F123456      # no sum of these tests
 
 
 def put_v(s, b, t, head, dims, x):
@@ -19,6 +21,20 @@ def put_v(s, b, t, head, dims, x):
 def put_k(s, b, t, head, dims, x):
     page, slot = int(s["table"][b][t // s["pages"].slots]), t % s["pages"].slots
     s["pages"].k[page, head, slot, dims] = x
+
+
+def marked_workspace(torch, yuear_lib, *sizes):
+    ws = yuear_lib.paged_workspace(*sizes)
+    ws[COUNTERS:] = UNSET
+    return ws
+
+
+def written_slots(torch, ws, group):
+    """Which partial sums of a decode call its workgroups left: [512, 2], for each
+    workgroup that of an item that began before it and that of one that begins in it."""
+    words = group * 130
+    part = ws[COUNTERS:COUNTERS + 1024 * words].view(1024, words)
+    return (part != UNSET).any(1).cpu().numpy().reshape(512, 2)
 
 
 # ---- infinities that a row sees ----
@@ -179,3 +195,47 @@ def test_decode_gives_equal_keys_equal_weights(torch, yuear_lib, size, pos):
         v = ref.gather(s["pages"].k, s["pages"].v, s["table"][b], p + 1)[1]
         want = v[:, big].mean(1)
         ref.check(out[b], want, ref.HALF * want.abs() + ref.FINE * v[:, big].abs().mean(1), f"sequence {b}")
+
+
+# ---- workgroups that walk several items or tiles ----
+
+def decode_on_gpu(torch, yuear_lib, heads, kv, slots, pos, absent, seed):
+    """decode_inputs() of many keys: one draw for the whole pool, NaN in slots that
+    no token wrote; `absent`: (sequence, page of it) pairs that the table does not have."""
+    rng = np.random.default_rng(seed)
+    gen = torch.Generator(device="cuda")
+    gen.manual_seed(seed)
+    lens = [max(p, 0) + 1 for p in pos]
+    n = sum((x + slots - 1) // slots for x in lens) + 3
+    s = dict(table=ref.tables(lens, slots, n, rng), pages=ref.Pages(n, kv, slots, "cuda"), pos=list(pos), heads=heads,
+             kv=kv, gains=[normal(torch, rng, 128, mean=1.3, std=0.1) for _ in range(2)],
+             qkv=normal(torch, rng, len(pos), (heads + 2 * kv) * 128), rope=rope(torch, yuear_lib, max(lens)))
+    pages = s["pages"]
+    pages.k = torch.randn(pages.k.shape, generator=gen, device="cuda").to(torch.bfloat16)
+    pages.v = torch.randn(pages.v.shape, generator=gen, device="cuda").to(torch.bfloat16)
+    held = set(s["table"].ravel().tolist()) - {-1}
+    loose = [p for p in range(n) if p not in held]
+    pages.k[loose], pages.v[loose] = float("nan"), float("nan")
+    for b, x in enumerate(lens):  # slots at and past the token's own
+        page, slot = int(s["table"][b][(x - 1) // slots]), (x - 1) % slots
+        pages.k[page, :, slot:] = float("nan")
+        blocks = pages.v[page].transpose(-1, -2).reshape(kv, slots, 128)
+        blocks[:, slot:] = float("nan")
+        pages.v[page] = blocks.reshape(kv, slots // 32, 32, 128).transpose(-1, -2)
+    for b, j in absent:
+        s["table"][b, j] = -1
+    return s
+
+
+@pytest.mark.parametrize("kv,batch,short,longest", [(8, 64, 370, 24570), (16, 32, 370, 12270)])
+def test_decode_of_one_long_sequence_among_short_ones(torch, yuear_lib, kv, batch, short, longest):
+    """The long one's keys are shared out over many workgroups."""
+    pos = [short] * batch
+    pos[batch // 2] = longest
+    s = decode_on_gpu(torch, yuear_lib, kv, kv, 128, pos, [], 45)
+    ws = marked_workspace(torch, yuear_lib, batch, kv, kv)
+    out = decode(torch, yuear_lib, s, workspace=ws)
+    check_decode(torch, s, out)
+    # its heads take at least half of the work and so of the 512 workgroups
+    assert written_slots(torch, ws, 1).any(1).sum() >= 200 and not ws[:COUNTERS].any()
+    assert same_bits(torch, out, decode(torch, yuear_lib, s, workspace=ws))

@@ -12,10 +12,12 @@
 // (sequence, kv head) item. The positions are read on the device, so one captured
 // launch serves every length. Two ways to cut the list into workgroups:
 //
-// - up to 512 items and 24 blocks a workgroup: each item into equal chunks, one
-//   workgroup each, as many as 512 workgroups and 64 parts an item allow, of at
-//   least a block a wave (one sequence of 4096 keys: 12.5 us, 15.9 cut the other
-//   way, 14 with two blocks a wave; one kv head of 20000: 21 and 65);
+// - up to 64 sequences, 512 items and 24 blocks a workgroup: each item into equal
+//   chunks, one workgroup each, as many as 512 workgroups and 64 parts an item allow,
+//   of at least a block a wave (one sequence of 4096 keys: 12.5 us, 15.9 cut the
+//   other way, 14 with two blocks a wave; one kv head of 20000: 21 and 65). Not
+//   where so many items take one chunk each that the rest would be cut into more
+//   than twice the blocks of equal shares;
 // - else into equal runs, whatever the lengths of the sequences, and a workgroup
 //   walks the items of its run (45 sequences of 150 to 24500 keys: 158 us, 189 in
 //   chunks). To begin an item (positions, page, q, the joining of the waves) costs
@@ -300,20 +302,30 @@ paged_decode_kernel(DecodeParams p, float qscale) {
   // dispatch goes round the 8 XCDs: each takes neighbouring runs
   int run = int(blockIdx.x % 8) * (p.groups / 8) + int(blockIdx.x / 8);
   int b, place, nb, kvh, x, u, u1, each = 0, more = 0, r0 = 0, r1 = 0, step = 1;
-  const bool chunks = p.batch <= 64 && total <= kChunkBlocks && items <= kChunks;
+  bool chunks = p.batch <= 64 && total <= kChunkBlocks && items <= kChunks;
   auto run_begin = [&](int g) { return g * each + min(g, more); };
   auto run_of = [&](int v) {
     return v < more * (each + 1) ? v / (each + 1) : more + (v - more * (each + 1)) / each;
   };
+  // blocks of a chunk, at most: one a wave, kChunks chunks, kParts of a sequence
+  int size = 0, count = 0;
+  auto cut = [&](int blocks) { return (blocks + size - 1) / size; };
+  auto chunks_of = [&](int blocks) {
+    size = blocks;
+    return count = __builtin_amdgcn_readlane(wave_scan(cut(my_blocks)), 63) * hkv;
+  };
+  if (chunks) {
+    const int longest = int(wave_max(float(my_blocks)));
+    const int least = max(max(kWaves, (longest + kParts - 1) / kParts), (total + kChunks - 1) / kChunks);
+    // many short items leave a long one few chunks: runs share it out (at 2 * least
+    // blocks a chunk, up to kChunks / 2 items always fit)
+    if (items > kChunks / 2)
+      chunks = chunks_of(2 * least) <= kChunks;
+    for (int s = least; chunks && chunks_of(s) > kChunks; ++s) {
+    }
+  }
   if (chunks) {
     const int n = my_blocks;
-    // blocks of a chunk, at most: one a wave, kChunks chunks, kParts of a sequence
-    const int longest = int(wave_max(float(n)));
-    int size = max(max(kWaves, (longest + kParts - 1) / kParts), (total + kChunks - 1) / kChunks);
-    auto cut = [&](int blocks) { return (blocks + size - 1) / size; };
-    int count;
-    while ((count = __builtin_amdgcn_readlane(wave_scan(cut(n)), 63) * hkv) > kChunks)
-      ++size;
     const int per = (count + 7) / 8;
     run = int(blockIdx.x % 8) * per + int(blockIdx.x / 8);
     if (int(blockIdx.x / 8) >= per ||
