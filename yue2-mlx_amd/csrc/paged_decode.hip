@@ -223,7 +223,9 @@ template <int G>
 __device__ __forceinline__ void walk_odd(const DecodeParams &p, float qscale, const Span &span,
                                          const int32_t *table, int kvh, int pos, int x, int x1,
                                          int wave, Shared<G> &sh) {
-  const int lane = threadIdx.x & 63, low = p.window > 0 ? pos - p.window : -1;
+  int lane = threadIdx.x & 63;
+  asm volatile("" : "+v"(lane));  // (anew, so that what this computes from it stays here)
+  const int low = p.window > 0 ? pos - p.window : -1;
   float *to = reinterpret_cast<float *>(sh.stage[wave][0]);
 #pragma unroll 1
   for (int h = 0; h < G; ++h) {
