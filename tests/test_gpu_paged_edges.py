@@ -1,11 +1,13 @@
 """Paged cache operators on the GPU where their plans and their arithmetic meet an
-edge. Bounds are paged_ref.py's."""
+edge: infinities that are seen, scores past 2^24, workgroups that walk several
+items or tiles, one long sequence among short ones, and the same cache through
+the contiguous operators. Bounds are paged_ref.py's."""
 import numpy as np
 import pytest
 
 import paged_ref as ref
-from test_gpu_paged import (check_decode, decode, decode_inputs, normal, prefill, prefill_inputs, rope, same_bits,
-                            torch)  # noqa: F401 (torch: the fixture)
+from test_gpu_paged import (check_decode, check_prefill, decode, decode_inputs, ints, normal, prefill, prefill_inputs,
+                            rope, same_bits, torch)  # noqa: F401 (torch: the fixture)
 
 pytestmark = pytest.mark.gpu
 INF = float("inf")
@@ -227,6 +229,55 @@ def decode_on_gpu(torch, yuear_lib, heads, kv, slots, pos, absent, seed):
     return s
 
 
+def check_some(torch, s, out, window, sinks, idle):
+    """check_decode() of the sequences that the call has, and the others' rows as they were."""
+    live = [b for b, p in enumerate(s["pos"]) if p >= 0]
+    assert sorted(set(range(len(s["pos"]))) - set(live)) == sorted(idle)
+    assert (out[idle] == 7).all()
+    part = dict(s, qkv=s["qkv"][live], table=s["table"][live], pos=[s["pos"][b] for b in live])
+    check_decode(torch, part, out[live], window, sinks)
+
+
+@pytest.mark.parametrize("heads,kv,batch,longest,window,sinks,both", [
+    (24, 8, 90, 1500, 0, 0, 50),
+    (24, 8, 90, 3000, 700, 37, 60),
+    (16, 8, 40, 4000, 0, 0, 200),   # up to 64 sequences, past 24 * 512 blocks
+    (6, 1, 200, 3000, 0, 0, 80),
+    (8, 1, 300, 1500, 0, 0, 80),
+    (4, 2, 300, 400, 0, 0, 20),
+])
+def test_decode_runs_that_cross_items(torch, yuear_lib, heads, kv, batch, longest, window, sinks, both):
+    """Equal runs of blocks whose workgroups end one item and begin the next, over
+    sequences, kv heads, absent pages and idle sequences."""
+    rng = np.random.default_rng(batch)
+    pos = [int(p) for p in np.exp(rng.uniform(0, np.log(longest), batch))]
+    pos[batch // 3] = longest
+    if batch <= 64 or kv == 1:
+        pos = [int(p) for p in rng.uniform(longest / 2 if batch <= 64 else 0, longest, batch)]
+    idle = [0, 1, batch // 2, batch - 1]
+    for b in idle:
+        pos[b] = -1
+    absent = [(b, j) for b in range(2, batch - 1, 7) for j in ([0, 2] if pos[b] > 300 else [0])]
+    s = decode_on_gpu(torch, yuear_lib, heads, kv, 64, pos, absent, batch + heads)
+    ws = marked_workspace(torch, yuear_lib, batch, heads, kv)
+    k, v = s["pages"].k.clone(), s["pages"].v.clone()
+    out = torch.full((batch, heads, 128), 7.0, dtype=torch.bfloat16, device="cuda")
+    decode(torch, yuear_lib, s, window, sinks, workspace=ws, out=out)
+    check_some(torch, s, out, window, sinks, idle)
+    slots = written_slots(torch, ws, heads // kv)
+    assert slots.all(1).sum() >= both and not ws[:COUNTERS].any()
+    # nothing but the tokens' own slots changed, and an equal call gives equal bits
+    for b, p in enumerate(pos):
+        page, slot = (int(s["table"][b][p // 64]), p % 64) if p >= 0 else (-1, 0)
+        if page >= 0:
+            k[page, :, slot] = s["pages"].k[page, :, slot]
+            v[page, :, slot // 32, :, slot % 32] = s["pages"].v[page, :, slot // 32, :, slot % 32]
+    assert same_bits(torch, k, s["pages"].k) and same_bits(torch, v, s["pages"].v)
+    again = torch.full_like(out, 7.0)
+    decode(torch, yuear_lib, s, window, sinks, workspace=ws, out=again)
+    assert same_bits(torch, out, again)
+
+
 @pytest.mark.parametrize("kv,batch,short,longest", [(8, 64, 370, 24570), (16, 32, 370, 12270)])
 def test_decode_of_one_long_sequence_among_short_ones(torch, yuear_lib, kv, batch, short, longest):
     """The long one's keys are shared out over many workgroups."""
@@ -239,3 +290,155 @@ def test_decode_of_one_long_sequence_among_short_ones(torch, yuear_lib, kv, batc
     # its heads take at least half of the work and so of the 512 workgroups
     assert written_slots(torch, ws, 1).any(1).sum() >= 200 and not ws[:COUNTERS].any()
     assert same_bits(torch, out, decode(torch, yuear_lib, s, workspace=ws))
+
+
+@pytest.mark.parametrize("heads,kv,lens,pos0,window,sinks,cross", [
+    (24, 8, [400], [3000], 0, 0, 5),
+    (24, 8, [200, 0, 700, 33], [2500, 5, 1500, 4000], 0, 0, 5),
+    (24, 8, [70, 0, 300, 33], [2500, 5, 0, 4000], 0, 0, 0),  # runs of about a tile's cost
+    (12, 6, [500], [2500], 0, 0, 5),
+    (16, 8, [400, 1, 300], [1000, 3000, 350], 1500, 33, 5),
+    (8, 1, [700, 500], [3000, 1200], 0, 0, 5),
+])
+@pytest.mark.parametrize("odd", [False, True])
+def test_prefill_runs_that_cross_tiles(torch, yuear_lib, heads, kv, lens, pos0, window, sinks, cross, odd):
+    """Dealt steps whose workgroups end one tile and begin the next, also of another
+    kv head; odd: some of the tiles hold infinite values that some rows see."""
+    rng = np.random.default_rng(heads + sum(lens) + odd)
+    rows, batch, group = sum(lens), len(lens), heads // kv
+    s = prefill_inputs(torch, rng, heads, kv, 64, lens, pos0, 300)
+    marks = []  # sequence, key, kv head
+    if odd:
+        marks = [(b, p + n * i // 7, h) for b, (p, n) in enumerate(zip(pos0, lens)) if n > 30 for i in (1, 3, 6)
+                 for h in range(0, kv, 3)]
+    for b, t, h in marks:
+        put_v(s, b, t, h, slice(0, 128, 9), 0.0)
+    clean = prefill(torch, yuear_lib, s, window, sinks)
+    check_prefill(torch, s, clean, window, sinks, some=12)
+    for b, t, h in marks:
+        put_v(s, b, t, h, slice(0, 128, 9), INF)
+    ws = marked_workspace(torch, yuear_lib, batch, heads, kv, rows)
+    out = prefill(torch, yuear_lib, s, window, sinks, workspace=ws)
+    seen = torch.zeros(rows, kv, dtype=torch.bool, device="cuda")
+    for b, t, h in marks:
+        p = np.arange(pos0[b], pos0[b] + lens[b])
+        sees = (t <= p) & ((p - t < window) | (t < sinks) if window else True)
+        seen[int(s["starts"][b]):int(s["starts"][b + 1]), h] |= torch.from_numpy(sees).cuda()
+    inf = torch.zeros(rows, heads, 128, dtype=torch.bool, device="cuda")
+    inf[:, :, ::9] = seen.repeat_interleave(group, 1)[:, :, None]
+    assert torch.equal(out == INF, inf)
+    for b, t, h in marks:
+        put_v(s, b, t, h, slice(0, 128, 9), 0.0)
+    check_prefill(torch, s, torch.where(inf, clean, out), window, sinks, some=12)
+    for b, t, h in marks:
+        put_v(s, b, t, h, slice(0, 128, 9), INF)
+    assert same_bits(torch, out, prefill(torch, yuear_lib, s, window, sinks, workspace=ws))
+    # the records of the tiles: their first and last run
+    tiles = rows * group // 128 + min(batch, rows)
+    info = ws[COUNTERS + 1024 * 16640:].cpu().numpy()
+    assert info[0] == sum((n * group + 127) // 128 for n in lens)
+    held = [set() for _ in range(512)]
+    for h in range(kv):
+        for i in range(info[0]):
+            first, last = info[8 * (1 + h * tiles + i):][:2]
+            for run in range(first, last + 1):
+                held[run].add((h, i))
+    assert sum(len(x) > 1 for x in held) >= cross
+    assert kv != 6 or sum(len({h for h, _ in x}) > 1 for x in held) >= 1
+
+
+def test_prefill_rounds_each_weight_once(torch, yuear_lib):
+    """Relative error of a whole call. A bf16 rounding of values with a mantissa m
+    of even logarithm leaves 2^-8 sqrt(E[1 / m^2] / 3) = 0.00166 (E = 3 / (8 ln 2));
+    values around zero take the outputs' one and the weights', independent of it:
+    0.00235 together, and a tenth for how the mantissas fall."""
+    rng = np.random.default_rng(46)
+    for lens, pos0 in (([97], [1000]), ([600], [0]), ([33, 210], [400, 7])):
+        s = prefill_inputs(torch, rng, 24, 8, 64, lens, pos0, 60)
+        s["pages"].v = normal(torch, rng, *s["pages"].v.shape)
+        out = prefill(torch, yuear_lib, s).double()
+        off = total = 0.0
+        for b, p0 in enumerate(pos0):
+            a, n = int(s["starts"][b]), lens[b]
+            k, v, _ = ref.gather(s["pages"].k, s["pages"].v, s["table"][b], p0 + n)
+            for i in range(0, n, 5):
+                want, _ = ref.attend(s["q"][a + i].double(), k[:, :p0 + i + 1], v[:, :p0 + i + 1], np.ones(p0 + i + 1, bool),
+                                     ref.HALF)
+                off += float(((out[a + i] - want) ** 2).sum())
+                total += float((want ** 2).sum())
+        assert (off / total) ** 0.5 <= 1.1 * 0.00235, (lens, (off / total) ** 0.5)
+
+
+# ---- beside the contiguous operators ----
+
+@pytest.mark.parametrize("heads,kv,n,before", [(24, 8, 130, 0), (24, 8, 1, 400), (16, 8, 77, 200), (8, 1, 33, 479)])
+def test_one_page_holds_what_a_contiguous_cache_does(torch, yuear_lib, heads, kv, n, before):
+    """A page of 512 slots is the contiguous cache of as many: both operators read
+    the same memory."""
+    rng = np.random.default_rng(heads + n)
+    pages = ref.Pages(1, kv, 512, "cuda")
+    pages.k[:], pages.v[:] = 0, 0
+    pages.put(np.zeros(1, np.int32), 0, normal(torch, rng, kv, before + n, 128), normal(torch, rng, kv, before + n, 128))
+    q = normal(torch, rng, n, heads, 128, std=1.5)
+    s = dict(q=q, pages=pages, table=np.zeros((1, 1), np.int32), pos0=[before], starts=np.array([0, n]), heads=heads, kv=kv)
+    paged = prefill(torch, yuear_lib, s)
+    other = torch.empty_like(paged)
+    assert yuear_lib.lib.yuear_op_attention_prefill(q.data_ptr(), pages.k.data_ptr(), pages.v.data_ptr(), n, before, heads,
+                                                    kv, 512, other.data_ptr(), None) == 0
+    torch.cuda.synchronize()
+    check_prefill(torch, s, paged)
+    check_prefill(torch, s, other)
+
+
+@pytest.mark.parametrize("heads,kv,pos", [(24, 8, 0), (24, 8, 400), (16, 8, 95), (8, 1, 511)])
+def test_a_step_on_one_page_is_one_on_a_contiguous_cache(torch, yuear_lib, heads, kv, pos):
+    """Rotation by nothing, no norm: both take the same queries and keep the same keys."""
+    rng = np.random.default_rng(heads + pos)
+    one, none = (torch.full((512, 64), x, dtype=torch.bfloat16, device="cuda") for x in (1.0, 0.0))
+    s = dict(qkv=normal(torch, rng, 1, (heads + 2 * kv) * 128), pages=ref.Pages(1, kv, 512, "cuda"),
+             table=np.zeros((1, 1), np.int32), gains=[None, None], pos=[pos], heads=heads, kv=kv, rope=(one, none))
+    if pos:
+        s["pages"].put(s["table"][0], 0, normal(torch, rng, kv, pos, 128), normal(torch, rng, kv, pos, 128))
+    k, v = s["pages"].k.clone(), s["pages"].v.clone()
+    paged = decode(torch, yuear_lib, s)
+    other = torch.empty_like(paged)
+    assert yuear_lib.lib.yuear_op_attention_decode(
+        s["qkv"].data_ptr(), None, None, 1e-5, one.data_ptr(), none.data_ptr(), k.data_ptr(), v.data_ptr(),
+        ints(torch, [pos]).data_ptr(), heads, kv, 512, 1, 16, other.data_ptr(), None) == 0
+    torch.cuda.synchronize()
+    check_decode(torch, s, paged)
+    check_decode(torch, s, other)
+    assert torch.equal(k.nan_to_num(7), s["pages"].k.nan_to_num(7))
+    # (V's slots after the token's in its block are the contiguous operator's own)
+    rows = [t[0].transpose(-1, -2).reshape(kv, 512, 128)[:, :pos + 1] for t in (v, s["pages"].v)]
+    assert torch.equal(rows[0], rows[1])
+
+
+def test_a_fork_decodes_into_a_page_of_its_own(torch, yuear_lib):
+    """A prompt, a second take of it, and a step of both: the tables are made after
+    the pool has given each its room."""
+    rng = np.random.default_rng(47)
+    heads, kv, slots, n = 6, 2, 32, 45
+    pool = yuear_lib.PagePool(10, slots)
+    pages = ref.Pages(10, kv, slots, "cuda")
+    cos, sin = rope(torch, yuear_lib, 100)
+    a = pool.open()
+    pool.extend(a, n)
+    table = pool.table([a], 3)
+    qkv = normal(torch, rng, n, (heads + 2 * kv) * 128)
+    yuear_lib.paged_append(qkv, pages.k, pages.v, ints(torch, table), ints(torch, [0, n]), ints(torch, [0]), cos, sin)
+    b = pool.fork(a)
+    takes = [a, b]
+    pos = [pool.length(t) for t in takes]
+    for t in takes:
+        yuear_lib.pages_copy(pages.k, pages.v, *pool.extend(t, 1))
+    both = pool.table(takes, 3)
+    assert both[0, 0] == both[1, 0] and both[0, 1] != both[1, 1]
+    s = dict(qkv=normal(torch, rng, 2, (heads + 2 * kv) * 128), pages=pages, table=both, gains=[None, None], pos=pos,
+             heads=heads, kv=kv, rope=(cos, sin))
+    check_decode(torch, s, decode(torch, yuear_lib, s))
+    x = s["qkv"].view(2, -1, 128)[:, heads + kv:]
+    for t in range(2):  # each take's page has its own token behind the shared prompt
+        values = ref.gather(pages.k, pages.v, both[t], n + 1)[1]
+        assert torch.equal(values[:, n], x[t].double())
+        assert torch.equal(values[:, :n], qkv.view(n, -1, 128)[:, heads + kv:].double().transpose(0, 1))
