@@ -70,6 +70,47 @@ def test_decode_gives_the_infinities_that_it_sees(torch, yuear_lib, pos):
     check_decode(torch, s, torch.where(odd, plain, out))
 
 
+@pytest.mark.parametrize("batch", [1, 70])
+def test_decode_keeps_unseen_slots_out_beside_infinities_that_it_sees(torch, yuear_lib, batch):
+    """Window, sinks, a page that is not there and slots past the token, all of them
+    NaN, in blocks that hold a seen infinity."""
+    rng = np.random.default_rng(39)
+    heads, kv, window, sinks = 8, 2, 105, 35
+    pos = [500 + i for i in range(batch)]
+    s = decode_inputs(torch, yuear_lib, rng, heads, kv, 32, pos, 20 * batch)
+    s["table"][:, 13] = -1  # keys 416 to 447 are not there
+    dims = slice(3, 128, 11)
+    marks = {0: [34], 1: [398 + batch, 500]}  # of a kv head: keys that every sequence sees
+
+    def fill(x):
+        for b, p in enumerate(pos):
+            for h, keys in marks.items():
+                for t in keys:
+                    if t < p:
+                        put_v(s, b, t, h, dims, x)
+    for b, p in enumerate(pos):
+        for t in [35, 63, p - window, p - window - 1]:
+            put_k(s, b, t, slice(None), slice(None), float("nan"))
+            put_v(s, b, t, slice(None), slice(None), float("nan"))
+    marks[1] = [t for t in marks[1] if t > pos[-1] - window]
+    fill(0.0)
+    plain = decode(torch, yuear_lib, s, window, sinks)
+    fill(INF)
+    out = decode(torch, yuear_lib, s, window, sinks)
+    odd = torch.zeros(batch, kv, heads // kv, 128, dtype=torch.bool, device="cuda")
+    odd[:, 0, :, dims] = True
+    for b, p in enumerate(pos):
+        odd[b, 1, :, dims] = any(t < p for t in marks[1])
+    odd = odd.view(batch, heads, 128)
+    assert torch.equal(out == INF, odd)
+    fill(0.0)
+    for b, p in enumerate(pos):
+        for t in [35, 63, p - window, p - window - 1]:
+            put_k(s, b, t, slice(None), slice(None), 0.0)
+            put_v(s, b, t, slice(None), slice(None), 0.0)
+    check_decode(torch, s, torch.where(odd, plain, out), window, sinks)
+
+
 @pytest.mark.parametrize("pos", [[40], [500, 40, 31, 700], [5000]])
 def test_decode_weighs_keys_with_an_infinity(torch, yuear_lib, pos):
     """A key whose score is -inf weighs nothing; one of +inf makes its rows NaN."""
@@ -136,14 +177,15 @@ def test_prefill_weighs_keys_with_an_infinity(torch, yuear_lib, width, odd):
 
 
 @pytest.mark.parametrize("width", [6, 128])
-def test_prefill_rows_that_see_no_page_stay_zeros_beside_ones_without_a_softmax(torch, yuear_lib, width):
+@pytest.mark.parametrize("window,sinks", [(0, 0), (40, 3), (1, 64)])
+def test_prefill_rows_that_see_no_page_stay_zeros_beside_ones_without_a_softmax(torch, yuear_lib, width, window, sinks):
     rng = np.random.default_rng(42)
     s = prefill_inputs(torch, rng, 3, 1, 64, [200], [40], 30, width=width)
     s["table"][0, 0] = -1              # rows at 40 to 63 see nothing
     for t in range(64, 128):
         put_k(s, 0, t, 0, 3, -INF)
     s["q"][:, :, 3] = s["q"][:, :, 3].abs() + 0.125  # rows at 64 to 127 see scores of -inf alone
-    out = prefill(torch, yuear_lib, s)
+    out = prefill(torch, yuear_lib, s, window, sinks)
     assert not out[:24].any() and torch.isnan(out[24:88]).all() and torch.isfinite(out[88:]).all()
 
 
