@@ -484,3 +484,115 @@ def test_a_fork_decodes_into_a_page_of_its_own(torch, yuear_lib):
         values = ref.gather(pages.k, pages.v, both[t], n + 1)[1]
         assert torch.equal(values[:, n], x[t].double())
         assert torch.equal(values[:, :n], qkv.view(n, -1, 128)[:, heads + kv:].double().transpose(0, 1))
+
+
+# ---- calls at once, in place, and through slices ----
+
+def test_calls_on_two_streams_at_once(torch, yuear_lib):
+    """Each with a workspace of its own, over one pool: equal bits to one after the other."""
+    rng = np.random.default_rng(48)
+    heads, kv = 24, 8
+    sizes = [([900, 5, 3000, 40], [70, 33], [2500, 400]), ([2000, 2100, 60, 7], [120, 5], [1500, 30])]
+    calls = []
+    for pos, lens, pos0 in sizes:
+        s = decode_inputs(torch, yuear_lib, rng, heads, kv, 64, pos, 150)
+        t = prefill_inputs(torch, rng, heads, kv, 64, lens, pos0, 150)
+        ws = yuear_lib.paged_workspace(4, heads, kv, sum(lens))
+        out = [torch.empty(4, heads, 128, dtype=torch.bfloat16, device="cuda"), torch.empty_like(t["q"])]
+        fixed = [ints(torch, x) for x in (s["table"], s["pos"], t["table"], t["starts"], t["pos0"])]
+        calls.append((s, t, ws, out, fixed))
+
+    def both(call, stream):
+        s, t, ws, out, (table, pos, table2, starts, pos0) = call
+        yuear_lib.paged_attention_decode(s["qkv"], s["pages"].k, s["pages"].v, table, pos, *s["rope"], workspace=ws,
+                                         out=out[0], stream=stream)
+        yuear_lib.paged_attention_prefill(t["q"], t["pages"].k, t["pages"].v, table2, starts, pos0, workspace=ws,
+                                          out=out[1], stream=stream)
+    want = []
+    for call in calls:
+        both(call, None)
+        want.append([o.clone() for o in call[3]])
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in calls]
+    for _ in range(5):
+        for call in calls:
+            for o in call[3]:
+                o.zero_()
+        torch.cuda.synchronize()
+        for _ in range(10):
+            for call, stream in zip(calls, streams):
+                both(call, stream.cuda_stream)
+        for stream in streams:
+            stream.synchronize()
+        for call, w in zip(calls, want):
+            assert all(same_bits(torch, a, b) for a, b in zip(call[3], w)) and not call[2][:COUNTERS].any()
+
+
+def test_two_graphs_take_turns_on_a_workspace(torch, yuear_lib):
+    rng = np.random.default_rng(49)
+    heads, kv = 16, 8
+    ws = yuear_lib.paged_workspace(3, heads, kv, 100)
+    s = decode_inputs(torch, yuear_lib, rng, heads, kv, 64, [3000, 50, 700], 100)
+    t = prefill_inputs(torch, rng, heads, kv, 64, [60, 9], [2700, 3], 100)
+    table, pos = ints(torch, s["table"]), ints(torch, s["pos"])
+    table2, starts, pos0 = (ints(torch, t[x]) for x in ("table", "starts", "pos0"))
+    out = torch.empty(3, heads, 128, dtype=torch.bfloat16, device="cuda"), torch.empty_like(t["q"])
+
+    def step(w, o):
+        yuear_lib.paged_attention_decode(s["qkv"], s["pages"].k, s["pages"].v, table, pos, *s["rope"], workspace=w, out=o)
+
+    def prompt(w, o):
+        yuear_lib.paged_attention_prefill(t["q"], t["pages"].k, t["pages"].v, table2, starts, pos0, workspace=w, out=o)
+    graphs = []
+    for call, o in ((step, out[0]), (prompt, out[1])):
+        call(ws, o)
+        torch.cuda.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            call(ws, o)
+        graphs.append(g)
+    own = yuear_lib.paged_workspace(3, heads, kv, 100)
+    for i in range(6):
+        s["qkv"].copy_(normal(torch, rng, *s["qkv"].shape))
+        t["q"].copy_(normal(torch, rng, *t["q"].shape))
+        for g in graphs[::1 - 2 * (i & 1)]:
+            g.replay()
+        want = [torch.empty_like(o) for o in out]
+        step(own, want[0])
+        prompt(own, want[1])
+        torch.cuda.synchronize()
+        assert all(same_bits(torch, a, b) for a, b in zip(out, want))
+
+
+@pytest.mark.parametrize("batch", [3, 70])
+def test_outputs_over_the_inputs(torch, yuear_lib, batch):
+    """Queries that the call turns into its output, in the same rows."""
+    rng = np.random.default_rng(50)
+    heads, kv, slots = 6, 2, 32
+    cos, sin = rope(torch, yuear_lib, 3100)
+    lens, before = [40 + i % 9 for i in range(batch)], [(500 if batch > 3 else 2900) - i for i in range(batch)]
+    rows = sum(lens)
+    ends = [n + p + 1 for n, p in zip(lens, before)]
+    n = sum((e + slots - 1) // slots for e in ends)
+    wide = torch.full((batch, n // batch + 9), -1, dtype=torch.int32)
+    table = ref.tables(ends, slots, n, rng)
+    wide[:, 3:3 + table.shape[1]] = torch.from_numpy(table)
+    table = wide.cuda()[:, 3:3 + table.shape[1]]  # rows of a wider table
+    starts, pos0 = ints(torch, np.concatenate([[0], np.cumsum(lens)])), ints(torch, before)
+    pos = ints(torch, [p + n_ for p, n_ in zip(before, lens)])
+    k = torch.randn(n, kv, slots, 128, device="cuda").to(torch.bfloat16)
+    v = torch.randn(n, kv, 1, 128, 32, device="cuda").to(torch.bfloat16)
+    qkv, new = normal(torch, rng, rows, (heads + 2 * kv) * 128), normal(torch, rng, batch, (heads + 2 * kv) * 128)
+    got = []
+    for over in (False, True):
+        a, b, k2, v2 = qkv.clone(), new.clone(), k.clone(), v.clone()
+        place = a[:, :heads * 128].unflatten(1, (heads, 128)) if over else None
+        q = yuear_lib.paged_append(a, k2, v2, table, starts, pos0, cos, sin, out=place)
+        y = yuear_lib.paged_attention_prefill(q, k2, v2, table, starts, pos0, out=place)
+        place = b[:, :heads * 128].unflatten(1, (heads, 128)) if over else None
+        z = yuear_lib.paged_attention_decode(b, k2, v2, table, pos, cos, sin, out=place)
+        got.append((y, z, k2, v2))
+        assert not over or (torch.equal(a[:, heads * 128:], qkv[:, heads * 128:])
+                            and torch.equal(b[:, heads * 128:], new[:, heads * 128:]))
+    assert torch.isfinite(got[0][0]).all() and torch.isfinite(got[0][1]).all()
+    assert all(torch.equal(x, y) for x, y in zip(*got))
