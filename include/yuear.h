@@ -452,7 +452,7 @@ int32_t yuear_op_pages_copy(uint16_t *dev_k_pages, uint16_t *dev_v_pages, int32_
                             int32_t page_slots, const int32_t *src, const int32_t *dst, int32_t n,
                             void *stream);
 /* Which sequence holds which page (host only; the pages' memory is the
- * caller's). Pages are handed out lowest first and shared by forks; a page goes
+ * caller's; at most 2^25 pages). Pages are handed out lowest first and shared by forks; a page goes
  * back when its last holder lets go of it. Calls that give copies expect the
  * caller to run them (yuear_op_pages_copy) before the cache is used again. */
 typedef struct yuear_pages yuear_pages;

@@ -228,3 +228,10 @@ def test_workspace_sizes_past_32_bits_are_refused(yuear_lib, sizes):
     """Not answered with the workspace of their low 32 bits."""
     with pytest.raises(ValueError, match="paged_workspace"):
         yuear_lib.paged_workspace(*sizes)
+
+
+@pytest.mark.parametrize("pages", [2 ** 25 + 1, 2 ** 31 - 1])
+def test_a_pool_of_more_pages_than_a_gpu_holds_is_refused(yuear_lib, pages):
+    """Its bookkeeping would take the host's memory."""
+    with pytest.raises(ValueError, match="2\\^25 pages"):
+        yuear_lib.PagePool(pages, 32)

@@ -255,6 +255,10 @@ hipError_t copy_pages(uint16_t *k, uint16_t *v, int layers, long long layer_stri
 }  // namespace
 }  // namespace yuear
 
+// Pages of a pool at most: one layer's smallest ones (16 KiB) would take 512 GiB. The
+// bookkeeping of 2^31 would take all of the host's memory.
+constexpr int32_t kMaxPages = 1 << 25;
+
 // Host bookkeeping of a pool of pages. Pages are handed out lowest first, so
 // the same calls give the same pages.
 struct yuear_pages {
@@ -309,6 +313,8 @@ yuear_status yuear_pages_create(int32_t pages, int32_t page_slots, yuear_pages *
       yuear::invalid("output pointer is required");
     if (pages < 1)
       yuear::invalid("a pool needs at least one page");
+    if (pages > kMaxPages)
+      yuear::invalid("a pool holds at most 2^25 pages");
     if (!yuear::paged::slots_ok(page_slots))
       yuear::invalid("page slots must be a power of two of at least 32");
     auto pool = std::make_unique<yuear_pages>();
