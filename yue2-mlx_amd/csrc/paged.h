@@ -98,6 +98,12 @@ __device__ __forceinline__ bool find_rows(const int32_t *starts, const int32_t *
   return true;
 }
 
+// Two values as bf16, rounded to the nearest (ties to even).
+__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
+  typedef float f32x2 __attribute__((ext_vector_type(2)));
+  return __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{lo, hi}, bf16x2_t));
+}
+
 // Value of lane ^ 8 (lanes of a 16-lane row turned by half a row).
 __device__ __forceinline__ float xor8(float v) { return dpp<0x128>(v); }
 

@@ -45,12 +45,8 @@ __device__ __forceinline__ void unpack8(u32x4 w, float (&x)[8]) {
   }
 }
 __device__ __forceinline__ u32x4 pack8(const float (&x)[8]) {
-  typedef float f32x2 __attribute__((ext_vector_type(2)));
-  uint32_t v[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-    v[i] = __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{x[2 * i], x[2 * i + 1]}, bf16x2_t));
-  return u32x4{v[0], v[1], v[2], v[3]};
+  return u32x4{paged::pack_bf16(x[0], x[1]), paged::pack_bf16(x[2], x[3]),
+               paged::pack_bf16(x[4], x[5]), paged::pack_bf16(x[6], x[7])};
 }
 
 // q/k RMSNorm + RoPE of prompt rows, q out, K and V into their pages. A

@@ -60,6 +60,7 @@ using attn::f32x4;
 using paged::Cache;
 using paged::D;
 using paged::kBlock;
+using paged::pack_bf16;
 using paged::wave_scan;
 
 constexpr int kWaves = 4;
@@ -102,11 +103,6 @@ __device__ __forceinline__ int blocks_at(const DecodeParams &p, int pos) {
 }
 __device__ __forceinline__ int blocks_of(const DecodeParams &p, int b) {
   return blocks_at(p, p.pos[b]);
-}
-
-__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
-  typedef float f32x2 __attribute__((ext_vector_type(2)));
-  return __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{lo, hi}, bf16x2_t));
 }
 
 // m (running maximum of the raw scores), l, and o of one head of a
