@@ -410,8 +410,9 @@ int32_t yuear_op_paged_append(const uint16_t *dev_qkv, int64_t qkv_stride,
 /* Attention of the rows that yuear_op_paged_append left (or any q): row i of
  * sequence b, at position p = pos0[b] + i, over the keys t <= p with
  * p - t < window or t < sinks (window 0: every t <= p) that the table has;
- * fp32 scores q . K / sqrt(128), softmax and sums, bf16 out [rows] of heads *
- * 128. Infinities and NaNs reach the rows that see their keys, no others. A row
+ * fp32 scores q . K / sqrt(128) and sums, weights rounded once to bf16 (half a
+ * step of 2^-8 of each; the contiguous prompt attention keeps them exact, and
+ * the decode form 16 bits of them), bf16 out [rows] of heads * 128. Infinities and NaNs reach the rows that see their keys, no others. A row
  * that sees no key gives zeros, one that sees scores of -inf alone NaNs; rows that the append leaves out for
  * their position in the table are left untouched here. workspace as below. */
 int32_t yuear_op_paged_attention_prefill(
@@ -436,8 +437,9 @@ int32_t yuear_op_paged_attention_decode(
     int32_t table_stride, const int32_t *dev_pos, int32_t batch, int32_t heads, int32_t kv_heads,
     int32_t window, int32_t sinks, void *dev_workspace, int64_t workspace_bytes,
     uint16_t *dev_out, int64_t out_stride, void *stream);
-/* Bytes of the workspace of the two attention calls (rows 0: the decode form),
- * 0 for invalid arguments. The caller zeroes its first
+/* Bytes of the workspace of the two attention calls (rows 0: the decode form;
+ * else with room for partial sums, also where a call comes to need none), 0 for
+ * invalid arguments. The caller zeroes its first
  * YUEAR_PAGED_COUNTER_BYTES once; every call leaves it ready for the next, of
  * any shape that it is large enough for. Calls that may overlap (other streams,
  * graphs replayed at once) need one each. */

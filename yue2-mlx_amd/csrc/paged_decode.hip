@@ -14,18 +14,21 @@
 //
 // - up to 64 sequences, 512 items and 24 blocks a workgroup: each item into equal
 //   chunks, one workgroup each, as many as 512 workgroups and 64 parts an item allow,
-//   of at least a block a wave (one sequence of 4096 keys: 12.5 us, 15.9 cut the
-//   other way, 14 with two blocks a wave; one kv head of 20000: 21 and 65). Not
-//   where so many items take one chunk each that the rest would be cut into more
-//   than twice the blocks of equal shares;
+//   of at least a block a wave (one sequence of 4096 keys: 12.3 us, 15.9 cut the
+//   other way, 14 with two blocks a wave; one kv head of 20000: 21 and 65). The
+//   sequences are a wave's lanes, so the 65th changes the plan: 64 of 30 to 100 keys
+//   11.8 us, 65 in runs 19.3; of 200 to 700 keys 27.7 and 31.0. Not where so many
+//   items take one chunk each that the rest would be cut into more than twice the
+//   blocks of equal shares (63 sequences of 370 keys and one of 24570: 414 us, in
+//   runs 43);
 // - else into equal runs, whatever the lengths of the sequences, and a workgroup
-//   walks the items of its run (45 sequences of 150 to 24500 keys: 158 us, 189 in
+//   walks the items of its run (45 sequences of 150 to 24500 keys: 155 us, 189 in
 //   chunks). To begin an item (positions, page, q, the joining of the waves) costs
 //   a workgroup about as much as 8 blocks, which the runs count (2: 172 us).
 //
 // Short caches are bound by a chain of dependent loads, 8.2 us for one block a
 // wave: positions, page numbers, K and V, each in turn, then what the waves leave in
-// LDS; the joining of parts adds 2.8 us (333 keys: 11.0).
+// LDS; the joining of parts adds 2.8 us (333 keys: 10.9).
 //
 // A part that is a whole item is finished there; else the workgroup leaves its
 // running maximum, sum and weighted values in its slots of the workspace, and
@@ -42,6 +45,8 @@
 // second product), with the G <= 8 heads in columns 0-7 as the leading bf16 piece
 // of q and in columns 8-15 as the rest, so that q counts to 16 bits and P, split
 // the same way, too: 2^-17 of each weight, at no more MFMAs than one piece each.
+// Sums that are not finite are formed once more without pieces (walk_odd; 0.2 us of
+// every call go into its being there and into looking at the sums).
 #include <algorithm>
 #include <cmath>
 

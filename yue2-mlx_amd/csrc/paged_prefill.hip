@@ -27,7 +27,7 @@
 // A step computes S of the step after it beside its own exponentials, and P V
 // beside the scaling of those scores; K is therefore loaded a step ahead of V.
 // Measured, 24 heads of 8 at 3000 rows / 16 of 8 and a window of 1024, 5 sequences of
-// 411 to 5003 (us): this form 72 / 109 (770 / 650 TFLOP/s; 12000 rows 1080); 64 rows a
+// 411 to 5003 (us): this form 73 / 111 (760 / 640 TFLOP/s; 12000 rows 1080); 64 rows a
 // wave, one wave a SIMD, 106 / 155; 8 waves and four steps of LDS, one workgroup a CU,
 // 88 / 130; S and P V of the same step one after the other 103 / 155.
 //
@@ -36,9 +36,13 @@
 // they are scaled, fma(score, scale, -m), weights of scores past 2^24 are wrong; as
 // fast). It is raised only when a score passes it by more than kSlack (the weights,
 // up to 2^20, are as exact in 32 bits and in bf16 as smaller ones), so almost no
-// step rescales the 64 sums. P is rounded to bf16, half a step of 2^-8 of each weight,
-// as the output is: one product per operand instead of two; the denominator sums
-// the rounded weights.
+// step rescales the 64 sums.
+//
+// P is rounded to bf16, half a step of 2^-8 of each weight, as the output is; the
+// denominator sums the rounded weights. Whole calls are off by 0.0020-0.0022 of 64
+// bits' (2-norm), of which the output's rounding is 0.0017. P in two pieces leaves
+// that alone and takes 16 more products a step: 3000 rows 75 -> 95 us, 12000 rows
+// 821 -> 1101, the windowed prompts 108 -> 133, 97 rows after 4000 keys 28 -> 29.
 //
 // A prompt piece of few rows behind many keys has fewer tiles than CUs (runs_of):
 // there the workgroups take equal runs of all tiles' steps, leave the sums of tiles
@@ -86,7 +90,8 @@ struct PrefillParams {
 };
 
 constexpr int kRuns = 512;  // workgroups of a dealt launch, at most
-// Steps that beginning a tile costs (97 rows after 4000 keys 27.8 us; 1: 29.5, 5: 27.4).
+// Steps that beginning a tile costs (97 rows after 4000 keys / 400 after 3000: 27.2 /
+// 40.3 us; 1: 29.4 / 42.7, 5: 27.5 / 40.4).
 constexpr int kTileCost = 3;
 // Sequences of a dealt launch, at most: every workgroup walks them all. Short pieces
 // after 2000 and 3000 keys (us), dealt / whole tiles: 32 sequences 30.7 / 35.0 and
@@ -149,8 +154,8 @@ __device__ __forceinline__ Tile tile_of(const PrefillParams &p, const paged::Row
 
 // The work of a dealt launch in units, a step each and kTileCost for beginning a
 // tile: the units of a kv head are those of its tiles, sequence by sequence. Every
-// wave holds the (at most 64) sequences, one a lane, and walks their tiles 64 at
-// a time.
+// wave holds the (at most kDealSequences) sequences, one a lane, and walks their
+// tiles 64 at a time.
 template <int G> struct Deal {
   const PrefillParams &p;
   paged::Rows mine;  // of the lane's sequence
@@ -769,7 +774,7 @@ paged_prefill_deal_kernel(PrefillParams p, float qscale) {
 // per 32 rows and 32 dims, a wave per quarter of the pieces, its lanes as the
 // tile's held them. Every load of a round of pieces is issued before the first is
 // used: what costs here is the latency of one round after the other (a wave for
-// all pieces: one row after 4000 keys 22.8 us in all, else 17.6).
+// all pieces: one row after 4000 keys 22.8 us in all, else 18.3).
 template <int G>
 __global__ __launch_bounds__(256) void paged_prefill_join_kernel(PrefillParams p, float qscale) {
   __shared__ f32x4 sums[kWaves][4][64];
@@ -867,9 +872,12 @@ long long tiles_at_most(int batch, int rows, int group) {
 // tables hold, at most. A workgroup that shares its CU does a step in two thirds of
 // the time, but shares more tiles: two a CU from 8 steps a workgroup on. 24 heads of
 // 8, time of whole tiles / dealt over 256 / over 512 (us):
-//   200 rows after 0 keys 11.3 / 15.8 / 17.8    97 after 4000   64.8 / 26.7 / 28.7
-//   700 after 0           18.6 / 24.2 / 26.3    400 after 3000  57.1 / 41.9 / 38.3
-//   1000 after 0          24.4 / 31.9 / 29.9    1000 after 3000 71.6 / 79.2 / 66.5
+//   200 rows after 0 keys 11.0 / 14.7 / 16.7    97 after 4000   61.6 / 25.7 / 25.8
+//   700 after 0           17.4 / 23.5 / 25.7    400 after 3000  55.9 / 41.0 / 37.2
+//   1000 after 0          23.0 / 31.0 / 29.8    1000 after 3000 68.7 / 82.3 / 66.3
+// The tables' width stands for the keys, which the host does not know: in a table of
+// 24576 slots, 64 / 200 / 700 / 1000 rows from position 0 are dealt, and take 12.6 /
+// 17.1 / 26.1 / 30.3 instead of 8.0 / 11.2 / 17.9 / 23.2.
 int runs_of(const PrefillParams &p, long long tiles) {
   constexpr int kDealTiles = 256, kDealSteps = 8;
   if (p.batch > kDealSequences || tiles >= kDealTiles)

@@ -669,8 +669,8 @@ def paged_attention_prefill(q, k_pages, v_pages, table, starts, pos0, window=0, 
                             stream=None):
     """Causal attention of rows q [rows, heads, 128] over pages: sequence b owns
     rows starts[b] to starts[b + 1], at positions from pos0[b]; a row at p sees
-    the keys t <= p with p - t < window or t < sinks (window 0: all). See
-    yuear_op_paged_attention_prefill."""
+    the keys t <= p with p - t < window or t < sinks (window 0: all). Each weight
+    is rounded to bf16 once. See yuear_op_paged_attention_prefill."""
     name, index = "paged_attention_prefill", q.get_device()
     stream = _stream(stream, index, name, out, workspace)
     n, hkv, slots = _check_pages(k_pages, v_pages, index, name)
