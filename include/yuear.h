@@ -412,7 +412,9 @@ int32_t yuear_op_paged_append(const uint16_t *dev_qkv, int64_t qkv_stride,
  * p - t < window or t < sinks (window 0: every t <= p) that the table has;
  * fp32 scores q . K / sqrt(128) and sums, weights rounded once to bf16 (half a
  * step of 2^-8 of each; the contiguous prompt attention keeps them exact, and
- * the decode form 16 bits of them), bf16 out [rows] of heads * 128. Infinities and NaNs reach the rows that see their keys, no others. A row
+ * the decode form 16 bits of them), bf16 out [rows] of heads * 128. (Weights
+ * are up to 2^20 before the division: finite values past 2^93 may overflow the
+ * sums.) Infinities and NaNs reach the rows that see their keys, no others. A row
  * that sees no key gives zeros, one that sees scores of -inf alone NaNs; rows that the append leaves out for
  * their position in the table are left untouched here. workspace as below. */
 int32_t yuear_op_paged_attention_prefill(
