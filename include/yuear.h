@@ -492,6 +492,60 @@ yuear_status yuear_pages_table(yuear_pages *pool, const int32_t *sequences, int3
 /* Tokens of a sequence (-1: no such sequence); pages that nobody holds. */
 int32_t yuear_pages_length(yuear_pages *pool, int32_t sequence);
 int32_t yuear_pages_unused(yuear_pages *pool);
+/* ---- block-scaled 8- and 4-bit rows (no counterpart in the reference, whose
+ * low-bit forms are the affine ones of yuear_op_qgemv) ----
+ * The operands of the matrix cores' scaled products: a row of k values is k
+ * codes, in 8 bits (e4m3: up to 448) or 4 (e2m1: 0, 0.5, 1, 1.5, 2, 3, 4, 6 and
+ * their negatives, two to a byte, the first in the low half), and k / 32 scale
+ * bytes (e8m0), one per 32 values: value = code * 2^(scale - 127), a scale of 255
+ * makes its 32 values NaN. k is a multiple of 32 up to 2^20. Codes are 16-byte
+ * aligned, their rows `codes_stride` bytes apart (a multiple of 16), the scales'
+ * rows `scales_stride` bytes; bf16 rows are 16-byte aligned with strides (in
+ * elements) that are multiples of 8, except yuear_op_mx_gemm's. Strides are at
+ * most 2^22. Invalid arguments, and outputs that share memory with an input or
+ * each other where it is not said below, return hipErrorInvalidValue (1) and
+ * launch nothing; empty calls (rows, m or n 0) return 0. The entry points run on
+ * `stream` of the current device, allocate nothing and can be captured. */
+/* codes and scales of bf16 rows x [rows][k]. Of 32 values with the largest
+ * magnitude t: scale 2^e, e = max(floor(log2 t) - E, -127) with E 8 (8 bits) or 2
+ * (4 bits), -127 for zeros; codes x / 2^e rounded to the nearest, ties to even,
+ * at most 448 or 6 in magnitude. 32 values with an infinity or NaN among them get
+ * scale 255 and codes 0. */
+int32_t yuear_op_mx_quantize(const uint16_t *dev_x, int64_t x_stride, int32_t rows, int32_t k,
+                             int32_t bits, uint8_t *dev_codes, int64_t codes_stride,
+                             uint8_t *dev_scales, int64_t scales_stride, void *stream);
+/* out [rows][k] = bf16(code * 2^(scale - 127)): exact where bf16 has the value. */
+int32_t yuear_op_mx_dequantize(const uint8_t *dev_codes, int64_t codes_stride,
+                               const uint8_t *dev_scales, int64_t scales_stride, int32_t rows,
+                               int32_t k, int32_t bits, uint16_t *dev_out, int64_t out_stride,
+                               void *stream);
+/* The residual addition and RMSNorm before a projection, with their output
+ * quantised as above: sum = bf16(x + residual) (which may be the same memory as x
+ * or residual, with the same stride), y = sum / sqrt(mean(sum^2) + eps) * gain in
+ * 32 bits, codes and scales of y. Null residual and sum: y of x. k up to 16384,
+ * gain [k], rows below 2^23. */
+int32_t yuear_op_mx_rms_norm(const uint16_t *dev_x, int64_t x_stride,
+                             const uint16_t *dev_residual, int64_t residual_stride,
+                             const uint16_t *dev_gain, float eps, int32_t rows, int32_t k,
+                             int32_t bits, uint8_t *dev_codes, int64_t codes_stride,
+                             uint8_t *dev_scales, int64_t scales_stride, uint16_t *dev_sum,
+                             int64_t sum_stride, void *stream);
+/* C[m][n] = bf16(A[m] . W[n]), bf16(residual[m][n] + A[m] . W[n]) with a residual
+ * (which may be C, with its stride), or, with swiglu 1 (no residual, n even), on
+ * interleaved gate / up rows, C[m][i] = bf16(silu(g) * u), g / u = A[m] . W[2i] /
+ * W[2i+1]: one rounding each (yuear_op_gemm's residual and SwiGLU forms keep the
+ * reference's roundings in between). A [m][k] in 8 or 4 bits, W [n][k] in 4, k a
+ * multiple of 128, scales and their strides multiples of 4 bytes; products exact
+ * and sums fp32, but for this of the matrix cores' 8-bit form: of eight
+ * neighbouring products (k = 8 i .. 8 i + 7) the bits more than 13 below the
+ * largest one's leading bit are dropped. residual and C rows of any stride below
+ * 2^31. */
+int32_t yuear_op_mx_gemm(const uint8_t *dev_a, int64_t a_stride, const uint8_t *dev_a_scales,
+                         int64_t a_scales_stride, int32_t a_bits, const uint8_t *dev_w,
+                         int64_t w_stride, const uint8_t *dev_w_scales, int64_t w_scales_stride,
+                         int32_t m, int32_t n, int32_t k, const uint16_t *dev_residual,
+                         int64_t residual_stride, uint16_t *dev_c, int64_t ldc, int32_t swiglu,
+                         void *stream);
 /* RoPE cos/sin tables exactly as the engine builds them (host). */
 void yuear_rope_table(int32_t positions, int32_t head_dim, double theta,
                       uint16_t *cos_out, uint16_t *sin_out);

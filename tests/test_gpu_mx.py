@@ -1,0 +1,450 @@
+"""Block-scaled rows on the GPU against their 64-bit definition (mx_ref.py): codes
+and scales bit for bit, norms within the reach of 32-bit arithmetic, products
+within derived bounds, at the sizes, strides and values where they can go wrong."""
+import numpy as np
+import pytest
+
+import mx_ref as ref
+
+pytestmark = pytest.mark.gpu
+EPS = 1e-5
+
+
+@pytest.fixture(scope="module")
+def torch():
+    import torch as t
+    t.cuda.init()
+    return t
+
+
+def bf16(torch, bits):
+    return torch.from_numpy(np.ascontiguousarray(bits, np.uint16).view(np.int16)).cuda().view(torch.bfloat16)
+
+
+def bits_of(torch, t):
+    return t.contiguous().view(torch.int16).cpu().numpy().view(np.uint16)
+
+
+def raw(torch, t):
+    return t.view(torch.uint8).cpu().numpy()
+
+
+def random_rows(rng, rows, k, kind):
+    """bf16 bits [rows, k]: "wide" any finite pattern, "near" values within 2^-14 of their block's
+    largest, on and beside the codes' midpoints, "plain" normal with channels of unlike size."""
+    if kind == "wide":
+        return rng.integers(0, 1 << 16, (rows, k), dtype=np.uint16) & np.uint16(0xBFFF)
+    if kind == "near":
+        e = np.repeat(rng.integers(1, 254, (rows, k // 32)), 32, 1) - rng.integers(0, 15, (rows, k))
+        sign = rng.integers(0, 2, (rows, k)) << 15
+        mantissa = rng.choice(np.array([0, 1, 7, 8, 9, 24, 31, 32, 33, 40, 56, 64, 72, 95, 96, 97, 100, 127]), (rows, k))
+        return (sign | np.maximum(e, 0) << 7 | mantissa).astype(np.uint16)
+    return ref.to_bf16(rng.standard_normal((rows, k)) * np.exp(0.8 * rng.standard_normal(k)))
+
+
+def pair_in(torch, rows, k, bits, gap=0, fill=0x5A):
+    """A pair whose rows lie `gap` 16-byte pieces (scales: 4 bytes) apart in wider buffers."""
+    wide = torch.full((rows, k * bits // 8 + 16 * gap), fill, dtype=torch.uint8, device="cuda")
+    wide_s = torch.full((rows, k // 32 + 4 * gap), fill, dtype=torch.uint8, device="cuda")
+    codes, scales = wide[:, :k * bits // 8], wide_s[:, :k // 32]
+    if bits == 8:
+        codes = codes.view(torch.float8_e4m3fn)
+    return (codes, scales.view(torch.float8_e8m0fnu)), (wide, wide_s)
+
+
+def untouched(wides, k, bits, fill=0x5A):
+    return bool((wides[0][:, k * bits // 8:] == fill).all() and (wides[1][:, k // 32:] == fill).all())
+
+
+def pair_of(torch, stored, scales, bits):
+    codes = torch.from_numpy(np.ascontiguousarray(stored)).cuda()
+    if bits == 8:
+        codes = codes.view(torch.float8_e4m3fn)
+    return codes, torch.from_numpy(np.ascontiguousarray(scales)).cuda().view(torch.float8_e8m0fnu)
+
+
+# ---- quantise, dequantise ----
+
+@pytest.mark.parametrize("bits", [8, 4])
+@pytest.mark.parametrize("kind", ["wide", "near", "plain"])
+@pytest.mark.parametrize("rows,k,gap", [(1, 32, 0), (3, 96, 0), (257, 1056, 1), (1027, 32, 2), (37, 2048, 0), (2, 16384, 0)])
+def test_quantize_and_back(torch, yuear_lib, bits, kind, rows, k, gap):
+    rng = np.random.default_rng(rows * 31 + k + bits)
+    x = random_rows(rng, rows, k, kind)
+    t = bf16(torch, x)
+    if gap:
+        wide = torch.full((rows, k + 8 * gap), 7.0, dtype=torch.bfloat16, device="cuda")
+        wide[:, :k] = t
+        t = wide[:, :k]
+    out, wides = pair_in(torch, rows, k, bits, gap)
+    got = yuear_lib.mx_quantize(t, bits, out=out)
+    assert got[0].data_ptr() == out[0].data_ptr() and untouched(wides, k, bits)
+    codes, scales = ref.quantize(ref.from_bf16(x), bits)
+    np.testing.assert_array_equal(raw(torch, got[1].contiguous()), scales)
+    np.testing.assert_array_equal(raw(torch, got[0].contiguous()), codes)
+    back = torch.full((rows, k + 8 * gap), 9.0, dtype=torch.bfloat16, device="cuda")
+    yuear_lib.mx_dequantize(got, out=back[:, :k])
+    np.testing.assert_array_equal(bits_of(torch, back[:, :k]), ref.to_bf16(ref.values(codes, scales, bits)))
+    assert (back[:, k:] == 9).all()
+
+
+@pytest.mark.parametrize("bits", [8, 4])
+def test_quantize_every_bf16_value(torch, yuear_lib, bits):
+    """All finite patterns, each in a block of its own exponent, of one 4 and of one 13 above it; zeros."""
+    e = np.arange(255)[:, None, None]
+    m = np.arange(128)[None, :, None]
+    sign = np.arange(2)[None, None, :] << 15
+    v = (sign | e << 7 | m).reshape(255, 256).astype(np.uint16)
+    rows = []
+    for up in (0, 4, 13):
+        top = (np.minimum(np.arange(255) + up, 254) << 7).astype(np.uint16)
+        block = np.concatenate([v, np.zeros((255, 23), np.uint16)], 1).reshape(255, 9, 31)  # 31 values and the top
+        rows.append(np.concatenate([block, np.broadcast_to(top[:, None, None], (255, 9, 1))], 2).reshape(255, 288))
+    x = np.concatenate(rows + [np.zeros((1, 288), np.uint16), np.full((1, 288), 0x8000, np.uint16)])
+    got = yuear_lib.mx_quantize(bf16(torch, x), bits)
+    codes, scales = ref.quantize(ref.from_bf16(x), bits)
+    np.testing.assert_array_equal(raw(torch, got[1]), scales)
+    np.testing.assert_array_equal(raw(torch, got[0]), codes)
+
+
+@pytest.mark.parametrize("bits", [8, 4])
+def test_not_finite_blocks(torch, yuear_lib, bits):
+    """An infinity or NaN, wherever in its block, makes that block alone NaN."""
+    rng = np.random.default_rng(3)
+    x = random_rows(rng, 96, 96, "plain")
+    for i in range(96):
+        x[i, i] = (0x7F80, 0xFF80, 0x7FC0, 0xFFFF, 0x7F81)[i % 5]
+    got = yuear_lib.mx_quantize(bf16(torch, x), bits)
+    codes, scales = ref.quantize(ref.from_bf16(x), bits)
+    assert (scales == 255).sum() == 96
+    np.testing.assert_array_equal(raw(torch, got[1]), scales)
+    np.testing.assert_array_equal(raw(torch, got[0]), codes)
+    back = yuear_lib.mx_dequantize(got)
+    np.testing.assert_array_equal(torch.isnan(back).cpu().numpy(), np.repeat(scales == 255, 32, 1))
+
+
+@pytest.mark.parametrize("bits", [8, 4])
+def test_dequantize_every_code_and_scale(torch, yuear_lib, bits):
+    codes = np.tile(np.arange(256, dtype=np.uint8), 256 // (2 if bits == 4 else 1)).reshape(-1, 32 * bits // 8)
+    codes = np.repeat(codes[:16 if bits == 4 else 8], 256, 0)
+    scales = np.tile(np.arange(256, dtype=np.uint8), codes.shape[0] // 256)[:, None]
+    got = yuear_lib.mx_dequantize(pair_of(torch, codes, scales, bits))
+    want = ref.to_bf16(ref.values(codes, scales, bits))
+    g = bits_of(torch, got)
+    nan = (want & 0x7FFF) > 0x7F80
+    assert ((g & 0x7FFF) > 0x7F80)[nan].all()
+    np.testing.assert_array_equal(g[~nan], want[~nan])
+
+
+# ---- norm ----
+
+# Of y in 32 bits: the squares' sum (k / 256 additions in a lane, 8 across) and its root, quotient and two products,
+# each half a step of 2^-24 of the value, the sum's halved by the root: under (8192 / 256 * 8 + 24) * 2^-25 = 2^-16.9.
+NORM_FINE = 2.0 ** -16
+
+
+def check_norm(torch, got, h, gain, bits):
+    """codes of y = h / sqrt(mean h^2 + eps) gain, for some y within NORM_FINE of the exact one."""
+    y = h / np.sqrt((h ** 2).mean(-1, keepdims=True) + EPS) * gain
+    rows, k = y.shape
+    scales = raw(torch, got[1].contiguous())
+    top = np.abs(y).reshape(rows, -1, 32).max(-1)
+    low, high = ref.scale_bytes(top * (1 - NORM_FINE), bits), ref.scale_bytes(top * (1 + NORM_FINE), bits)
+    assert ((scales == low) | (scales == high)).all()
+    s = np.repeat(ref.power(scales), 32, 1)
+    codes = ref.unpack(raw(torch, got[0].contiguous()), bits)
+    a = np.abs(y) / s
+    low, high = ref.nearest(a * (1 - NORM_FINE), bits), ref.nearest(a * (1 + NORM_FINE), bits)
+    magnitude = codes & ((1 << (bits - 1)) - 1)
+    assert ((magnitude >= low) & (magnitude <= high)).all()
+    assert (magnitude == ref.nearest(a, bits)).mean() > 0.999
+    nonzero = y != 0
+    assert ((codes >> (bits - 1) != 0) == np.signbit(y))[nonzero].all()
+
+
+@pytest.mark.parametrize("rows,k,gap,bits,residual", [
+    (1, 32, 0, 8, True), (1, 3072, 0, 8, True), (7, 96, 1, 8, True), (5, 512, 0, 4, False), (9, 544, 0, 8, True),
+    (3, 2048, 2, 8, False), (4, 2080, 0, 8, True), (3, 4096, 1, 4, True), (2, 4128, 0, 8, True), (3, 8192, 0, 8, True),
+    (2, 8224, 0, 8, False), (3, 16384, 0, 8, True), (1030, 64, 0, 8, True), (300, 2048, 0, 8, True),
+])
+def test_norm(torch, yuear_lib, rows, k, gap, bits, residual):
+    rng = np.random.default_rng(rows + k)
+    x, r = random_rows(rng, rows, k, "plain"), random_rows(rng, rows, k, "plain")
+    gain = ref.to_bf16(1 + 0.2 * rng.standard_normal(k))
+    wide = torch.zeros(rows, k + 8 * gap, dtype=torch.bfloat16, device="cuda")
+    t = wide[:, :k]
+    t.copy_(bf16(torch, x))
+    total = torch.full((rows, k + 16), 5.0, dtype=torch.bfloat16, device="cuda")
+    out, wides = pair_in(torch, rows, k, bits, gap)
+    got, h = yuear_lib.mx_rms_norm(t, bf16(torch, gain), EPS, residual=bf16(torch, r) if residual else None, bits=bits,
+                                   out=out, sum_out=total[:, :k] if residual else None)
+    want = ref.from_bf16(x)
+    if residual:
+        want = ref.from_bf16(ref.to_bf16(want + ref.from_bf16(r)))
+        np.testing.assert_array_equal(ref.from_bf16(bits_of(torch, h)), want)
+        assert (total[:, k:] == 5).all()
+    else:
+        assert h is None and (total == 5).all()
+    assert untouched(wides, k, bits)
+    check_norm(torch, got, want, ref.from_bf16(gain), bits)
+
+
+def test_norm_in_place(torch, yuear_lib):
+    """The sum over the residual, and over x, give the same bits as apart."""
+    rng = np.random.default_rng(8)
+    x, r = (bf16(torch, random_rows(rng, 33, 1024, "plain")) for _ in range(2))
+    gain = bf16(torch, ref.to_bf16(1 + 0.1 * rng.standard_normal(1024)))
+    want, h = yuear_lib.mx_rms_norm(x, gain, residual=r)
+    for over in (0, 1):
+        a, b = x.clone(), r.clone()
+        got, s = yuear_lib.mx_rms_norm(a, gain, residual=b, sum_out=(a, b)[over])
+        assert s.data_ptr() == (a, b)[over].data_ptr() and torch.equal(s, h)
+        assert all(torch.equal(u.view(torch.uint8), v.view(torch.uint8)) for u, v in zip(got, want))
+
+
+def test_norm_rows_that_are_not_finite(torch, yuear_lib):
+    """An infinity or NaN spoils its row alone; a sum that overflows is one; zeros stay zeros."""
+    rng = np.random.default_rng(9)
+    x, r = random_rows(rng, 6, 256, "plain"), random_rows(rng, 6, 256, "plain")
+    x[1, 3], x[2, 200], x[4, 7], r[4, 7] = 0x7F80, 0x7FC0, 0x7F7F, 0x7F7F
+    x[5] = r[5] = 0
+    gain = bf16(torch, np.full(256, 0x3F80))
+    got, h = yuear_lib.mx_rms_norm(bf16(torch, x), gain, residual=bf16(torch, r))
+    scales, codes = raw(torch, got[1]), raw(torch, got[0])
+    # an infinity's row: inf * 0 in its own block is NaN, the other values are 0
+    assert scales[1, 0] == 255 and (codes[1, 32:] & 0x7F == 0).all() and torch.isinf(h[1, 3])
+    assert (scales[2] == 255).all() and scales[4, 0] == 255 and torch.isinf(h[4, 7])
+    assert not codes[5].any() and not scales[5].any()
+    sound = [0, 3]
+    check_norm(torch, (got[0][sound], got[1].view(torch.uint8)[sound].view(torch.float8_e8m0fnu)),
+               ref.from_bf16(bits_of(torch, h[sound])), np.ones(256), 8)
+
+
+# ---- product ----
+
+def random_pair(rng, rows, k, bits, kind="codes"):
+    """(stored codes, scales) of random codes with scales near 1, or of quantised normal rows."""
+    if kind == "codes":
+        n = 127 if bits == 8 else 8
+        c = rng.integers(0, n, (rows, k)).astype(np.uint8) | (rng.integers(0, 2, (rows, k)) << (bits - 1)).astype(np.uint8)
+        return ref.pack(c, bits), rng.integers(121, 132, (rows, k // 32)).astype(np.uint8)
+    return ref.quantize(rng.standard_normal((rows, k)) * np.exp(0.8 * rng.standard_normal(k)), bits)
+
+
+def check_gemm(torch, out, a, w, a_bits, epilogue, r=None):
+    y, off = ref.product(a, w, a_bits)
+    got = ref.from_bf16(bits_of(torch, out))
+    if epilogue == "residual":
+        y = y + r
+        off = off + 2.0 ** -24 * np.abs(y)
+    elif epilogue == "swiglu":
+        g, u = y[:, 0::2], y[:, 1::2]
+        dg, du = off[:, 0::2], off[:, 1::2]
+        sig = 1 / (1 + np.exp(-g))
+        y = g * sig * u
+        # |d silu| <= 1.1, exp and the quotient 2^-21 of the result (expf within 2 units, at |g| up to 88)
+        off = 1.1 * dg * np.abs(u) + (np.abs(g * sig) + 1.1 * dg) * du + 2.0 ** -20 * np.abs(y)
+    bound = (1 + ref.HALF_BF16) * off + ref.HALF_BF16 * np.abs(y) + 2.0 ** -133
+    err = np.abs(got - y)
+    assert (err <= bound).all(), f"{(err > bound).sum()} of {err.size} off, worst {np.nanmax(err / bound):.3g}"
+
+
+GEMMS = [
+    (1, 1, 128, 8, "store"), (1, 16, 128, 4, "store"), (1, 256, 1024, 8, "store"), (2, 50, 384, 8, "swiglu"),
+    (5, 33, 640, 4, "residual"), (8, 512, 512, 8, "swiglu"), (15, 17, 256, 8, "residual"), (16, 96, 896, 4, "swiglu"),
+    (17, 130, 128, 8, "store"), (31, 64, 1152, 8, "residual"), (32, 258, 256, 4, "store"), (33, 100, 512, 8, "swiglu"),
+    (48, 16, 2048, 8, "store"), (64, 192, 384, 8, "residual"), (65, 66, 768, 4, "swiglu"), (97, 301, 512, 8, "store"),
+    (128, 128, 256, 8, "swiglu"), (130, 257, 640, 4, "residual"), (197, 384, 1024, 8, "residual"),
+    (255, 510, 128, 8, "store"), (257, 514, 384, 8, "swiglu"), (300, 700, 256, 4, "store"), (513, 258, 128, 8, "residual"),
+    (1, 3, 8192, 8, "store"), (600, 130, 512, 4, "swiglu"), (1030, 520, 256, 8, "store"),
+]
+
+
+@pytest.mark.parametrize("m,n,k,bits,epilogue", GEMMS)
+@pytest.mark.parametrize("kind", ["codes", "quantised"])
+def test_gemm(torch, yuear_lib, m, n, k, bits, epilogue, kind):
+    rng = np.random.default_rng(m * 7 + n + k)
+    a, w = random_pair(rng, m, k, bits, kind), random_pair(rng, n, k, 4, kind)
+    width = n // 2 if epilogue == "swiglu" else n
+    wide = torch.full((m + 1, width + 3), 3.0, dtype=torch.bfloat16, device="cuda")
+    r = ref.to_bf16(4 * rng.standard_normal((m, n))) if epilogue == "residual" else None
+    out = yuear_lib.mx_gemm(pair_of(torch, *a, bits), pair_of(torch, *w, 4), swiglu=epilogue == "swiglu",
+                            residual=bf16(torch, r) if r is not None else None, out=wide[:m, :width])
+    assert out.data_ptr() == wide.data_ptr() and (wide[m:] == 3).all() and (wide[:, width:] == 3).all()
+    check_gemm(torch, out, ref.values(*a, bits), ref.values(*w, 4), bits, epilogue,
+               ref.from_bf16(r) if r is not None else None)
+
+
+@pytest.mark.parametrize("m,n,k,bits", [(3, 40, 256, 8), (70, 140, 384, 4), (300, 300, 256, 8)])
+def test_gemm_rows_apart(torch, yuear_lib, m, n, k, bits):
+    """Operands that are columns of wider buffers; what lies between their rows is NaN."""
+    rng = np.random.default_rng(k)
+    a, w = random_pair(rng, m, k, bits), random_pair(rng, n, k, 4)
+    pairs = []
+    for (codes, scales), b in ((a, bits), (w, 4)):
+        p, _ = pair_in(torch, codes.shape[0], k, b, 3, fill=0xFF)
+        p[0].view(torch.uint8).copy_(torch.from_numpy(codes))
+        p[1].view(torch.uint8).copy_(torch.from_numpy(scales))
+        pairs.append(p)
+    out = yuear_lib.mx_gemm(*pairs)
+    check_gemm(torch, out, ref.values(*a, bits), ref.values(*w, 4), bits, "store")
+    same = yuear_lib.mx_gemm(pair_of(torch, *a, bits), pair_of(torch, *w, 4))
+    assert torch.equal(out, same)
+
+
+@pytest.mark.parametrize("m", [3, 40, 300])
+def test_gemm_not_finite(torch, yuear_lib, m):
+    """NaN scales and NaN codes reach their rows and columns, nothing else. Sums past 2^128 are not finite:
+    infinities, or NaN where partial sums of either sign overflow."""
+    rng = np.random.default_rng(m)
+    n, k = 50, 512
+    a, w = random_pair(rng, m, k, 8), random_pair(rng, n, k, 4)
+    a[0][1, 100] = 0x7F
+    a[1][2, 15] = 255
+    w[1][7, 3] = 255
+    a[1][0], w[1][9] = 200, 200  # 2^73 each
+    out = yuear_lib.mx_gemm(pair_of(torch, *a, 8), pair_of(torch, *w, 4))
+    nan = torch.isnan(out).cpu().numpy()
+    want = np.zeros((m, n), bool)
+    want[1], want[2], want[:, 7] = True, True, True
+    assert not torch.isfinite(out[0, 9])
+    nan[0, 9] = False
+    np.testing.assert_array_equal(nan, want)
+    fine = np.ones((m, n), bool)
+    fine[0], fine[:, 9], fine[want] = False, False, False
+    rows, cols = [i for i in range(m) if i > 2], [j for j in range(n) if j not in (7, 9)]
+    if rows:
+        y, off = ref.product(ref.values(a[0][rows], a[1][rows], 8), ref.values(w[0][cols], w[1][cols], 4), 8)
+        got = ref.from_bf16(bits_of(torch, out))[np.ix_(rows, cols)]
+        assert (np.abs(got - y) <= ref.HALF_BF16 * np.abs(y) + (1 + ref.HALF_BF16) * off).all()
+
+
+def test_gemm_into_its_residual(torch, yuear_lib):
+    rng = np.random.default_rng(4)
+    for m in (2, 90, 400):
+        a, w = pair_of(torch, *random_pair(rng, m, 256, 8), 8), pair_of(torch, *random_pair(rng, 200, 256, 4), 4)
+        r = bf16(torch, ref.to_bf16(rng.standard_normal((m, 200))))
+        want = yuear_lib.mx_gemm(a, w, residual=r)
+        got = yuear_lib.mx_gemm(a, w, residual=r, out=r)
+        assert got is r and torch.equal(got, want)
+
+
+def test_refused_on_the_gpu(torch, yuear_lib):
+    x = torch.zeros(4, 128, dtype=torch.bfloat16, device="cuda")
+    a, w = yuear_lib.mx_quantize(x), yuear_lib.mx_quantize(x, 4)
+    other = yuear_lib.mx_quantize(torch.zeros(4, 256, dtype=torch.bfloat16, device="cuda"), 4)
+    for call in (
+            lambda: yuear_lib.mx_quantize(x.float()), lambda: yuear_lib.mx_quantize(x, 6),
+            lambda: yuear_lib.mx_quantize(x[:, :40]), lambda: yuear_lib.mx_quantize(x.T),
+            lambda: yuear_lib.mx_quantize(x[:, 4:100]), lambda: yuear_lib.mx_quantize(x, 4, out=a),
+            lambda: yuear_lib.mx_dequantize((a[0], a[1][:2])), lambda: yuear_lib.mx_dequantize((x, a[1])),
+            lambda: yuear_lib.mx_dequantize(a, out=x.float()), lambda: yuear_lib.mx_rms_norm(x, x[0, :64]),
+            lambda: yuear_lib.mx_rms_norm(x, x[0], sum_out=x), lambda: yuear_lib.mx_rms_norm(x, x[0], residual=x[:2]),
+            lambda: yuear_lib.mx_gemm(a, a), lambda: yuear_lib.mx_gemm(a, other), lambda: yuear_lib.mx_gemm(x, w),
+            lambda: yuear_lib.mx_gemm(a, w, residual=x), lambda: yuear_lib.mx_gemm(a, w, swiglu=True, residual=x),
+            lambda: yuear_lib.mx_gemm((a[0][:, :32], a[1][:, :1]), (w[0][:, :16], w[1][:, :1])),
+            lambda: yuear_lib.mx_quantize(x, stream=torch.cuda.Stream().cuda_stream),
+    ):
+        with pytest.raises((ValueError, TypeError)):
+            call()
+
+
+def test_empty(torch, yuear_lib):
+    x = torch.zeros(0, 128, dtype=torch.bfloat16, device="cuda")
+    gain = torch.ones(128, dtype=torch.bfloat16, device="cuda")
+    a = yuear_lib.mx_quantize(x)
+    w = yuear_lib.mx_quantize(torch.zeros(6, 128, dtype=torch.bfloat16, device="cuda"), 4)
+    assert yuear_lib.mx_dequantize(a).shape == (0, 128) and yuear_lib.mx_gemm(a, w).shape == (0, 6)
+    assert yuear_lib.mx_rms_norm(x, gain, residual=x)[1].shape == (0, 128)
+    some = yuear_lib.mx_quantize(torch.ones(3, 128, dtype=torch.bfloat16, device="cuda"))
+    assert yuear_lib.mx_gemm(some, (w[0][:0], w[1][:0])).shape == (3, 0)
+
+
+# ---- together ----
+
+def mlp(yuear_lib, x, stream, gain, w_up, w_down, **kw):
+    """A decoder layer's second half: norm of the sum, gate/up, down into the residual stream."""
+    a, h = yuear_lib.mx_rms_norm(x, gain, EPS, residual=stream)
+    y = yuear_lib.mx_gemm(a, w_up, swiglu=True)
+    return yuear_lib.mx_gemm(yuear_lib.mx_quantize(y), w_down, residual=h)
+
+
+def mlp_inputs(torch, rng, m, h=512, f=1024):
+    x, stream = (bf16(torch, random_rows(rng, m, h, "plain")) for _ in range(2))
+    gain = bf16(torch, ref.to_bf16(1 + 0.1 * rng.standard_normal(h)))
+    up = bf16(torch, ref.to_bf16(0.04 * rng.standard_normal((2 * f, h))))
+    down = bf16(torch, ref.to_bf16(0.04 * rng.standard_normal((h, f))))
+    return x, stream, gain, up, down
+
+
+@pytest.mark.parametrize("m", [1, 8, 70, 300])
+def test_mlp_together(torch, yuear_lib, m):
+    """The run of operators against the same steps in 64 bits, each from the one before as it was stored."""
+    rng = np.random.default_rng(m)
+    x, stream, gain, up, down = mlp_inputs(torch, rng, m)
+    w_up, w_down = yuear_lib.mx_quantize(up, 4), yuear_lib.mx_quantize(down, 4)
+    a, h = yuear_lib.mx_rms_norm(x, gain, EPS, residual=stream)
+    want_h = ref.from_bf16(ref.to_bf16(ref.from_bf16(bits_of(torch, x)) + ref.from_bf16(bits_of(torch, stream))))
+    np.testing.assert_array_equal(ref.from_bf16(bits_of(torch, h)), want_h)
+    check_norm(torch, a, want_h, ref.from_bf16(bits_of(torch, gain)), 8)
+
+    def held(pair, bits):
+        return ref.values(raw(torch, pair[0]), raw(torch, pair[1]), bits)
+
+    y = yuear_lib.mx_gemm(a, w_up, swiglu=True)
+    check_gemm(torch, y, held(a, 8), held(w_up, 4), 8, "swiglu")
+    q = yuear_lib.mx_quantize(y)
+    codes, scales = ref.quantize(ref.from_bf16(bits_of(torch, y)), 8)
+    np.testing.assert_array_equal(raw(torch, q[0]), codes)
+    np.testing.assert_array_equal(raw(torch, q[1]), scales)
+    out = yuear_lib.mx_gemm(q, w_down, residual=h)
+    check_gemm(torch, out, held(q, 8), held(w_down, 4), 8, "residual", want_h)
+    assert torch.equal(out, mlp(yuear_lib, x, stream, gain, w_up, w_down))
+
+
+@pytest.mark.parametrize("m", [2, 200])
+def test_captured_and_replayed(torch, yuear_lib, m):
+    """A captured run of them, replayed with eager work and other inputs between, gives the eager bits."""
+    rng = np.random.default_rng(11)
+    x, stream, gain, up, down = mlp_inputs(torch, rng, m)
+    w_up, w_down = yuear_lib.mx_quantize(up, 4), yuear_lib.mx_quantize(down, 4)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        mlp(yuear_lib, x, stream, gain, w_up, w_down)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = mlp(yuear_lib, x, stream, gain, w_up, w_down)
+    for i in range(4):
+        x.copy_(bf16(torch, random_rows(rng, m, 512, "plain")))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, mlp(yuear_lib, x, stream, gain, w_up, w_down))
+
+
+def test_two_streams_and_given_outputs(torch, yuear_lib):
+    """Calls on a given stream with given outputs, two streams at once, against calls in order."""
+    rng = np.random.default_rng(12)
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    w = yuear_lib.mx_quantize(bf16(torch, ref.to_bf16(rng.standard_normal((640, 512)))), 4)
+    gain = bf16(torch, np.full(512, 0x3F80))
+    rows = [bf16(torch, random_rows(rng, m, 512, "plain")) for m in (9, 150)]
+    want = [yuear_lib.mx_gemm(yuear_lib.mx_rms_norm(x, gain)[0], w) for x in rows]
+    outs = [(yuear_lib.mx_quantize(x), torch.empty(x.shape[0], 640, dtype=torch.bfloat16, device="cuda")) for x in rows]
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for st, x, (pair, out) in zip(streams, rows, outs):
+            yuear_lib.mx_rms_norm(x, gain, out=pair, stream=st.cuda_stream)
+            yuear_lib.mx_gemm(pair, w, out=out, stream=st.cuda_stream)
+    torch.cuda.synchronize()
+    assert all(torch.equal(out, y) for (_, out), y in zip(outs, want))
+
+
+def test_equal_calls_give_equal_bits(torch, yuear_lib):
+    rng = np.random.default_rng(13)
+    w = pair_of(torch, *random_pair(rng, 1000, 1024, 4), 4)
+    for m in (1, 20, 100, 500):
+        a = pair_of(torch, *random_pair(rng, m, 1024, 8), 8)
+        first = yuear_lib.mx_gemm(a, w)
+        assert all(torch.equal(first, yuear_lib.mx_gemm(a, w)) for _ in range(3))

@@ -192,6 +192,20 @@ _SIGS = {
             C.c_void_p, C.c_int32]),
     "yuear_pages_unused": (C.c_int32, [
             C.c_void_p]),
+    "yuear_op_mx_quantize": (C.c_int32, [
+            C.c_void_p, C.c_int64, C.c_int32, C.c_int32, C.c_int32, C.c_void_p, C.c_int64,
+            C.c_void_p, C.c_int64, C.c_void_p]),
+    "yuear_op_mx_dequantize": (C.c_int32, [
+            C.c_void_p, C.c_int64, C.c_void_p, C.c_int64, C.c_int32, C.c_int32, C.c_int32,
+            C.c_void_p, C.c_int64, C.c_void_p]),
+    "yuear_op_mx_rms_norm": (C.c_int32, [
+            C.c_void_p, C.c_int64, C.c_void_p, C.c_int64, C.c_void_p, C.c_float, C.c_int32,
+            C.c_int32, C.c_int32, C.c_void_p, C.c_int64, C.c_void_p, C.c_int64, C.c_void_p,
+            C.c_int64, C.c_void_p]),
+    "yuear_op_mx_gemm": (C.c_int32, [
+            C.c_void_p, C.c_int64, C.c_void_p, C.c_int64, C.c_int32, C.c_void_p, C.c_int64,
+            C.c_void_p, C.c_int64, C.c_int32, C.c_int32, C.c_int32, C.c_void_p, C.c_int64,
+            C.c_void_p, C.c_int64, C.c_int32, C.c_void_p]),
     "yuear_tokenizer_load": (C.c_int, [C.c_char_p, _P(C.c_void_p), _P(C.c_void_p)]),
     "yuear_tokenizer_destroy": (None, [C.c_void_p]),
     "yuear_tokenizer_encode": (C.c_int, [C.c_void_p, C.c_char_p, C.c_int64, _P(i32p),
@@ -485,14 +499,16 @@ def _hip_check(status, name):
 
 def _torch():
     """torch; the first call sets its types that the checks compare with."""
-    global _T, _BF16, _INT32
+    global _T, _BF16, _INT32, _UINT8, _E4M3, _E8M0
     if _T is None:
         import torch
-        _T, _BF16, _INT32 = torch, torch.bfloat16, torch.int32
+        _BF16, _INT32, _UINT8 = torch.bfloat16, torch.int32, torch.uint8
+        _E4M3, _E8M0 = torch.float8_e4m3fn, torch.float8_e8m0fnu
+        _T = torch
     return _T
 
 
-_T = _BF16 = _INT32 = None
+_T = _BF16 = _INT32 = _UINT8 = _E4M3 = _E8M0 = None
 _LAYOUT = ("pages are contiguous bfloat16 tensors on one device: k [pages, kv heads, slots, 128] and "
            "v [pages, kv heads, slots / 32, 128, 32]")
 
@@ -719,6 +735,138 @@ def paged_attention_decode(qkv, k_pages, v_pages, table, pos, cos, sin, q_norm=N
           cos.data_ptr(), sin.data_ptr(), positions, k_pages.data_ptr(), v_pages.data_ptr(), n, slots,
           table.data_ptr(), width, table_stride, pos.data_ptr(), batch, heads, hkv, window, sinks,
           workspace.data_ptr(), _workspace(workspace, index, name), out.data_ptr(), out_stride, stream)
+    return out
+
+
+# ---- block-scaled 8- and 4-bit rows: pairs (codes, scales) of tensors, codes
+# float8_e4m3fn [rows, k] or, in 4 bits, uint8 [rows, k / 2] (two to a byte, the
+# first in the low half), scales float8_e8m0fnu [rows, k / 32] ----
+
+_MX = ("block-scaled rows are (codes, scales) on one device: codes float8_e4m3fn [rows, k] or uint8 [rows, k / 2] "
+       "with whole rows, scales float8_e8m0fnu [rows, k / 32] with whole rows, k a multiple of 32")
+
+
+def _mx_rows(packed, index, name):
+    """(rows, k, bits, codes' address, row stride, scales' address, row stride) of a pair."""
+    codes, scales = packed
+    shape, ss = codes.shape, scales.shape
+    if len(shape) == 2 and len(ss) == 2 and scales.dtype is _E8M0:
+        dtype, k = codes.dtype, ss[1] * 32
+        bits = 8 if dtype is _E4M3 and shape[1] == k else 4 if dtype is _UINT8 and 2 * shape[1] == k else 0
+        rows = shape[0]
+        if bits and k and ss[0] == rows and codes.get_device() == index and scales.get_device() == index:
+            stride, scale_stride = codes.stride(), scales.stride()
+            if stride[1] == 1 and (scale_stride[1] == 1 or k == 32):
+                return (rows, k, bits, codes.data_ptr(), stride[0] if rows > 1 else shape[1], scales.data_ptr(),
+                        scale_stride[0] if rows > 1 else ss[1])
+    _refuse(name, _MX)
+
+
+def _mx_bf16(t, rows, k, index, name, what):
+    """Row stride of a bfloat16 tensor [rows, k]."""
+    if t.dtype is _BF16 and t.shape == (rows, k) and t.get_device() == index:
+        stride = t.stride()
+        if stride[1] == 1 or k == 1:
+            return stride[0] if rows > 1 else k
+    _refuse(name, f"{what} is bfloat16 [{rows}, {k}] with whole rows on the operands' device")
+
+
+def _mx_out(x, rows, k, bits, out, index, name):
+    """The given pair, or a new one, and its numbers."""
+    if out is None:
+        if bits == 8:
+            codes = _T.empty((rows, k), dtype=_E4M3, device=x.device)
+        elif bits == 4:
+            codes = _T.empty((rows, k // 2), dtype=_UINT8, device=x.device)
+        else:
+            _refuse(name, "bits is 8 or 4")
+        out = codes, _T.empty((rows, k // 32), dtype=_E8M0, device=x.device)
+    got = _mx_rows(out, index, name)
+    if got[:3] != (rows, k, bits):
+        _refuse(name, f"out is a pair of [{rows}, {k}] values in {bits} bits")
+    return out, got
+
+
+def _mx_shape(x, name):
+    """(rows, k) of what is quantised."""
+    shape = x.shape
+    if len(shape) != 2 or shape[1] % 32 or not shape[1]:
+        _refuse(name, "x is bfloat16 [rows, k] with k a multiple of 32")
+    return shape
+
+
+def mx_quantize(x, bits=8, out=None, stream=None):
+    """bfloat16 rows [rows, k] as a pair (codes, scales) in 8 or 4 bits, one scale
+    per 32 values. See yuear_op_mx_quantize."""
+    name, index = "mx_quantize", x.get_device()
+    stream = _stream(stream, index, name, out)
+    rows, k = _mx_shape(x, name)
+    x_stride = _mx_bf16(x, rows, k, index, name, "x")
+    out, (_, _, _, codes, stride, scales, scale_stride) = _mx_out(x, rows, k, bits, out, index, name)
+    _call(lib.yuear_op_mx_quantize, name, index, x.data_ptr(), x_stride, rows, k, bits, codes, stride, scales,
+          scale_stride, stream)
+    return out
+
+
+def mx_dequantize(packed, out=None, stream=None):
+    """The bfloat16 values [rows, k] of a pair (codes, scales). See yuear_op_mx_dequantize."""
+    name, index = "mx_dequantize", packed[0].get_device()
+    stream = _stream(stream, index, name, out)
+    rows, k, bits, codes, stride, scales, scale_stride = _mx_rows(packed, index, name)
+    if out is None:
+        out = _T.empty((rows, k), dtype=_BF16, device=packed[0].device)
+    out_stride = _mx_bf16(out, rows, k, index, name, "out")
+    _call(lib.yuear_op_mx_dequantize, name, index, codes, stride, scales, scale_stride, rows, k, bits, out.data_ptr(),
+          out_stride, stream)
+    return out
+
+
+def mx_rms_norm(x, gain, eps=1e-5, residual=None, bits=8, out=None, sum_out=None, stream=None):
+    """(pair, sum): RMSNorm of sum = bfloat16(x + residual) (of x and None without a
+    residual) times the gain [k], as a pair (codes, scales) in 8 or 4 bits. sum_out
+    may be x or residual. See yuear_op_mx_rms_norm."""
+    name, index = "mx_rms_norm", x.get_device()
+    stream = _stream(stream, index, name, out, *(() if residual is None else (sum_out,)))
+    rows, k = _mx_shape(x, name)
+    x_stride = _mx_bf16(x, rows, k, index, name, "x")
+    if not (gain.dtype is _BF16 and gain.shape == (k,) and gain.get_device() == index and gain.is_contiguous()):
+        _refuse(name, f"gain is contiguous bfloat16 [{k}] on the operands' device")
+    residual_at, residual_stride, sum_at, sum_stride = None, 0, None, 0
+    if residual is not None:
+        residual_at, residual_stride = residual.data_ptr(), _mx_bf16(residual, rows, k, index, name, "residual")
+        if sum_out is None:
+            sum_out = _T.empty((rows, k), dtype=_BF16, device=x.device)
+        sum_at, sum_stride = sum_out.data_ptr(), _mx_bf16(sum_out, rows, k, index, name, "sum_out")
+    elif sum_out is not None:
+        _refuse(name, "sum_out comes with a residual")
+    out, (_, _, _, codes, stride, scales, scale_stride) = _mx_out(x, rows, k, bits, out, index, name)
+    _call(lib.yuear_op_mx_rms_norm, name, index, x.data_ptr(), x_stride, residual_at, residual_stride, gain.data_ptr(),
+          eps, rows, k, bits, codes, stride, scales, scale_stride, sum_at, sum_stride, stream)
+    return out, sum_out
+
+
+def mx_gemm(a, w, residual=None, swiglu=False, out=None, stream=None):
+    """bfloat16 [m, n] products of pairs a [m, k] in 8 or 4 bits and w [n, k] in 4
+    bits, k a multiple of 128; plus a residual [m, n] (which out may be), or, with
+    swiglu, silu(gate) * up [m, n / 2] of w's interleaved gate and up rows. See
+    yuear_op_mx_gemm."""
+    name, index = "mx_gemm", a[0].get_device()
+    stream = _stream(stream, index, name, out)
+    m, k, a_bits, a_codes, a_stride, a_scales, a_scale_stride = _mx_rows(a, index, name)
+    n, wk, w_bits, w_codes, w_stride, w_scales, w_scale_stride = _mx_rows(w, index, name)
+    if wk != k or w_bits != 4 or k % 128:
+        _refuse(name, "w is a pair in 4 bits of rows as long as a's, k a multiple of 128")
+    if swiglu and (n % 2 or residual is not None):
+        _refuse(name, "swiglu takes an even number of rows of w and no residual")
+    width = n // 2 if swiglu else n
+    residual_at, residual_stride = None, 0
+    if residual is not None:
+        residual_at, residual_stride = residual.data_ptr(), _mx_bf16(residual, m, n, index, name, "residual")
+    if out is None:
+        out = _T.empty((m, width), dtype=_BF16, device=a[0].device)
+    ldc = _mx_bf16(out, m, width, index, name, "out")
+    _call(lib.yuear_op_mx_gemm, name, index, a_codes, a_stride, a_scales, a_scale_stride, a_bits, w_codes, w_stride,
+          w_scales, w_scale_stride, m, n, k, residual_at, residual_stride, out.data_ptr(), ldc, 1 if swiglu else 0, stream)
     return out
 
 
