@@ -1,6 +1,9 @@
 // C[m][n] = bf16(epilogue(sum_k A[m][k] W[n][k])) of rows with a scale per 32
 // values (mx.h): activations in 8 or 4 bits, weights in 4, on gfx950's scaled
 // MFMA, 128 of K at a time with sums in fp32.
+#include <algorithm>
+#include <type_traits>
+
 #include "kernels.h"
 #include "mx.h"
 
@@ -34,8 +37,16 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_rsrc(const uint8_t *base,
   return __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t *>(base), 0, int(n), 0x00020000);
 }
 
+// silu(gate) * up with e^-gate as 2^t, t = -gate log2 e: what rounding takes off t, up
+// to 2^-18 of the result where gate is large, is given back in the first order (and
+// kept small where gate is past all exponents). expf and a division made a third of
+// the SwiGLU tiles' time past the last product.
 __device__ __forceinline__ float silu_times(float gate, float up) {
-  return gate / (1.0f + expf(-gate)) * up;
+  constexpr float kLog2e = 1.44269502f, kRest = 1.92596299e-8f;  // log2 e in two parts
+  const float t = gate * -kLog2e;
+  const float off = __builtin_amdgcn_fmed3f(fmaf(gate, -kLog2e, -t) - gate * kRest, -1.f, 1.f);
+  const float s = __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(t));
+  return gate * fmaf(s * (s - 1.0f), off * 0.693147182f, s) * up;
 }
 
 // A lane's features n .. n + 3 (n a multiple of 4) of token row m < p.m.
@@ -62,13 +73,23 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
   return uint32_t(f2bf(lo)) | uint32_t(f2bf(hi)) << 16;
 }
 
+// What finish32() adds, read ahead of it.
+__device__ __forceinline__ void residual32(const GemmArgs &p, int m, int n, int h,
+                                           u32x4 (&residual)[2]) {
+  if (!p.wide || n + 32 > p.n || m >= p.m)
+    return;
+  const uint16_t *r = p.residual + m * p.residual_stride + n + 16 * h;
+  residual[0] = *reinterpret_cast<const u32x4 *>(r);
+  residual[1] = *reinterpret_cast<const u32x4 *>(r + 8);
+}
+
 // A 32 x 32 MFMA tile, lane 32 h + r with features n + 8 q + 4 h + [0, 4) of token m
 // at v[4 q ..]. Where the rows allow it (p.wide, whole tile) the lanes of a token
 // trade halves first, so that each stores 16 bytes: h = 0 the features (SwiGLU
 // outputs) below 16 (8), h = 1 the others.
 template <int EPI>
 __device__ __forceinline__ void finish32(const GemmArgs &p, int m, int n, int h,
-                                         const float (&v)[16]) {
+                                         const float (&v)[16], const u32x4 (&residual)[2]) {
   if (!p.wide || n + 32 > p.n) {
     if (m < p.m)
 #pragma unroll
@@ -108,7 +129,7 @@ __device__ __forceinline__ void finish32(const GemmArgs &p, int m, int n, int h,
       x[4 + e] = bits_f32(f[8 + 4 * q + e]);
     }
     if (EPI == kResidual) {
-      const u32x4 r = *reinterpret_cast<const u32x4 *>(p.residual + m * p.residual_stride + at);
+      const u32x4 r = residual[q];
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         x[2 * e] += bflo(r[e]);
@@ -214,27 +235,30 @@ __global__ __launch_bounds__(KW * 64) void rows_kernel(GemmArgs p) {
 
 // ---- many token rows: tiles through LDS ----
 //
-// A workgroup of WM x WN waves computes a BM x BN tile of C, each wave BM / WM
-// tokens by BN / WN features as 32 x 32 MFMA tiles, 64 of K at a time. K advances
-// by steps of 128 bytes of each A row (128 of K in 8 bits, 256 in 4) through a
-// two-stage LDS ring that direct-to-LDS loads fill (1 KiB an instruction). The
-// operands of the next 64 of K are read from LDS under the MFMAs of these. One
-// barrier a step, before its last 64: past it every wave has read all of the
-// stage, which takes the step after the next, and the next step's loads have
-// landed.
+// A workgroup of WM x WN waves computes BM x BN tiles of C, each wave BM / WM tokens
+// by BN / WN features as 32 x 32 MFMA tiles, 64 of K at a time. K advances by steps
+// of KSTEP through a ring of LDS stages that direct-to-LDS loads fill (1 KiB an
+// instruction). The operands of the next 64 of K are read from LDS under the MFMAs
+// of these. One barrier a step, before its last 64: past it every wave has read all
+// of the stage, which takes the step that the ring has room for, and the next step's
+// loads have landed.
 //
-// Scales come 512 of K at a time, 16 bytes a row, into two buffers behind the
-// ring; a lane reads the byte of its row and k-block.
+// There is a workgroup for each CU, which takes one tile after another, and the ring
+// does not stop between them: the last steps of a tile load the first ones of the
+// next, whose products go on while this one's results are on their way to memory.
 //
-// MFMA operands, lane l = 32 h + r: W (4 bits) row r, k 32 h .. 32 h + 31 of the
-// 64, the same of A in 4 bits; A in 8 bits k 16 h .. 16 h + 15 and 32 + 16 h ..; the
-// scale of k-block h of row r. D: features 8 q + 4 h + [0, 4) of token r.
+// Scales come 512 of K (a group) at a time, 16 bytes a row, into two buffers behind
+// the ring, a group in use and the one after it; a lane reads the bytes of its row
+// and step and shifts them so that k-block h of each 64 is at byte 0 or 2.
 //
-// LDS rows of 128 bytes (A, and W beside 4-bit A) keep their 16-byte chunk c at
-// slot c ^ (row >> 1 & 7); rows of 64 bytes (W beside 8-bit A) at c ^ (bit 2 of the
-// row | bit 4 << 1). A ds_read_b128 is served 16 lanes at a time (bit 5 of the
-// lane, and bit 3 ^ bit 4): rows 0-7 and 24-31, or 8-23, with one chunk, which
-// either layout spreads over all 16 slots of 256 bytes.
+// MFMA operands, lane l = 32 h + r: in 4 bits row r, k 32 h .. 32 h + 31 of the 64;
+// in 8 bits k 16 h .. 16 h + 15 and 32 + 16 h ..; the scale of k-block h of row r.
+// D: features 8 q + 4 h + [0, 4) of token r.
+//
+// LDS rows of 128 bytes keep their 16-byte chunk c at slot c ^ (row >> 1 & 7), rows
+// of 64 bytes at c ^ (bit 2 of the row | bit 4 << 1). A ds_read_b128 is served 16
+// lanes at a time (bit 5 of the lane, and bit 3 ^ bit 4): rows 0-7 and 24-31, or
+// 8-23, with one chunk, which either layout spreads over all 16 slots of 256 bytes.
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef __attribute__((address_space(3))) void *lds_ptr_t;
 
@@ -242,229 +266,368 @@ typedef __attribute__((address_space(3))) void *lds_ptr_t;
 // stage from the reads of the other.
 extern __shared__ __attribute__((aligned(1024))) char mx_lds[];
 
-template <int ABITS, int BM, int BN, int WM, int WN> struct Tile {
-  static constexpr int kWaves = WM * WN;
-  static constexpr int kWRow = ABITS == 8 ? 64 : 128;    // bytes of a W row a step
-  static constexpr int kStepK = ABITS == 8 ? 128 : 256;  // K of a step
-  static constexpr int kStage = BM * 128 + BN * kWRow;
-  static constexpr int kScales = (BM + BN) * 16;         // of 512 of K
-  static constexpr int kLds = 2 * kStage + 2 * kScales;
+constexpr int kGroupK = 512;  // K of a group of scales
+
+template <int ABITS, int BM, int BN, int WM, int WN, int KSTEP, int STAGES> struct Tile {
+  static constexpr int kWaves = WM * WN, kBM = BM, kBN = BN;
+  static constexpr int kARow = KSTEP * ABITS / 8, kWRow = KSTEP / 2;  // bytes of a row a step
+  static constexpr int kStage = BM * kARow + BN * kWRow;
+  static constexpr int kScales = (BM + BN) * 16;
+  static constexpr int kStages = STAGES;
+  static constexpr int kLds = kStages * kStage + 2 * kScales;
+  static_assert(kLds <= 160 * 1024, "LDS");
 };
 
-// Tile of workgroup b. Workgroups go to the 8 XCDs in turn, each with its own L2:
-// XCD x takes one contiguous range of an order in columns of four tile rows, so
-// that the tiles that share an L2 form a compact block of A and W rows.
-__device__ __forceinline__ void tile_of(int b, int tiles_m, int tiles_n, int &tm, int &tn) {
+// Tiles of workgroup b of `grid` (a multiple of 8): the n-th, counted from 0. Workgroups
+// go to the 8 XCDs in turn, each with its own L2: XCD x takes one contiguous range of
+// an order in columns of four tile rows, so that the tiles that share an L2 form a
+// compact block of A and W rows.
+__device__ __forceinline__ bool tile_of(int b, int grid, int n, int tiles_m, int tiles_n, int &tm,
+                                        int &tn) {
   constexpr int kXcds = 8, kGroup = 4;
   const int total = tiles_m * tiles_n, each = total / kXcds, more = total % kXcds;
-  const int x = b % kXcds;
-  const int t = x * each + min(x, more) + b / kXcds;
+  const int x = b % kXcds, at = b / kXcds + n * (grid / kXcds);
+  if (at >= each + (x < more))
+    return false;
+  const int t = x * each + min(x, more) + at;
   const int per = kGroup * tiles_n, first = t / per * kGroup;
   const int rows = min(tiles_m - first, kGroup), r = t % per;
   tm = first + r % rows;
   tn = r / rows;
+  return true;
 }
 
-__device__ __forceinline__ int slot128(int row, int chunk) { return chunk ^ ((row >> 1) & 7); }
-__device__ __forceinline__ int slot64(int row, int chunk) {
-  return chunk ^ (((row >> 2) & 1) | ((row >> 3) & 2));
+__device__ __forceinline__ int slot_of(int bytes, int row, int chunk) {
+  return bytes == 128 ? chunk ^ ((row >> 1) & 7) : chunk ^ (((row >> 2) & 1) | ((row >> 3) & 2));
 }
 
-template <int ABITS, int EPI, int BM, int BN, int WM, int WN>
+// s_waitcnt for all but the last `loads` vector memory operations, and every LDS read.
+constexpr int waitcnt(int loads) { return (loads & 15) | (loads >> 4) << 14 | 0x0070; }
+// The workgroup's barrier, after the wave's LDS reads and, from step FROM on, all but the last
+// LOADS of its vector memory operations. (__syncthreads() would wait for every load into LDS,
+// those of the steps ahead too. The branch is in the assembly so that a step stays one block for
+// the scheduler.)
+template <int LOADS, int FROM> __device__ __forceinline__ void wait_and_meet(int step) {
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_sched_barrier(0);
+  asm volatile("s_cmp_lt_i32 %0, %2\n\t"
+               "s_cbranch_scc1 .Lmeet%=\n\t"
+               "s_waitcnt vmcnt(%1)\n"
+               ".Lmeet%=:" ::"s"(__builtin_amdgcn_readfirstlane(step)), "n"(LOADS), "n"(FROM)
+               : "scc", "memory");
+  __builtin_amdgcn_s_waitcnt(waitcnt(63));
+  __builtin_amdgcn_s_barrier();
+  __builtin_amdgcn_sched_barrier(0);
+  asm volatile("" ::: "memory");
+}
+
+// What a wave loads of a tile: its rows of A, of W, and its blocks of scales.
+template <int SPW> struct Source {
+  const uint8_t *a, *w, *s[SPW];
+  int a_bytes, w_bytes, s_bytes[SPW];  // past which nothing is read
+};
+__device__ __forceinline__ int range(int64_t stride, int rows, int bytes) {
+  return int((rows - 1) * stride + bytes);
+}
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t rsrc(const uint8_t *base, int bytes) {
+  return __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t *>(base), 0, bytes, 0x00020000);
+}
+
+// With k up to 512 (fewer than two groups of scales) loads could reach past the next
+// tile: the launch gives each workgroup one tile then, and they read nothing.
+template <int ABITS, int EPI, int BM, int BN, int WM, int WN, int KSTEP, int STAGES>
 __device__ __forceinline__ void tile(const GemmArgs &p) {
-  using T = Tile<ABITS, BM, BN, WM, WN>;
-  constexpr int TM = BM / WM / 32, TN = BN / WN / 32;
-  constexpr int AQ = ABITS / 4;            // 16-byte pieces of A of a lane and 64 of K
-  constexpr int PARTS = T::kStepK / 64;
-  constexpr int APW = BM / 8 / T::kWaves, WPW = BN * T::kWRow / 1024 / T::kWaves;
-  constexpr int kGroupSteps = 512 / T::kStepK;
-  static_assert(APW * T::kWaves * 8 == BM && WPW * T::kWaves * 1024 == BN * T::kWRow &&
-                    TM * 32 * WM == BM && TN * 32 * WN == BN,
+  using T = Tile<ABITS, BM, BN, WM, WN, KSTEP, STAGES>;
+  constexpr int TM = BM / WM / 32, TN = BN / WN / 32, PARTS = KSTEP / 64;
+  constexpr int kGroupSteps = kGroupK / KSTEP;
+  constexpr int AQ = ABITS / 4;  // 16-byte pieces of A of a lane and 64 of K
+  constexpr int APW = BM * T::kARow / 1024 / T::kWaves, WPW = BN * T::kWRow / 1024 / T::kWaves;
+  constexpr int SB = (BM + BN) / 64, SPW = (SB + T::kWaves - 1) / T::kWaves;  // blocks of scales
+  static_assert(APW * T::kWaves * 1024 == BM * T::kARow && WPW * T::kWaves * 1024 == BN * T::kWRow &&
+                    TM * 32 * WM == BM && TN * 32 * WN == BN && BM % 64 == 0 && BN % 64 == 0 &&
+                    (STAGES == 2 || STAGES == 3) && kGroupSteps >= 2,
                 "tile");
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wm = wave / WN, wn = wave % WN;
   const int r = lane & 31, h = lane >> 5;
-  int tm, tn;
-  tile_of(int(blockIdx.x), (p.m + BM - 1) / BM, (p.n + BN - 1) / BN, tm, tn);
-  const int m0 = tm * BM, n0 = tn * BN;
-  const int rows_a = min(p.m - m0, BM), rows_w = min(p.n - n0, BN);
-  const auto ra = rows_rsrc(p.a + m0 * p.a_stride, p.a_stride, rows_a, p.k * ABITS / 8);
-  const auto rw = rows_rsrc(p.w + n0 * p.w_stride, p.w_stride, rows_w, p.k / 2);
+  const int tiles_m = (p.m + BM - 1) / BM, tiles_n = (p.n + BN - 1) / BN;
 
-  // this wave's KiB blocks of A and of W: lane l fills slot l
-  uint32_t from_a[APW], from_w[WPW];
+  // this wave's KiB blocks of a stage's A and W: lane l fills slot l
+  // (blocks two apart have their rows' slots alike: 16 rows of 128 bytes, 32 of 64)
+  constexpr int kARows = 1024 / T::kARow, kWRows = 1024 / T::kWRow;  // of a block
+  static_assert(APW % 2 == 0 && WPW % 2 == 0, "pairs of blocks");
+  uint32_t from_a[2], from_w[2], from_s[SPW];
 #pragma unroll
-  for (int i = 0; i < APW; ++i) {
-    const int row = 8 * (wave * APW + i) + (lane >> 3);
-    from_a[i] = uint32_t(row * int(p.a_stride) + slot128(row, lane & 7) * 16);
+  for (int i = 0; i < 2; ++i) {
+    const int ar = kARows * (wave * APW + i) + lane / (64 / kARows);
+    from_a[i] = uint32_t(ar * int(p.a_stride) + slot_of(T::kARow, ar, lane % (64 / kARows)) * 16);
+    const int wr = kWRows * (wave * WPW + i) + lane / (64 / kWRows);
+    from_w[i] = uint32_t(wr * int(p.w_stride) + slot_of(T::kWRow, wr, lane % (64 / kWRows)) * 16);
   }
+  // 64 rows of scales a block, A's first; waves past the last block repeat it
+  auto block = [&](int i) { return min(wave + i * T::kWaves, SB - 1); };
 #pragma unroll
-  for (int i = 0; i < WPW; ++i) {
-    constexpr int kRows = 1024 / T::kWRow;
-    const int row = kRows * (wave * WPW + i) + lane / (64 / kRows);
-    from_w[i] = uint32_t(row * int(p.w_stride) +
-                         (T::kWRow == 64 ? slot64(row, lane & 3) : slot128(row, lane & 7)) * 16);
+  for (int i = 0; i < SPW; ++i) {
+    const bool is_a = block(i) < BM / 64;
+    from_s[i] = uint32_t((64 * (is_a ? block(i) : block(i) - BM / 64) + lane) *
+                         int(is_a ? p.a_scale_stride : p.w_scale_stride));
   }
-  auto load = [&](int step) {
-    char *stage = mx_lds + (step & 1) * T::kStage;
+  auto source = [&](int m0, int n0) {
+    const int rows_a = min(p.m - m0, BM), rows_w = min(p.n - n0, BN);
+    Source<SPW> s;
+    s.a = p.a + m0 * p.a_stride;
+    s.w = p.w + n0 * p.w_stride;
+    s.a_bytes = range(p.a_stride, rows_a, p.k * ABITS / 8);
+    s.w_bytes = range(p.w_stride, rows_w, p.k / 2);
+#pragma unroll
+    for (int i = 0; i < SPW; ++i) {
+      const bool is_a = block(i) < BM / 64;
+      s.s[i] = is_a ? p.a_scales + m0 * p.a_scale_stride : p.w_scales + n0 * p.w_scale_stride;
+      s.s_bytes[i] = is_a ? range(p.a_scale_stride, rows_a, p.k / 32)
+                          : range(p.w_scale_stride, rows_w, p.k / 32);
+    }
+    return s;
+  };
+
+  int tm, tn;
+  if (!tile_of(int(blockIdx.x), int(gridDim.x), 0, tiles_m, tiles_n, tm, tn))
+    return;
+  int m0 = tm * BM, n0 = tn * BN;
+  Source<SPW> now = source(m0, n0), then = now;
+
+  const int steps = p.k / KSTEP, groups = (p.k + kGroupK - 1) / kGroupK;
+  // step `step` of this tile, or step - steps of the next, into the stage that begins at `stage`
+  auto load = [&](int stage, int step) {
+    const bool here = step < steps;
+    const int at = here ? step : step - steps;
+    const auto ra = rsrc(here ? now.a : then.a, here ? now.a_bytes : then.a_bytes);
+    const auto rw = rsrc(here ? now.w : then.w, here ? now.w_bytes : then.w_bytes);
 #pragma unroll
     for (int i = 0; i < APW; ++i)
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(ra, (lds_ptr_t)(stage + (wave * APW + i) * 1024), 16,
-                                               from_a[i] + step * 128, 0, 0, 0);
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(
+          ra, (lds_ptr_t)(mx_lds + stage + (wave * APW + i) * 1024), 16,
+          from_a[i & 1] + (at * T::kARow + (i & ~1) * kARows * int(p.a_stride)), 0, 0, 0);
 #pragma unroll
     for (int i = 0; i < WPW; ++i)
       __builtin_amdgcn_raw_ptr_buffer_load_lds(
-          rw, (lds_ptr_t)(stage + BM * 128 + (wave * WPW + i) * 1024), 16,
-          from_w[i] + step * T::kWRow, 0, 0, 0);
+          rw, (lds_ptr_t)(mx_lds + stage + BM * T::kARow + (wave * WPW + i) * 1024), 16,
+          from_w[i & 1] + (at * T::kWRow + (i & ~1) * kWRows * int(p.w_stride)), 0, 0, 0);
   };
-  // 64 rows of scales a wave, A's first; waves past the last block repeat it
-  constexpr int SB = (BM + BN) / 64;
-  static_assert(SB <= T::kWaves && BM % 64 == 0, "scale blocks");
-  const int sb = min(wave, SB - 1);
-  const bool sb_a = sb < BM / 64;
-  const auto rs = rows_rsrc(sb_a ? p.a_scales + m0 * p.a_scale_stride : p.w_scales + n0 * p.w_scale_stride,
-                            sb_a ? p.a_scale_stride : p.w_scale_stride, sb_a ? rows_a : rows_w, p.k / 32);
-  const uint32_t from_s = uint32_t((64 * (sb_a ? sb : sb - BM / 64) + lane) *
-                                   int(sb_a ? p.a_scale_stride : p.w_scale_stride));
+  constexpr int kScalesAt = T::kStages * T::kStage;
+  int odd = 0;  // the buffer of this tile's first group
   auto load_scales = [&](int group) {
-    __builtin_amdgcn_raw_ptr_buffer_load_lds(
-        rs, (lds_ptr_t)(mx_lds + 2 * T::kStage + (group & 1) * T::kScales + sb * 1024), 16,
-        from_s + group * 16, 0, 0, 0);
+    const bool here = group < groups;
+    const int at = here ? group : group - groups;
+#pragma unroll
+    for (int i = 0; i < SPW; ++i)
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(
+          rsrc(here ? now.s[i] : then.s[i], here ? now.s_bytes[i] : then.s_bytes[i]),
+          (lds_ptr_t)(mx_lds + kScalesAt + ((group + odd) & 1) * T::kScales + block(i) * 1024), 16,
+          from_s[i] + at * 16, 0, 0, 0);
   };
 
+  const int a_row = wm * (BM / WM) + r, w_row = wn * (BN / WN) + r;  // of the first MFMA tiles
   f32x16 acc[TM][TN];
-#pragma unroll
-  for (int i = 0; i < TM; ++i)
-#pragma unroll
-    for (int j = 0; j < TN; ++j)
-#pragma unroll
-      for (int e = 0; e < 16; ++e)
-        acc[i][j][e] = 0.f;
-
-  const int a_row = wm * (BM / WM) + r, w_row = wn * (BN / WN) + r;  // of the first tiles
   u32x4 af[2][TM][AQ], wf[2][TN];
-  int as[2][TM], ws[2][TN];
-  // operands of part s of a step (64 of K), from the stage and scale buffers that hold it
-  auto read = [&](int buf, int step, int s) {
-    const char *a = mx_lds + (step & 1) * T::kStage + a_row * 128;
-    const char *w = mx_lds + (step & 1) * T::kStage + BM * 128 + w_row * T::kWRow;
-    const int at = PARTS * step + s;
-    const uint8_t *sc = reinterpret_cast<const uint8_t *>(mx_lds) + 2 * T::kStage +
-                        (at >> 3 & 1) * T::kScales + 2 * (at & 7) + h;
+  constexpr int SW = PARTS / 2;  // 4-byte words of a row's scales a step
+  int as[SW][TM], ws[SW][TN], as_next[SW][TM], ws_next[SW][TN];
+  // operands of part s of a step from its stage
+  auto read = [&](int stage, int s) {
+    const char *a = mx_lds + stage + a_row * T::kARow;
+    const char *w = mx_lds + stage + BM * T::kARow + w_row * T::kWRow;
 #pragma unroll
     for (int x = 0; x < (TM > TN ? TM : TN); ++x) {
-      if (x < TN) {
-        wf[buf][x] = *reinterpret_cast<const u32x4 *>(
-            w + x * 32 * T::kWRow +
-            (T::kWRow == 64 ? slot64(r, 2 * s + h) : slot128(r, 2 * s + h)) * 16);
-        ws[buf][x] = sc[(BM + w_row + 32 * x) * 16];
-      }
-      if (x < TM) {
+      if (x < TN)
+        wf[s & 1][x] = *reinterpret_cast<const u32x4 *>(w + x * 32 * T::kWRow +
+                                                        slot_of(T::kWRow, r, 2 * s + h) * 16);
+      if (x < TM)
 #pragma unroll
         for (int q = 0; q < AQ; ++q)
-          af[buf][x][q] = *reinterpret_cast<const u32x4 *>(
-              a + x * 32 * 128 + slot128(r, (ABITS == 8 ? 4 * s + 2 * q : 2 * s) + h) * 16);
-        as[buf][x] = sc[(a_row + 32 * x) * 16];
-      }
+          af[s & 1][x][q] = *reinterpret_cast<const u32x4 *>(
+              a + x * 32 * T::kARow +
+              slot_of(T::kARow, r, (ABITS == 8 ? 4 * s + 2 * q : 2 * s) + h) * 16);
     }
   };
-  auto multiply = [&](int buf) {
+  // scales of step `at` of the group in buffer `buffer`
+  auto read_scales = [&](int buffer, int at) {
+    const char *sc = mx_lds + kScalesAt + buffer * T::kScales + at * (KSTEP / 32);
+#pragma unroll
+    for (int x = 0; x < TN; ++x)
+#pragma unroll
+      for (int e = 0; e < SW; ++e)
+        ws_next[e][x] = *reinterpret_cast<const int *>(sc + (BM + w_row + 32 * x) * 16 + 4 * e);
+#pragma unroll
+    for (int x = 0; x < TM; ++x)
+#pragma unroll
+      for (int e = 0; e < SW; ++e)
+        as_next[e][x] = *reinterpret_cast<const int *>(sc + (a_row + 32 * x) * 16 + 4 * e);
+  };
+  auto take_scales = [&] {
+#pragma unroll
+    for (int e = 0; e < SW; ++e) {
+#pragma unroll
+      for (int x = 0; x < TN; ++x)
+        ws[e][x] = int(uint32_t(ws_next[e][x]) >> (8 * h));
+#pragma unroll
+      for (int x = 0; x < TM; ++x)
+        as[e][x] = int(uint32_t(as_next[e][x]) >> (8 * h));
+    }
+  };
+  auto multiply = [&](auto part) {
+    constexpr int s = decltype(part)::value, e = s / 2, byte = 2 * (s & 1);
 #pragma unroll
     for (int i = 0; i < TM; ++i)
 #pragma unroll
       for (int j = 0; j < TN; ++j) {
-        const u32x4 w = wf[buf][j], lo = af[buf][i][0], hi = af[buf][i][AQ - 1];
+        const u32x4 w = wf[s & 1][j], lo = af[s & 1][i][0], hi = af[s & 1][i][AQ - 1];
         const i32x8 wv = {int(w.x), int(w.y), int(w.z), int(w.w), 0, 0, 0, 0};
         const i32x8 av = {int(lo.x), int(lo.y), int(lo.z), int(lo.w),
                           int(hi.x), int(hi.y), int(hi.z), int(hi.w)};
         acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(
-            wv, av, acc[i][j], 4, ABITS == 8 ? 0 : 4, 0, ws[buf][j], 0, as[buf][i]);
+            wv, av, acc[i][j], 4, ABITS == 8 ? 0 : 4, byte, ws[e][j], byte, as[e][i]);
       }
   };
 
-  // Step `step`, whose last barrier lets the ring take step + 2 and, at the end of a group of
-  // scales, their buffer the next but one. Reads and loads go between the MFMAs.
-  constexpr int kReads = TN + TM * AQ + TM + TN, kMfmas = TM * TN;
-  auto advance = [&](int step, int s_last) {
-#pragma unroll
-    for (int s = 0; s + 1 < PARTS; ++s) {
-      read((s + 1) & 1, step, s + 1);
-      multiply(s & 1);
+  // A step, with the next one's stage at `next` and scales at (buffer, at). Past its barrier the
+  // ring takes step + STAGES, and, where the step ends a group, that group's buffer the group
+  // after the next. Reads and loads go between the MFMAs.
+  constexpr int kReads = TN + TM * AQ, kScaleReads = SW * (TM + TN), kMfmas = TM * TN,
+                kLoads = APW + WPW, kHalf = kMfmas / 2;
+  auto advance = [&](auto ends, int stage, int next, int step, int buffer, int at, int group) {
+    auto part = [&](auto s) {
+      read(stage, s + 1);
+      multiply(s);
 #pragma unroll
       for (int x = 0; x < kMfmas; ++x) {
         __builtin_amdgcn_sched_group_barrier(0x100, (kReads + kMfmas - 1) / kMfmas, 0);
         __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
       }
       __builtin_amdgcn_sched_barrier(0);
+    };
+    part(std::integral_constant<int, 0>());
+    if constexpr (PARTS == 4) {
+      part(std::integral_constant<int, 1>());
+      part(std::integral_constant<int, 2>());
     }
-    __builtin_amdgcn_s_waitcnt(0);
-    __syncthreads();
-    __builtin_amdgcn_sched_barrier(0);
-    read(0, step + 1, 0);
-    load(step + 2);
-    if (s_last)
-      load_scales(step / kGroupSteps + 2);
-    multiply(1);
+    // (a tile's first steps find theirs waited for below, or in the prologue)
+    wait_and_meet<(STAGES - 2) * kLoads, STAGES - 1>(step);
+    read(next, 0);
+    read_scales(buffer, at);
+    if constexpr (decltype(ends)::value)
+      load_scales(group + 2);
+    load(stage, step + STAGES);
+    multiply(std::integral_constant<int, PARTS - 1>());
 #pragma unroll
     for (int x = 0; x < kMfmas; ++x) {
-      if (x < kMfmas / 2)
-        __builtin_amdgcn_sched_group_barrier(0x100, (kReads + kMfmas / 2 - 1) / (kMfmas / 2), 0);
+      if (x < kHalf)
+        __builtin_amdgcn_sched_group_barrier(0x100, (kReads + kScaleReads + kHalf - 1) / kHalf, 0);
       else
-        __builtin_amdgcn_sched_group_barrier(0x020, (APW + WPW + 1 + kMfmas / 2 - 1) / (kMfmas / 2), 0);
+        __builtin_amdgcn_sched_group_barrier(0x020, (kLoads + SPW + kHalf - 1) / kHalf, 0);
       __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
     }
     __builtin_amdgcn_sched_barrier(0);
+    take_scales();
   };
-  const int steps = p.k / T::kStepK;
-  load(0);
+  using Ends = std::true_type;
+  using Goes = std::false_type;
+
   load_scales(0);
   load_scales(1);
-  __builtin_amdgcn_s_waitcnt(0);  // (a barrier waits for no global load)
-  load(1);                        // past K, here and below: read by nobody
-  __syncthreads();
-  read(0, 0, 0);
-  int step = 0;
-  for (; step + kGroupSteps <= steps; step += kGroupSteps)
 #pragma unroll
-    for (int s = 0; s < kGroupSteps; ++s)
-      advance(step + s, s == kGroupSteps - 1);
-  for (; step < steps; ++step)
-    advance(step, 0);
-  if (p.k % T::kStepK) {  // 4 bits: an odd number of 128s leaves half of a step
-    read(1, step, 1);
-    multiply(0);
-    multiply(1);
-  }
-  __builtin_amdgcn_s_waitcnt(0);  // loads past K still in flight
+  for (int s = 0; s < STAGES; ++s)
+    load(s * T::kStage, s);
+  wait_and_meet<0, 0>(0);
+  read(0, 0);
+  read_scales(0, 0);
+  take_scales();
+  int stage = 0;
+  auto after = [](int at) { return at + T::kStage == STAGES * T::kStage ? 0 : at + T::kStage; };
 
+  for (int turn = 1;; ++turn) {
+    const bool more = tile_of(int(blockIdx.x), int(gridDim.x), turn, tiles_m, tiles_n, tm, tn);
+    then = source(more ? tm * BM : m0, more ? tn * BN : n0);
+    if (!more) {
+      then.a_bytes = then.w_bytes = 0;
 #pragma unroll
-  for (int i = 0; i < TM; ++i)
-#pragma unroll
-    for (int j = 0; j < TN; ++j) {
-      float v[16];
-#pragma unroll
-      for (int e = 0; e < 16; ++e)
-        v[e] = acc[i][j][e];
-      finish32<EPI>(p, m0 + a_row + 32 * i, n0 + wn * (BN / WN) + 32 * j, h, v);
+      for (int i = 0; i < SPW; ++i)
+        then.s_bytes[i] = 0;
     }
+#pragma unroll
+    for (int i = 0; i < TM; ++i)
+#pragma unroll
+      for (int j = 0; j < TN; ++j)
+#pragma unroll
+        for (int e = 0; e < 16; ++e)
+          acc[i][j][e] = 0.f;
+
+    auto one = [&](auto ends, int step, int s, int g) {  // step s of group g
+      const int next = after(stage);
+      const bool last = s == kGroupSteps - 1 || step == steps - 1;
+      advance(ends, stage, next, step, (last ? g + 1 + odd : g + odd) & 1, last ? 0 : s + 1, g);
+      stage = next;
+    };
+    int step = 0, g = 0;
+    for (; step + kGroupSteps <= steps; step += kGroupSteps, ++g)
+#pragma unroll
+      for (int s = 0; s < kGroupSteps; ++s) {
+        if (s == kGroupSteps - 1)
+          one(Ends(), step + s, s, g);
+        else
+          one(Goes(), step + s, s, g);
+      }
+    if (step < steps) {
+      int s = 0;
+      for (; step + 1 < steps; ++step, ++s)
+        one(Goes(), step, s, g);
+      one(Ends(), step, s, g);
+    }
+
+    // the loads of the next tile's first steps, before this one's stores queue up behind them
+    __builtin_amdgcn_s_waitcnt(waitcnt(0) | 0x0f00);
+#pragma unroll
+    for (int i = 0; i < TM; ++i) {
+      const int m = m0 + a_row + 32 * i, n = n0 + wn * (BN / WN);
+      u32x4 residual[2][2];  // of this tile and the next
+      if (EPI == kResidual)
+        residual32(p, m, n, h, residual[0]);
+#pragma unroll
+      for (int j = 0; j < TN; ++j) {
+        if (EPI == kResidual && j + 1 < TN)
+          residual32(p, m, n + 32 * (j + 1), h, residual[(j + 1) & 1]);
+        float v[16];
+#pragma unroll
+        for (int e = 0; e < 16; ++e)
+          v[e] = acc[i][j][e];
+        finish32<EPI>(p, m, n + 32 * j, h, v, residual[j & 1]);
+      }
+    }
+    if (!more)
+      break;
+    odd = (odd + groups) & 1;
+    m0 = tm * BM;
+    n0 = tn * BN;
+    now = then;
+  }
 }
 
-template <int ABITS, int EPI, int BM, int BN, int WM, int WN>
-__global__ __launch_bounds__(WM * WN * 64) void tile_kernel(GemmArgs p) {
-  tile<ABITS, EPI, BM, BN, WM, WN>(p);
+template <int ABITS, int EPI, int BM, int BN, int WM, int WN, int KSTEP, int STAGES>
+__global__ __launch_bounds__(WM * WN * 64, 2) void tile_kernel(GemmArgs p) {
+  tile<ABITS, EPI, BM, BN, WM, WN, KSTEP, STAGES>(p);
 }
 
 template <class T>
-hipError_t launch_tile(void (*kernel)(GemmArgs), int bm, int bn, const GemmArgs &p, hipStream_t s) {
-  const int64_t tiles = ((int64_t(p.m) + bm - 1) / bm) * ((int64_t(p.n) + bn - 1) / bn);
-  if (tiles * T::kWaves * 64 >= int64_t(1) << 32)
+hipError_t launch_tile(void (*kernel)(GemmArgs), const GemmArgs &p, hipStream_t s) {
+  const int64_t tiles = ((int64_t(p.m) + T::kBM - 1) / T::kBM) * ((int64_t(p.n) + T::kBN - 1) / T::kBN);
+  if (tiles >= int64_t(1) << 22)  // threads of the grid count in 32 bits
     return hipErrorInvalidValue;
   const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void *>(kernel),
                                            hipFuncAttributeMaxDynamicSharedMemorySize, T::kLds);
   if (e != hipSuccess)
     return e;
-  hipLaunchKernelGGL(kernel, dim3(unsigned(tiles)), dim3(T::kWaves * 64), T::kLds, s, p);
+  const int64_t all = (tiles + 7) / 8 * 8, cus = std::max(gemm_cus() / 8 * 8, 8);
+  const unsigned grid = unsigned(p.k > kGroupK ? std::min(cus, all) : all);
+  hipLaunchKernelGGL(kernel, dim3(grid), dim3(T::kWaves * 64), T::kLds, s, p);
   return hipGetLastError();
 }
 
@@ -480,7 +643,14 @@ template <int ABITS, int EPI> hipError_t launch_form(const GemmArgs &p, hipStrea
     return go(rows_kernel<ABITS, EPI, 1, 1, 4>, 1, 1, 4);
   if (p.m <= 512)
     return go(rows_kernel<ABITS, EPI, 4, 4, 4>, 4, 4, 4);
-  return launch_tile<Tile<ABITS, 256, 256, 4, 2>>(tile_kernel<ABITS, EPI, 256, 256, 4, 2>, 256, 256, p, s);
+#define YUEAR_MX_TILE(...)                                                                 \
+  launch_tile<Tile<ABITS, __VA_ARGS__>>(tile_kernel<ABITS, EPI, __VA_ARGS__>, p, s)
+  if constexpr (ABITS == 4) {
+    if (p.k % 256 == 0)
+      return YUEAR_MX_TILE(256, 256, 4, 2, 256, 2);
+  }
+  return YUEAR_MX_TILE(256, 256, 4, 2, 128, 3);
+#undef YUEAR_MX_TILE
 }
 
 template <int ABITS> hipError_t launch(const GemmArgs &p, hipStream_t s) {
