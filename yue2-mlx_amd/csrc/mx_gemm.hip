@@ -141,91 +141,136 @@ __device__ __forceinline__ void finish32(const GemmArgs &p, int m, int n, int h,
   }
 }
 
-// Few token rows: a workgroup computes 16 FT features of 16 MT tokens, its KW
-// waves a part of K each with all operands straight from memory into registers,
-// then adds the waves' sums in order.
+// ---- few token rows ----
 //
-// MFMA operands, lane l = 16 g + r: W (4 bits) row r, k 32 g .. 32 g + 31 of the
-// step, the same of A in 4 bits; A in 8 bits k 16 g .. 16 g + 15 and 64 + 16 g ..;
-// the scale of k-block g of row r in either case. D: features 4 g .. 4 g + 3 of
-// token r.
-template <int ABITS, int EPI, int MT, int FT, int KW>
-__global__ __launch_bounds__(KW * 64) void rows_kernel(GemmArgs p) {
-  constexpr int AQ = ABITS / 4;  // 16-byte pieces of A of a lane and step
-  constexpr int kBatch = 4;      // steps whose loads go out together
-  __shared__ f32x4 sums[KW][FT * MT][64];
+// A workgroup computes 16 FT features of up to 16 MT tokens, its waves 512 of K each
+// (and the next 512 that no wave has, where K is longer), then adds the waves' sums in
+// order. A wave brings its rows into an LDS region of its own by direct-to-LDS loads,
+// 1 KiB of whole 256- or 512-byte row pieces an instruction, and reads them back as
+// MFMA operands: no barrier before the sums. (Operands loaded straight into registers
+// have neighbouring lanes in different rows: some 55 cycles a load instead of 16, and
+// 137 MB of weights in 35 to 45 us.)
+//
+// 16 x 16 x 128 MFMAs, lane l = 16 g + r: row r; W and 4-bit A k 32 g .. 32 g + 31 of the
+// 128, 8-bit A k 16 g .. 16 g + 15 and 64 + 16 g ..; the scale of k-block g. D: features
+// 4 g .. 4 g + 3 of token r. Rows of A past m are not loaded: what the region holds there
+// reaches only their own, unwritten, tokens.
+//
+// The 16-byte chunk c of a row is at slot c ^ (row & 15) within 256 bytes: the 16 rows
+// that a ds_read_b128 serves at a time, with one chunk of two neighbours, lie in 16
+// different slots.
+typedef __attribute__((address_space(3))) void *lds_ptr_t;
+
+// The kernels' only LDS object, so that the compiler tells the loads into one
+// place from the reads of another.
+extern __shared__ __attribute__((aligned(1024))) char mx_lds[];
+
+constexpr int kSliceK = 512;
+// Bytes of a wave's region: pieces of W and A, then their scales.
+template <int ABITS, int FT> constexpr int region(int a_rows) {
+  return 16 * FT * (kSliceK / 2 + 16) + a_rows * (kSliceK * ABITS / 8 + 16);
+}
+
+template <int ABITS, int EPI, int MT, int FT>
+__global__ __launch_bounds__(1024) void rows_kernel(GemmArgs p, int a_rows) {
+  constexpr int AQ = ABITS / 4;              // 16-byte pieces of A of a lane and MFMA
+  constexpr int kARow = kSliceK * ABITS / 8;  // bytes of an A row's piece
+  constexpr int kWAt = 0, kAAt = 16 * FT * (kSliceK / 2);
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int waves = int(blockDim.x) >> 6;
   const int r = lane & 15, g = lane >> 4;
   const int n0 = int(blockIdx.x) * (16 * FT), m0 = int(blockIdx.y) * (16 * MT);
-  const auto ra = rows_rsrc(p.a + m0 * p.a_stride, p.a_stride, min(p.m - m0, 16 * MT), p.k * ABITS / 8);
-  const auto rw = rows_rsrc(p.w + n0 * p.w_stride, p.w_stride, min(p.n - n0, 16 * FT), p.k / 2);
-  const auto rsa =
-      rows_rsrc(p.a_scales + m0 * p.a_scale_stride, p.a_scale_stride,
-                             min(p.m - m0, 16 * MT), p.k / 32);
-  const auto rsw =
-      rows_rsrc(p.w_scales + n0 * p.w_scale_stride, p.w_scale_stride,
-                             min(p.n - n0, 16 * FT), p.k / 32);
-  const int steps = p.k / kStep;
-  const int begin = steps * wave / KW, end = steps * (wave + 1) / KW;
+  const int rows_a = min(p.m - m0, a_rows), rows_w = min(p.n - n0, 16 * FT);
+  const auto ra = rows_rsrc(p.a + m0 * p.a_stride, p.a_stride, rows_a, p.k * ABITS / 8);
+  const auto rw = rows_rsrc(p.w + n0 * p.w_stride, p.w_stride, rows_w, p.k / 2);
+  const auto rsa = rows_rsrc(p.a_scales + m0 * p.a_scale_stride, p.a_scale_stride, rows_a, p.k / 32);
+  const auto rsw = rows_rsrc(p.w_scales + n0 * p.w_scale_stride, p.w_scale_stride, rows_w, p.k / 32);
+  char *const mine = mx_lds + wave * region<ABITS, FT>(a_rows);
+  char *const w_scales = mine + kAAt + a_rows * kARow, *const a_scales = w_scales + 16 * FT * 16;
+
   f32x4 acc[FT][MT];
 #pragma unroll
   for (int f = 0; f < FT; ++f)
 #pragma unroll
     for (int t = 0; t < MT; ++t)
       acc[f][t] = f32x4{0.f, 0.f, 0.f, 0.f};
-  for (int s = begin; s < end; s += kBatch) {
-    u32x4 w[FT][kBatch], a[MT][kBatch][AQ], ws[FT], as[MT];
+  for (int k0 = wave * kSliceK; k0 < p.k; k0 += waves * kSliceK) {
+    // (what lies past K in a piece belongs to other rows, and is not used)
 #pragma unroll
-    for (int f = 0; f < FT; ++f) {
-      const int row = 16 * f + r;
-      ws[f] = __builtin_amdgcn_raw_buffer_load_b128(rsw, row * int(p.w_scale_stride) + 4 * s, 0, 0);
-#pragma unroll
-      for (int j = 0; j < kBatch; ++j)
-        w[f][j] = __builtin_amdgcn_raw_buffer_load_b128(
-            rw, row * int(p.w_stride) + (s + j) * (kStep / 2) + 16 * g, 0, 0);
+    for (int i = 0; i < 4 * FT; ++i) {
+      const int row = 4 * i + (lane >> 4);
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(
+          rw, (lds_ptr_t)(mine + kWAt + i * 1024), 16,
+          row * int(p.w_stride) + k0 / 2 + ((lane & 15) ^ (row & 15)) * 16, 0, 0, 0);
     }
+    for (int i = 0; i < a_rows * kARow / 1024; ++i) {
+      constexpr int kSlots = kARow / 16;
+      const int row = 64 / kSlots * i + lane / kSlots, slot = lane % kSlots;
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(
+          ra, (lds_ptr_t)(mine + kAAt + i * 1024), 16,
+          row * int(p.a_stride) + k0 * ABITS / 8 + (slot ^ (row & 15)) * 16, 0, 0, 0);
+    }
+    if (lane < 16 * FT)
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(rsw, (lds_ptr_t)w_scales, 16,
+                                               lane * int(p.w_scale_stride) + k0 / 32, 0, 0, 0);
+    if (lane < a_rows)
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(rsa, (lds_ptr_t)a_scales, 16,
+                                               lane * int(p.a_scale_stride) + k0 / 32, 0, 0, 0);
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_waitcnt(0x0f70);  // the wave's own loads: nobody else reads them
+    asm volatile("" ::: "memory");
+    u32x4 ws[FT], as[MT];
 #pragma unroll
-    for (int t = 0; t < MT; ++t) {
-      const int row = 16 * t + r;
-      as[t] = __builtin_amdgcn_raw_buffer_load_b128(rsa, row * int(p.a_scale_stride) + 4 * s, 0, 0);
+    for (int f = 0; f < FT; ++f)
+      ws[f] = *reinterpret_cast<const u32x4 *>(w_scales + (16 * f + r) * 16);
 #pragma unroll
-      for (int j = 0; j < kBatch; ++j)
+    for (int t = 0; t < MT; ++t)
+      as[t] = *reinterpret_cast<const u32x4 *>(a_scales + min(16 * t + r, a_rows - 1) * 16);
+#pragma unroll
+    for (int s = 0; s < kSliceK / kStep; ++s) {
+      if (k0 + s * kStep >= p.k)
+        break;
+      u32x4 w[FT], a[MT][AQ];
+#pragma unroll
+      for (int f = 0; f < FT; ++f)
+        w[f] = *reinterpret_cast<const u32x4 *>(mine + kWAt + (16 * f + r) * (kSliceK / 2) +
+                                                ((4 * s + g) ^ r) * 16);
+#pragma unroll
+      for (int t = 0; t < MT; ++t)
 #pragma unroll
         for (int q = 0; q < AQ; ++q)
-          a[t][j][q] = __builtin_amdgcn_raw_buffer_load_b128(
-              ra, row * int(p.a_stride) + (s + j) * (kStep * ABITS / 8) + 64 * q + 16 * g, 0, 0);
-    }
-#pragma unroll
-    for (int j = 0; j < kBatch; ++j) {
-      if (s + j >= end)  // what was read past the wave's part counts for nothing
-        break;
+          a[t][q] = *reinterpret_cast<const u32x4 *>(
+              mine + kAAt + min(16 * t + r, a_rows - 1) * kARow +
+              ((ABITS == 8 ? 8 * s + 4 * q + g : 4 * s + g) ^ r) * 16);
 #pragma unroll
       for (int f = 0; f < FT; ++f)
 #pragma unroll
         for (int t = 0; t < MT; ++t) {
-          const u32x4 lo = a[t][j][0], hi = a[t][j][AQ - 1];
-          const i32x8 wv = {int(w[f][j].x), int(w[f][j].y), int(w[f][j].z), int(w[f][j].w), 0, 0, 0, 0};
+          const u32x4 lo = a[t][0], hi = a[t][AQ - 1];
+          const i32x8 wv = {int(w[f].x), int(w[f].y), int(w[f].z), int(w[f].w), 0, 0, 0, 0};
           const i32x8 av = {int(lo.x), int(lo.y), int(lo.z), int(lo.w),
                             int(hi.x), int(hi.y), int(hi.z), int(hi.w)};
           acc[f][t] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(
-              wv, av, acc[f][t], 4, ABITS == 8 ? 0 : 4, 0, int(ws[f][j] >> (8 * g)), 0,
-              int(as[t][j] >> (8 * g)));
+              wv, av, acc[f][t], 4, ABITS == 8 ? 0 : 4, 0, int(ws[f][s] >> (8 * g)), 0,
+              int(as[t][s] >> (8 * g)));
         }
     }
+    __builtin_amdgcn_s_waitcnt(0xc07f);  // every read, before the next loads
+    asm volatile("" ::: "memory");
   }
+  f32x4 *const sums = reinterpret_cast<f32x4 *>(mine);  // the region's pieces are used up
 #pragma unroll
   for (int f = 0; f < FT; ++f)
 #pragma unroll
     for (int t = 0; t < MT; ++t)
-      sums[wave][f * MT + t][lane] = acc[f][t];
+      sums[(f * MT + t) * 64 + lane] = acc[f][t];
   __syncthreads();
-  for (int i = threadIdx.x; i < FT * MT * 64; i += KW * 64) {
+  for (int i = threadIdx.x; i < FT * MT * 64; i += int(blockDim.x)) {
     const int tile = i >> 6, l = i & 63;
-    f32x4 sum = sums[0][tile][l];
-#pragma unroll
-    for (int q = 1; q < KW; ++q)
-      sum += sums[q][tile][l];
+    f32x4 sum = {0.f, 0.f, 0.f, 0.f};
+    for (int q = 0; q < waves; ++q)
+      sum += *reinterpret_cast<const f32x4 *>(mx_lds + q * region<ABITS, FT>(a_rows) + i * 16);
     const int m = m0 + 16 * (tile % MT) + (l & 15), n = n0 + 16 * (tile / MT) + 4 * (l >> 4);
     const float v[4] = {sum[0], sum[1], sum[2], sum[3]};
     if (m < p.m)
@@ -260,11 +305,6 @@ __global__ __launch_bounds__(KW * 64) void rows_kernel(GemmArgs p) {
 // lanes at a time (bit 5 of the lane, and bit 3 ^ bit 4): rows 0-7 and 24-31, or
 // 8-23, with one chunk, which either layout spreads over all 16 slots of 256 bytes.
 typedef float f32x16 __attribute__((ext_vector_type(16)));
-typedef __attribute__((address_space(3))) void *lds_ptr_t;
-
-// The kernel's only LDS object, so that the compiler tells the loads into one
-// stage from the reads of the other.
-extern __shared__ __attribute__((aligned(1024))) char mx_lds[];
 
 constexpr int kGroupK = 512;  // K of a group of scales
 
@@ -631,18 +671,33 @@ hipError_t launch_tile(void (*kernel)(GemmArgs), const GemmArgs &p, hipStream_t 
   return hipGetLastError();
 }
 
+template <int ABITS, int MT, int FT>
+hipError_t launch_rows(void (*kernel)(GemmArgs, int), const GemmArgs &p, hipStream_t s) {
+  const int64_t x = (int64_t(p.n) + 16 * FT - 1) / (16 * FT), y = (int64_t(p.m) + 16 * MT - 1) / (16 * MT);
+  if (x >= int64_t(1) << 22 || y > 65535)  // threads of the grid count in 32 bits
+    return hipErrorInvalidValue;
+  // whole KiB of A's rows; at least the sums fit a region
+  const int per_kib = 1024 / (kSliceK * ABITS / 8), rows = std::min(p.m, 16 * MT);
+  const int a_rows = (rows + per_kib - 1) / per_kib * per_kib;
+  const int bytes = region<ABITS, FT>(a_rows);
+  static_assert(16 * FT * (kSliceK / 2) >= 1024 * FT * MT, "sums");
+  const int waves = std::min({(p.k + kSliceK - 1) / kSliceK, 160 * 1024 / bytes, 16});
+  const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void *>(kernel),
+                                           hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024);
+  if (e != hipSuccess)
+    return e;
+  hipLaunchKernelGGL(kernel, dim3(unsigned(x), unsigned(y)), dim3(unsigned(waves * 64)), waves * bytes, s, p,
+                     a_rows);
+  return hipGetLastError();
+}
+
 template <int ABITS, int EPI> hipError_t launch_form(const GemmArgs &p, hipStream_t s) {
-  auto go = [&](auto kernel, int mt, int ft, int kw) {
-    const int64_t x = (int64_t(p.n) + 16 * ft - 1) / (16 * ft), y = (int64_t(p.m) + 16 * mt - 1) / (16 * mt);
-    if (x * kw * 64 >= int64_t(1) << 32 || y > 65535)
-      return hipErrorInvalidValue;
-    hipLaunchKernelGGL(kernel, dim3(unsigned(x), unsigned(y)), dim3(unsigned(kw * 64)), 0, s, p);
-    return hipGetLastError();
-  };
+#define YUEAR_MX_ROWS(MT, FT) launch_rows<ABITS, MT, FT>(rows_kernel<ABITS, EPI, MT, FT>, p, s)
   if (p.m <= 16)
-    return go(rows_kernel<ABITS, EPI, 1, 1, 4>, 1, 1, 4);
+    return YUEAR_MX_ROWS(1, 1);
   if (p.m <= 512)
-    return go(rows_kernel<ABITS, EPI, 4, 4, 4>, 4, 4, 4);
+    return YUEAR_MX_ROWS(2, 2);
+#undef YUEAR_MX_ROWS
 #define YUEAR_MX_TILE(...)                                                                 \
   launch_tile<Tile<ABITS, __VA_ARGS__>>(tile_kernel<ABITS, EPI, __VA_ARGS__>, p, s)
   if constexpr (ABITS == 4) {
