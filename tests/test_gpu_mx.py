@@ -275,6 +275,64 @@ def test_gemm(torch, yuear_lib, m, n, k, bits, epilogue, kind):
                ref.from_bf16(r) if r is not None else None)
 
 
+def forced(torch, yuear_lib, form, a, w, a_bits, out, residual=None, swiglu=False):
+    (ac, asc), (wc, wsc) = a, w
+    status = yuear_lib.lib.yuear_op_mx_gemm_form(
+        ac.data_ptr(), ac.stride(0), asc.data_ptr(), asc.stride(0), a_bits, wc.data_ptr(), wc.stride(0),
+        wsc.data_ptr(), wsc.stride(0), ac.shape[0], wc.shape[0], asc.shape[1] * 32,
+        residual.data_ptr() if residual is not None else None, residual.stride(0) if residual is not None else 0,
+        out.data_ptr(), out.stride(0), int(swiglu), form, torch.cuda.current_stream().cuda_stream)
+    assert status == 0
+
+
+# tokens, features, K: one and two rounds of a ring, odd numbers of 128s and of 512s, tiles with one
+# row or column, more tiles than a workgroup's first (256 x 256: 300 x 35000 has 274 of them)
+FORMS = [(1, 2, 128), (5, 40, 384), (16, 66, 640), (33, 34, 1152), (65, 130, 512), (130, 62, 1664), (257, 300, 896),
+         (40, 514, 2304), (300, 130, 4224)]
+
+
+@pytest.mark.parametrize("form", range(7))
+@pytest.mark.parametrize("m,n,k", FORMS)
+@pytest.mark.parametrize("bits", [8, 4])
+def test_every_form(torch, yuear_lib, form, m, n, k, bits):
+    """Each form at any shape, stored rows and their surroundings, with each epilogue in turn."""
+    rng = np.random.default_rng(form + m + k)
+    a, w = random_pair(rng, m, k, bits), random_pair(rng, n, k, 4)
+    va, vw = ref.values(*a, bits), ref.values(*w, 4)
+    pa, pw = pair_of(torch, *a, bits), pair_of(torch, *w, 4)
+    r = ref.to_bf16(4 * rng.standard_normal((m, n)))
+    for epilogue, pad in (("store", 8), ("swiglu", 0), ("residual", 3)):
+        width = n // 2 if epilogue == "swiglu" else n
+        wide = torch.full((m + 2, width + pad), 3.0, dtype=torch.bfloat16, device="cuda")
+        forced(torch, yuear_lib, form, pa, pw, bits, wide[:m, :width], bf16(torch, r) if epilogue == "residual" else None,
+               epilogue == "swiglu")
+        assert (wide[m:] == 3).all() and (wide[:, width:] == 3).all()
+        check_gemm(torch, wide[:m, :width], va, vw, bits, epilogue, ref.from_bf16(r) if epilogue == "residual" else None)
+
+
+@pytest.mark.parametrize("bits,k", [(8, 640), (8, 1024), (4, 768), (4, 896), (4, 1024)])
+@pytest.mark.parametrize("epilogue", ["store", "swiglu", "residual"])
+def test_tiles_one_after_another(torch, yuear_lib, bits, k, epilogue):
+    """More 256 x 256 tiles than CUs: the ring runs on into the next tile (ragged last ones), the same
+    bits as the tiles of 128 x 128, whose sums have the same order."""
+    rng = np.random.default_rng(k)
+    m, n = 300, 35002
+    a, w = pair_of(torch, *random_pair(rng, m, k, bits), bits), pair_of(torch, *random_pair(rng, n, k, 4), 4)
+    width = n // 2 if epilogue == "swiglu" else n
+    r = bf16(torch, ref.to_bf16(rng.standard_normal((m, n)))) if epilogue == "residual" else None
+    outs = []
+    for form in (6, 5):
+        for ld in (width, width + (-width) % 8 + 8):
+            out = torch.full((m, ld), 7.0, dtype=torch.bfloat16, device="cuda")[:, :width]
+            forced(torch, yuear_lib, form, a, w, bits, out, r, epilogue == "swiglu")
+            outs.append(out)
+    assert all(torch.equal(outs[0], o) for o in outs[1:])
+    rows = [0, 1, 255, 256, 299]
+    check_gemm(torch, outs[0][rows][:, :2000], ref.values(raw(torch, a[0])[rows], raw(torch, a[1])[rows], bits),
+               ref.values(raw(torch, w[0])[:2000 * n // width], raw(torch, w[1])[:2000 * n // width], 4), bits, epilogue,
+               ref.from_bf16(bits_of(torch, r))[rows][:, :2000] if r is not None else None)
+
+
 @pytest.mark.parametrize("m,n,k,bits", [(3, 40, 256, 8), (70, 140, 384, 4), (300, 300, 256, 8)])
 def test_gemm_rows_apart(torch, yuear_lib, m, n, k, bits):
     """Operands that are columns of wider buffers; what lies between their rows is NaN."""
@@ -290,10 +348,13 @@ def test_gemm_rows_apart(torch, yuear_lib, m, n, k, bits):
     check_gemm(torch, out, ref.values(*a, bits), ref.values(*w, 4), bits, "store")
     same = yuear_lib.mx_gemm(pair_of(torch, *a, bits), pair_of(torch, *w, 4))
     assert torch.equal(out, same)
+    for form in range(7):
+        forced(torch, yuear_lib, form, *pairs, bits, out)
+        check_gemm(torch, out, ref.values(*a, bits), ref.values(*w, 4), bits, "store")
 
 
-@pytest.mark.parametrize("m", [3, 40, 300])
-def test_gemm_not_finite(torch, yuear_lib, m):
+@pytest.mark.parametrize("m,form", [(3, 0), (3, 1), (40, 2), (40, 3), (40, 4), (300, 5), (300, 6)])
+def test_gemm_not_finite(torch, yuear_lib, m, form):
     """NaN scales and NaN codes reach their rows and columns, nothing else. Sums past 2^128 are not finite:
     infinities, or NaN where partial sums of either sign overflow."""
     rng = np.random.default_rng(m)
@@ -303,7 +364,8 @@ def test_gemm_not_finite(torch, yuear_lib, m):
     a[1][2, 15] = 255
     w[1][7, 3] = 255
     a[1][0], w[1][9] = 200, 200  # 2^73 each
-    out = yuear_lib.mx_gemm(pair_of(torch, *a, 8), pair_of(torch, *w, 4))
+    out = torch.empty(m, n, dtype=torch.bfloat16, device="cuda")
+    forced(torch, yuear_lib, form, pair_of(torch, *a, 8), pair_of(torch, *w, 4), 8, out)
     nan = torch.isnan(out).cpu().numpy()
     want = np.zeros((m, n), bool)
     want[1], want[2], want[:, 7] = True, True, True

@@ -1,6 +1,4 @@
 """What the block-scaled entry points refuse, before anything is launched: runs without a GPU."""
-import ctypes as C
-
 import numpy as np
 import pytest
 
@@ -79,6 +77,12 @@ def gemm(lib, a=BASE, a_stride=256, a_scales=BASE + (1 << 20), a_scales_stride=8
 ])
 def test_gemm_refused(yuear_lib, bad):
     assert gemm(yuear_lib.lib, **bad) == 1
+
+
+def test_forms_refused(yuear_lib):
+    for form in (-2, 7):
+        assert yuear_lib.lib.yuear_op_mx_gemm_form(BASE, 256, BASE + (1 << 20), 8, 8, BASE + (2 << 20), 128, BASE + (3 << 20),
+                                                   8, 4, 6, 256, None, 0, BASE + (4 << 20), 6, 0, form, None) == 1
 
 
 def test_empty_calls(yuear_lib):

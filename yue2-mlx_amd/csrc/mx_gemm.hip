@@ -2,6 +2,7 @@
 // values (mx.h): activations in 8 or 4 bits, weights in 4, on gfx950's scaled
 // MFMA, 128 of K at a time with sums in fp32.
 #include <algorithm>
+#include <cmath>
 #include <type_traits>
 
 #include "kernels.h"
@@ -308,13 +309,15 @@ typedef float f32x16 __attribute__((ext_vector_type(16)));
 
 constexpr int kGroupK = 512;  // K of a group of scales
 
-template <int ABITS, int BM, int BN, int WM, int WN, int KSTEP, int STAGES> struct Tile {
-  static constexpr int kWaves = WM * WN, kBM = BM, kBN = BN;
+template <int ABITS, int BM, int BN, int WM, int WN, int KS, int KSTEP, int STAGES> struct Tile {
+  static constexpr int kTeam = WM * WN, kWaves = kTeam * KS, kBM = BM, kBN = BN;
   static constexpr int kARow = KSTEP * ABITS / 8, kWRow = KSTEP / 2;  // bytes of a row a step
   static constexpr int kStage = BM * kARow + BN * kWRow;
   static constexpr int kScales = (BM + BN) * 16;
   static constexpr int kStages = STAGES;
-  static constexpr int kLds = kStages * kStage + 2 * kScales;
+  static constexpr int kRing = kStages * kStage + 2 * kScales;  // of a team
+  static constexpr int kLds = KS * kRing;
+  static constexpr bool kOnward = KS == 1 && STAGES <= 3;  // takes one tile after another
   static_assert(kLds <= 160 * 1024, "LDS");
 };
 
@@ -338,7 +341,9 @@ __device__ __forceinline__ bool tile_of(int b, int grid, int n, int tiles_m, int
 }
 
 __device__ __forceinline__ int slot_of(int bytes, int row, int chunk) {
-  return bytes == 128 ? chunk ^ ((row >> 1) & 7) : chunk ^ (((row >> 2) & 1) | ((row >> 3) & 2));
+  return bytes == 256   ? chunk ^ (row & 15)
+         : bytes == 128 ? chunk ^ ((row >> 1) & 7)
+                        : chunk ^ (((row >> 2) & 1) | ((row >> 3) & 2));
 }
 
 // s_waitcnt for all but the last `loads` vector memory operations, and every LDS read.
@@ -347,7 +352,7 @@ constexpr int waitcnt(int loads) { return (loads & 15) | (loads >> 4) << 14 | 0x
 // LOADS of its vector memory operations. (__syncthreads() would wait for every load into LDS,
 // those of the steps ahead too. The branch is in the assembly so that a step stays one block for
 // the scheduler.)
-template <int LOADS, int FROM> __device__ __forceinline__ void wait_and_meet(int step) {
+template <int LOADS, int FROM, bool MEET> __device__ __forceinline__ void wait_and_meet(int step) {
   asm volatile("" ::: "memory");
   __builtin_amdgcn_sched_barrier(0);
   asm volatile("s_cmp_lt_i32 %0, %2\n\t"
@@ -356,7 +361,8 @@ template <int LOADS, int FROM> __device__ __forceinline__ void wait_and_meet(int
                ".Lmeet%=:" ::"s"(__builtin_amdgcn_readfirstlane(step)), "n"(LOADS), "n"(FROM)
                : "scc", "memory");
   __builtin_amdgcn_s_waitcnt(waitcnt(63));
-  __builtin_amdgcn_s_barrier();
+  if constexpr (MEET)
+    __builtin_amdgcn_s_barrier();
   __builtin_amdgcn_sched_barrier(0);
   asm volatile("" ::: "memory");
 }
@@ -375,38 +381,52 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t rsrc(const uint8_t *base, int 
 
 // With k up to 512 (fewer than two groups of scales) loads could reach past the next
 // tile: the launch gives each workgroup one tile then, and they read nothing.
-template <int ABITS, int EPI, int BM, int BN, int WM, int WN, int KSTEP, int STAGES>
+//
+// KS > 1: one wave has the whole tile, and KS of them a part of K and a ring each, with
+// no barrier before their sums are added.
+template <int ABITS, int EPI, int BM, int BN, int WM, int WN, int KS, int KSTEP, int STAGES>
 __device__ __forceinline__ void tile(const GemmArgs &p) {
-  using T = Tile<ABITS, BM, BN, WM, WN, KSTEP, STAGES>;
+  using T = Tile<ABITS, BM, BN, WM, WN, KS, KSTEP, STAGES>;
   constexpr int TM = BM / WM / 32, TN = BN / WN / 32, PARTS = KSTEP / 64;
   constexpr int kGroupSteps = kGroupK / KSTEP;
   constexpr int AQ = ABITS / 4;  // 16-byte pieces of A of a lane and 64 of K
-  constexpr int APW = BM * T::kARow / 1024 / T::kWaves, WPW = BN * T::kWRow / 1024 / T::kWaves;
-  constexpr int SB = (BM + BN) / 64, SPW = (SB + T::kWaves - 1) / T::kWaves;  // blocks of scales
-  static_assert(APW * T::kWaves * 1024 == BM * T::kARow && WPW * T::kWaves * 1024 == BN * T::kWRow &&
+  constexpr int APW = BM * T::kARow / 1024 / T::kTeam, WPW = BN * T::kWRow / 1024 / T::kTeam;
+  constexpr int SB = (BM + BN) / 64, SPW = (SB + T::kTeam - 1) / T::kTeam;  // blocks of scales
+  // A group of scales is asked for at the end of the group before the last one, so kGroupSteps
+  // steps ahead, and waited for with the loads of STAGES - 2 steps later.
+  static_assert(APW * T::kTeam * 1024 == BM * T::kARow && WPW * T::kTeam * 1024 == BN * T::kWRow &&
                     TM * 32 * WM == BM && TN * 32 * WN == BN && BM % 64 == 0 && BN % 64 == 0 &&
-                    (STAGES == 2 || STAGES == 3) && kGroupSteps >= 2,
+                    STAGES >= 2 && STAGES - 2 <= kGroupSteps && kGroupSteps >= 2 &&
+                    (KS == 1 || (T::kTeam == 1 && TM * TN == KS)),
                 "tile");
   const int tid = threadIdx.x, lane = tid & 63;
-  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wave_id = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int team = wave_id / T::kTeam, wave = wave_id % T::kTeam;
+  const int ring = team * T::kRing;
+  const int k_begin = p.k / KSTEP * team / KS * KSTEP;  // this team's K
+  const int k_len = p.k / KSTEP * (team + 1) / KS * KSTEP - k_begin;
   const int wm = wave / WN, wn = wave % WN;
   const int r = lane & 31, h = lane >> 5;
   const int tiles_m = (p.m + BM - 1) / BM, tiles_n = (p.n + BN - 1) / BN;
 
   // this wave's KiB blocks of a stage's A and W: lane l fills slot l
-  // (blocks two apart have their rows' slots alike: 16 rows of 128 bytes, 32 of 64)
+  // (the slots repeat after 16 rows, of 64 bytes after 32: blocks that far apart share an offset)
   constexpr int kARows = 1024 / T::kARow, kWRows = 1024 / T::kWRow;  // of a block
-  static_assert(APW % 2 == 0 && WPW % 2 == 0, "pairs of blocks");
-  uint32_t from_a[2], from_w[2], from_s[SPW];
+  constexpr int AP = kARows == 4 ? 4 : 2, WP = kWRows == 4 ? 4 : 2;  // blocks of 16 or 32 rows
+  static_assert((APW % AP == 0 || APW == 1) && (WPW % WP == 0 || WPW == 1), "blocks");
+  uint32_t from_a[AP], from_w[WP], from_s[SPW];
 #pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const int ar = kARows * (wave * APW + i) + lane / (64 / kARows);
-    from_a[i] = uint32_t(ar * int(p.a_stride) + slot_of(T::kARow, ar, lane % (64 / kARows)) * 16);
-    const int wr = kWRows * (wave * WPW + i) + lane / (64 / kWRows);
-    from_w[i] = uint32_t(wr * int(p.w_stride) + slot_of(T::kWRow, wr, lane % (64 / kWRows)) * 16);
+  for (int i = 0; i < AP; ++i) {
+    const int row = kARows * (wave * APW + i) + lane / (64 / kARows);
+    from_a[i] = uint32_t(row * int(p.a_stride) + slot_of(T::kARow, row, lane % (64 / kARows)) * 16);
+  }
+#pragma unroll
+  for (int i = 0; i < WP; ++i) {
+    const int row = kWRows * (wave * WPW + i) + lane / (64 / kWRows);
+    from_w[i] = uint32_t(row * int(p.w_stride) + slot_of(T::kWRow, row, lane % (64 / kWRows)) * 16);
   }
   // 64 rows of scales a block, A's first; waves past the last block repeat it
-  auto block = [&](int i) { return min(wave + i * T::kWaves, SB - 1); };
+  auto block = [&](int i) { return min(wave + i * T::kTeam, SB - 1); };
 #pragma unroll
   for (int i = 0; i < SPW; ++i) {
     const bool is_a = block(i) < BM / 64;
@@ -416,16 +436,17 @@ __device__ __forceinline__ void tile(const GemmArgs &p) {
   auto source = [&](int m0, int n0) {
     const int rows_a = min(p.m - m0, BM), rows_w = min(p.n - n0, BN);
     Source<SPW> s;
-    s.a = p.a + m0 * p.a_stride;
-    s.w = p.w + n0 * p.w_stride;
-    s.a_bytes = range(p.a_stride, rows_a, p.k * ABITS / 8);
-    s.w_bytes = range(p.w_stride, rows_w, p.k / 2);
+    s.a = p.a + m0 * p.a_stride + k_begin * ABITS / 8;
+    s.w = p.w + n0 * p.w_stride + k_begin / 2;
+    s.a_bytes = range(p.a_stride, rows_a, (p.k - k_begin) * ABITS / 8);
+    s.w_bytes = range(p.w_stride, rows_w, (p.k - k_begin) / 2);
 #pragma unroll
     for (int i = 0; i < SPW; ++i) {
       const bool is_a = block(i) < BM / 64;
-      s.s[i] = is_a ? p.a_scales + m0 * p.a_scale_stride : p.w_scales + n0 * p.w_scale_stride;
-      s.s_bytes[i] = is_a ? range(p.a_scale_stride, rows_a, p.k / 32)
-                          : range(p.w_scale_stride, rows_w, p.k / 32);
+      s.s[i] = (is_a ? p.a_scales + m0 * p.a_scale_stride : p.w_scales + n0 * p.w_scale_stride) +
+               k_begin / 32;
+      s.s_bytes[i] = is_a ? range(p.a_scale_stride, rows_a, (p.k - k_begin) / 32)
+                          : range(p.w_scale_stride, rows_w, (p.k - k_begin) / 32);
     }
     return s;
   };
@@ -436,7 +457,7 @@ __device__ __forceinline__ void tile(const GemmArgs &p) {
   int m0 = tm * BM, n0 = tn * BN;
   Source<SPW> now = source(m0, n0), then = now;
 
-  const int steps = p.k / KSTEP, groups = (p.k + kGroupK - 1) / kGroupK;
+  const int steps = k_len / KSTEP, groups = (k_len + kGroupK - 1) / kGroupK;
   // step `step` of this tile, or step - steps of the next, into the stage that begins at `stage`
   auto load = [&](int stage, int step) {
     const bool here = step < steps;
@@ -447,14 +468,14 @@ __device__ __forceinline__ void tile(const GemmArgs &p) {
     for (int i = 0; i < APW; ++i)
       __builtin_amdgcn_raw_ptr_buffer_load_lds(
           ra, (lds_ptr_t)(mx_lds + stage + (wave * APW + i) * 1024), 16,
-          from_a[i & 1] + (at * T::kARow + (i & ~1) * kARows * int(p.a_stride)), 0, 0, 0);
+          from_a[i % AP] + (at * T::kARow + i / AP * AP * kARows * int(p.a_stride)), 0, 0, 0);
 #pragma unroll
     for (int i = 0; i < WPW; ++i)
       __builtin_amdgcn_raw_ptr_buffer_load_lds(
           rw, (lds_ptr_t)(mx_lds + stage + BM * T::kARow + (wave * WPW + i) * 1024), 16,
-          from_w[i & 1] + (at * T::kWRow + (i & ~1) * kWRows * int(p.w_stride)), 0, 0, 0);
+          from_w[i % WP] + (at * T::kWRow + i / WP * WP * kWRows * int(p.w_stride)), 0, 0, 0);
   };
-  constexpr int kScalesAt = T::kStages * T::kStage;
+  const int scales_at = ring + T::kStages * T::kStage;
   int odd = 0;  // the buffer of this tile's first group
   auto load_scales = [&](int group) {
     const bool here = group < groups;
@@ -463,7 +484,7 @@ __device__ __forceinline__ void tile(const GemmArgs &p) {
     for (int i = 0; i < SPW; ++i)
       __builtin_amdgcn_raw_ptr_buffer_load_lds(
           rsrc(here ? now.s[i] : then.s[i], here ? now.s_bytes[i] : then.s_bytes[i]),
-          (lds_ptr_t)(mx_lds + kScalesAt + ((group + odd) & 1) * T::kScales + block(i) * 1024), 16,
+          (lds_ptr_t)(mx_lds + scales_at + ((group + odd) & 1) * T::kScales + block(i) * 1024), 16,
           from_s[i] + at * 16, 0, 0, 0);
   };
 
@@ -491,7 +512,7 @@ __device__ __forceinline__ void tile(const GemmArgs &p) {
   };
   // scales of step `at` of the group in buffer `buffer`
   auto read_scales = [&](int buffer, int at) {
-    const char *sc = mx_lds + kScalesAt + buffer * T::kScales + at * (KSTEP / 32);
+    const char *sc = mx_lds + scales_at + buffer * T::kScales + at * (KSTEP / 32);
 #pragma unroll
     for (int x = 0; x < TN; ++x)
 #pragma unroll
@@ -533,7 +554,8 @@ __device__ __forceinline__ void tile(const GemmArgs &p) {
   // ring takes step + STAGES, and, where the step ends a group, that group's buffer the group
   // after the next. Reads and loads go between the MFMAs.
   constexpr int kReads = TN + TM * AQ, kScaleReads = SW * (TM + TN), kMfmas = TM * TN,
-                kLoads = APW + WPW, kHalf = kMfmas / 2;
+                kLoads = APW + WPW, kHalf = (kMfmas + 1) / 2;
+  int ahead = STAGES;  // the first tile's loads are in order from its first step on
   auto advance = [&](auto ends, int stage, int next, int step, int buffer, int at, int group) {
     auto part = [&](auto s) {
       read(stage, s + 1);
@@ -550,8 +572,8 @@ __device__ __forceinline__ void tile(const GemmArgs &p) {
       part(std::integral_constant<int, 1>());
       part(std::integral_constant<int, 2>());
     }
-    // (a tile's first steps find theirs waited for below, or in the prologue)
-    wait_and_meet<(STAGES - 2) * kLoads, STAGES - 1>(step);
+    // (the first steps of a later tile find theirs waited for before the last one's stores)
+    wait_and_meet<(STAGES - 2) * kLoads, STAGES - 1, (T::kTeam > 1)>(step + ahead);
     read(next, 0);
     read_scales(buffer, at);
     if constexpr (decltype(ends)::value)
@@ -576,16 +598,19 @@ __device__ __forceinline__ void tile(const GemmArgs &p) {
   load_scales(1);
 #pragma unroll
   for (int s = 0; s < STAGES; ++s)
-    load(s * T::kStage, s);
-  wait_and_meet<0, 0>(0);
-  read(0, 0);
+    load(ring + s * T::kStage, s);
+  wait_and_meet<(STAGES - 1) * kLoads, 0, (T::kTeam > 1)>(0);
+  read(ring, 0);
   read_scales(0, 0);
   take_scales();
-  int stage = 0;
-  auto after = [](int at) { return at + T::kStage == STAGES * T::kStage ? 0 : at + T::kStage; };
+  int stage = ring;
+  auto after = [&](int at) {
+    return at + T::kStage == ring + STAGES * T::kStage ? ring : at + T::kStage;
+  };
 
   for (int turn = 1;; ++turn) {
-    const bool more = tile_of(int(blockIdx.x), int(gridDim.x), turn, tiles_m, tiles_n, tm, tn);
+    const bool more =
+        T::kOnward && tile_of(int(blockIdx.x), int(gridDim.x), turn, tiles_m, tiles_n, tm, tn);
     then = source(more ? tm * BM : m0, more ? tn * BN : n0);
     if (!more) {
       then.a_bytes = then.w_bytes = 0;
@@ -625,6 +650,36 @@ __device__ __forceinline__ void tile(const GemmArgs &p) {
 
     // the loads of the next tile's first steps, before this one's stores queue up behind them
     __builtin_amdgcn_s_waitcnt(waitcnt(0) | 0x0f00);
+    if constexpr (KS > 1) {  // team t finishes MFMA tile t, from everybody's sums in order
+      f32x4 *const sums = reinterpret_cast<f32x4 *>(mx_lds) + lane;
+      static_assert(KS * BM * BN * 4 <= T::kLds, "sums");
+      __syncthreads();
+#pragma unroll
+      for (int t = 0; t < KS; ++t)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const f32x16 &a = acc[t / TN][t % TN];
+          sums[((team * KS + t) * 4 + q) * 64] = f32x4{a[4 * q], a[4 * q + 1], a[4 * q + 2], a[4 * q + 3]};
+        }
+      __syncthreads();
+      float v[16];
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        f32x4 sum = sums[(team * 4 + q) * 64];
+#pragma unroll
+        for (int t = 1; t < KS; ++t)
+          sum += sums[((t * KS + team) * 4 + q) * 64];
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          v[4 * q + e] = sum[e];
+      }
+      const int m = m0 + r + team / TN * 32, n = n0 + team % TN * 32;
+      u32x4 residual[2];
+      if (EPI == kResidual)
+        residual32(p, m, n, h, residual);
+      finish32<EPI>(p, m, n, h, v, residual);
+      return;
+    }
 #pragma unroll
     for (int i = 0; i < TM; ++i) {
       const int m = m0 + a_row + 32 * i, n = n0 + wn * (BN / WN);
@@ -644,6 +699,7 @@ __device__ __forceinline__ void tile(const GemmArgs &p) {
     }
     if (!more)
       break;
+    ahead = 0;
     odd = (odd + groups) & 1;
     m0 = tm * BM;
     n0 = tn * BN;
@@ -651,9 +707,9 @@ __device__ __forceinline__ void tile(const GemmArgs &p) {
   }
 }
 
-template <int ABITS, int EPI, int BM, int BN, int WM, int WN, int KSTEP, int STAGES>
-__global__ __launch_bounds__(WM * WN * 64, 2) void tile_kernel(GemmArgs p) {
-  tile<ABITS, EPI, BM, BN, WM, WN, KSTEP, STAGES>(p);
+template <int ABITS, int EPI, int BM, int BN, int WM, int WN, int KS, int KSTEP, int STAGES>
+__global__ __launch_bounds__(WM * WN * KS * 64, 2) void tile_kernel(GemmArgs p) {
+  tile<ABITS, EPI, BM, BN, WM, WN, KS, KSTEP, STAGES>(p);
 }
 
 template <class T>
@@ -666,7 +722,7 @@ hipError_t launch_tile(void (*kernel)(GemmArgs), const GemmArgs &p, hipStream_t 
   if (e != hipSuccess)
     return e;
   const int64_t all = (tiles + 7) / 8 * 8, cus = std::max(gemm_cus() / 8 * 8, 8);
-  const unsigned grid = unsigned(p.k > kGroupK ? std::min(cus, all) : all);
+  const unsigned grid = unsigned(T::kOnward && p.k > kGroupK ? std::min(cus, all) : all);
   hipLaunchKernelGGL(kernel, dim3(grid), dim3(T::kWaves * 64), T::kLds, s, p);
   return hipGetLastError();
 }
@@ -691,48 +747,114 @@ hipError_t launch_rows(void (*kernel)(GemmArgs, int), const GemmArgs &p, hipStre
   return hipGetLastError();
 }
 
-template <int ABITS, int EPI> hipError_t launch_form(const GemmArgs &p, hipStream_t s) {
+// ---- the forms, and which one a call takes ----
+
+enum Form : int { kRows16, kRows32, kRows32x32, kTile64, kTile64x128, kTile128, kTile256, kForms };
+
+template <int ABITS, int EPI> hipError_t launch_form(int form, const GemmArgs &p, hipStream_t s) {
 #define YUEAR_MX_ROWS(MT, FT) launch_rows<ABITS, MT, FT>(rows_kernel<ABITS, EPI, MT, FT>, p, s)
-  if (p.m <= 16)
-    return YUEAR_MX_ROWS(1, 1);
-  if (p.m <= 512)
-    return YUEAR_MX_ROWS(2, 2);
-#undef YUEAR_MX_ROWS
 #define YUEAR_MX_TILE(...)                                                                 \
   launch_tile<Tile<ABITS, __VA_ARGS__>>(tile_kernel<ABITS, EPI, __VA_ARGS__>, p, s)
-  if constexpr (ABITS == 4) {
-    if (p.k % 256 == 0)
-      return YUEAR_MX_TILE(256, 256, 4, 2, 256, 2);
+  switch (form) {
+  case kRows16: return YUEAR_MX_ROWS(1, 1);
+  case kRows32: return YUEAR_MX_ROWS(1, 2);
+  case kRows32x32: return YUEAR_MX_ROWS(2, 2);
+  case kTile64: return YUEAR_MX_TILE(64, 64, 1, 1, 4, 128, (ABITS == 8 ? 3 : 4));
+  case kTile64x128: return YUEAR_MX_TILE(64, 128, 1, 4, 1, 128, 6);
+  case kTile128: return YUEAR_MX_TILE(128, 128, 2, 2, 1, 128, 3);
+  case kTile256:
+    // 4 bits: rows of 128 bytes (256 of K) a load where K has them; 64 bytes ask L2 as often
+    if constexpr (ABITS == 4)
+      if (p.k % 256 == 0)
+        return YUEAR_MX_TILE(256, 256, 4, 2, 1, 256, 2);
+    return YUEAR_MX_TILE(256, 256, 4, 2, 1, 128, 3);
   }
-  return YUEAR_MX_TILE(256, 256, 4, 2, 128, 3);
+#undef YUEAR_MX_ROWS
 #undef YUEAR_MX_TILE
+  return hipErrorInvalidValue;
 }
 
-template <int ABITS> hipError_t launch(const GemmArgs &p, hipStream_t s) {
+template <int ABITS> hipError_t launch(int form, const GemmArgs &p, hipStream_t s) {
   switch (p.epilogue) {
-  case kSwiglu: return launch_form<ABITS, kSwiglu>(p, s);
-  case kResidual: return launch_form<ABITS, kResidual>(p, s);
-  default: return launch_form<ABITS, kStore>(p, s);
+  case kSwiglu: return launch_form<ABITS, kSwiglu>(form, p, s);
+  case kResidual: return launch_form<ABITS, kResidual>(form, p, s);
+  default: return launch_form<ABITS, kStore>(form, p, s);
   }
+}
+
+// Estimated us of m x n x k by a form, fitted on MI355X with the weights from HBM to 1100
+// calls (1-3072 tokens, 16-98304 features, K 256-8192; 4-16% rms).
+double form_time(int form, int bits, int m, int n, int k, int cus) {
+  const bool a8 = bits == 8;
+  const double kk = k / 1024.0;
+  auto tiles = [&](int bm, int bn) { return double((m + bm - 1) / bm) * double((n + bn - 1) / bn); };
+  if (form <= kRows32x32) {
+    // the launch, each 512 of K that a wave takes after another, the bytes of W and of A
+    const int bm = form == kRows32x32 ? 32 : 16, bn = form == kRows16 ? 16 : 32;
+    const int per_kib = a8 ? 2 : 4, rows = (std::min(m, bm) + per_kib - 1) / per_kib * per_kib;
+    const int region = bn * (kSliceK / 2 + 16) + rows * (kSliceK * bits / 8 + 16);
+    const int slices = (k + kSliceK - 1) / kSliceK;
+    const int waves = std::min({slices, 160 * 1024 / region, 16});
+    static const double fit[2][3][5] = {
+        {{2.097, 0.781, 0.021, 0.014, 0.003}, {1.789, 1.261, 0.021, 0.022, 0.019}, {3.232, 0.377, 0.031, 0.0, 0.16}},
+        {{2.819, 0.0, 0.02, 0.018, 0.006}, {1.667, 1.308, 0.021, 0.023, 0.023}, {3.107, 0.321, 0.027, 0.0, 0.183}}};
+    const double *c = fit[a8 ? 0 : 1][form];
+    const double t = tiles(bm, bn) / cus;
+    return c[0] + c[1] * ((slices + waves - 1) / waves) + t * (kk * (c[2] * bn + c[3] * rows * bits / 8) + c[4]);
+  }
+  // the launch, full rounds of tiles, and a last one by how many CUs it has work for
+  static const int shape[4][3] = {{64, 64, 1}, {64, 128, 1}, {128, 128, 2}, {256, 256, 1}};
+  static const double fit[2][4][7] = {{{1.524, 3.182, 1.706, 2.885, 0.787, 0.189, 1.072},
+                                       {1.627, 2.555, 3.051, 2.061, 1.73, 0.436, 1.28},
+                                       {4.05, 3.489, 8.666, 0.0, 2.487, 3.698, 4.451},
+                                       {6.695, 6.056, 12.041, 1.699, 7.315, 3.586, 3.695}},
+                                      {{1.331, 3.193, 1.467, 2.832, 0.55, 0.31, 1.083},
+                                       {2.798, 1.22, 2.497, 0.556, 1.473, 0.586, 0.994},
+                                       {3.756, 3.377, 7.138, 0.0, 1.919, 3.606, 3.907},
+                                       {5.723, 6.185, 8.392, 1.894, 4.788, 3.998, 2.257}}};
+  const int *of = shape[form - kTile64];
+  const double *c = fit[a8 ? 0 : 1][form - kTile64];
+  const double slots = double(cus) * of[2], t = tiles(of[0], of[1]), full = std::floor(t / slots), rest = t / slots - full;
+  return c[0] + full * (c[1] + c[2] * kk) + (rest > 0 ? c[3] + c[4] * kk + rest * (c[5] + c[6] * kk) : 0.0);
+}
+
+// The form of least estimated time: rows where there are few tokens, the larger tiles the
+// more there are to fill the CUs with. The sum over K is split as the form is (by waves, in
+// order), so the form decides the order of the sums.
+int pick_form(int bits, int m, int n, int k) {
+  const int cus = gemm_cus();
+  int best = 0;
+  double least = __builtin_inf();
+  for (int form = 0; form < kForms; ++form) {
+    const double t = form_time(form, bits, m, n, k, cus);
+    if (t < least) {
+      least = t;
+      best = form;
+    }
+  }
+  return best;
 }
 
 }  // namespace
 }  // namespace mx
 }  // namespace yuear
 
-extern "C" int32_t yuear_op_mx_gemm(const uint8_t *a, int64_t a_stride, const uint8_t *a_scales,
-                                    int64_t a_scales_stride, int32_t a_bits, const uint8_t *w,
-                                    int64_t w_stride, const uint8_t *w_scales,
-                                    int64_t w_scales_stride, int32_t m, int32_t n, int32_t k,
-                                    const uint16_t *residual, int64_t residual_stride, uint16_t *c,
-                                    int64_t ldc, int32_t swiglu, void *stream) {
+extern "C" {
+
+int32_t yuear_op_mx_gemm_form(const uint8_t *a, int64_t a_stride, const uint8_t *a_scales,
+                              int64_t a_scales_stride, int32_t a_bits, const uint8_t *w,
+                              int64_t w_stride, const uint8_t *w_scales, int64_t w_scales_stride,
+                              int32_t m, int32_t n, int32_t k, const uint16_t *residual,
+                              int64_t residual_stride, uint16_t *c, int64_t ldc, int32_t swiglu,
+                              int32_t form, void *stream) {
   using namespace yuear;
   if (m == 0 || n == 0)
     return 0;
   if (m < 0 || n < 0 || k % mx::kStep || (swiglu != 0 && swiglu != 1) || (swiglu && (n % 2 || residual)) ||
       !mx::rows_ok(a, a_stride, a_scales, a_scales_stride, k, a_bits) ||
       !mx::rows_ok(w, w_stride, w_scales, w_scales_stride, k, 4) || !mx::aligned(a_scales, 4) ||
-      !mx::aligned(w_scales, 4) || a_scales_stride % 4 || w_scales_stride % 4 || !mx::aligned(c, 2))
+      !mx::aligned(w_scales, 4) || a_scales_stride % 4 || w_scales_stride % 4 || !mx::aligned(c, 2) || form < -1 ||
+      form >= mx::kForms)
     return int32_t(hipErrorInvalidValue);
   const int width = swiglu ? n / 2 : n;
   constexpr int64_t kMostLd = int64_t(1) << 31;
@@ -748,11 +870,24 @@ extern "C" int32_t yuear_op_mx_gemm(const uint8_t *a, int64_t a_stride, const ui
   if (residual && !(residual == c && residual_stride == ldc) &&
       mx::overlap(mx::bf16_span(residual, residual_stride, m, width), out))
     return int32_t(hipErrorInvalidValue);
-  const mx::GemmArgs p{a,      a_scales, w, w_scales, a_stride, a_scales_stride, w_stride, w_scales_stride, m, n, k,
+  const mx::GemmArgs p{a, a_scales, w, w_scales, a_stride, a_scales_stride, w_stride, w_scales_stride, m, n, k,
                        residual, c, residual_stride, ldc,
                        swiglu ? mx::kSwiglu : residual ? mx::kResidual : mx::kStore,
                        mx::aligned(c, 16) && ldc % 8 == 0 &&
                            (!residual || (mx::aligned(residual, 16) && residual_stride % 8 == 0))};
   const hipStream_t st = static_cast<hipStream_t>(stream);
-  return int32_t(a_bits == 8 ? mx::launch<8>(p, st) : mx::launch<4>(p, st));
+  if (form < 0)
+    form = mx::pick_form(a_bits, m, n, k);
+  return int32_t(a_bits == 8 ? mx::launch<8>(form, p, st) : mx::launch<4>(form, p, st));
 }
+
+int32_t yuear_op_mx_gemm(const uint8_t *a, int64_t a_stride, const uint8_t *a_scales,
+                         int64_t a_scales_stride, int32_t a_bits, const uint8_t *w, int64_t w_stride,
+                         const uint8_t *w_scales, int64_t w_scales_stride, int32_t m, int32_t n,
+                         int32_t k, const uint16_t *residual, int64_t residual_stride, uint16_t *c,
+                         int64_t ldc, int32_t swiglu, void *stream) {
+  return yuear_op_mx_gemm_form(a, a_stride, a_scales, a_scales_stride, a_bits, w, w_stride, w_scales,
+                               w_scales_stride, m, n, k, residual, residual_stride, c, ldc, swiglu, -1, stream);
+}
+
+}  // extern "C"

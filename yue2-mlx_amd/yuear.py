@@ -206,6 +206,10 @@ _SIGS = {
             C.c_void_p, C.c_int64, C.c_void_p, C.c_int64, C.c_int32, C.c_void_p, C.c_int64,
             C.c_void_p, C.c_int64, C.c_int32, C.c_int32, C.c_int32, C.c_void_p, C.c_int64,
             C.c_void_p, C.c_int64, C.c_int32, C.c_void_p]),
+    "yuear_op_mx_gemm_form": (C.c_int32, [
+            C.c_void_p, C.c_int64, C.c_void_p, C.c_int64, C.c_int32, C.c_void_p, C.c_int64,
+            C.c_void_p, C.c_int64, C.c_int32, C.c_int32, C.c_int32, C.c_void_p, C.c_int64,
+            C.c_void_p, C.c_int64, C.c_int32, C.c_int32, C.c_void_p]),
     "yuear_tokenizer_load": (C.c_int, [C.c_char_p, _P(C.c_void_p), _P(C.c_void_p)]),
     "yuear_tokenizer_destroy": (None, [C.c_void_p]),
     "yuear_tokenizer_encode": (C.c_int, [C.c_void_p, C.c_char_p, C.c_int64, _P(i32p),
