@@ -546,10 +546,11 @@ int32_t yuear_op_mx_gemm(const uint8_t *dev_a, int64_t a_stride, const uint8_t *
                          int32_t m, int32_t n, int32_t k, const uint16_t *dev_residual,
                          int64_t residual_stride, uint16_t *dev_c, int64_t ldc, int32_t swiglu,
                          void *stream);
-/* Test hook: yuear_op_mx_gemm with its form forced, 0..6 = 16 and 32 features by up to 16
- * tokens, 32 by 32, tiles of 64x64, 64x128 (tokens x features), 128x128, 256x256;
- * -1 the one that yuear_op_mx_gemm takes; other values return
- * hipErrorInvalidValue (1). */
+/* Test hook: yuear_op_mx_gemm with its form forced, 0..8 = workgroups of 16 and 32 features by
+ * up to 16 tokens, 32 by 32, tiles of 64x64, 64x128 (tokens x features), 128x128, 256x256,
+ * 16 and 32 features one after another by up to 16 tokens (m up to 16 and operands of all K that
+ * fit a CU's LDS, else hipErrorInvalidValue); -1 the one that yuear_op_mx_gemm takes; other
+ * values return hipErrorInvalidValue (1). */
 int32_t yuear_op_mx_gemm_form(const uint8_t *dev_a, int64_t a_stride, const uint8_t *dev_a_scales,
                               int64_t a_scales_stride, int32_t a_bits, const uint8_t *dev_w,
                               int64_t w_stride, const uint8_t *dev_w_scales,

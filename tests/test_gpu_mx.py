@@ -275,14 +275,14 @@ def test_gemm(torch, yuear_lib, m, n, k, bits, epilogue, kind):
                ref.from_bf16(r) if r is not None else None)
 
 
-def forced(torch, yuear_lib, form, a, w, a_bits, out, residual=None, swiglu=False):
+def forced(torch, yuear_lib, form, a, w, a_bits, out, residual=None, swiglu=False, expect=0):
     (ac, asc), (wc, wsc) = a, w
     status = yuear_lib.lib.yuear_op_mx_gemm_form(
         ac.data_ptr(), ac.stride(0), asc.data_ptr(), asc.stride(0), a_bits, wc.data_ptr(), wc.stride(0),
         wsc.data_ptr(), wsc.stride(0), ac.shape[0], wc.shape[0], asc.shape[1] * 32,
         residual.data_ptr() if residual is not None else None, residual.stride(0) if residual is not None else 0,
         out.data_ptr(), out.stride(0), int(swiglu), form, torch.cuda.current_stream().cuda_stream)
-    assert status == 0
+    assert status == expect
 
 
 # tokens, features, K: one and two rounds of a ring, odd numbers of 128s and of 512s, tiles with one
@@ -333,6 +333,26 @@ def test_tiles_one_after_another(torch, yuear_lib, bits, k, epilogue):
                ref.from_bf16(bits_of(torch, r))[rows][:, :2000] if r is not None else None)
 
 
+@pytest.mark.parametrize("form", [7, 8])
+@pytest.mark.parametrize("m,n,k,bits", [(1, 2, 128, 8), (5, 40, 384, 4), (16, 66, 640, 8), (3, 20002, 1152, 8),
+                                        (7, 70034, 640, 4), (15, 9000, 512, 8), (2, 16390, 4096, 4)])
+@pytest.mark.parametrize("epilogue", ["store", "swiglu", "residual"])
+def test_streamed_rows(torch, yuear_lib, form, m, n, k, bits, epilogue):
+    """Features one workgroup after another: the sums of the rows form (0), whose order is the same."""
+    rng = np.random.default_rng(n)
+    a, w = pair_of(torch, *random_pair(rng, m, k, bits), bits), pair_of(torch, *random_pair(rng, n, k, 4), 4)
+    width = n // 2 if epilogue == "swiglu" else n
+    r = bf16(torch, ref.to_bf16(rng.standard_normal((m, n)))) if epilogue == "residual" else None
+    wide = torch.full((m + 1, width + 5), 3.0, dtype=torch.bfloat16, device="cuda")
+    want = torch.empty(m, width, dtype=torch.bfloat16, device="cuda")
+    if (form, k) == (8, 4096):  # two buffers of 32 rows for eight waves do not fit a CU's LDS
+        forced(torch, yuear_lib, form, a, w, bits, wide[:m, :width], r, epilogue == "swiglu", expect=1)
+        return
+    forced(torch, yuear_lib, form, a, w, bits, wide[:m, :width], r, epilogue == "swiglu")
+    forced(torch, yuear_lib, 0, a, w, bits, want, r, epilogue == "swiglu")
+    assert torch.equal(wide[:m, :width], want) and (wide[m:] == 3).all() and (wide[:, width:] == 3).all()
+
+
 @pytest.mark.parametrize("m,n,k,bits", [(3, 40, 256, 8), (70, 140, 384, 4), (300, 300, 256, 8)])
 def test_gemm_rows_apart(torch, yuear_lib, m, n, k, bits):
     """Operands that are columns of wider buffers; what lies between their rows is NaN."""
@@ -353,7 +373,7 @@ def test_gemm_rows_apart(torch, yuear_lib, m, n, k, bits):
         check_gemm(torch, out, ref.values(*a, bits), ref.values(*w, 4), bits, "store")
 
 
-@pytest.mark.parametrize("m,form", [(3, 0), (3, 1), (40, 2), (40, 3), (40, 4), (300, 5), (300, 6)])
+@pytest.mark.parametrize("m,form", [(3, 0), (3, 1), (3, 7), (3, 8), (40, 2), (40, 3), (40, 4), (300, 5), (300, 6)])
 def test_gemm_not_finite(torch, yuear_lib, m, form):
     """NaN scales and NaN codes reach their rows and columns, nothing else. Sums past 2^128 are not finite:
     infinities, or NaN where partial sums of either sign overflow."""

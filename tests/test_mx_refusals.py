@@ -80,7 +80,7 @@ def test_gemm_refused(yuear_lib, bad):
 
 
 def test_forms_refused(yuear_lib):
-    for form in (-2, 7):
+    for form in (-2, 9):
         assert yuear_lib.lib.yuear_op_mx_gemm_form(BASE, 256, BASE + (1 << 20), 8, 8, BASE + (2 << 20), 128, BASE + (3 << 20),
                                                    8, 4, 6, 256, None, 0, BASE + (4 << 20), 6, 0, form, None) == 1
 

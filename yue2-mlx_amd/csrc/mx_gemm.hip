@@ -172,23 +172,125 @@ template <int ABITS, int FT> constexpr int region(int a_rows) {
   return 16 * FT * (kSliceK / 2 + 16) + a_rows * (kSliceK * ABITS / 8 + 16);
 }
 
+constexpr int kWPiece = kSliceK / 2;
+template <int ABITS> constexpr int a_piece() { return kSliceK * ABITS / 8; }
+
+// 512 of K from k0 on of 16 FT rows of W and of A's rows, with their scales, into LDS at the
+// places given. (What lies past K in a piece belongs to other rows, and is not used.)
+template <int FT>
+__device__ __forceinline__ void load_w(const GemmArgs &p, __amdgpu_buffer_rsrc_t rw,
+                                       __amdgpu_buffer_rsrc_t rsw, char *w, char *scales, int k0) {
+  const int lane = threadIdx.x & 63;
+#pragma unroll
+  for (int i = 0; i < 4 * FT; ++i) {
+    const int row = 4 * i + (lane >> 4);
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(
+        rw, (lds_ptr_t)(w + i * 1024), 16,
+        row * int(p.w_stride) + k0 / 2 + ((lane & 15) ^ (row & 15)) * 16, 0, 0, 0);
+  }
+  if (lane < 16 * FT)
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(rsw, (lds_ptr_t)scales, 16,
+                                             lane * int(p.w_scale_stride) + k0 / 32, 0, 0, 0);
+}
+template <int ABITS>
+__device__ __forceinline__ void load_a(const GemmArgs &p, __amdgpu_buffer_rsrc_t ra,
+                                       __amdgpu_buffer_rsrc_t rsa, char *a, char *scales, int k0,
+                                       int a_rows) {
+  constexpr int kSlots = a_piece<ABITS>() / 16;
+  const int lane = threadIdx.x & 63;
+  for (int i = 0; i < a_rows * a_piece<ABITS>() / 1024; ++i) {
+    const int row = 64 / kSlots * i + lane / kSlots, slot = lane % kSlots;
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(
+        ra, (lds_ptr_t)(a + i * 1024), 16,
+        row * int(p.a_stride) + k0 * ABITS / 8 + (slot ^ (row & 15)) * 16, 0, 0, 0);
+  }
+  if (lane < a_rows)
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(rsa, (lds_ptr_t)scales, 16,
+                                             lane * int(p.a_scale_stride) + k0 / 32, 0, 0, 0);
+}
+
+// acc += W A^T over the 512 of K from k0 on that those loads brought.
+template <int ABITS, int MT, int FT>
+__device__ __forceinline__ void multiply_slice(const GemmArgs &p, const char *w_at,
+                                               const char *w_scales, const char *a_at,
+                                               const char *a_scales, int k0, int a_rows,
+                                               f32x4 (&acc)[FT][MT]) {
+  constexpr int AQ = ABITS / 4;  // 16-byte pieces of A of a lane and MFMA
+  const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
+  u32x4 ws[FT], as[MT];
+#pragma unroll
+  for (int f = 0; f < FT; ++f)
+    ws[f] = *reinterpret_cast<const u32x4 *>(w_scales + (16 * f + r) * 16);
+#pragma unroll
+  for (int t = 0; t < MT; ++t)
+    as[t] = *reinterpret_cast<const u32x4 *>(a_scales + min(16 * t + r, a_rows - 1) * 16);
+#pragma unroll
+  for (int s = 0; s < kSliceK / kStep; ++s) {
+    if (k0 + s * kStep >= p.k)
+      break;
+    u32x4 w[FT], a[MT][AQ];
+#pragma unroll
+    for (int f = 0; f < FT; ++f)
+      w[f] = *reinterpret_cast<const u32x4 *>(w_at + (16 * f + r) * kWPiece + ((4 * s + g) ^ r) * 16);
+#pragma unroll
+    for (int t = 0; t < MT; ++t)
+#pragma unroll
+      for (int q = 0; q < AQ; ++q)
+        a[t][q] = *reinterpret_cast<const u32x4 *>(
+            a_at + min(16 * t + r, a_rows - 1) * a_piece<ABITS>() +
+            ((ABITS == 8 ? 8 * s + 4 * q + g : 4 * s + g) ^ r) * 16);
+#pragma unroll
+    for (int f = 0; f < FT; ++f)
+#pragma unroll
+      for (int t = 0; t < MT; ++t) {
+        const u32x4 lo = a[t][0], hi = a[t][AQ - 1];
+        const i32x8 wv = {int(w[f].x), int(w[f].y), int(w[f].z), int(w[f].w), 0, 0, 0, 0};
+        const i32x8 av = {int(lo.x), int(lo.y), int(lo.z), int(lo.w),
+                          int(hi.x), int(hi.y), int(hi.z), int(hi.w)};
+        acc[f][t] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(
+            wv, av, acc[f][t], 4, ABITS == 8 ? 0 : 4, 0, int(ws[f][s] >> (8 * g)), 0,
+            int(as[t][s] >> (8 * g)));
+      }
+  }
+}
+
+// Sums of all waves at `sums` (a wave's `stride` bytes apart) to memory.
+template <int EPI, int MT, int FT>
+__device__ __forceinline__ void add_and_finish(const GemmArgs &p, const char *sums, int stride,
+                                               int m0, int n0) {
+  const int waves = int(blockDim.x) >> 6;
+  for (int i = threadIdx.x; i < FT * MT * 64; i += int(blockDim.x)) {
+    const int tile = i >> 6, l = i & 63;
+    f32x4 sum = {0.f, 0.f, 0.f, 0.f};
+    for (int q = 0; q < waves; ++q)
+      sum += *reinterpret_cast<const f32x4 *>(sums + q * stride + i * 16);
+    const int m = m0 + 16 * (tile % MT) + (l & 15), n = n0 + 16 * (tile / MT) + 4 * (l >> 4);
+    const float v[4] = {sum[0], sum[1], sum[2], sum[3]};
+    if (m < p.m)
+      finish4<EPI>(p, m, n, v);
+  }
+}
+
+// s_waitcnt for all but the last `loads` vector memory operations.
+template <int LOADS> __device__ __forceinline__ void wait_loads() {
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_waitcnt((LOADS & 15) | (LOADS >> 4) << 14 | 0x0f70);
+  asm volatile("" ::: "memory");
+}
+
 template <int ABITS, int EPI, int MT, int FT>
 __global__ __launch_bounds__(1024) void rows_kernel(GemmArgs p, int a_rows) {
-  constexpr int AQ = ABITS / 4;              // 16-byte pieces of A of a lane and MFMA
-  constexpr int kARow = kSliceK * ABITS / 8;  // bytes of an A row's piece
-  constexpr int kWAt = 0, kAAt = 16 * FT * (kSliceK / 2);
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int waves = int(blockDim.x) >> 6;
-  const int r = lane & 15, g = lane >> 4;
   const int n0 = int(blockIdx.x) * (16 * FT), m0 = int(blockIdx.y) * (16 * MT);
   const int rows_a = min(p.m - m0, a_rows), rows_w = min(p.n - n0, 16 * FT);
   const auto ra = rows_rsrc(p.a + m0 * p.a_stride, p.a_stride, rows_a, p.k * ABITS / 8);
   const auto rw = rows_rsrc(p.w + n0 * p.w_stride, p.w_stride, rows_w, p.k / 2);
   const auto rsa = rows_rsrc(p.a_scales + m0 * p.a_scale_stride, p.a_scale_stride, rows_a, p.k / 32);
   const auto rsw = rows_rsrc(p.w_scales + n0 * p.w_scale_stride, p.w_scale_stride, rows_w, p.k / 32);
-  char *const mine = mx_lds + wave * region<ABITS, FT>(a_rows);
-  char *const w_scales = mine + kAAt + a_rows * kARow, *const a_scales = w_scales + 16 * FT * 16;
+  char *const w = mx_lds + wave * region<ABITS, FT>(a_rows), *const a = w + 16 * FT * kWPiece;
+  char *const w_scales = a + a_rows * a_piece<ABITS>(), *const a_scales = w_scales + 16 * FT * 16;
 
   f32x4 acc[FT][MT];
 #pragma unroll
@@ -197,85 +299,75 @@ __global__ __launch_bounds__(1024) void rows_kernel(GemmArgs p, int a_rows) {
     for (int t = 0; t < MT; ++t)
       acc[f][t] = f32x4{0.f, 0.f, 0.f, 0.f};
   for (int k0 = wave * kSliceK; k0 < p.k; k0 += waves * kSliceK) {
-    // (what lies past K in a piece belongs to other rows, and is not used)
-#pragma unroll
-    for (int i = 0; i < 4 * FT; ++i) {
-      const int row = 4 * i + (lane >> 4);
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(
-          rw, (lds_ptr_t)(mine + kWAt + i * 1024), 16,
-          row * int(p.w_stride) + k0 / 2 + ((lane & 15) ^ (row & 15)) * 16, 0, 0, 0);
-    }
-    for (int i = 0; i < a_rows * kARow / 1024; ++i) {
-      constexpr int kSlots = kARow / 16;
-      const int row = 64 / kSlots * i + lane / kSlots, slot = lane % kSlots;
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(
-          ra, (lds_ptr_t)(mine + kAAt + i * 1024), 16,
-          row * int(p.a_stride) + k0 * ABITS / 8 + (slot ^ (row & 15)) * 16, 0, 0, 0);
-    }
-    if (lane < 16 * FT)
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(rsw, (lds_ptr_t)w_scales, 16,
-                                               lane * int(p.w_scale_stride) + k0 / 32, 0, 0, 0);
-    if (lane < a_rows)
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(rsa, (lds_ptr_t)a_scales, 16,
-                                               lane * int(p.a_scale_stride) + k0 / 32, 0, 0, 0);
-    asm volatile("" ::: "memory");
-    __builtin_amdgcn_s_waitcnt(0x0f70);  // the wave's own loads: nobody else reads them
-    asm volatile("" ::: "memory");
-    u32x4 ws[FT], as[MT];
-#pragma unroll
-    for (int f = 0; f < FT; ++f)
-      ws[f] = *reinterpret_cast<const u32x4 *>(w_scales + (16 * f + r) * 16);
-#pragma unroll
-    for (int t = 0; t < MT; ++t)
-      as[t] = *reinterpret_cast<const u32x4 *>(a_scales + min(16 * t + r, a_rows - 1) * 16);
-#pragma unroll
-    for (int s = 0; s < kSliceK / kStep; ++s) {
-      if (k0 + s * kStep >= p.k)
-        break;
-      u32x4 w[FT], a[MT][AQ];
-#pragma unroll
-      for (int f = 0; f < FT; ++f)
-        w[f] = *reinterpret_cast<const u32x4 *>(mine + kWAt + (16 * f + r) * (kSliceK / 2) +
-                                                ((4 * s + g) ^ r) * 16);
-#pragma unroll
-      for (int t = 0; t < MT; ++t)
-#pragma unroll
-        for (int q = 0; q < AQ; ++q)
-          a[t][q] = *reinterpret_cast<const u32x4 *>(
-              mine + kAAt + min(16 * t + r, a_rows - 1) * kARow +
-              ((ABITS == 8 ? 8 * s + 4 * q + g : 4 * s + g) ^ r) * 16);
-#pragma unroll
-      for (int f = 0; f < FT; ++f)
-#pragma unroll
-        for (int t = 0; t < MT; ++t) {
-          const u32x4 lo = a[t][0], hi = a[t][AQ - 1];
-          const i32x8 wv = {int(w[f].x), int(w[f].y), int(w[f].z), int(w[f].w), 0, 0, 0, 0};
-          const i32x8 av = {int(lo.x), int(lo.y), int(lo.z), int(lo.w),
-                            int(hi.x), int(hi.y), int(hi.z), int(hi.w)};
-          acc[f][t] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(
-              wv, av, acc[f][t], 4, ABITS == 8 ? 0 : 4, 0, int(ws[f][s] >> (8 * g)), 0,
-              int(as[t][s] >> (8 * g)));
-        }
-    }
+    load_w<FT>(p, rw, rsw, w, w_scales, k0);
+    load_a<ABITS>(p, ra, rsa, a, a_scales, k0, a_rows);
+    wait_loads<0>();  // the wave's own: nobody else reads them
+    multiply_slice<ABITS, MT, FT>(p, w, w_scales, a, a_scales, k0, a_rows, acc);
     __builtin_amdgcn_s_waitcnt(0xc07f);  // every read, before the next loads
     asm volatile("" ::: "memory");
   }
-  f32x4 *const sums = reinterpret_cast<f32x4 *>(mine);  // the region's pieces are used up
+  f32x4 *const sums = reinterpret_cast<f32x4 *>(w);  // the region's pieces are used up
 #pragma unroll
   for (int f = 0; f < FT; ++f)
 #pragma unroll
     for (int t = 0; t < MT; ++t)
       sums[(f * MT + t) * 64 + lane] = acc[f][t];
   __syncthreads();
-  for (int i = threadIdx.x; i < FT * MT * 64; i += int(blockDim.x)) {
-    const int tile = i >> 6, l = i & 63;
-    f32x4 sum = {0.f, 0.f, 0.f, 0.f};
-    for (int q = 0; q < waves; ++q)
-      sum += *reinterpret_cast<const f32x4 *>(mx_lds + q * region<ABITS, FT>(a_rows) + i * 16);
-    const int m = m0 + 16 * (tile % MT) + (l & 15), n = n0 + 16 * (tile / MT) + 4 * (l >> 4);
-    const float v[4] = {sum[0], sum[1], sum[2], sum[3]};
-    if (m < p.m)
-      finish4<EPI>(p, m, n, v);
+  add_and_finish<EPI, MT, FT>(p, mx_lds, region<ABITS, FT>(a_rows), m0, n0);
+}
+
+// The same for weights of many features, k up to 512 a wave: a workgroup keeps A and goes
+// from one 16 FT features to another, the next ones' weights on their way under the products
+// and sums of these. (A workgroup for each 16 features spends half of its time on its start
+// and end: 5 x 83968 x 3072 31 us.)
+template <int ABITS, int FT> constexpr int stream_region(int a_rows) {
+  return 2 * (16 * FT * (kWPiece + 16) + FT * 1024) + a_rows * (a_piece<ABITS>() + 16);
+}
+template <int ABITS, int EPI, int FT>
+__global__ __launch_bounds__(1024) void stream_kernel(GemmArgs p, int a_rows) {
+  constexpr int kW = 16 * FT * (kWPiece + 16);  // a buffer's rows and scales
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int k0 = wave * kSliceK, stride = stream_region<ABITS, FT>(a_rows);
+  const auto ra = rows_rsrc(p.a, p.a_stride, min(p.m, a_rows), p.k * ABITS / 8);
+  const auto rsa = rows_rsrc(p.a_scales, p.a_scale_stride, min(p.m, a_rows), p.k / 32);
+  char *const mine = mx_lds + wave * stride;  // two buffers of W, two of sums, A
+  char *const a = mine + 2 * (kW + FT * 1024), *const a_scales = a + a_rows * a_piece<ABITS>();
+  auto load = [&](int n0, int buffer) {
+    const int rows = min(p.n - n0, 16 * FT);
+    char *const w = mine + buffer * kW;
+    load_w<FT>(p, rows_rsrc(p.w + n0 * p.w_stride, p.w_stride, rows, p.k / 2),
+               rows_rsrc(p.w_scales + n0 * p.w_scale_stride, p.w_scale_stride, rows, p.k / 32), w,
+               w + 16 * FT * kWPiece, k0);
+  };
+  load_a<ABITS>(p, ra, rsa, a, a_scales, k0, a_rows);
+  const int tiles = (p.n + 16 * FT - 1) / (16 * FT);
+  load(int(blockIdx.x) * (16 * FT), 0);
+  int buffer = 0;
+  for (int tile = int(blockIdx.x); tile < tiles; tile += int(gridDim.x), buffer ^= 1) {
+    const int next = tile + int(gridDim.x);
+    if (next < tiles) {
+      load(next * (16 * FT), buffer ^ 1);
+      wait_loads<4 * FT + 1>();
+    } else {
+      wait_loads<0>();
+    }
+    f32x4 acc[FT][1];
+#pragma unroll
+    for (int f = 0; f < FT; ++f)
+      acc[f][0] = f32x4{0.f, 0.f, 0.f, 0.f};
+    const char *const w = mine + buffer * kW;
+    multiply_slice<ABITS, 1, FT>(p, w, w + 16 * FT * kWPiece, a, a_scales, k0, a_rows, acc);
+    f32x4 *const sums = reinterpret_cast<f32x4 *>(mine + 2 * kW + buffer * FT * 1024);
+#pragma unroll
+    for (int f = 0; f < FT; ++f)
+      sums[f * 64 + lane] = acc[f][0];
+    // Sums and the weights just read are written again after the next barrier but this one.
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_waitcnt(0xc07f);
+    __builtin_amdgcn_s_barrier();  // (__syncthreads() would wait for the next weights)
+    asm volatile("" ::: "memory");
+    add_and_finish<EPI, 1, FT>(p, mx_lds + 2 * kW + buffer * FT * 1024, stride, 0, tile * (16 * FT));
   }
 }
 
@@ -749,7 +841,26 @@ hipError_t launch_rows(void (*kernel)(GemmArgs, int), const GemmArgs &p, hipStre
 
 // ---- the forms, and which one a call takes ----
 
-enum Form : int { kRows16, kRows32, kRows32x32, kTile64, kTile64x128, kTile128, kTile256, kForms };
+enum Form : int { kRows16, kRows32, kRows32x32, kTile64, kTile64x128, kTile128, kTile256, kStream16, kStream32, kForms };
+
+// k up to 512 a wave, m up to 16.
+template <int ABITS, int FT>
+hipError_t launch_stream(void (*kernel)(GemmArgs, int), const GemmArgs &p, hipStream_t s) {
+  const int per_kib = 1024 / (kSliceK * ABITS / 8);
+  const int a_rows = (p.m + per_kib - 1) / per_kib * per_kib;
+  const int waves = (p.k + kSliceK - 1) / kSliceK, bytes = waves * stream_region<ABITS, FT>(a_rows);
+  if (p.m > 16 || waves > 16 || bytes > 160 * 1024)
+    return hipErrorInvalidValue;
+  const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void *>(kernel),
+                                           hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024);
+  if (e != hipSuccess)
+    return e;
+  const int64_t tiles = (int64_t(p.n) + 16 * FT - 1) / (16 * FT);
+  const int per_cu = std::max(1, std::min(160 * 1024 / bytes, 32 / waves));
+  hipLaunchKernelGGL(kernel, dim3(unsigned(std::min<int64_t>(tiles, int64_t(gemm_cus()) * per_cu))),
+                     dim3(unsigned(waves * 64)), bytes, s, p, a_rows);
+  return hipGetLastError();
+}
 
 template <int ABITS, int EPI> hipError_t launch_form(int form, const GemmArgs &p, hipStream_t s) {
 #define YUEAR_MX_ROWS(MT, FT) launch_rows<ABITS, MT, FT>(rows_kernel<ABITS, EPI, MT, FT>, p, s)
@@ -768,6 +879,8 @@ template <int ABITS, int EPI> hipError_t launch_form(int form, const GemmArgs &p
       if (p.k % 256 == 0)
         return YUEAR_MX_TILE(256, 256, 4, 2, 1, 256, 2);
     return YUEAR_MX_TILE(256, 256, 4, 2, 1, 128, 3);
+  case kStream16: return launch_stream<ABITS, 1>(stream_kernel<ABITS, EPI, 1>, p, s);
+  case kStream32: return launch_stream<ABITS, 2>(stream_kernel<ABITS, EPI, 2>, p, s);
   }
 #undef YUEAR_MX_ROWS
 #undef YUEAR_MX_TILE
@@ -782,25 +895,40 @@ template <int ABITS> hipError_t launch(int form, const GemmArgs &p, hipStream_t 
   }
 }
 
-// Estimated us of m x n x k by a form, fitted on MI355X with the weights from HBM to 1100
-// calls (1-3072 tokens, 16-98304 features, K 256-8192; 4-16% rms).
+// Estimated us of m x n x k by a form, infinite where it cannot run; fitted on MI355X with the
+// weights from HBM to 2000 calls of up to 16 tokens (16-84000 features, K 256-8192; 7-12% rms)
+// and 500 of more (up to 3072; 4-16%).
 double form_time(int form, int bits, int m, int n, int k, int cus) {
   const bool a8 = bits == 8;
   const double kk = k / 1024.0;
   auto tiles = [&](int bm, int bn) { return double((m + bm - 1) / bm) * double((n + bn - 1) / bn); };
-  if (form <= kRows32x32) {
-    // the launch, each 512 of K that a wave takes after another, the bytes of W and of A
-    const int bm = form == kRows32x32 ? 32 : 16, bn = form == kRows16 ? 16 : 32;
+  if (form <= kRows32x32 || form >= kStream16) {
+    const bool stream = form >= kStream16;
+    const int bm = form == kRows32x32 ? 32 : 16, bn = form == kRows16 || form == kStream16 ? 16 : 32;
     const int per_kib = a8 ? 2 : 4, rows = (std::min(m, bm) + per_kib - 1) / per_kib * per_kib;
-    const int region = bn * (kSliceK / 2 + 16) + rows * (kSliceK * bits / 8 + 16);
+    const int a_bytes = rows * (kSliceK * bits / 8 + 16), w_bytes = bn * (kSliceK / 2 + 16);
     const int slices = (k + kSliceK - 1) / kSliceK;
-    const int waves = std::min({slices, 160 * 1024 / region, 16});
-    static const double fit[2][3][5] = {
-        {{2.097, 0.781, 0.021, 0.014, 0.003}, {1.789, 1.261, 0.021, 0.022, 0.019}, {3.232, 0.377, 0.031, 0.0, 0.16}},
-        {{2.819, 0.0, 0.02, 0.018, 0.006}, {1.667, 1.308, 0.021, 0.023, 0.023}, {3.107, 0.321, 0.027, 0.0, 0.183}}};
-    const double *c = fit[a8 ? 0 : 1][form];
-    const double t = tiles(bm, bn) / cus;
-    return c[0] + c[1] * ((slices + waves - 1) / waves) + t * (kk * (c[2] * bn + c[3] * rows * bits / 8) + c[4]);
+    const double t = tiles(bm, bn);
+    if (!stream) {
+      // the launch, each 512 of K that a wave takes after another, the bytes of W and of A
+      const int waves = std::min({slices, 160 * 1024 / (w_bytes + a_bytes), 16});
+      static const double fit[2][3][5] = {
+          {{1.771, 1.134, 0.0199, 0.0169, 0.0}, {1.968, 1.104, 0.0217, 0.0196, 0.0}, {3.232, 0.377, 0.031, 0.0, 0.16}},
+          {{0.0, 2.815, 0.0199, 0.019, 0.0}, {1.763, 1.264, 0.021, 0.0245, 0.0}, {3.107, 0.321, 0.027, 0.0, 0.183}}};
+      const double *c = fit[a8 ? 0 : 1][form];
+      return c[0] + c[1] * ((slices + waves - 1) / waves) +
+             t / cus * (kk * (c[2] * bn + c[3] * rows * bits / 8) + c[4]);
+    }
+    // the launch, each 16 or 32 features of a workgroup, the bytes of W and once those of A
+    const int bytes = slices * (2 * (w_bytes + bn * 64) + a_bytes);
+    if (m > 16 || slices > 16 || bytes > 160 * 1024)
+      return __builtin_inf();
+    const double grid = std::min(t, double(cus) * std::max(1, std::min(160 * 1024 / bytes, 32 / slices)));
+    static const double fit[2][2][5] = {{{2.041, 0.714, 0.0142, 0.0049, 0.0843}, {2.161, 0.823, 0.0128, 0.0115, 0.0486}},
+                                        {{2.052, 0.643, 0.0151, 0.0, 0.0788}, {2.036, 0.77, 0.0129, 0.0242, 0.0656}}};
+    const double *c = fit[a8 ? 0 : 1][form - kStream16];
+    return c[0] + c[1] * std::ceil(t / grid) + c[2] * t / cus * kk * bn + c[3] * grid / cus * kk * rows * bits / 8 +
+           c[4] * kk;
   }
   // the launch, full rounds of tiles, and a last one by how many CUs it has work for
   static const int shape[4][3] = {{64, 64, 1}, {64, 128, 1}, {128, 128, 2}, {256, 256, 1}};
@@ -818,8 +946,9 @@ double form_time(int form, int bits, int m, int n, int k, int cus) {
   return c[0] + full * (c[1] + c[2] * kk) + (rest > 0 ? c[3] + c[4] * kk + rest * (c[5] + c[6] * kk) : 0.0);
 }
 
-// The form of least estimated time: rows where there are few tokens, the larger tiles the
-// more there are to fill the CUs with. The sum over K is split as the form is (by waves, in
+// The form of least estimated time: for few tokens rows, streamed where a workgroup can keep A
+// (137 MB of weights, 5 tokens: 31 -> 23 us), the larger tiles the more there are to fill the
+// CUs with. The sum over K is split as the form is (by waves, in
 // order), so the form decides the order of the sums.
 int pick_form(int bits, int m, int n, int k) {
   const int cus = gemm_cus();

@@ -776,19 +776,20 @@ def _mx_bf16(t, rows, k, index, name, what):
 
 
 def _mx_out(x, rows, k, bits, out, index, name):
-    """The given pair, or a new one, and its numbers."""
+    """The given pair, or a new one, and (codes' address, row stride, scales' address, row stride)."""
     if out is None:
         if bits == 8:
-            codes = _T.empty((rows, k), dtype=_E4M3, device=x.device)
+            codes = x.new_empty((rows, k), dtype=_E4M3)
         elif bits == 4:
-            codes = _T.empty((rows, k // 2), dtype=_UINT8, device=x.device)
+            codes = x.new_empty((rows, k // 2), dtype=_UINT8)
         else:
             _refuse(name, "bits is 8 or 4")
-        out = codes, _T.empty((rows, k // 32), dtype=_E8M0, device=x.device)
+        scales = x.new_empty((rows, k // 32), dtype=_E8M0)
+        return (codes, scales), codes.data_ptr(), k * bits // 8, scales.data_ptr(), k // 32
     got = _mx_rows(out, index, name)
     if got[:3] != (rows, k, bits):
         _refuse(name, f"out is a pair of [{rows}, {k}] values in {bits} bits")
-    return out, got
+    return out, *got[3:]
 
 
 def _mx_shape(x, name):
@@ -806,7 +807,7 @@ def mx_quantize(x, bits=8, out=None, stream=None):
     stream = _stream(stream, index, name, out)
     rows, k = _mx_shape(x, name)
     x_stride = _mx_bf16(x, rows, k, index, name, "x")
-    out, (_, _, _, codes, stride, scales, scale_stride) = _mx_out(x, rows, k, bits, out, index, name)
+    out, codes, stride, scales, scale_stride = _mx_out(x, rows, k, bits, out, index, name)
     _call(lib.yuear_op_mx_quantize, name, index, x.data_ptr(), x_stride, rows, k, bits, codes, stride, scales,
           scale_stride, stream)
     return out
@@ -818,8 +819,9 @@ def mx_dequantize(packed, out=None, stream=None):
     stream = _stream(stream, index, name, out)
     rows, k, bits, codes, stride, scales, scale_stride = _mx_rows(packed, index, name)
     if out is None:
-        out = _T.empty((rows, k), dtype=_BF16, device=packed[0].device)
-    out_stride = _mx_bf16(out, rows, k, index, name, "out")
+        out, out_stride = packed[0].new_empty((rows, k), dtype=_BF16), k
+    else:
+        out_stride = _mx_bf16(out, rows, k, index, name, "out")
     _call(lib.yuear_op_mx_dequantize, name, index, codes, stride, scales, scale_stride, rows, k, bits, out.data_ptr(),
           out_stride, stream)
     return out
@@ -839,11 +841,13 @@ def mx_rms_norm(x, gain, eps=1e-5, residual=None, bits=8, out=None, sum_out=None
     if residual is not None:
         residual_at, residual_stride = residual.data_ptr(), _mx_bf16(residual, rows, k, index, name, "residual")
         if sum_out is None:
-            sum_out = _T.empty((rows, k), dtype=_BF16, device=x.device)
-        sum_at, sum_stride = sum_out.data_ptr(), _mx_bf16(sum_out, rows, k, index, name, "sum_out")
+            sum_out, sum_stride = x.new_empty((rows, k)), k
+        else:
+            sum_stride = _mx_bf16(sum_out, rows, k, index, name, "sum_out")
+        sum_at = sum_out.data_ptr()
     elif sum_out is not None:
         _refuse(name, "sum_out comes with a residual")
-    out, (_, _, _, codes, stride, scales, scale_stride) = _mx_out(x, rows, k, bits, out, index, name)
+    out, codes, stride, scales, scale_stride = _mx_out(x, rows, k, bits, out, index, name)
     _call(lib.yuear_op_mx_rms_norm, name, index, x.data_ptr(), x_stride, residual_at, residual_stride, gain.data_ptr(),
           eps, rows, k, bits, codes, stride, scales, scale_stride, sum_at, sum_stride, stream)
     return out, sum_out
@@ -867,8 +871,9 @@ def mx_gemm(a, w, residual=None, swiglu=False, out=None, stream=None):
     if residual is not None:
         residual_at, residual_stride = residual.data_ptr(), _mx_bf16(residual, m, n, index, name, "residual")
     if out is None:
-        out = _T.empty((m, width), dtype=_BF16, device=a[0].device)
-    ldc = _mx_bf16(out, m, width, index, name, "out")
+        out, ldc = a[0].new_empty((m, width), dtype=_BF16), width
+    else:
+        ldc = _mx_bf16(out, m, width, index, name, "out")
     _call(lib.yuear_op_mx_gemm, name, index, a_codes, a_stride, a_scales, a_scale_stride, a_bits, w_codes, w_stride,
           w_scales, w_scale_stride, m, n, k, residual_at, residual_stride, out.data_ptr(), ldc, 1 if swiglu else 0, stream)
     return out
