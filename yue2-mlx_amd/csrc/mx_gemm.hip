@@ -493,7 +493,7 @@ __device__ __forceinline__ void tile(const GemmArgs &p) {
                 "tile");
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave_id = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int team = wave_id / T::kTeam, wave = wave_id % T::kTeam;
+  const int team = KS == 1 ? 0 : wave_id / T::kTeam, wave = KS == 1 ? wave_id : wave_id % T::kTeam;
   const int ring = team * T::kRing;
   const int k_begin = p.k / KSTEP * team / KS * KSTEP;  // this team's K
   const int k_len = p.k / KSTEP * (team + 1) / KS * KSTEP - k_begin;
