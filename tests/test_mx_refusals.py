@@ -73,14 +73,14 @@ def gemm(lib, a=BASE, a_stride=256, a_scales=BASE + (1 << 20), a_scales_stride=8
     dict(swiglu=1, residual=BASE + (5 << 20), residual_stride=6), dict(residual=BASE + (5 << 20), residual_stride=5),
     dict(residual=BASE + (4 << 20) + 2, residual_stride=6), dict(residual=BASE + (4 << 20), residual_stride=8),
     dict(c=BASE), dict(c=BASE + (1 << 20)), dict(c=BASE + (2 << 20) - 16), dict(c=BASE + (3 << 20) + 4),
-    dict(ldc=1 << 31), dict(w_stride=(1 << 22) + 16),
+    dict(ldc=1 << 31), dict(m=(1 << 30) + 1), dict(n=(1 << 30) + 1, ldc=1 << 31), dict(w_stride=(1 << 22) + 16),
 ])
 def test_gemm_refused(yuear_lib, bad):
     assert gemm(yuear_lib.lib, **bad) == 1
 
 
 def test_forms_refused(yuear_lib):
-    for form in (-2, 9):
+    for form in (-2, 10):
         assert yuear_lib.lib.yuear_op_mx_gemm_form(BASE, 256, BASE + (1 << 20), 8, 8, BASE + (2 << 20), 128, BASE + (3 << 20),
                                                    8, 4, 6, 256, None, 0, BASE + (4 << 20), 6, 0, form, None) == 1
 

@@ -28,7 +28,8 @@ struct GemmArgs {
   int wide;  // 16-byte stores (and residual loads) where a tile is whole
 };
 
-constexpr int kStep = 128;  // K of an MFMA
+constexpr int kStep = 128;           // K of an MFMA
+constexpr int kMaxRows = 1 << 30;    // tokens, features
 
 // Range of a tile's `rows` rows (at most 256) from `base`, of which the last ends
 // with its data: what lies past it reads as zero.
@@ -433,9 +434,7 @@ __device__ __forceinline__ bool tile_of(int b, int grid, int n, int tiles_m, int
 }
 
 __device__ __forceinline__ int slot_of(int bytes, int row, int chunk) {
-  return bytes == 256   ? chunk ^ (row & 15)
-         : bytes == 128 ? chunk ^ ((row >> 1) & 7)
-                        : chunk ^ (((row >> 2) & 1) | ((row >> 3) & 2));
+  return bytes == 128 ? chunk ^ ((row >> 1) & 7) : chunk ^ (((row >> 2) & 1) | ((row >> 3) & 2));
 }
 
 // s_waitcnt for all but the last `loads` vector memory operations, and every LDS read.
@@ -504,8 +503,8 @@ __device__ __forceinline__ void tile(const GemmArgs &p) {
   // this wave's KiB blocks of a stage's A and W: lane l fills slot l
   // (the slots repeat after 16 rows, of 64 bytes after 32: blocks that far apart share an offset)
   constexpr int kARows = 1024 / T::kARow, kWRows = 1024 / T::kWRow;  // of a block
-  constexpr int AP = kARows == 4 ? 4 : 2, WP = kWRows == 4 ? 4 : 2;  // blocks of 16 or 32 rows
-  static_assert((APW % AP == 0 || APW == 1) && (WPW % WP == 0 || WPW == 1), "blocks");
+  constexpr int AP = APW % 2 ? APW : 2, WP = WPW % 2 ? WPW : 2;
+  static_assert(kARows >= 8 && kWRows >= 8, "blocks");
   uint32_t from_a[AP], from_w[WP], from_s[SPW];
 #pragma unroll
   for (int i = 0; i < AP; ++i) {
@@ -800,14 +799,14 @@ __device__ __forceinline__ void tile(const GemmArgs &p) {
 }
 
 template <int ABITS, int EPI, int BM, int BN, int WM, int WN, int KS, int KSTEP, int STAGES>
-__global__ __launch_bounds__(WM * WN * KS * 64, 2) void tile_kernel(GemmArgs p) {
+__global__ __launch_bounds__(WM * WN * KS * 64, BM * BN > WM * WN * 8192 ? 1 : 2) void tile_kernel(GemmArgs p) {
   tile<ABITS, EPI, BM, BN, WM, WN, KS, KSTEP, STAGES>(p);
 }
 
 template <class T>
 hipError_t launch_tile(void (*kernel)(GemmArgs), const GemmArgs &p, hipStream_t s) {
   const int64_t tiles = ((int64_t(p.m) + T::kBM - 1) / T::kBM) * ((int64_t(p.n) + T::kBN - 1) / T::kBN);
-  if (tiles >= int64_t(1) << 22)  // threads of the grid count in 32 bits
+  if (tiles > int64_t(1) << 22)  // threads of the grid count in 32 bits (m, n <= 2^30 and what memory holds stay below)
     return hipErrorInvalidValue;
   const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void *>(kernel),
                                            hipFuncAttributeMaxDynamicSharedMemorySize, T::kLds);
@@ -841,7 +840,19 @@ hipError_t launch_rows(void (*kernel)(GemmArgs, int), const GemmArgs &p, hipStre
 
 // ---- the forms, and which one a call takes ----
 
-enum Form : int { kRows16, kRows32, kRows32x32, kTile64, kTile64x128, kTile128, kTile256, kStream16, kStream32, kForms };
+enum Form : int {
+  kRows16,
+  kRows32,
+  kRows32x32,
+  kTile64,
+  kTile64x128,
+  kTile128,
+  kTile192,
+  kTile256,
+  kStream16,
+  kStream32,
+  kForms
+};
 
 // k up to 512 a wave, m up to 16.
 template <int ABITS, int FT>
@@ -873,8 +884,13 @@ template <int ABITS, int EPI> hipError_t launch_form(int form, const GemmArgs &p
   case kTile64: return YUEAR_MX_TILE(64, 64, 1, 1, 4, 128, (ABITS == 8 ? 3 : 4));
   case kTile64x128: return YUEAR_MX_TILE(64, 128, 1, 4, 1, 128, 6);
   case kTile128: return YUEAR_MX_TILE(128, 128, 2, 2, 1, 128, 3);
+  // 4 bits: rows of 128 bytes (256 of K) a load where K has them; 64 bytes ask L2 as often
+  case kTile192:
+    if constexpr (ABITS == 4)
+      if (p.k % 256 == 0)
+        return YUEAR_MX_TILE(192, 192, 2, 2, 1, 256, 3);
+    return YUEAR_MX_TILE(192, 192, 2, 2, 1, 128, 3);
   case kTile256:
-    // 4 bits: rows of 128 bytes (256 of K) a load where K has them; 64 bytes ask L2 as often
     if constexpr (ABITS == 4)
       if (p.k % 256 == 0)
         return YUEAR_MX_TILE(256, 256, 4, 2, 1, 256, 2);
@@ -895,9 +911,9 @@ template <int ABITS> hipError_t launch(int form, const GemmArgs &p, hipStream_t 
   }
 }
 
-// Estimated us of m x n x k by a form, infinite where it cannot run; fitted on MI355X with the
-// weights from HBM to 2000 calls of up to 16 tokens (16-84000 features, K 256-8192; 7-12% rms)
-// and 500 of more (up to 3072; 4-16%).
+// Estimated us of m x n x k by a form, infinite where it cannot run; fitted on MI355X to 2200
+// calls of up to 16 tokens (48-84000 features, K 256-8192; 7-12% rms) and 900 of more (up to 3072
+// tokens; 4-13%, 32 x 32 features 15%).
 double form_time(int form, int bits, int m, int n, int k, int cus) {
   const bool a8 = bits == 8;
   const double kk = k / 1024.0;
@@ -910,6 +926,8 @@ double form_time(int form, int bits, int m, int n, int k, int cus) {
     const int slices = (k + kSliceK - 1) / kSliceK;
     const double t = tiles(bm, bn);
     if (!stream) {
+      if (n / bn >= (1 << 22) - 1 || m / bm >= 65535)  // past a launch's grid
+        return __builtin_inf();
       // the launch, each 512 of K that a wave takes after another, the bytes of W and of A
       const int waves = std::min({slices, 160 * 1024 / (w_bytes + a_bytes), 16});
       static const double fit[2][3][5] = {
@@ -931,16 +949,20 @@ double form_time(int form, int bits, int m, int n, int k, int cus) {
            c[4] * kk;
   }
   // the launch, full rounds of tiles, and a last one by how many CUs it has work for
-  static const int shape[4][3] = {{64, 64, 1}, {64, 128, 1}, {128, 128, 2}, {256, 256, 1}};
-  static const double fit[2][4][7] = {{{1.524, 3.182, 1.706, 2.885, 0.787, 0.189, 1.072},
-                                       {1.627, 2.555, 3.051, 2.061, 1.73, 0.436, 1.28},
-                                       {4.05, 3.489, 8.666, 0.0, 2.487, 3.698, 4.451},
-                                       {6.695, 6.056, 12.041, 1.699, 7.315, 3.586, 3.695}},
-                                      {{1.331, 3.193, 1.467, 2.832, 0.55, 0.31, 1.083},
-                                       {2.798, 1.22, 2.497, 0.556, 1.473, 0.586, 0.994},
-                                       {3.756, 3.377, 7.138, 0.0, 1.919, 3.606, 3.907},
-                                       {5.723, 6.185, 8.392, 1.894, 4.788, 3.998, 2.257}}};
+  static const int shape[5][3] = {{64, 64, 1}, {64, 128, 1}, {128, 128, 2}, {192, 192, 1}, {256, 256, 1}};
+  static const double fit[2][5][7] = {{{1.552, 3.05, 1.521, 2.75, 0.914, 0.0, 0.844},
+                                       {1.674, 2.585, 2.717, 2.049, 1.792, 0.305, 0.848},
+                                       {4.318, 3.74, 7.629, 0.0, 2.066, 3.503, 5.039},
+                                       {4.678, 4.909, 7.272, 1.57, 5.477, 2.678, 1.316},
+                                       {5.413, 6.405, 11.547, 2.506, 7.678, 4.157, 2.53}},
+                                      {{1.54, 3.019, 1.377, 2.755, 0.499, 0.0, 0.93},
+                                       {2.802, 1.283, 2.168, 0.659, 1.475, 0.109, 0.928},
+                                       {2.964, 4.056, 6.095, 0.0, 2.187, 4.893, 3.66},
+                                       {5.008, 4.674, 4.908, 1.048, 3.729, 3.404, 1.039},
+                                       {4.81, 6.567, 7.868, 2.784, 4.682, 3.522, 2.669}}};
   const int *of = shape[form - kTile64];
+  if (form != kTile256 && tiles(of[0], of[1]) >= (1 << 22))
+    return __builtin_inf();
   const double *c = fit[a8 ? 0 : 1][form - kTile64];
   const double slots = double(cus) * of[2], t = tiles(of[0], of[1]), full = std::floor(t / slots), rest = t / slots - full;
   return c[0] + full * (c[1] + c[2] * kk) + (rest > 0 ? c[3] + c[4] * kk + rest * (c[5] + c[6] * kk) : 0.0);
@@ -979,7 +1001,7 @@ int32_t yuear_op_mx_gemm_form(const uint8_t *a, int64_t a_stride, const uint8_t 
   using namespace yuear;
   if (m == 0 || n == 0)
     return 0;
-  if (m < 0 || n < 0 || k % mx::kStep || (swiglu != 0 && swiglu != 1) || (swiglu && (n % 2 || residual)) ||
+  if (m < 0 || n < 0 || m > mx::kMaxRows || n > mx::kMaxRows || k % mx::kStep || (swiglu != 0 && swiglu != 1) || (swiglu && (n % 2 || residual)) ||
       !mx::rows_ok(a, a_stride, a_scales, a_scales_stride, k, a_bits) ||
       !mx::rows_ok(w, w_stride, w_scales, w_scales_stride, k, 4) || !mx::aligned(a_scales, 4) ||
       !mx::aligned(w_scales, 4) || a_scales_stride % 4 || w_scales_stride % 4 || !mx::aligned(c, 2) || form < -1 ||
