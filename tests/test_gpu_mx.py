@@ -442,6 +442,47 @@ def test_empty(torch, yuear_lib):
     assert yuear_lib.mx_gemm(some, (w[0][:0], w[1][:0])).shape == (3, 0)
 
 
+def test_rows_past_32_bits(torch, yuear_lib):
+    """Arrays of more than 2^32 bytes: the last rows' codes, norm, values and products."""
+    rng = np.random.default_rng(21)
+    rows, k, n = 540_000, 8192, 24
+    tail = random_rows(rng, 40, k, "plain")
+    x = torch.zeros(rows, k, dtype=torch.bfloat16, device="cuda")
+    x[-40:] = bf16(torch, tail)
+    codes, scales = ref.quantize(ref.from_bf16(tail), 8)
+    a = yuear_lib.mx_quantize(x)
+    assert a[0].numel() > 2 ** 32
+    np.testing.assert_array_equal(raw(torch, a[0][-40:]), codes)
+    np.testing.assert_array_equal(raw(torch, a[1].view(torch.uint8)[-40:]), scales)
+    assert not a[0].view(torch.uint8)[:-40].any()
+    w = random_pair(rng, n, k, 4)
+    out = yuear_lib.mx_gemm(a, pair_of(torch, *w, 4))
+    assert not out[:-40].any()
+    check_gemm(torch, out[-40:], ref.values(codes, scales, 8), ref.values(*w, 4), 8, "store")
+    back = yuear_lib.mx_dequantize(a, out=x)
+    np.testing.assert_array_equal(bits_of(torch, back[-40:]), ref.to_bf16(ref.values(codes, scales, 8)))
+    x[-40:] = bf16(torch, tail)
+    got, _ = yuear_lib.mx_rms_norm(x, torch.ones(k, dtype=torch.bfloat16, device="cuda"), EPS, out=a)
+    check_norm(torch, (got[0][-40:], got[1].view(torch.uint8)[-40:].view(torch.float8_e8m0fnu)), ref.from_bf16(tail),
+               np.ones(k), 8)
+    assert not got[0].view(torch.uint8)[:-40].any()
+
+
+def test_outputs_past_32_bits(torch, yuear_lib):
+    """A product of more than 2^31 values, each form's last rows and columns."""
+    rng = np.random.default_rng(22)
+    m, n, k = 40_000, 65_600, 128
+    a, w = pair_of(torch, *random_pair(rng, m, k, 8), 8), pair_of(torch, *random_pair(rng, n, k, 4), 4)
+    out = torch.empty(m, n, dtype=torch.bfloat16, device="cuda")
+    rows, cols = slice(m - 300, m), slice(n - 300, n)
+    va = ref.values(raw(torch, a[0][rows]), raw(torch, a[1].view(torch.uint8)[rows]), 8)
+    vw = ref.values(raw(torch, w[0][cols]), raw(torch, w[1].view(torch.uint8)[cols]), 4)
+    for form in (-1, 2, 4, 5, 6, 7):
+        out[rows].zero_()
+        forced(torch, yuear_lib, form, a, w, 8, out)
+        check_gemm(torch, out[rows, cols], va, vw, 8, "store")
+
+
 # ---- together ----
 
 def mlp(yuear_lib, x, stream, gain, w_up, w_down, **kw):
