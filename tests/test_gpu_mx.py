@@ -373,6 +373,28 @@ def test_gemm_rows_apart(torch, yuear_lib, m, n, k, bits):
         check_gemm(torch, out, ref.values(*a, bits), ref.values(*w, 4), bits, "store")
 
 
+@pytest.mark.parametrize("m,n,form", [(1, 38, 0), (9, 70, 1), (9, 70, 8), (16, 102, 9), (33, 71, 2), (65, 133, 3), (66, 262, 4),
+                                      (130, 263, 5), (200, 390, 6), (261, 519, 7)])
+@pytest.mark.parametrize("epilogue", ["store", "swiglu", "residual"])
+@pytest.mark.parametrize("at,more", [(1, 2), (2, 1), (3, 5), (4, 4)])
+def test_outputs_at_any_even_address(torch, yuear_lib, m, n, form, epilogue, at, more):
+    """Outputs and residuals that are columns of wider arrays of odd and even widths."""
+    if epilogue == "swiglu":
+        n -= n % 2
+    rng = np.random.default_rng(n + at)
+    a, w = random_pair(rng, m, 384, 8), random_pair(rng, n, 384, 4)
+    width = n // 2 if epilogue == "swiglu" else n
+    wide = torch.full((m + 1, at + width + more), 3.0, dtype=torch.bfloat16, device="cuda")
+    r = rng.standard_normal((m, width))
+    resid = torch.full((m, width + 3 + at), float("nan"), dtype=torch.bfloat16, device="cuda")
+    r = resid[:, 3:3 + width].copy_(torch.from_numpy(r))
+    out = wide[:m, at:at + width]
+    forced(torch, yuear_lib, form, pair_of(torch, *a, 8), pair_of(torch, *w, 4), 8, out,
+           r if epilogue == "residual" else None, epilogue == "swiglu")
+    check_gemm(torch, out, ref.values(*a, 8), ref.values(*w, 4), 8, epilogue, ref.from_bf16(bits_of(torch, r)))
+    assert (wide[m:] == 3).all() and (wide[:, :at] == 3).all() and (wide[:, at + width:] == 3).all()
+
+
 @pytest.mark.parametrize("m,form", [(3, 0), (3, 1), (3, 8), (3, 9), (40, 2), (40, 3), (40, 4), (300, 5), (300, 6), (300, 7)])
 def test_gemm_not_finite(torch, yuear_lib, m, form):
     """NaN scales and NaN codes reach their rows and columns, nothing else. Sums past 2^128 are not finite:

@@ -14,6 +14,7 @@ namespace {
 
 typedef int i32x8 __attribute__((ext_vector_type(8)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 
 enum Epilogue : int { kStore = 0, kResidual = 1, kSwiglu = 2 };
 
@@ -25,8 +26,17 @@ struct GemmArgs {
   uint16_t *c;
   int64_t residual_stride, ldc;
   int epilogue;
-  int wide;  // 16-byte stores (and residual loads) where a tile is whole
 };
+
+// Outputs and residuals lie at any even address: the hardware takes loads and stores of 4 to 16
+// bytes there, and the type tells the compiler that this is one.
+template <class T> struct __attribute__((packed, aligned(2))) AtHalves { T v; };
+template <class T> __device__ __forceinline__ T load_at(const uint16_t *p) {
+  return reinterpret_cast<const AtHalves<T> *>(p)->v;
+}
+template <class T> __device__ __forceinline__ void store_at(uint16_t *p, T v) {
+  reinterpret_cast<AtHalves<T> *>(p)->v = v;
+}
 
 constexpr int kStep = 128;           // K of an MFMA
 constexpr int kMaxRows = 1 << 30;    // tokens, features
@@ -51,48 +61,62 @@ __device__ __forceinline__ float silu_times(float gate, float up) {
   return gate * fmaf(s * (s - 1.0f), off * 0.693147182f, s) * up;
 }
 
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+  return uint32_t(f2bf(lo)) | uint32_t(f2bf(hi)) << 16;
+}
+
 // A lane's features n .. n + 3 (n a multiple of 4) of token row m < p.m.
 template <int EPI>
 __device__ __forceinline__ void finish4(const GemmArgs &p, int m, int n, const float (&v)[4]) {
-  if (n >= p.n)
-    return;
+  const bool whole = n + 4 <= p.n;
   if (EPI == kSwiglu) {
     uint16_t *c = p.c + m * p.ldc + (n >> 1);
-    c[0] = f2bf(silu_times(v[0], v[1]));
-    if (n + 2 < p.n)
-      c[1] = f2bf(silu_times(v[2], v[3]));
+    const uint32_t out = pack2(silu_times(v[0], v[1]), silu_times(v[2], v[3]));
+    if (whole)
+      store_at(c, out);
+    else if (n < p.n)
+      c[0] = uint16_t(out);
     return;
   }
   uint16_t *c = p.c + m * p.ldc + n;
   const uint16_t *r = p.residual + m * p.residual_stride + n;
+  if (whole) {
+    float x[4] = {v[0], v[1], v[2], v[3]};
+    if (EPI == kResidual) {
+      const u32x2 add = load_at<u32x2>(r);
 #pragma unroll
-  for (int e = 0; e < 4; ++e)
+      for (int e = 0; e < 2; ++e) {
+        x[2 * e] += bflo(add[e]);
+        x[2 * e + 1] += bfhi(add[e]);
+      }
+    }
+    store_at(c, u32x2{pack2(x[0], x[1]), pack2(x[2], x[3])});
+    return;
+  }
+#pragma unroll
+  for (int e = 0; e < 3; ++e)
     if (n + e < p.n)
       c[e] = f2bf(EPI == kResidual ? bf2f(r[e]) + v[e] : v[e]);
-}
-
-__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
-  return uint32_t(f2bf(lo)) | uint32_t(f2bf(hi)) << 16;
 }
 
 // What finish32() adds, read ahead of it.
 __device__ __forceinline__ void residual32(const GemmArgs &p, int m, int n, int h,
                                            u32x4 (&residual)[2]) {
-  if (!p.wide || n + 32 > p.n || m >= p.m)
+  if (n + 32 > p.n || m >= p.m)
     return;
   const uint16_t *r = p.residual + m * p.residual_stride + n + 16 * h;
-  residual[0] = *reinterpret_cast<const u32x4 *>(r);
-  residual[1] = *reinterpret_cast<const u32x4 *>(r + 8);
+  residual[0] = load_at<u32x4>(r);
+  residual[1] = load_at<u32x4>(r + 8);
 }
 
 // A 32 x 32 MFMA tile, lane 32 h + r with features n + 8 q + 4 h + [0, 4) of token m
-// at v[4 q ..]. Where the rows allow it (p.wide, whole tile) the lanes of a token
-// trade halves first, so that each stores 16 bytes: h = 0 the features (SwiGLU
-// outputs) below 16 (8), h = 1 the others.
+// at v[4 q ..]. Where all features exist the lanes of a token trade halves first, so
+// that each stores 16 bytes: h = 0 the features (SwiGLU outputs) below 16 (8), h = 1
+// the others.
 template <int EPI>
 __device__ __forceinline__ void finish32(const GemmArgs &p, int m, int n, int h,
                                          const float (&v)[16], const u32x4 (&residual)[2]) {
-  if (!p.wide || n + 32 > p.n) {
+  if (n + 32 > p.n) {
     if (m < p.m)
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
@@ -109,7 +133,7 @@ __device__ __forceinline__ void finish32(const GemmArgs &p, int m, int n, int h,
     permlane32_swap(w[0], w[2]);
     permlane32_swap(w[1], w[3]);
     if (m < p.m)
-      *reinterpret_cast<u32x4 *>(p.c + m * p.ldc + (n >> 1) + 8 * h) = u32x4{w[0], w[2], w[1], w[3]};
+      store_at(p.c + m * p.ldc + (n >> 1) + 8 * h, u32x4{w[0], w[2], w[1], w[3]});
     return;
   }
   uint32_t f[16];
@@ -138,8 +162,8 @@ __device__ __forceinline__ void finish32(const GemmArgs &p, int m, int n, int h,
         x[2 * e + 1] += bfhi(r[e]);
       }
     }
-    *reinterpret_cast<u32x4 *>(p.c + m * p.ldc + at) =
-        u32x4{pack2(x[0], x[1]), pack2(x[2], x[3]), pack2(x[4], x[5]), pack2(x[6], x[7])};
+    store_at(p.c + m * p.ldc + at,
+             u32x4{pack2(x[0], x[1]), pack2(x[2], x[3]), pack2(x[4], x[5]), pack2(x[6], x[7])});
   }
 }
 
@@ -1023,9 +1047,7 @@ int32_t yuear_op_mx_gemm_form(const uint8_t *a, int64_t a_stride, const uint8_t 
     return int32_t(hipErrorInvalidValue);
   const mx::GemmArgs p{a, a_scales, w, w_scales, a_stride, a_scales_stride, w_stride, w_scales_stride, m, n, k,
                        residual, c, residual_stride, ldc,
-                       swiglu ? mx::kSwiglu : residual ? mx::kResidual : mx::kStore,
-                       mx::aligned(c, 16) && ldc % 8 == 0 &&
-                           (!residual || (mx::aligned(residual, 16) && residual_stride % 8 == 0))};
+                       swiglu ? mx::kSwiglu : residual ? mx::kResidual : mx::kStore};
   const hipStream_t st = static_cast<hipStream_t>(stream);
   if (form < 0)
     form = mx::pick_form(a_bits, m, n, k);
