@@ -56,13 +56,15 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_rsrc(const uint8_t *base,
 __device__ __forceinline__ float silu_times(float gate, float up) {
   constexpr float kLog2e = 1.44269502f, kRest = 1.92596299e-8f;  // log2 e in two parts
   const float t = gate * -kLog2e;
-  const float off = __builtin_amdgcn_fmed3f(fmaf(gate, -kLog2e, -t) - gate * kRest, -1.f, 1.f);
+  const float off = fmaf(gate, -kRest, fmaf(gate, -kLog2e, -t)) * 0.693147182f;
   const float s = __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(t));
-  return gate * fmaf(s * (s - 1.0f), off * 0.693147182f, s) * up;
+  return gate * fmaf(fmaf(s, s, -s), __builtin_amdgcn_fmed3f(off, -1.f, 1.f), s) * up;
 }
 
 __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
-  return uint32_t(f2bf(lo)) | uint32_t(f2bf(hi)) << 16;
+  typedef float f32x2 __attribute__((ext_vector_type(2)));
+  typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+  return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{lo, hi}), bf16x2));
 }
 
 // A lane's features n .. n + 3 (n a multiple of 4) of token row m < p.m.
