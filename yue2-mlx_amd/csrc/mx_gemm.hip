@@ -937,9 +937,9 @@ template <int ABITS> hipError_t launch(int form, const GemmArgs &p, hipStream_t 
   }
 }
 
-// Estimated us of m x n x k by a form, infinite where it cannot run; fitted on MI355X to 2200
-// calls of up to 16 tokens (48-84000 features, K 256-8192; 7-12% rms) and 900 of more (up to 3072
-// tokens; 4-13%, 32 x 32 features 15%).
+// Estimated us of m x n x k by a form, infinite where it cannot run; fitted on MI355X to 4400
+// shapes in all forms (to 6000 tokens, 84000 features, K 128-8192; 6-13% rms where a form is
+// within 1.6 of the fastest). Over them what it picks takes 1.0% more than the fastest form.
 double form_time(int form, int bits, int m, int n, int k, int cus) {
   const bool a8 = bits == 8;
   const double kk = k / 1024.0;
@@ -954,38 +954,40 @@ double form_time(int form, int bits, int m, int n, int k, int cus) {
     if (!stream) {
       if (n / bn >= (1 << 22) - 1 || m / bm >= 65535)  // past a launch's grid
         return __builtin_inf();
-      // the launch, each 512 of K that a wave takes after another, the bytes of W and of A
+      // the launch, each 512 of K that a wave takes after another, each round of the workgroups
+      // that the CUs hold, the bytes of W, each workgroup
       const int waves = std::min({slices, 160 * 1024 / (w_bytes + a_bytes), 16});
+      const int held = std::max(1, std::min(160 * 1024 / (waves * (w_bytes + a_bytes)), 32 / waves));
       static const double fit[2][3][5] = {
-          {{1.771, 1.134, 0.0199, 0.0169, 0.0}, {1.968, 1.104, 0.0217, 0.0196, 0.0}, {3.232, 0.377, 0.031, 0.0, 0.16}},
-          {{0.0, 2.815, 0.0199, 0.019, 0.0}, {1.763, 1.264, 0.021, 0.0245, 0.0}, {3.107, 0.321, 0.027, 0.0, 0.183}}};
+          {{0.254, 1.274, 1.444, 0.0203, 0.0}, {0.681, 1.135, 1.365, 0.0189, 0.0}, {0.541, 1.268, 1.818, 0.0193, 0.0501}},
+          {{0.0, 1.708, 1.174, 0.0188, 0.0}, {0.697, 1.11, 1.303, 0.0182, 0.0}, {1.274, 1.147, 1.076, 0.0173, 0.0918}}};
       const double *c = fit[a8 ? 0 : 1][form];
-      return c[0] + c[1] * ((slices + waves - 1) / waves) +
-             t / cus * (kk * (c[2] * bn + c[3] * rows * bits / 8) + c[4]);
+      return c[0] + c[1] * ((slices + waves - 1) / waves) + c[2] * std::ceil(t / (double(cus) * held)) +
+             t / cus * (c[3] * kk * bn + c[4]);
     }
     // the launch, each 16 or 32 features of a workgroup, the bytes of W and once those of A
     const int bytes = slices * (2 * (w_bytes + bn * 64) + a_bytes);
     if (m > 16 || slices > 16 || bytes > 160 * 1024)
       return __builtin_inf();
     const double grid = std::min(t, double(cus) * std::max(1, std::min(160 * 1024 / bytes, 32 / slices)));
-    static const double fit[2][2][5] = {{{2.041, 0.714, 0.0142, 0.0049, 0.0843}, {2.161, 0.823, 0.0128, 0.0115, 0.0486}},
-                                        {{2.052, 0.643, 0.0151, 0.0, 0.0788}, {2.036, 0.77, 0.0129, 0.0242, 0.0656}}};
+    static const double fit[2][2][5] = {{{1.926, 0.757, 0.0138, 0.002, 0.0997}, {1.626, 1.285, 0.0088, 0.0101, 0.0998}},
+                                        {{1.901, 0.741, 0.0142, 0.0, 0.0663}, {1.506, 1.274, 0.0087, 0.0204, 0.0766}}};
     const double *c = fit[a8 ? 0 : 1][form - kStream16];
     return c[0] + c[1] * std::ceil(t / grid) + c[2] * t / cus * kk * bn + c[3] * grid / cus * kk * rows * bits / 8 +
            c[4] * kk;
   }
   // the launch, full rounds of tiles, and a last one by how many CUs it has work for
   static const int shape[5][3] = {{64, 64, 1}, {64, 128, 1}, {128, 128, 2}, {192, 192, 1}, {256, 256, 1}};
-  static const double fit[2][5][7] = {{{1.552, 3.05, 1.521, 2.75, 0.914, 0.0, 0.844},
-                                       {1.674, 2.585, 2.717, 2.049, 1.792, 0.305, 0.848},
-                                       {4.318, 3.74, 7.629, 0.0, 2.066, 3.503, 5.039},
-                                       {4.678, 4.909, 7.272, 1.57, 5.477, 2.678, 1.316},
-                                       {5.413, 6.405, 11.547, 2.506, 7.678, 4.157, 2.53}},
-                                      {{1.54, 3.019, 1.377, 2.755, 0.499, 0.0, 0.93},
-                                       {2.802, 1.283, 2.168, 0.659, 1.475, 0.109, 0.928},
-                                       {2.964, 4.056, 6.095, 0.0, 2.187, 4.893, 3.66},
-                                       {5.008, 4.674, 4.908, 1.048, 3.729, 3.404, 1.039},
-                                       {4.81, 6.567, 7.868, 2.784, 4.682, 3.522, 2.669}}};
+  static const double fit[2][5][7] = {{{1.957, 3.111, 1.389, 2.548, 0.748, 0.18, 0.795},
+                                       {1.234, 2.978, 2.319, 2.314, 1.868, 0.776, 0.654},
+                                       {0.85, 5.63, 6.703, 4.271, 1.741, 1.694, 5.379},
+                                       {3.525, 6.613, 6.164, 2.594, 5.338, 5.195, 0.645},
+                                       {0.591, 10.876, 9.663, 5.976, 7.548, 8.132, 1.331}},
+                                      {{1.35, 2.936, 1.339, 2.938, 0.478, 0.0, 0.971},
+                                       {2.87, 1.481, 1.862, 0.528, 1.506, 0.809, 0.599},
+                                       {2.458, 4.555, 5.584, 1.916, 1.703, 3.449, 3.095},
+                                       {5.728, 5.124, 4.198, 0.0, 3.757, 5.692, 0.15},
+                                       {3.142, 8.015, 6.513, 2.969, 4.77, 8.5, 0.893}}};
   const int *of = shape[form - kTile64];
   if (form != kTile256 && tiles(of[0], of[1]) >= (1 << 22))
     return __builtin_inf();
