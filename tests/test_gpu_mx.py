@@ -465,15 +465,15 @@ def test_empty(torch, yuear_lib):
 
 
 def test_rows_past_32_bits(torch, yuear_lib):
-    """Arrays of more than 2^32 bytes: the last rows' codes, norm, values and products."""
+    """More than 2^31 chunks of 8 values, 2^35 bytes: the last rows' codes, norm, values and products."""
     rng = np.random.default_rng(21)
-    rows, k, n = 540_000, 8192, 24
+    rows, k, n = 2_200_000, 8192, 24
     tail = random_rows(rng, 40, k, "plain")
     x = torch.zeros(rows, k, dtype=torch.bfloat16, device="cuda")
     x[-40:] = bf16(torch, tail)
     codes, scales = ref.quantize(ref.from_bf16(tail), 8)
     a = yuear_lib.mx_quantize(x)
-    assert a[0].numel() > 2 ** 32
+    assert a[0].numel() > 2 ** 34
     np.testing.assert_array_equal(raw(torch, a[0][-40:]), codes)
     np.testing.assert_array_equal(raw(torch, a[1].view(torch.uint8)[-40:]), scales)
     assert not a[0].view(torch.uint8)[:-40].any()

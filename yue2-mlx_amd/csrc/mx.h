@@ -13,6 +13,15 @@ constexpr int kBlock = 32;            // values of a scale
 constexpr int kMaxK = 1 << 20;        // values of a row
 constexpr int64_t kMaxStride = 1 << 22;  // bytes from row to row: 256 rows count in 32 bits
 
+// The workgroup's barrier after a wave's LDS operations. (__syncthreads() would wait for its
+// global memory operations too, loads into LDS and stores.)
+__device__ __forceinline__ void lds_barrier() {
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0)
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
+
 // ---- host-side checks ----
 inline bool aligned(const void *p, int bytes) {
   return p && (reinterpret_cast<uintptr_t>(p) & uintptr_t(bytes - 1)) == 0;

@@ -390,10 +390,7 @@ __global__ __launch_bounds__(1024) void stream_kernel(GemmArgs p, int a_rows) {
     for (int f = 0; f < FT; ++f)
       sums[f * 64 + lane] = acc[f][0];
     // Sums and the weights just read are written again after the next barrier but this one.
-    asm volatile("" ::: "memory");
-    __builtin_amdgcn_s_waitcnt(0xc07f);
-    __builtin_amdgcn_s_barrier();  // (__syncthreads() would wait for the next weights)
-    asm volatile("" ::: "memory");
+    lds_barrier();  // the next weights' loads go on
     add_and_finish<EPI, 1, FT>(p, mx_lds + 2 * kW + buffer * FT * 1024, stride, 0, tile * (16 * FT));
   }
 }

@@ -12,6 +12,8 @@
 //
 // All three are bound by memory: a lane moves 8 values, 16 bytes of bf16, so a
 // wave reads whole KiB, and four lanes share a scale (two DPP steps).
+#include <algorithm>
+
 #include "kernels.h"
 #include "mx.h"
 
@@ -79,51 +81,38 @@ __device__ __forceinline__ void store_codes(uint8_t *p, const uint32_t (&w)[BITS
     *reinterpret_cast<uint32_t *>(p) = w[0];
 }
 
-// Chunk of 8 values: row and place in it of chunk `first + t` of rows of `per`
-// chunks, first in chunk `at0` of row `row0`.
+// The rows' chunks of 8 values, `per` a row, in one sequence. A thread has one, and a
+// workgroup 256 of them: with four a thread, all read before the first is used, 3000 x
+// 8192 values in 8 bits take 15.8 us instead of 13.5, and 517 x 2048 in 4 bits and back
+// 6.7 instead of 4.8. (Past the grid's limit a thread goes on to the chunk that lies
+// all threads further.)
 struct Place {
   int64_t row;
   uint32_t chunk;
 };
-__device__ __forceinline__ Place place(int64_t row0, uint32_t at0, uint32_t t, uint32_t per) {
-  const uint32_t i = at0 + t, down = i / per;
-  return Place{row0 + down, i - down * per};
+__device__ __forceinline__ Place place(int64_t i, uint32_t per) {
+  const int64_t row = i / per;
+  return Place{row, uint32_t(i - row * per)};
 }
 
 constexpr int kThreads = 256;
-constexpr int kLoads = 4;  // chunks of a thread, all read before the first is used
+constexpr int64_t kMaxValues = int64_t(1) << 40;  // of a call: more than memory holds
 
 template <int BITS>
 __global__ __launch_bounds__(kThreads) void quantize_kernel(const uint16_t *x, int64_t x_stride,
                                                             int64_t chunks, uint32_t per,
                                                             uint8_t *codes, int64_t stride,
                                                             uint8_t *scales, int64_t scale_stride) {
-  const int64_t first = int64_t(blockIdx.x) * (kThreads * kLoads);
-  const int64_t row0 = first / per;
-  const uint32_t at0 = uint32_t(first - row0 * per);
-  const uint32_t left = uint32_t(min(chunks - first, int64_t(kThreads * kLoads)));
-  u32x4 in[kLoads];
-#pragma unroll
-  for (int u = 0; u < kLoads; ++u) {
-    const uint32_t t = u * kThreads + threadIdx.x;
-    if (t < left) {
-      const Place at = place(row0, at0, t, per);
-      in[u] = *reinterpret_cast<const u32x4 *>(x + at.row * x_stride + at.chunk * 8);
-    }
-  }
-#pragma unroll
-  for (int u = 0; u < kLoads; ++u) {
-    const uint32_t t = u * kThreads + threadIdx.x;
-    if (t < left) {  // whole blocks: four lanes agree
-      const Place at = place(row0, at0, t, per);
-      float v[8];
-      unpack8(in[u], v);
-      uint32_t w[BITS / 4], scale;
-      encode<BITS>(v, w, scale);
-      store_codes<BITS>(codes + at.row * stride + at.chunk * BITS, w);
-      if ((threadIdx.x & 3) == 0)
-        scales[at.row * scale_stride + (at.chunk >> 2)] = uint8_t(scale);
-    }
+  for (int64_t i = int64_t(blockIdx.x) * kThreads + threadIdx.x; i < chunks;
+       i += int64_t(gridDim.x) * kThreads) {  // whole blocks: four lanes agree
+    const Place at = place(i, per);
+    float v[8];
+    unpack8(*reinterpret_cast<const u32x4 *>(x + at.row * x_stride + at.chunk * 8), v);
+    uint32_t w[BITS / 4], scale;
+    encode<BITS>(v, w, scale);
+    store_codes<BITS>(codes + at.row * stride + at.chunk * BITS, w);
+    if ((threadIdx.x & 3) == 0)
+      scales[at.row * scale_stride + (at.chunk >> 2)] = uint8_t(scale);
   }
 }
 
@@ -135,55 +124,32 @@ __global__ __launch_bounds__(kThreads) void dequantize_kernel(const uint8_t *cod
                                                               int64_t scale_stride, int64_t chunks,
                                                               uint32_t per, uint16_t *out,
                                                               int64_t out_stride) {
-  const int64_t first = int64_t(blockIdx.x) * (kThreads * kLoads);
-  const int64_t row0 = first / per;
-  const uint32_t at0 = uint32_t(first - row0 * per);
-  const uint32_t left = uint32_t(min(chunks - first, int64_t(kThreads * kLoads)));
-  uint32_t in[kLoads][BITS / 4], scale[kLoads];
-#pragma unroll
-  for (int u = 0; u < kLoads; ++u) {
-    const uint32_t t = u * kThreads + threadIdx.x;
-    if (t < left) {
-      const Place at = place(row0, at0, t, per);
-      const uint8_t *p = codes + at.row * stride + at.chunk * BITS;
-      scale[u] = scales[at.row * scale_stride + (at.chunk >> 2)];
-      if (BITS == 8) {
-        const uint2 w = *reinterpret_cast<const uint2 *>(p);
-        in[u][0] = w.x;
-        in[u][BITS / 4 - 1] = w.y;
-      } else {
-        in[u][0] = *reinterpret_cast<const uint32_t *>(p);
-      }
+  for (int64_t i = int64_t(blockIdx.x) * kThreads + threadIdx.x; i < chunks;
+       i += int64_t(gridDim.x) * kThreads) {
+    const Place at = place(i, per);
+    const uint8_t *p = codes + at.row * stride + at.chunk * BITS;
+    const uint32_t scale = scales[at.row * scale_stride + (at.chunk >> 2)];
+    const float s = bits_f32(scale ? scale << 23 : 0x00400000u);
+    auto two = [&](auto pair) {
+      return uint32_t(f2bf(pair[0])) | uint32_t(f2bf(pair[1])) << 16;
+    };
+    u32x4 w;
+    if (BITS == 8) {
+      const uint2 in = *reinterpret_cast<const uint2 *>(p);
+      w[0] = two(__builtin_amdgcn_cvt_scalef32_pk_f32_fp8(in.x, s, false));
+      w[1] = two(__builtin_amdgcn_cvt_scalef32_pk_f32_fp8(in.x, s, true));
+      w[2] = two(__builtin_amdgcn_cvt_scalef32_pk_f32_fp8(in.y, s, false));
+      w[3] = two(__builtin_amdgcn_cvt_scalef32_pk_f32_fp8(in.y, s, true));
+    } else {
+      const uint32_t in = *reinterpret_cast<const uint32_t *>(p);
+      w[0] = two(__builtin_amdgcn_cvt_scalef32_pk_f32_fp4(in, s, 0));
+      w[1] = two(__builtin_amdgcn_cvt_scalef32_pk_f32_fp4(in, s, 1));
+      w[2] = two(__builtin_amdgcn_cvt_scalef32_pk_f32_fp4(in, s, 2));
+      w[3] = two(__builtin_amdgcn_cvt_scalef32_pk_f32_fp4(in, s, 3));
     }
-  }
-#pragma unroll
-  for (int u = 0; u < kLoads; ++u) {
-    const uint32_t t = u * kThreads + threadIdx.x;
-    if (t < left) {
-      const Place at = place(row0, at0, t, per);
-      const float s = scale[u] == 255u ? __builtin_nanf("")
-                                       : bits_f32(scale[u] ? scale[u] << 23 : 0x00400000u);
-      uint32_t w[4];
-      auto two = [&](auto pair) {
-        return uint32_t(f2bf(pair[0])) | uint32_t(f2bf(pair[1])) << 16;
-      };
-      if (BITS == 8) {
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          w[2 * i] = two(__builtin_amdgcn_cvt_scalef32_pk_f32_fp8(in[u][i % (BITS / 4)], s, false));
-          w[2 * i + 1] = two(__builtin_amdgcn_cvt_scalef32_pk_f32_fp8(in[u][i % (BITS / 4)], s, true));
-        }
-      } else {
-        w[0] = two(__builtin_amdgcn_cvt_scalef32_pk_f32_fp4(in[u][0], s, 0));
-        w[1] = two(__builtin_amdgcn_cvt_scalef32_pk_f32_fp4(in[u][0], s, 1));
-        w[2] = two(__builtin_amdgcn_cvt_scalef32_pk_f32_fp4(in[u][0], s, 2));
-        w[3] = two(__builtin_amdgcn_cvt_scalef32_pk_f32_fp4(in[u][0], s, 3));
-      }
-      if (scale[u] == 255u)
-        w[0] = w[1] = w[2] = w[3] = 0x7fc07fc0u;
-      *reinterpret_cast<u32x4 *>(out + at.row * out_stride + at.chunk * 8) =
-          u32x4{w[0], w[1], w[2], w[3]};
-    }
+    if (scale == 255u)
+      w = u32x4{0x7fc07fc0u, 0x7fc07fc0u, 0x7fc07fc0u, 0x7fc07fc0u};
+    *reinterpret_cast<u32x4 *>(out + at.row * out_stride + at.chunk * 8) = w;
   }
 }
 
@@ -196,33 +162,30 @@ struct NormArgs {
   float eps;
 };
 
-// h = bf16(x + residual) (or x), y = h / sqrt(mean h^2 + eps) * gain in 32 bits,
-// y quantised without a rounding in between. WPR waves have a row, each lane C
-// chunks of 8 in registers from the read to the codes, so a row is read once.
-template <int BITS, int WPR, int C>
-__global__ __launch_bounds__(256) void norm_kernel(NormArgs p) {
-  constexpr int kRows = 4 / WPR;  // rows of a workgroup
-  __shared__ float part[4];
-  const int wave = threadIdx.x >> 6;
-  const int row = int(blockIdx.x) * kRows + wave / WPR;
-  const int t = threadIdx.x & (WPR * 64 - 1);
-  const int chunks = p.k >> 3;
-  const bool in_row = row < p.rows;
-  u32x4 x[C], r[C];
+// h = bf16(x + residual) (or x), y = h * gain / sqrt(mean h^2 + eps) in 32 bits, y
+// quantised without a rounding in between. A workgroup has a row, each lane C chunks
+// of 8 in registers from the read to the codes, so a row is read once.
+template <int BITS, int C>
+__global__ __launch_bounds__(1024) void norm_kernel(NormArgs p) {
+  __shared__ float part[16];
+  const int waves = int(blockDim.x) >> 6, chunks = p.k >> 3;
+  const int64_t row = blockIdx.x;
+  u32x4 x[C], r[C], gain[C];
 #pragma unroll
   for (int c = 0; c < C; ++c) {
-    const int i = c * WPR * 64 + t;
-    if (in_row && i < chunks) {
+    const int i = c * int(blockDim.x) + int(threadIdx.x);
+    if (i < chunks) {
       x[c] = *reinterpret_cast<const u32x4 *>(p.x + row * p.x_stride + i * 8);
       if (p.residual)
         r[c] = *reinterpret_cast<const u32x4 *>(p.residual + row * p.residual_stride + i * 8);
+      gain[c] = *reinterpret_cast<const u32x4 *>(p.gain + i * 8);
     }
   }
   float v[C][8], squares = 0.f;
 #pragma unroll
   for (int c = 0; c < C; ++c) {
-    const int i = c * WPR * 64 + t;
-    if (!(in_row && i < chunks))
+    const int i = c * int(blockDim.x) + int(threadIdx.x);
+    if (i >= chunks)
       continue;
     unpack8(x[c], v[c]);
     if (p.residual) {
@@ -242,20 +205,22 @@ __global__ __launch_bounds__(256) void norm_kernel(NormArgs p) {
       squares = fmaf(v[c][e], v[c][e], squares);
   }
   float total = wave_sum(squares);
-  if (WPR > 1) {
+  if (waves > 1) {
     if ((threadIdx.x & 63) == 0)
-      part[wave] = total;
-    __syncthreads();
-    total = (part[0] + part[1]) + (part[2] + part[3]);
+      part[threadIdx.x >> 6] = total;
+    lds_barrier();  // the stores of h go on
+    total = part[0];
+    for (int w = 1; w < waves; ++w)
+      total += part[w];
   }
   const float scale = 1.0f / __builtin_sqrtf(total / float(p.k) + p.eps);
 #pragma unroll
   for (int c = 0; c < C; ++c) {
-    const int i = c * WPR * 64 + t;
-    if (!(in_row && i < chunks))
+    const int i = c * int(blockDim.x) + int(threadIdx.x);
+    if (i >= chunks)
       continue;
     float g[8];
-    unpack8(*reinterpret_cast<const u32x4 *>(p.gain + i * 8), g);
+    unpack8(gain[c], g);
 #pragma unroll
     for (int e = 0; e < 8; ++e)
       v[c][e] = v[c][e] * g[e] * scale;  // the first product, of two bf16 values, is exact
@@ -269,27 +234,35 @@ __global__ __launch_bounds__(256) void norm_kernel(NormArgs p) {
 
 constexpr int kMaxNormK = 16384;
 
-template <int BITS>
-hipError_t launch_norm(const NormArgs &p, hipStream_t s) {
-  auto go = [&](auto kernel, int rows) {
-    hipLaunchKernelGGL(kernel, dim3(unsigned((p.rows + rows - 1) / rows)), dim3(256), 0, s, p);
-    return hipGetLastError();
-  };
-  if (p.k <= 512)
-    return go(norm_kernel<BITS, 1, 1>, 4);
-  if (p.k <= 2048)
-    return go(norm_kernel<BITS, 4, 1>, 1);
-  if (p.k <= 4096)
-    return go(norm_kernel<BITS, 4, 2>, 1);
-  if (p.k <= 8192)
-    return go(norm_kernel<BITS, 4, 4>, 1);
-  return go(norm_kernel<BITS, 4, 8>, 1);
+// One chunk a lane and k / 512 waves are the quickest for few rows, two the quickest for
+// many long ones (us, with a residual; four waves for every row as before 3.0, 31.0):
+//    1 x 3072: 2.70, 2.87    8000 x 3072: 29.7, 29.0    8000 x 2048: 18.9, 18.6
+//    1 x 2048: 2.50, 2.82    3000 x 8192: 31.2, 29.3    8000 x 1024: 11.4, 10.8
+// The choice goes by k alone, so that a row's sum has one order however many rows there are.
+template <int BITS> hipError_t launch_norm(NormArgs p, hipStream_t s) {
+  const int each = p.k <= 2048 ? 1 : 2, threads = (p.k / 8 + 64 * each - 1) / (64 * each) * 64;
+  constexpr int kMost = 1 << 21;  // of a launch, whose threads count in 32 bits
+  for (int left = p.rows; left > 0; left -= kMost) {
+    p.rows = std::min(left, kMost);
+    hipLaunchKernelGGL((each == 1 ? norm_kernel<BITS, 1> : norm_kernel<BITS, 2>),
+                       dim3(unsigned(p.rows)), dim3(unsigned(threads)), 0, s, p);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess)
+      return e;
+    p.x += p.rows * p.x_stride;
+    if (p.residual) {
+      p.residual += p.rows * p.residual_stride;
+      p.sum += p.rows * p.sum_stride;
+    }
+    p.codes += p.rows * p.stride;
+    p.scales += p.rows * p.scale_stride;
+  }
+  return hipSuccess;
 }
 
-// Workgroups of a call over `chunks` chunks, 0 where the grid cannot hold them.
+// Workgroups of a call over `chunks` chunks.
 unsigned groups(int64_t chunks) {
-  const int64_t n = (chunks + kThreads * kLoads - 1) / (kThreads * kLoads);
-  return n < (int64_t(1) << 31) / kThreads ? unsigned(n) : 0u;
+  return unsigned(std::min<int64_t>((chunks + kThreads - 1) / kThreads, 1 << 23));
 }
 
 }  // namespace
@@ -305,17 +278,18 @@ int32_t yuear_op_mx_quantize(const uint16_t *x, int64_t x_stride, int32_t rows, 
                              int64_t scales_stride, void *stream) {
   if (rows == 0)
     return 0;
-  if (rows < 0 || !mx::rows_ok(codes, codes_stride, scales, scales_stride, k, bits) ||
+  if (rows < 0 || int64_t(rows) * k > mx::kMaxValues ||
+      !mx::rows_ok(codes, codes_stride, scales, scales_stride, k, bits) ||
       !mx::wide_ok(x, x_stride, k))
     return int32_t(hipErrorInvalidValue);
   const mx::Span in = mx::bf16_span(x, x_stride, rows, k),
                  c = mx::codes_span(codes, codes_stride, rows, k, bits),
                  s = mx::scales_span(scales, scales_stride, rows, k);
-  const unsigned grid = mx::groups(int64_t(rows) * (k / 8));
-  if (mx::overlap(in, c) || mx::overlap(in, s) || mx::overlap(c, s) || !grid)
+  if (mx::overlap(in, c) || mx::overlap(in, s) || mx::overlap(c, s))
     return int32_t(hipErrorInvalidValue);
-  hipLaunchKernelGGL(bits == 8 ? mx::quantize_kernel<8> : mx::quantize_kernel<4>, dim3(grid),
-                     dim3(mx::kThreads), 0, static_cast<hipStream_t>(stream), x, x_stride,
+  hipLaunchKernelGGL(bits == 8 ? mx::quantize_kernel<8> : mx::quantize_kernel<4>,
+                     dim3(mx::groups(int64_t(rows) * (k / 8))), dim3(mx::kThreads), 0,
+                     static_cast<hipStream_t>(stream), x, x_stride,
                      int64_t(rows) * (k / 8), uint32_t(k / 8), codes, codes_stride, scales,
                      scales_stride);
   return int32_t(hipGetLastError());
@@ -326,16 +300,17 @@ int32_t yuear_op_mx_dequantize(const uint8_t *codes, int64_t codes_stride, const
                                uint16_t *out, int64_t out_stride, void *stream) {
   if (rows == 0)
     return 0;
-  if (rows < 0 || !mx::rows_ok(codes, codes_stride, scales, scales_stride, k, bits) ||
+  if (rows < 0 || int64_t(rows) * k > mx::kMaxValues ||
+      !mx::rows_ok(codes, codes_stride, scales, scales_stride, k, bits) ||
       !mx::wide_ok(out, out_stride, k))
     return int32_t(hipErrorInvalidValue);
   const mx::Span o = mx::bf16_span(out, out_stride, rows, k);
-  const unsigned grid = mx::groups(int64_t(rows) * (k / 8));
   if (mx::overlap(o, mx::codes_span(codes, codes_stride, rows, k, bits)) ||
-      mx::overlap(o, mx::scales_span(scales, scales_stride, rows, k)) || !grid)
+      mx::overlap(o, mx::scales_span(scales, scales_stride, rows, k)))
     return int32_t(hipErrorInvalidValue);
-  hipLaunchKernelGGL(bits == 8 ? mx::dequantize_kernel<8> : mx::dequantize_kernel<4>, dim3(grid),
-                     dim3(mx::kThreads), 0, static_cast<hipStream_t>(stream), codes, codes_stride,
+  hipLaunchKernelGGL(bits == 8 ? mx::dequantize_kernel<8> : mx::dequantize_kernel<4>,
+                     dim3(mx::groups(int64_t(rows) * (k / 8))), dim3(mx::kThreads), 0,
+                     static_cast<hipStream_t>(stream), codes, codes_stride,
                      scales, scales_stride, int64_t(rows) * (k / 8), uint32_t(k / 8), out,
                      out_stride);
   return int32_t(hipGetLastError());
@@ -348,7 +323,7 @@ int32_t yuear_op_mx_rms_norm(const uint16_t *x, int64_t x_stride, const uint16_t
                              uint16_t *sum, int64_t sum_stride, void *stream) {
   if (rows == 0)
     return 0;
-  if (rows < 0 || rows >= 1 << 23 || k > mx::kMaxNormK ||
+  if (rows < 0 || k > mx::kMaxNormK ||
       !mx::rows_ok(codes, codes_stride, scales, scales_stride, k, bits) ||
       !mx::wide_ok(x, x_stride, k) || !mx::aligned(gain, 16) || !residual != !sum ||
       (residual &&
