@@ -353,6 +353,29 @@ def test_streamed_rows(torch, yuear_lib, form, m, n, k, bits, epilogue):
     assert torch.equal(wide[:m, :width], want) and (wide[m:] == 3).all() and (wide[:, width:] == 3).all()
 
 
+@pytest.mark.parametrize("form", [8, 9])
+@pytest.mark.parametrize("bits", [8, 4])
+@pytest.mark.parametrize("epilogue", ["store", "swiglu", "residual"])
+def test_streamed_weights_past_the_cache(torch, yuear_lib, form, bits, epilogue):
+    """More than 64 MiB of weights: the same bits as by form 0, whose last columns are checked."""
+    rng = np.random.default_rng(31)
+    m, n, k = 3, 140_002, 1024
+    a, rows = random_pair(rng, m, k, bits), random_pair(rng, 1009, k, 4)
+    w = tuple(t.view(torch.uint8)[torch.arange(n, device="cuda") * 7 % 1009] for t in pair_of(torch, *rows, 4))
+    w = (w[0], w[1].view(torch.float8_e8m0fnu))
+    width = n // 2 if epilogue == "swiglu" else n
+    r = bf16(torch, ref.to_bf16(rng.standard_normal((m, width)))) if epilogue == "residual" else None
+    out, want = (torch.empty(m, width, dtype=torch.bfloat16, device="cuda") for _ in range(2))
+    forced(torch, yuear_lib, form, pair_of(torch, *a, bits), w, bits, out, r, epilogue == "swiglu")
+    forced(torch, yuear_lib, 0, pair_of(torch, *a, bits), w, bits, want, r, epilogue == "swiglu")
+    assert torch.equal(out, want)
+    last = 202
+    at = width - (last // 2 if epilogue == "swiglu" else last)
+    check_gemm(torch, want[:, at:], ref.values(*a, bits),
+               ref.values(raw(torch, w[0][-last:]), raw(torch, w[1].view(torch.uint8)[-last:]), 4), bits, epilogue,
+               ref.from_bf16(bits_of(torch, r[:, at:])) if r is not None else None)
+
+
 @pytest.mark.parametrize("m,n,k,bits", [(3, 40, 256, 8), (70, 140, 384, 4), (300, 300, 256, 8)])
 def test_gemm_rows_apart(torch, yuear_lib, m, n, k, bits):
     """Operands that are columns of wider buffers; what lies between their rows is NaN."""

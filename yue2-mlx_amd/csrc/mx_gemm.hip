@@ -194,6 +194,7 @@ typedef __attribute__((address_space(3))) void *lds_ptr_t;
 extern __shared__ __attribute__((aligned(1024))) char mx_lds[];
 
 constexpr int kSliceK = 512;
+constexpr int kNonTemporal = 2;  // of a load: what it brings goes from the caches first
 // Bytes of a wave's region: pieces of W and A, then their scales.
 template <int ABITS, int FT> constexpr int region(int a_rows) {
   return 16 * FT * (kSliceK / 2 + 16) + a_rows * (kSliceK * ABITS / 8 + 16);
@@ -204,7 +205,7 @@ template <int ABITS> constexpr int a_piece() { return kSliceK * ABITS / 8; }
 
 // 512 of K from k0 on of 16 FT rows of W and of A's rows, with their scales, into LDS at the
 // places given. (What lies past K in a piece belongs to other rows, and is not used.)
-template <int FT>
+template <int FT, bool ONCE = false>
 __device__ __forceinline__ void load_w(const GemmArgs &p, __amdgpu_buffer_rsrc_t rw,
                                        __amdgpu_buffer_rsrc_t rsw, char *w, char *scales, int k0) {
   const int lane = threadIdx.x & 63;
@@ -213,7 +214,7 @@ __device__ __forceinline__ void load_w(const GemmArgs &p, __amdgpu_buffer_rsrc_t
     const int row = 4 * i + (lane >> 4);
     __builtin_amdgcn_raw_ptr_buffer_load_lds(
         rw, (lds_ptr_t)(w + i * 1024), 16,
-        row * int(p.w_stride) + k0 / 2 + ((lane & 15) ^ (row & 15)) * 16, 0, 0, 0);
+        row * int(p.w_stride) + k0 / 2 + ((lane & 15) ^ (row & 15)) * 16, 0, 0, ONCE ? kNonTemporal : 0);
   }
   if (lane < 16 * FT)
     __builtin_amdgcn_raw_ptr_buffer_load_lds(rsw, (lds_ptr_t)scales, 16,
@@ -345,12 +346,18 @@ __global__ __launch_bounds__(1024) void rows_kernel(GemmArgs p, int a_rows) {
 
 // The same for weights of many features, k up to 512 a wave: a workgroup keeps A and goes
 // from one 16 FT features to another, the next ones' weights on their way under the products
-// and sums of these. (A workgroup for each 16 features spends half of its time on its start
-// and end: 5 x 83968 x 3072 31 us.)
+// and sums of these. (A workgroup for each 16 or 32 features spends half of its time on its
+// start and end. 5 x 83968 x 3072 in 8 bits, weights from HBM: 30.5 and 29.3 us, this 26.7;
+// 8 x 16384 x 3072: 8.2, 7.7, this 7.4.)
+//
+// ONCE: weights of more than 64 MiB, which the last-level cache (256 MB) does not keep until
+// the next token's turn, are loaded past it: 5 x 83968 x 3072 26.7 -> 24.5 us (5.6 TB/s), 5 x
+// 200000 x 3072 57 -> 52; kept in the cache by calls of them alone 22.2 -> 23.6. 61 MB 12.9
+// either way, 25 MB from the cache 5.1 -> 5.4.
 template <int ABITS, int FT> constexpr int stream_region(int a_rows) {
   return 2 * (16 * FT * (kWPiece + 16) + FT * 1024) + a_rows * (a_piece<ABITS>() + 16);
 }
-template <int ABITS, int EPI, int FT>
+template <int ABITS, int EPI, int FT, bool ONCE>
 __global__ __launch_bounds__(1024) void stream_kernel(GemmArgs p, int a_rows) {
   constexpr int kW = 16 * FT * (kWPiece + 16);  // a buffer's rows and scales
   const int lane = threadIdx.x & 63;
@@ -363,9 +370,9 @@ __global__ __launch_bounds__(1024) void stream_kernel(GemmArgs p, int a_rows) {
   auto load = [&](int n0, int buffer) {
     const int rows = min(p.n - n0, 16 * FT);
     char *const w = mine + buffer * kW;
-    load_w<FT>(p, rows_rsrc(p.w + n0 * p.w_stride, p.w_stride, rows, p.k / 2),
-               rows_rsrc(p.w_scales + n0 * p.w_scale_stride, p.w_scale_stride, rows, p.k / 32), w,
-               w + 16 * FT * kWPiece, k0);
+    load_w<FT, ONCE>(p, rows_rsrc(p.w + n0 * p.w_stride, p.w_stride, rows, p.k / 2),
+                     rows_rsrc(p.w_scales + n0 * p.w_scale_stride, p.w_scale_stride, rows, p.k / 32), w,
+                     w + 16 * FT * kWPiece, k0);
   };
   load_a<ABITS>(p, ra, rsa, a, a_scales, k0, a_rows);
   const int tiles = (p.n + 16 * FT - 1) / (16 * FT);
@@ -412,6 +419,19 @@ __global__ __launch_bounds__(1024) void stream_kernel(GemmArgs p, int a_rows) {
 // Scales come 512 of K (a group) at a time, 16 bytes a row, into two buffers behind
 // the ring, a group in use and the one after it; a lane reads the bytes of its row
 // and step and shifts them so that k-block h of each 64 is at byte 0 or 2.
+//
+// us of stores:                 64x64  64x128  128x128  192x192  256x256
+//   8 bits, 100 x 5120 x 3072      8.5    10.5     13.2
+//   8 bits, 300 x 5120 x 3072     15.8    11.6     14.1     24.5
+//   8 bits, 1000 x 5120 x 3072    36.6    29.1     25.5     26.0     33.7
+//   8 bits, 3000 x 3072 x 8192             109     86.8     64.7     74.5
+//   8 bits, 3000 x 16384 x 3072            207      149      141      117
+//   4 bits, 6001 x 12288 x 2048            165      124      104       95
+// The largest run at 2.6 PFLOP/s (8 bits, 2.9 at K 8192) and 3.3 (4 bits, 4.2): matrix
+// cores busy 59 and 34% of the cycles at the 2.0 GHz that the power limit leaves (operands of
+// zeros run 27-30% faster), in 4 bits the results' way to memory a quarter of the time (K 2048).
+// The smallest are bound by LDS: 64 x 64 tiles of 197 x 3072 x 8192 bring 768 KiB a CU at 70
+// KB/us of the 66 (rows of 64 bytes) to 120 (128) that loads into LDS reach, 15.6 us.
 //
 // MFMA operands, lane l = 32 h + r: in 4 bits row r, k 32 h .. 32 h + 31 of the 64;
 // in 8 bits k 16 h .. 16 h + 15 and 32 + 16 h ..; the scale of k-block h of row r.
@@ -878,13 +898,15 @@ enum Form : int {
 };
 
 // k up to 512 a wave, m up to 16.
-template <int ABITS, int FT>
-hipError_t launch_stream(void (*kernel)(GemmArgs, int), const GemmArgs &p, hipStream_t s) {
+template <int ABITS, int EPI, int FT> hipError_t launch_stream(const GemmArgs &p, hipStream_t s) {
   const int per_kib = 1024 / (kSliceK * ABITS / 8);
   const int a_rows = (p.m + per_kib - 1) / per_kib * per_kib;
   const int waves = (p.k + kSliceK - 1) / kSliceK, bytes = waves * stream_region<ABITS, FT>(a_rows);
   if (p.m > 16 || waves > 16 || bytes > 160 * 1024)
     return hipErrorInvalidValue;
+  void (*const kernel)(GemmArgs, int) = int64_t(p.n) * (p.k / 2) > int64_t(64) << 20
+                                            ? stream_kernel<ABITS, EPI, FT, true>
+                                            : stream_kernel<ABITS, EPI, FT, false>;
   const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void *>(kernel),
                                            hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024);
   if (e != hipSuccess)
@@ -918,8 +940,8 @@ template <int ABITS, int EPI> hipError_t launch_form(int form, const GemmArgs &p
       if (p.k % 256 == 0)
         return YUEAR_MX_TILE(256, 256, 4, 2, 1, 256, 2);
     return YUEAR_MX_TILE(256, 256, 4, 2, 1, 128, 3);
-  case kStream16: return launch_stream<ABITS, 1>(stream_kernel<ABITS, EPI, 1>, p, s);
-  case kStream32: return launch_stream<ABITS, 2>(stream_kernel<ABITS, EPI, 2>, p, s);
+  case kStream16: return launch_stream<ABITS, EPI, 1>(p, s);
+  case kStream32: return launch_stream<ABITS, EPI, 2>(p, s);
   }
 #undef YUEAR_MX_ROWS
 #undef YUEAR_MX_TILE
@@ -993,10 +1015,9 @@ double form_time(int form, int bits, int m, int n, int k, int cus) {
   return c[0] + full * (c[1] + c[2] * kk) + (rest > 0 ? c[3] + c[4] * kk + rest * (c[5] + c[6] * kk) : 0.0);
 }
 
-// The form of least estimated time: for few tokens rows, streamed where a workgroup can keep A
-// (137 MB of weights, 5 tokens: 31 -> 23 us), the larger tiles the more there are to fill the
-// CUs with. The sum over K is split as the form is (by waves, in
-// order), so the form decides the order of the sums.
+// The form of least estimated time: for few tokens rows, streamed where a workgroup can keep
+// A, the larger tiles the more there are to fill the CUs with. The sum over K is split as the
+// form is (by waves, in order), so the form decides the order of the sums.
 int pick_form(int bits, int m, int n, int k) {
   const int cus = gemm_cus();
   int best = 0;
