@@ -160,14 +160,25 @@ struct NormArgs {
   int64_t x_stride, residual_stride, sum_stride, stride, scale_stride;
   int rows, k;
   float eps;
+  double inverse_k;
 };
 
+// Sum over the wave's lanes: over 16 of them in 32 bits, their sums in 64.
+__device__ __forceinline__ double wave_sum64(float v) {
+  const int rows = int(f32_bits(row_sum16(v)));
+  auto row = [&](int lane) { return double(bits_f32(uint32_t(__builtin_amdgcn_readlane(rows, lane)))); };
+  return (row(0) + row(16)) + (row(32) + row(48));
+}
+
 // h = bf16(x + residual) (or x), y = h * gain / sqrt(mean h^2 + eps) in 32 bits, y
-// quantised without a rounding in between. A workgroup has a row, each lane C chunks
-// of 8 in registers from the read to the codes, so a row is read once.
+// quantised without a rounding in between but y's own to 32 bits. A workgroup has a row, each
+// lane C chunks of 8 in registers from the read to the codes, so a row is read once. The
+// squares of 16 lanes and more are added, and the root taken, in 64 bits (the factor in two parts
+// of 32): a row's values all carry its factor's error, and one that it takes past a code's edge
+// is off by a whole step of the code.
 template <int BITS, int C>
 __global__ __launch_bounds__(1024) void norm_kernel(NormArgs p) {
-  __shared__ float part[16];
+  __shared__ double part[16];
   const int waves = int(blockDim.x) >> 6, chunks = p.k >> 3;
   const int64_t row = blockIdx.x;
   u32x4 x[C], r[C], gain[C];
@@ -204,7 +215,7 @@ __global__ __launch_bounds__(1024) void norm_kernel(NormArgs p) {
     for (int e = 0; e < 8; ++e)
       squares = fmaf(v[c][e], v[c][e], squares);
   }
-  float total = wave_sum(squares);
+  double total = wave_sum64(squares);
   if (waves > 1) {
     if ((threadIdx.x & 63) == 0)
       part[threadIdx.x >> 6] = total;
@@ -213,7 +224,11 @@ __global__ __launch_bounds__(1024) void norm_kernel(NormArgs p) {
     for (int w = 1; w < waves; ++w)
       total += part[w];
   }
-  const float scale = 1.0f / __builtin_sqrtf(total / float(p.k) + p.eps);
+  const double mean = fma(total, p.inverse_k, double(p.eps));
+  const float scale = 1.0f / __builtin_sqrtf(float(mean));
+  // a Newton step; none where the factor is 0 or infinite
+  float rest = float(0.5 * scale * fma(-mean * scale, double(scale), 1.0));
+  rest = fabsf(rest) < scale * 1e-6f ? rest : 0.f;
 #pragma unroll
   for (int c = 0; c < C; ++c) {
     const int i = c * int(blockDim.x) + int(threadIdx.x);
@@ -223,7 +238,7 @@ __global__ __launch_bounds__(1024) void norm_kernel(NormArgs p) {
     unpack8(gain[c], g);
 #pragma unroll
     for (int e = 0; e < 8; ++e)
-      v[c][e] = v[c][e] * g[e] * scale;  // the first product, of two bf16 values, is exact
+      v[c][e] = fmaf(v[c][e] * g[e], scale, v[c][e] * g[e] * rest);  // v g of bf16 values is exact
     uint32_t w[BITS / 4], s;
     encode<BITS>(v[c], w, s);
     store_codes<BITS>(p.codes + row * p.stride + i * BITS, w);
@@ -347,7 +362,7 @@ int32_t yuear_op_mx_rms_norm(const uint16_t *x, int64_t x_stride, const uint16_t
     return int32_t(hipErrorInvalidValue);
   const mx::NormArgs p{x,        residual,        gain,       sum,          codes,
                        scales,   x_stride,        residual_stride, sum_stride, codes_stride,
-                       scales_stride, rows,       k,          eps};
+                       scales_stride, rows,       k,          eps, 1.0 / k};
   const hipStream_t st = static_cast<hipStream_t>(stream);
   return int32_t(bits == 8 ? mx::launch_norm<8>(p, st) : mx::launch_norm<4>(p, st));
 }
