@@ -476,6 +476,18 @@ def test_refused_on_the_gpu(torch, yuear_lib):
             call()
 
 
+def test_rows_past_32_bits_of_values_are_refused(torch, yuear_lib):
+    """k of 2^32 + 32 is not taken for 32."""
+    k = 2 ** 32 + 32
+    x = torch.empty(1, k, dtype=torch.bfloat16, device="cuda")
+    pair = (x.view(torch.uint8)[:, :k].view(torch.float8_e4m3fn), x.view(torch.uint8)[:, :k // 32].view(torch.float8_e8m0fnu))
+    small = pair_of(torch, *random_pair(np.random.default_rng(1), 2, 128, 4), 4)
+    for call in (lambda: yuear_lib.mx_quantize(x), lambda: yuear_lib.mx_dequantize(pair),
+                 lambda: yuear_lib.mx_rms_norm(x, x[0]), lambda: yuear_lib.mx_gemm(pair, small)):
+        with pytest.raises(ValueError):
+            call()
+
+
 def test_empty(torch, yuear_lib):
     x = torch.zeros(0, 128, dtype=torch.bfloat16, device="cuda")
     gain = torch.ones(128, dtype=torch.bfloat16, device="cuda")
