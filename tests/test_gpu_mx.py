@@ -446,6 +446,27 @@ def test_gemm_not_finite(torch, yuear_lib, m, form):
         assert (np.abs(got - y) <= ref.HALF_BF16 * np.abs(y) + (1 + ref.HALF_BF16) * off).all()
 
 
+@pytest.mark.parametrize("m", [1, 9, 70, 300])
+@pytest.mark.parametrize("bits", [8, 4])
+def test_swiglu_at_far_gates(torch, yuear_lib, m, bits):
+    """Gates down to where e^-gate leaves 32 bits, and up; the sums are one product each, exact."""
+    gates = np.array([-104, -96, -88, -80, -64, -40, -16, -2, 0, 1, 12, 80, 96, 104]) if bits == 8 else np.array(
+        [-96, -64, -48, -24, -4, -1, 0, 2, 32, 96])
+    x = np.zeros((m, 128))
+    x[:, 0] = np.resize(gates, m)
+    x[:, 32] = 1
+    w = np.zeros((64, 128))
+    w[0::2, 0], w[1::2, 32] = 1, np.resize(2.0 ** np.arange(-12, 20, 3), 32)
+    a, w = yuear_lib.mx_quantize(bf16(torch, ref.to_bf16(x)), bits), yuear_lib.mx_quantize(bf16(torch, ref.to_bf16(w)), 4)
+    got = ref.from_bf16(bits_of(torch, yuear_lib.mx_gemm(a, w, swiglu=True)))
+    g = x[:, :1]
+    want = g / (1 + np.exp(-g)) * ref.values(raw(torch, w[0]), raw(torch, w[1].view(torch.uint8)), 4)[1::2, 32]
+    # of the result: the argument's roundings, exp2's, the reciprocal's and five more of 32 bits, then bf16's
+    near = np.abs(got - want) <= np.abs(want) * (np.abs(g) * 7.4e-8 + 9 * 2.0 ** -24 + ref.HALF_BF16) * (1 + 2.0 ** -8) + 2.0 ** -134
+    lost = g < -88.7  # e^-gate is infinite in 32 bits
+    assert (near | (lost & (got == 0))).all()
+
+
 def test_gemm_into_its_residual(torch, yuear_lib):
     rng = np.random.default_rng(4)
     for m in (2, 90, 400):

@@ -49,16 +49,15 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_rsrc(const uint8_t *base,
   return __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t *>(base), 0, int(n), 0x00020000);
 }
 
-// silu(gate) * up with e^-gate as 2^t, t = -gate log2 e: what rounding takes off t, up
-// to 2^-18 of the result where gate is large, is given back in the first order (and
-// kept small where gate is past all exponents). expf and a division made a third of
-// the SwiGLU tiles' time past the last product.
+// silu(gate) * up with e^-gate as 2^t. Rounding t = -gate log2 e moves the result by up to
+// |gate| 7.3e-8 of it, no more than half a step of gate, a 32-bit sum, does (|gate| 6e-8). A
+// quarter of the quotient's parts: 1 / (1 + e^-gate) itself would be subnormal, which the
+// reciprocal takes for zero, from gate = -87.3 on, where the result need not be. Eight operations a
+// value, two of them of quarter rate: with expf and a division they were a third of the SwiGLU
+// tiles' time past the last product.
 __device__ __forceinline__ float silu_times(float gate, float up) {
-  constexpr float kLog2e = 1.44269502f, kRest = 1.92596299e-8f;  // log2 e in two parts
-  const float t = gate * -kLog2e;
-  const float off = fmaf(gate, -kRest, fmaf(gate, -kLog2e, -t)) * 0.693147182f;
-  const float s = __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(t));
-  return gate * fmaf(fmaf(s, s, -s), __builtin_amdgcn_fmed3f(off, -1.f, 1.f), s) * up;
+  const float r = __builtin_amdgcn_rcpf(fmaf(__builtin_amdgcn_exp2f(gate * -1.44269502f), 0.25f, 0.25f));
+  return gate * 0.25f * r * up;
 }
 
 __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
