@@ -979,8 +979,12 @@ double form_time(int form, int bits, int m, int n, int k, int cus) {
       const int waves = std::min({slices, 160 * 1024 / (w_bytes + a_bytes), 16});
       const int held = std::max(1, std::min(160 * 1024 / (waves * (w_bytes + a_bytes)), 32 / waves));
       static const double fit[2][3][5] = {
-          {{0.254, 1.274, 1.444, 0.0203, 0.0}, {0.681, 1.135, 1.365, 0.0189, 0.0}, {0.541, 1.268, 1.818, 0.0193, 0.0501}},
-          {{0.0, 1.708, 1.174, 0.0188, 0.0}, {0.697, 1.11, 1.303, 0.0182, 0.0}, {1.274, 1.147, 1.076, 0.0173, 0.0918}}};
+          {{0.254, 1.274, 1.444, 0.0203, 0.0},
+           {0.681, 1.135, 1.365, 0.0189, 0.0},
+           {0.541, 1.268, 1.818, 0.0193, 0.0501}},
+          {{0.0, 1.708, 1.174, 0.0188, 0.0},
+           {0.697, 1.11, 1.303, 0.0182, 0.0},
+           {1.274, 1.147, 1.076, 0.0173, 0.0918}}};
       const double *c = fit[a8 ? 0 : 1][form];
       return c[0] + c[1] * ((slices + waves - 1) / waves) + c[2] * std::ceil(t / (double(cus) * held)) +
              t / cus * (c[3] * kk * bn + c[4]);
@@ -1012,7 +1016,8 @@ double form_time(int form, int bits, int m, int n, int k, int cus) {
   if (form != kTile256 && tiles(of[0], of[1]) >= (1 << 22))
     return __builtin_inf();
   const double *c = fit[a8 ? 0 : 1][form - kTile64];
-  const double slots = double(cus) * of[2], t = tiles(of[0], of[1]), full = std::floor(t / slots), rest = t / slots - full;
+  const double slots = double(cus) * of[2], t = tiles(of[0], of[1]);
+  const double full = std::floor(t / slots), rest = t / slots - full;
   return c[0] + full * (c[1] + c[2] * kk) + (rest > 0 ? c[3] + c[4] * kk + rest * (c[5] + c[6] * kk) : 0.0);
 }
 
@@ -1048,7 +1053,8 @@ int32_t yuear_op_mx_gemm_form(const uint8_t *a, int64_t a_stride, const uint8_t 
   using namespace yuear;
   if (m == 0 || n == 0)
     return 0;
-  if (m < 0 || n < 0 || m > mx::kMaxRows || n > mx::kMaxRows || k % mx::kStep || (swiglu != 0 && swiglu != 1) || (swiglu && (n % 2 || residual)) ||
+  if (m < 0 || n < 0 || m > mx::kMaxRows || n > mx::kMaxRows || k % mx::kStep ||
+      (swiglu != 0 && swiglu != 1) || (swiglu && (n % 2 || residual)) ||
       !mx::rows_ok(a, a_stride, a_scales, a_scales_stride, k, a_bits) ||
       !mx::rows_ok(w, w_stride, w_scales, w_scales_stride, k, 4) || !mx::aligned(a_scales, 4) ||
       !mx::aligned(w_scales, 4) || a_scales_stride % 4 || w_scales_stride % 4 || !mx::aligned(c, 2) || form < -1 ||
@@ -1060,8 +1066,9 @@ int32_t yuear_op_mx_gemm_form(const uint8_t *a, int64_t a_stride, const uint8_t 
       (residual && (!mx::aligned(residual, 2) || residual_stride < width || residual_stride >= kMostLd)))
     return int32_t(hipErrorInvalidValue);
   const mx::Span out = mx::bf16_span(c, ldc, m, width);
-  for (const mx::Span &in : {mx::codes_span(a, a_stride, m, k, a_bits), mx::scales_span(a_scales, a_scales_stride, m, k),
-                             mx::codes_span(w, w_stride, n, k, 4), mx::scales_span(w_scales, w_scales_stride, n, k)})
+  for (const mx::Span &in :
+       {mx::codes_span(a, a_stride, m, k, a_bits), mx::scales_span(a_scales, a_scales_stride, m, k),
+        mx::codes_span(w, w_stride, n, k, 4), mx::scales_span(w_scales, w_scales_stride, n, k)})
     if (mx::overlap(in, out))
       return int32_t(hipErrorInvalidValue);
   // the output may replace the residual: a lane reads its values before it writes them
