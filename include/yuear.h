@@ -521,9 +521,10 @@ int32_t yuear_op_mx_dequantize(const uint8_t *dev_codes, int64_t codes_stride,
                                void *stream);
 /* The residual addition and RMSNorm before a projection, with their output
  * quantised as above: sum = bf16(x + residual) (which may be the same memory as x
- * or residual, with the same stride), y = sum * gain / sqrt(mean(sum^2) + eps) in
- * 32 bits, in that order, codes and scales of y. Null residual and sum: y of x. k up
- * to 16384, gain [k]. */
+ * or residual, with the same stride), y = sum * gain / sqrt(mean(sum^2) + eps), codes
+ * and scales of y: those of 64-bit arithmetic, where sum * gain and the squares of the
+ * sum stay within the exponents of 32 bits. Null residual and sum: y of x. k up to
+ * 16384, gain [k]. */
 int32_t yuear_op_mx_rms_norm(const uint16_t *dev_x, int64_t x_stride,
                              const uint16_t *dev_residual, int64_t residual_stride,
                              const uint16_t *dev_gain, float eps, int32_t rows, int32_t k,

@@ -189,6 +189,32 @@ def test_norm(torch, yuear_lib, rows, k, gap, bits, residual):
     check_norm(torch, got, want, ref.from_bf16(gain), bits)
 
 
+@pytest.mark.parametrize("rows,k,bits", [(1500, 3072, 8), (1500, 3072, 4), (9000, 256, 8), (300, 16384, 4)])
+def test_norm_codes_are_those_of_64_bits(torch, yuear_lib, rows, k, bits):
+    """Every code, of millions; a product would have to come within 2^-45 of a tie to differ."""
+    rng = np.random.default_rng(rows + bits)
+    x, gain = random_rows(rng, rows, k, "plain"), ref.to_bf16(1 + 0.2 * rng.standard_normal(k))
+    got, _ = yuear_lib.mx_rms_norm(bf16(torch, x), bf16(torch, gain), EPS, bits=bits)
+    h = ref.from_bf16(x)
+    codes, scales = ref.quantize(h / np.sqrt((h ** 2).mean(-1, keepdims=True) + EPS) * ref.from_bf16(gain), bits)
+    np.testing.assert_array_equal(raw(torch, got[1]), scales)
+    np.testing.assert_array_equal(raw(torch, got[0]), codes)
+
+
+@pytest.mark.parametrize("bits", [8, 4])
+def test_norm_ties_where_the_factor_is_exact(torch, yuear_lib, bits):
+    """Rows of +-1, +-2, +-0.25 without eps: the products are the gains, ties among them."""
+    rng = np.random.default_rng(5)
+    k = 2080
+    x = np.where(rng.integers(0, 2, (6, k)), 1.0, -1.0) * np.array([1, 2, 0.25, 1, 2.0 ** 20, 2.0 ** -20])[:, None]
+    gain = ref.from_bf16(ref.to_bf16(rng.integers(128, 256, k) / 128.0 * 2.0 ** rng.integers(-6, 3, k)))
+    gain[::7] = 0
+    got, _ = yuear_lib.mx_rms_norm(bf16(torch, ref.to_bf16(x)), bf16(torch, ref.to_bf16(gain)), 0.0, bits=bits)
+    codes, scales = ref.quantize(np.sign(x) * gain, bits)
+    np.testing.assert_array_equal(raw(torch, got[1]), scales)
+    np.testing.assert_array_equal(raw(torch, got[0]), codes)
+
+
 def test_norm_in_place(torch, yuear_lib):
     """The sum over the residual, and over x, give the same bits as apart."""
     rng = np.random.default_rng(8)

@@ -428,9 +428,9 @@ __global__ __launch_bounds__(1024) void stream_kernel(GemmArgs p, int a_rows) {
 //   8 bits, 3000 x 3072 x 8192             109     86.8     64.7     74.5
 //   8 bits, 3000 x 16384 x 3072            207      149      141      117
 //   4 bits, 6001 x 12288 x 2048            165      124      104       95
-// The largest run at 2.6 PFLOP/s (8 bits, 2.9 at K 8192) and 3.3 (4 bits, 4.2): matrix
-// cores busy 59 and 34% of the cycles at the 2.0 GHz that the power limit leaves (operands of
-// zeros run 27-30% faster), in 4 bits the results' way to memory a quarter of the time (K 2048).
+// The largest run at 2.6 PFLOP/s (8 bits, 2.9 at K 8192) and 3.4 (4 bits, 4.2): matrix
+// cores busy 61 and 36% of the cycles at the 2.0 GHz that the power limit leaves (operands of
+// zeros run 27-30% faster), in 4 bits SwiGLU a sixth of the time (K 2048).
 // The smallest are bound by LDS: 64 x 64 tiles of 197 x 3072 x 8192 bring 768 KiB a CU at 70
 // KB/us of the 66 (rows of 64 bytes) to 120 (128) that loads into LDS reach, 15.6 us.
 //

@@ -166,19 +166,58 @@ struct NormArgs {
   double inverse_k;
 };
 
-// Sum over the wave's lanes: over 16 of them in 32 bits, their sums in 64.
-__device__ __forceinline__ double wave_sum64(float v) {
-  const int rows = int(f32_bits(row_sum16(v)));
-  auto row = [&](int lane) { return double(bits_f32(uint32_t(__builtin_amdgcn_readlane(rows, lane)))); };
+// Sum over the wave's lanes.
+template <int CTRL> __device__ __forceinline__ double dpp64(double v) {
+  const uint64_t b = __builtin_bit_cast(uint64_t, v);
+  const uint32_t lo = uint32_t(__builtin_amdgcn_mov_dpp(int(b), CTRL, 0xF, 0xF, false));
+  const uint32_t hi = uint32_t(__builtin_amdgcn_mov_dpp(int(b >> 32), CTRL, 0xF, 0xF, false));
+  return __builtin_bit_cast(double, uint64_t(hi) << 32 | lo);
+}
+__device__ __forceinline__ double wave_sum64(double v) {
+  v += dpp64<0xB1>(v);   // lane ^ 1
+  v += dpp64<0x4E>(v);   // lane ^ 2
+  v += dpp64<0x141>(v);  // the other quad of the half-row
+  v += dpp64<0x140>(v);  // the other half of the row of 16
+  const uint64_t b = __builtin_bit_cast(uint64_t, v);
+  auto row = [&](int lane) {
+    const uint32_t lo = uint32_t(__builtin_amdgcn_readlane(int(b), lane));
+    const uint32_t hi = uint32_t(__builtin_amdgcn_readlane(int(b >> 32), lane));
+    return __builtin_bit_cast(double, uint64_t(hi) << 32 | lo);
+  };
   return (row(0) + row(16)) + (row(32) + row(48));
 }
 
-// h = bf16(x + residual) (or x), y = h * gain / sqrt(mean h^2 + eps) in 32 bits, y
-// quantised without a rounding in between but y's own to 32 bits. A workgroup has a row, each
-// lane C chunks of 8 in registers from the read to the codes, so a row is read once. The
-// squares of 16 lanes and more are added, and the root taken, in 64 bits (the factor in two parts
-// of 32): a row's values all carry its factor's error, and one that it takes past a code's edge
-// is off by a whole step of the code.
+// p (scale + rest) in 32 bits rounded to odd: towards zero, and the last bit set where the
+// product goes on, as it does where rest is not 0. So rounded, a product lies on the same side of
+// every tie of the codes, and of every power of two, as it does exactly.
+__device__ __forceinline__ void scaled8(const float (&p)[8], float scale, float rest, float (&y)[8]) {
+#pragma unroll
+  for (int e = 0; e < 8; ++e)
+    y[e] = p[e] * rest;
+  asm("s_setreg_imm32_b32 hwreg(HW_REG_MODE, 0, 2), 3\n\t"  // fp32 rounds towards zero
+      "v_fmac_f32 %0, %8, %16\n\t"
+      "v_fmac_f32 %1, %9, %16\n\t"
+      "v_fmac_f32 %2, %10, %16\n\t"
+      "v_fmac_f32 %3, %11, %16\n\t"
+      "v_fmac_f32 %4, %12, %16\n\t"
+      "v_fmac_f32 %5, %13, %16\n\t"
+      "v_fmac_f32 %6, %14, %16\n\t"
+      "v_fmac_f32 %7, %15, %16\n\t"
+      "s_setreg_imm32_b32 hwreg(HW_REG_MODE, 0, 2), 0"  // to nearest
+      : "+&v"(y[0]), "+&v"(y[1]), "+&v"(y[2]), "+&v"(y[3]), "+&v"(y[4]), "+&v"(y[5]), "+&v"(y[6]), "+&v"(y[7])
+      : "v"(p[0]), "v"(p[1]), "v"(p[2]), "v"(p[3]), "v"(p[4]), "v"(p[5]), "v"(p[6]), "v"(p[7]), "v"(scale));
+  const uint32_t goes_on = rest != 0.f;
+#pragma unroll
+  for (int e = 0; e < 8; ++e)
+    y[e] = bits_f32(f32_bits(y[e]) | goes_on);
+}
+
+// h = bf16(x + residual) (or x), y = h * gain / sqrt(mean h^2 + eps), y quantised without a
+// rounding in between. A workgroup has a row, each lane C chunks of 8 in registers from
+// the read to the codes, so a row is read once. The squares are added, and the root taken,
+// in 64 bits (the factor in two parts of 32), which with scaled8() makes the codes those of
+// 64-bit arithmetic: a row's values all carry its factor's error, and one that it takes past a
+// code's edge is off by a whole step of the code (7 in 9 million with all of it in 32 bits).
 template <int BITS, int C>
 __global__ __launch_bounds__(1024) void norm_kernel(NormArgs p) {
   __shared__ double part[16];
@@ -195,7 +234,8 @@ __global__ __launch_bounds__(1024) void norm_kernel(NormArgs p) {
       gain[c] = *reinterpret_cast<const u32x4 *>(p.gain + i * 8);
     }
   }
-  float v[C][8], squares = 0.f;
+  float v[C][8];
+  double squares = 0.0;
 #pragma unroll
   for (int c = 0; c < C; ++c) {
     const int i = c * int(blockDim.x) + int(threadIdx.x);
@@ -216,7 +256,7 @@ __global__ __launch_bounds__(1024) void norm_kernel(NormArgs p) {
     }
 #pragma unroll
     for (int e = 0; e < 8; ++e)
-      squares = fmaf(v[c][e], v[c][e], squares);
+      squares = fma(double(v[c][e]), double(v[c][e]), squares);
   }
   double total = wave_sum64(squares);
   if (waves > 1) {
@@ -237,13 +277,14 @@ __global__ __launch_bounds__(1024) void norm_kernel(NormArgs p) {
     const int i = c * int(blockDim.x) + int(threadIdx.x);
     if (i >= chunks)
       continue;
-    float g[8];
+    float g[8], y[8];
     unpack8(gain[c], g);
 #pragma unroll
     for (int e = 0; e < 8; ++e)
-      v[c][e] = fmaf(v[c][e] * g[e], scale, v[c][e] * g[e] * rest);  // v g of bf16 values is exact
+      g[e] *= v[c][e];  // exact, of two bf16 values
+    scaled8(g, scale, rest, y);
     uint32_t w[BITS / 4], s;
-    encode<BITS>(v[c], w, s);
+    encode<BITS>(y, w, s);
     store_codes<BITS>(p.codes + row * p.stride + i * BITS, w);
     if ((threadIdx.x & 3) == 0)
       p.scales[row * p.scale_stride + (i >> 2)] = uint8_t(s);
