@@ -959,7 +959,7 @@ template <int ABITS> hipError_t launch(int form, const GemmArgs &p, hipStream_t 
 
 // Estimated us of m x n x k by a form, infinite where it cannot run; fitted on MI355X to 4400
 // shapes in all forms (to 6000 tokens, 84000 features, K 128-8192; 6-13% rms where a form is
-// within 1.6 of the fastest). Over them what it picks takes 1.0% more than the fastest form.
+// within 1.6 of the fastest). Over them what it picks takes 0.7% more than the fastest form.
 double form_time(int form, int bits, int m, int n, int k, int cus) {
   const bool a8 = bits == 8;
   const double kk = k / 1024.0;
@@ -1004,12 +1004,12 @@ double form_time(int form, int bits, int m, int n, int k, int cus) {
   static const int shape[5][3] = {{64, 64, 1}, {64, 128, 1}, {128, 128, 2}, {192, 192, 1}, {256, 256, 1}};
   static const double fit[2][5][7] = {{{1.957, 3.111, 1.389, 2.548, 0.748, 0.18, 0.795},
                                        {1.234, 2.978, 2.319, 2.314, 1.868, 0.776, 0.654},
-                                       {0.85, 5.63, 6.703, 4.271, 1.741, 1.694, 5.379},
+                                       {1.634, 5.877, 6.484, 3.391, 2.459, 0.488, 2.216},
                                        {3.525, 6.613, 6.164, 2.594, 5.338, 5.195, 0.645},
                                        {0.591, 10.876, 9.663, 5.976, 7.548, 8.132, 1.331}},
                                       {{1.35, 2.936, 1.339, 2.938, 0.478, 0.0, 0.971},
                                        {2.87, 1.481, 1.862, 0.528, 1.506, 0.809, 0.599},
-                                       {2.458, 4.555, 5.584, 1.916, 1.703, 3.449, 3.095},
+                                       {2.423, 4.764, 5.324, 2.061, 2.014, 1.129, 1.981},
                                        {5.728, 5.124, 4.198, 0.0, 3.757, 5.692, 0.15},
                                        {3.142, 8.015, 6.513, 2.969, 4.77, 8.5, 0.893}}};
   const int *of = shape[form - kTile64];
@@ -1017,7 +1017,11 @@ double form_time(int form, int bits, int m, int n, int k, int cus) {
     return __builtin_inf();
   const double *c = fit[a8 ? 0 : 1][form - kTile64];
   const double slots = double(cus) * of[2], t = tiles(of[0], of[1]);
-  const double full = std::floor(t / slots), rest = t / slots - full;
+  double full = std::floor(t / slots), rest = t / slots - full;
+  if (of[2] == 2 && rest > 0.5) {  // some CU has both of its tiles again
+    full += 1;
+    rest = 0;
+  }
   return c[0] + full * (c[1] + c[2] * kk) + (rest > 0 ? c[3] + c[4] * kk + rest * (c[5] + c[6] * kk) : 0.0);
 }
 
