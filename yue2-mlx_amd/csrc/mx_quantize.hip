@@ -13,8 +13,8 @@
 // All three are bound by memory: a lane moves 8 values, 16 bytes of bf16, so a
 // wave reads whole KiB, and four lanes share a scale (two DPP steps). MI355X, where a
 // plain copy reaches 4.7 TB/s: quantising 3000 x 8192 in 8 bits 13.5 us (5.5 TB/s), 16384 x 3072
-// in 4 bits 26 us, back 21; the norm of 3000 x 3072 with its residual 12.4 us (5.2 TB/s). One
-// row of 3072: 2.0 to 2.4 and 2.4 to 2.9 us, a launch.
+// in 4 bits 26 us, back 21; the norm of 3000 x 3072 with its residual 12.6 us (5.1 TB/s). One
+// row of 3072: 2.0 to 2.4 and 2.4 to 3.0 us, a launch.
 #include <algorithm>
 
 #include "kernels.h"
