@@ -14,7 +14,6 @@ apart), what is held in 4 bits as the bfloat16 values that it stands for.
 `own` False: the operators in elementary torch operations in 32 bits. `own`
 True: the library's calls.
 """
-import functools
 import importlib
 import math
 
@@ -203,7 +202,6 @@ def _plain_gemm(s):
 
 # ---- the library's calls ----
 
-@functools.cache
 def _library():
     return importlib.import_module("yue2-mlx_amd.yuear")
 
