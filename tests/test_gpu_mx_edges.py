@@ -38,3 +38,55 @@ def test_norm_of_a_mean_that_is_exact(torch, yuear_lib, k, bits):
     got, _ = yuear_lib.mx_rms_norm(bf16(torch, ref.to_bf16(x * np.array([[1], [2], [0.25], [1]]))),
                                    bf16(torch, ref.to_bf16(gain)), 0.0, bits=bits)
     check_codes(torch, got, x * gain, bits)
+
+
+# Rows of one magnitude: their root is that magnitude, its reciprocal no float, and y is sign * gain.
+# The last row's eps adds to a square: sqrt(2 * 2 + 2.25) is 2.5.
+@pytest.mark.parametrize("bits", [8, 4])
+@pytest.mark.parametrize("k,residual", [(1024, False), (2080, True), (3072, False), (3136, True), (16384, False)])
+@pytest.mark.parametrize("magnitude,eps", [(3, 0.0), (1.5, 0.0), (7 * 2.0 ** 20, 0.0), (0.625, 0.0), (100, 0.0), (2, 2.25)])
+def test_norm_ties_where_the_factor_is_not_exact(torch, yuear_lib, k, residual, magnitude, eps, bits):
+    rng = np.random.default_rng(k)
+    x = np.where(rng.integers(0, 2, (5, k)), 1.0, -1.0)
+    root = np.sqrt(magnitude ** 2 + eps)
+    gain = tied_gains(rng, k) * (1.25 if eps else 1.0)  # 2 * 1.25 / 2.5 = 1
+    gain = ref.from_bf16(ref.to_bf16(gain))
+    h = x * magnitude
+    part = np.where(rng.integers(0, 2, (5, k)), 0.25 * magnitude, -magnitude) if residual else 0 * h
+    got, total = yuear_lib.mx_rms_norm(bf16(torch, ref.to_bf16(h - part)), bf16(torch, ref.to_bf16(gain)), eps,
+                                       residual=bf16(torch, ref.to_bf16(part)) if residual else None, bits=bits)
+    if residual:
+        np.testing.assert_array_equal(ref.from_bf16(bits_of(torch, total)), h)
+    check_codes(torch, got, h * gain / root, bits)  # exact wherever it is a tie
+
+
+@pytest.mark.parametrize("bits", [8, 4])
+def test_norm_of_one_value_in_nine(torch, yuear_lib, bits):
+    """32 of 288 values are 1: a mean of 1/9, which no float is, and y is three times the gain."""
+    rng = np.random.default_rng(2)
+    x = np.zeros((3, 288))
+    x[0, ::9], x[1, 4::9], x[2, 8::9] = 1, -2, 0.5
+    gain = tied_gains(rng, 288)
+    gain[gain == 0] = 1
+    got, _ = yuear_lib.mx_rms_norm(bf16(torch, ref.to_bf16(x)), bf16(torch, ref.to_bf16(gain)), 0.0, bits=bits)
+    check_codes(torch, got, 3 * np.sign(x) * gain, bits)
+
+
+@pytest.mark.parametrize("rows,k,gap,bits,eps", [
+    (1500, 3072, 0, 8, 1e-5), (1500, 2048, 0, 4, 1e-6), (700, 3136, 1, 8, 1e-5), (9000, 256, 0, 8, 1e-5),
+    (300, 16384, 0, 4, 1e-5), (5, 8224, 2, 8, 0.0), (1, 3072, 0, 8, 1e-5),
+])
+def test_norm_of_a_sum_has_the_codes_of_64_bits(torch, yuear_lib, rows, k, gap, bits, eps):
+    """With a residual, rows apart, the eps as the float that the call takes."""
+    rng = np.random.default_rng(rows + k)
+    x, r = random_rows(rng, rows, k, "plain"), random_rows(rng, rows, k, "plain")
+    gain = ref.to_bf16(1 + 0.2 * rng.standard_normal(k))
+    wide = torch.full((rows, k + 8 * gap), 7.0, dtype=torch.bfloat16, device="cuda")
+    wide[:, :k] = bf16(torch, x)
+    out, wides = pair_in(torch, rows, k, bits, gap)
+    got, total = yuear_lib.mx_rms_norm(wide[:, :k], bf16(torch, gain), eps, residual=bf16(torch, r), bits=bits, out=out)
+    h = ref.from_bf16(ref.to_bf16(ref.from_bf16(x) + ref.from_bf16(r)))
+    np.testing.assert_array_equal(ref.from_bf16(bits_of(torch, total)), h)
+    mean = (h ** 2).mean(-1, keepdims=True) + np.float64(np.float32(eps))
+    check_codes(torch, got, h / np.sqrt(mean) * ref.from_bf16(gain), bits)
+    assert untouched(wides, k, bits)

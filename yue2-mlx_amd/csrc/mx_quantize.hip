@@ -163,6 +163,7 @@ struct NormArgs {
   int64_t x_stride, residual_stride, sum_stride, stride, scale_stride;
   int rows, k;
   float eps;
+  double inverse_k;
 };
 
 // Sum over the wave's lanes.
@@ -186,37 +187,43 @@ __device__ __forceinline__ double wave_sum64(double v) {
   return (row(0) + row(16)) + (row(32) + row(48));
 }
 
-// p (scale + rest) in 32 bits rounded to odd: towards zero, and the last bit set where the
-// product goes on, as it does where rest is not 0. So rounded, a product lies on the same side of
-// every tie of the codes, and of every power of two, as it does exactly.
-__device__ __forceinline__ void scaled8(const float (&p)[8], float scale, float rest, float (&y)[8]) {
+// The edges of the codes, their ties, and the powers of two, where a block's scale changes, end in
+// 19 zeros. y = p scale in 32 bits is less than 4 units of its last place off (3.5 roundings: half
+// a one in the mean's root, the root's, the quotient's, the product's), so where its last 19 bits
+// are more than 4 away from zeros it lies on the side that it would lie on exactly. A wave's 512
+// values have one nearer in 1 of 100 cases. (Zeros, two in a row of a sum's 3072, are none, or
+// the branch cost 0.2 us a row: what is added, 5 units, leaves products from 2^-122 on.)
+__device__ __forceinline__ bool near_an_edge(const float (&p)[8], float scale) {
+  uint32_t least = ~0u;
 #pragma unroll
   for (int e = 0; e < 8; ++e)
-    y[e] = p[e] * rest;
-  asm("s_setreg_imm32_b32 hwreg(HW_REG_MODE, 0, 2), 3\n\t"  // fp32 rounds towards zero
-      "v_fmac_f32 %0, %8, %16\n\t"
-      "v_fmac_f32 %1, %9, %16\n\t"
-      "v_fmac_f32 %2, %10, %16\n\t"
-      "v_fmac_f32 %3, %11, %16\n\t"
-      "v_fmac_f32 %4, %12, %16\n\t"
-      "v_fmac_f32 %5, %13, %16\n\t"
-      "v_fmac_f32 %6, %14, %16\n\t"
-      "v_fmac_f32 %7, %15, %16\n\t"
-      "s_setreg_imm32_b32 hwreg(HW_REG_MODE, 0, 2), 0"  // to nearest
-      : "+&v"(y[0]), "+&v"(y[1]), "+&v"(y[2]), "+&v"(y[3]), "+&v"(y[4]), "+&v"(y[5]), "+&v"(y[6]), "+&v"(y[7])
-      : "v"(p[0]), "v"(p[1]), "v"(p[2]), "v"(p[3]), "v"(p[4]), "v"(p[5]), "v"(p[6]), "v"(p[7]), "v"(scale));
-  const uint32_t goes_on = rest != 0.f;
+    least = min(least, (f32_bits(fmaf(p[e], scale, bits_f32(5u))) << 13) + (4u << 13));
+  return least < 9u << 13;
+}
+
+// The same in 64 bits, scale with a Newton step (none where it is 0 or infinite): 1.5 times the
+// square of scale's 2.5 roundings of 2^-24 is left, 2^-44.7. Products may lie on an edge itself
+// though their factor is no float (rows of one magnitude: 3 gain / 3), so what is within 2^-43 of
+// one is taken for it; the rest is rounded to odd, towards zero and the last bit set, which keeps
+// its side.
+__device__ __forceinline__ void settle8(const float (&p)[8], double mean, float scale, float (&y)[8]) {
+  asm volatile("" : "+v"(scale));  // or the step is taken ahead of the branch
+  const double s = scale, off = fma(-mean * s, s, 1.0), factor = fabs(off) < 1e-6 ? fma(0.5 * s, off, s) : s;
 #pragma unroll
-  for (int e = 0; e < 8; ++e)
-    y[e] = bits_f32(f32_bits(y[e]) | goes_on);
+  for (int e = 0; e < 8; ++e) {
+    const uint64_t b = (__builtin_bit_cast(uint64_t, double(p[e]) * factor) + 0x200u) & ~uint64_t(0x3ff);
+    const uint64_t top = b & ~((uint64_t(1) << 29) - 1);
+    y[e] = bits_f32(f32_bits(float(__builtin_bit_cast(double, top))) | uint32_t(b != top));
+  }
 }
 
 // h = bf16(x + residual) (or x), y = h * gain / sqrt(mean h^2 + eps), y quantised without a
 // rounding in between. A workgroup has a row, each lane C chunks of 8 in registers from
-// the read to the codes, so a row is read once. The squares are added, and the root taken,
-// in 64 bits (the factor in two parts of 32), which with scaled8() makes the codes those of
+// the read to the codes, so a row is read once. The squares are added in 64 bits, and products
+// whose side of a code's edge is in doubt are taken again in 64 bits, which makes the codes those of
 // 64-bit arithmetic: a row's values all carry its factor's error, and one that it takes past a
-// code's edge is off by a whole step of the code (7 in 9 million with all of it in 32 bits).
+// code's edge is off by a whole step of the code (7 in 9 million with all of it in 32 bits, and
+// one in 30 of a row of one magnitude).
 template <int BITS, int C>
 __global__ __launch_bounds__(1024) void norm_kernel(NormArgs p) {
   __shared__ double part[16];
@@ -266,11 +273,8 @@ __global__ __launch_bounds__(1024) void norm_kernel(NormArgs p) {
     for (int w = 1; w < waves; ++w)
       total += part[w];
   }
-  const double mean = total / p.k + double(p.eps);  // (times 1 / k rounded, 1 in 15 of the widths miss a mean of 1)
+  const double mean = fma(total, p.inverse_k, double(p.eps));
   const float scale = 1.0f / __builtin_sqrtf(float(mean));
-  // a Newton step; none where the factor is 0 or infinite
-  float rest = float(0.5 * scale * fma(-mean * scale, double(scale), 1.0));
-  rest = fabsf(rest) < scale * 1e-6f ? rest : 0.f;
 #pragma unroll
   for (int c = 0; c < C; ++c) {
     const int i = c * int(blockDim.x) + int(threadIdx.x);
@@ -280,8 +284,9 @@ __global__ __launch_bounds__(1024) void norm_kernel(NormArgs p) {
     unpack8(gain[c], g);
 #pragma unroll
     for (int e = 0; e < 8; ++e)
-      g[e] *= v[c][e];  // exact, of two bf16 values
-    scaled8(g, scale, rest, y);
+      y[e] = (g[e] *= v[c][e]) * scale;  // the first product, of two bf16 values, is exact
+    if (__builtin_expect(near_an_edge(g, scale), 0))
+      settle8(g, mean, scale, y);
     uint32_t w[BITS / 4], s;
     encode<BITS>(y, w, s);
     store_codes<BITS>(p.codes + row * p.stride + i * BITS, w);
@@ -405,7 +410,7 @@ int32_t yuear_op_mx_rms_norm(const uint16_t *x, int64_t x_stride, const uint16_t
     return int32_t(hipErrorInvalidValue);
   const mx::NormArgs p{x,        residual,        gain,       sum,          codes,
                        scales,   x_stride,        residual_stride, sum_stride, codes_stride,
-                       scales_stride, rows,       k,          eps};
+                       scales_stride, rows,       k,          eps, 1.0 / k};
   const hipStream_t st = static_cast<hipStream_t>(stream);
   return int32_t(bits == 8 ? mx::launch_norm<8>(p, st) : mx::launch_norm<4>(p, st));
 }
