@@ -90,3 +90,19 @@ def test_norm_of_a_sum_has_the_codes_of_64_bits(torch, yuear_lib, rows, k, gap, 
     mean = (h ** 2).mean(-1, keepdims=True) + np.float64(np.float32(eps))
     check_codes(torch, got, h / np.sqrt(mean) * ref.from_bf16(gain), bits)
     assert untouched(wides, k, bits)
+
+
+@pytest.mark.parametrize("bits", [8, 4])
+@pytest.mark.parametrize("ones", [1, 2])
+def test_norm_of_values_past_32_bits(torch, yuear_lib, bits, ones):
+    """A row of few values has a factor of 128 (ones = 1) or 90.5: values from 2^128 on count as infinite and
+    make their block NaN, those below keep their codes."""
+    k = 16384
+    x, gain = np.zeros((4, k)), np.ones(k)
+    x[0, :ones], x[1, 64:64 + ones], x[2, 128:128 + ones], x[3, 5000:5000 + ones] = 1, -1, 1, -3
+    gain[:64], gain[64:128], gain[128:192], gain[4992:5024] = 2.0 ** 122 * 1.5, 2.0 ** 127, 2.0 ** 120 * 1.25, 2.0 ** 126
+    got, _ = yuear_lib.mx_rms_norm(bf16(torch, ref.to_bf16(x)), bf16(torch, ref.to_bf16(gain)), 0.0, bits=bits)
+    y = x / np.sqrt((x ** 2).mean(-1, keepdims=True)) * gain
+    past = np.abs(y) >= 2.0 ** 128
+    assert past.any(1).tolist() == [True, True, False, True]
+    check_codes(torch, got, np.where(past, np.copysign(np.inf, y), y), bits)
