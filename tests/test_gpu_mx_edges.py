@@ -106,3 +106,28 @@ def test_norm_of_values_past_32_bits(torch, yuear_lib, bits, ones):
     past = np.abs(y) >= 2.0 ** 128
     assert past.any(1).tolist() == [True, True, False, True]
     check_codes(torch, got, np.where(past, np.copysign(np.inf, y), y), bits)
+
+
+# ---- product ----
+
+@pytest.mark.parametrize("m,form", [(m, form) for m in (1, 5, 40, 70, 130, 300) for form in range(-1, 10 if m <= 16 else 8)])
+def test_swiglu_where_the_exponential_leaves_32_bits(torch, yuear_lib, m, form):
+    """Gates from -64 to -224 beside ups that make ordinary numbers of their results again, and beside
+    ordinary gates of the same waves; the sums are one product each, exact."""
+    gates = np.array([-64, -80, -88, -96, -104, -112, 2, -128, -144, -160, 0, -176, -192, -208, -224, 12])
+    x = np.zeros((m, 128))
+    x[:, 0], x[:, 32] = np.resize(gates if m > 1 else [-96], m), 1
+    ups = np.resize(np.concatenate([2.0 ** np.arange(-24, 125, 7), -2.0 ** np.arange(3, 127, 11)]), 96)
+    w = np.zeros((192, 128))
+    w[0::2, 0], w[1::2, 32] = 1, ups
+    a, wq = ref.quantize(x, 8), ref.quantize(w, 4)
+    assert (ref.values(*a, 8) == x).all() and (ref.values(*wq, 4) == w).all()
+    out = torch.empty(m, 96, dtype=torch.bfloat16, device="cuda")
+    forced(torch, yuear_lib, form, pair_of(torch, *a, 8), pair_of(torch, *wq, 4), 8, out, swiglu=True)
+    got, g = ref.from_bf16(bits_of(torch, out)), x[:, :1]
+    want = g / (1 + np.exp(-g)) * ups
+    # of the result: the exponent's roundings, of t and of its constant, ln 2 |t| 2^-23 = |g| 2^-23; one unit each of
+    # three exponentials; eight roundings of half a step; then bf16's. Below its least number: half a step of that.
+    off = np.abs(want) * (np.abs(g) * 2.0 ** -23 + 3 * 2.0 ** -23 + 8 * 2.0 ** -24)
+    assert (np.abs(got - want) <= off * (1 + 2.0 ** -8) + np.abs(want) * ref.HALF_BF16 + 2.0 ** -134).all()
+    assert (np.abs(want)[g[:, 0] < -88.7] > 2.0 ** -120).any()

@@ -59,6 +59,28 @@ __device__ __forceinline__ float silu_times(float gate, float up) {
   const float r = __builtin_amdgcn_rcpf(fmaf(__builtin_amdgcn_exp2f(gate * -1.44269502f), 0.25f, 0.25f));
   return gate * 0.25f * r * up;
 }
+// The same below kFarGate, where e^-gate goes out of 32 bits (at -88.7) while a large up brings the
+// result back: 1 / (1 + e^-gate) is e^gate there, to 2^-125 of it, and the cube of a third of it
+// is multiplied in one by one, so that nothing is lost that the result has.
+constexpr float kFarGate = -87.f;
+__device__ __forceinline__ float far_silu_times(float gate, float up) {
+  const float third = __builtin_amdgcn_exp2f(gate * 0.480898347f);
+  return gate * third * up * third * third;
+}
+// N values of interleaved gates and ups. (Negative numbers compare by their bits the other way.)
+template <int N> __device__ __forceinline__ void swiglu(const float (&v)[2 * N], float (&y)[N]) {
+  uint32_t far = 0;
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    y[i] = silu_times(v[2 * i], v[2 * i + 1]);
+    far = max(far, f32_bits(v[2 * i]));
+  }
+  if (__builtin_expect(far > f32_bits(kFarGate), 0))
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      if (v[2 * i] < kFarGate)
+        y[i] = far_silu_times(v[2 * i], v[2 * i + 1]);
+}
 
 __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
   typedef float f32x2 __attribute__((ext_vector_type(2)));
@@ -72,7 +94,9 @@ __device__ __forceinline__ void finish4(const GemmArgs &p, int m, int n, const f
   const bool whole = n + 4 <= p.n;
   if (EPI == kSwiglu) {
     uint16_t *c = p.c + m * p.ldc + (n >> 1);
-    const uint32_t out = pack2(silu_times(v[0], v[1]), silu_times(v[2], v[3]));
+    float y[2];
+    swiglu<2>(v, y);
+    const uint32_t out = pack2(y[0], y[1]);
     if (whole)
       store_at(c, out);
     else if (n < p.n)
@@ -127,10 +151,12 @@ __device__ __forceinline__ void finish32(const GemmArgs &p, int m, int n, int h,
     return;
   }
   if (EPI == kSwiglu) {
+    float y[8];
+    swiglu<8>(v, y);
     uint32_t w[4];
 #pragma unroll
     for (int q = 0; q < 4; ++q)
-      w[q] = pack2(silu_times(v[4 * q], v[4 * q + 1]), silu_times(v[4 * q + 2], v[4 * q + 3]));
+      w[q] = pack2(y[2 * q], y[2 * q + 1]);
     permlane32_swap(w[0], w[2]);
     permlane32_swap(w[1], w[3]);
     if (m < p.m)
