@@ -507,7 +507,8 @@ def _torch():
     if _T is None:
         import torch
         _BF16, _INT32, _UINT8 = torch.bfloat16, torch.int32, torch.uint8
-        _E4M3, _E8M0 = torch.float8_e4m3fn, torch.float8_e8m0fnu
+        # (the paged operators need neither; a torch without them refuses block-scaled rows)
+        _E4M3, _E8M0 = getattr(torch, "float8_e4m3fn", None), getattr(torch, "float8_e8m0fnu", None)
         _T = torch
     return _T
 
@@ -779,6 +780,8 @@ def _mx_bf16(t, rows, k, index, name, what):
 def _mx_out(x, rows, k, bits, out, index, name):
     """The given pair, or a new one, and (codes' address, row stride, scales' address, row stride)."""
     if out is None:
+        if _E4M3 is None or _E8M0 is None:
+            _refuse(name, "torch has no float8_e4m3fn and float8_e8m0fnu")
         if bits == 8:
             codes = x.new_empty((rows, k), dtype=_E4M3)
         elif bits == 4:
