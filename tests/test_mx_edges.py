@@ -1,5 +1,5 @@
 """Block-scaled rows where no GPU is needed: the binding on a torch without the types of their
-scales."""
+scales, and sizes that a launch takes."""
 import pytest
 
 
@@ -28,3 +28,16 @@ def test_block_scaled_rows_without_their_types_are_refused(yuear_lib, old_torch)
     pair = old_torch.zeros(4, 128, dtype=old_torch.float8_e4m3fn), old_torch.zeros(4, 4, dtype=old_torch.uint8)
     with pytest.raises(ValueError, match="block-scaled rows"):
         yuear_lib._mx_rows(pair, -1, "mx_dequantize")
+
+
+def test_products_of_the_largest_sizes_are_not_refused(yuear_lib):
+    """257 x (2^29 + 256) in SwiGLU, 138 GB of outputs, are more than 2^22 tiles of 256 x 256. (Without a GPU the
+    launch itself fails, with another error than that of invalid arguments.)"""
+    import torch
+    if torch.cuda.device_count():
+        pytest.skip("nothing is to be launched on these addresses")
+    base, m, n = 1 << 40, 257, (1 << 29) + 256
+    for k in (128, 512, 640):
+        status = yuear_lib.lib.yuear_op_mx_gemm(base, k, base + (1 << 20), k // 32, 8, base + (1 << 41), k // 2,
+                                                base + (1 << 40), k // 32, m, n, k, None, 0, base + (1 << 43), n // 2, 1, None)
+        assert status not in (0, 1)

@@ -876,15 +876,16 @@ __global__ __launch_bounds__(WM * WN * KS * 64, BM * BN > WM * WN * 8192 ? 1 : 2
 template <class T>
 hipError_t launch_tile(void (*kernel)(GemmArgs), const GemmArgs &p, hipStream_t s) {
   const int64_t tiles = ((int64_t(p.m) + T::kBM - 1) / T::kBM) * ((int64_t(p.n) + T::kBN - 1) / T::kBN);
-  if (tiles > int64_t(1) << 22)  // threads of the grid count in 32 bits (m, n <= 2^30 and what memory holds stay below)
+  const int64_t all = (tiles + 7) / 8 * 8, cus = std::max(gemm_cus() / 8 * 8, 8);
+  const int64_t grid = T::kOnward && p.k > kGroupK ? std::min(cus, all) : all;
+  // threads of the grid count in 32 bits, tiles in 31 (the largest ones of what memory holds do)
+  if (grid * T::kWaves * 64 >= int64_t(1) << 32 || tiles > int64_t(1) << 30)
     return hipErrorInvalidValue;
   const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void *>(kernel),
                                            hipFuncAttributeMaxDynamicSharedMemorySize, T::kLds);
   if (e != hipSuccess)
     return e;
-  const int64_t all = (tiles + 7) / 8 * 8, cus = std::max(gemm_cus() / 8 * 8, 8);
-  const unsigned grid = unsigned(T::kOnward && p.k > kGroupK ? std::min(cus, all) : all);
-  hipLaunchKernelGGL(kernel, dim3(grid), dim3(T::kWaves * 64), T::kLds, s, p);
+  hipLaunchKernelGGL(kernel, dim3(unsigned(grid)), dim3(T::kWaves * 64), T::kLds, s, p);
   return hipGetLastError();
 }
 
