@@ -131,3 +131,35 @@ def test_swiglu_where_the_exponential_leaves_32_bits(torch, yuear_lib, m, form):
     off = np.abs(want) * (np.abs(g) * 2.0 ** -23 + 3 * 2.0 ** -23 + 8 * 2.0 ** -24)
     assert (np.abs(got - want) <= off * (1 + 2.0 ** -8) + np.abs(want) * ref.HALF_BF16 + 2.0 ** -134).all()
     assert (np.abs(want)[g[:, 0] < -88.7] > 2.0 ** -120).any()
+
+
+@pytest.mark.parametrize("form", [5, 6, 7])
+@pytest.mark.parametrize("bits,k", [(8, 640), (8, 1152), (4, 768), (4, 896)])
+@pytest.mark.parametrize("epilogue", ["store", "swiglu", "residual"])
+def test_every_value_of_tiles_after_the_first(torch, yuear_lib, form, bits, k, epilogue):
+    """300 x 35002 are 274 tiles of 256 x 256 and more of the smaller ones, past the 256 workgroups of a launch:
+    all of them against 64 bits, whose products are those of 1009 rows of W (an odd number, so that tiles differ)."""
+    rng = np.random.default_rng(k + form)
+    m, n, some = 300, 35002, 1009
+    a, w = random_pair(rng, m, k, bits), random_pair(rng, some, k, 4)
+    which = np.arange(n) * 7 % some
+    width = n // 2 if epilogue == "swiglu" else n
+    r = bf16(torch, ref.to_bf16(rng.standard_normal((m, n)))) if epilogue == "residual" else None
+    out = torch.full((m, width), 7.0, dtype=torch.bfloat16, device="cuda")
+    forced(torch, yuear_lib, form, pair_of(torch, *a, bits), pair_of(torch, w[0][which], w[1][which], 4), bits, out, r,
+           epilogue == "swiglu")
+    y, off = ref.product(ref.values(*a, bits), ref.values(*w, 4), bits)
+    y, off = y[:, which], off[:, which]
+    if epilogue == "residual":
+        y = y + ref.from_bf16(bits_of(torch, r))
+        off = off + 2.0 ** -24 * np.abs(y)
+    elif epilogue == "swiglu":
+        g, u, dg, du = y[:, 0::2], y[:, 1::2], off[:, 0::2], off[:, 1::2]
+        with np.errstate(over="ignore"):
+            silu = g / (1 + np.exp(-g))
+        # |d silu| <= 1.1; the exponential and the quotient 2^-20 of the result, its argument's roundings |g| 2^-23
+        y = silu * u
+        off = 1.1 * dg * np.abs(u) + (np.abs(silu) + 1.1 * dg) * du + (2.0 ** -20 + np.abs(g) * 2.0 ** -23) * np.abs(y)
+    bound = (1 + ref.HALF_BF16) * off + ref.HALF_BF16 * np.abs(y) + 2.0 ** -133
+    err = np.abs(ref.from_bf16(bits_of(torch, out)) - y)
+    assert (err <= bound).all(), f"{(err > bound).sum()} of {err.size} off, first at {np.argwhere(err > bound)[0]}"
