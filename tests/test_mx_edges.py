@@ -1,5 +1,5 @@
 """Block-scaled rows where no GPU is needed: the binding on a torch without the types of their
-scales, and sizes that a launch takes."""
+scales, numbers of rows past 32 bits, and sizes that a launch takes."""
 import pytest
 
 
@@ -41,3 +41,16 @@ def test_products_of_the_largest_sizes_are_not_refused(yuear_lib):
         status = yuear_lib.lib.yuear_op_mx_gemm(base, k, base + (1 << 20), k // 32, 8, base + (1 << 41), k // 2,
                                                 base + (1 << 40), k // 32, m, n, k, None, 0, base + (1 << 43), n // 2, 1, None)
         assert status not in (0, 1)
+
+
+@pytest.mark.parametrize("rows", [1 << 31, (1 << 32) + 5])
+def test_rows_that_32_bits_do_not_count_are_refused(yuear_lib, rows):
+    """2^32 + 5 rows (of weights in 4 bits with k 128: 292 GB) are not taken for 5."""
+    import torch
+    yuear_lib._torch()
+    codes, scales = torch.zeros(1, 64, dtype=torch.uint8), torch.zeros(1, 4, dtype=torch.float8_e8m0fnu)
+    assert yuear_lib._mx_rows((codes, scales), -1, "mx_gemm")[:3] == (1, 128, 4)
+    with pytest.raises(ValueError, match="2.31"):
+        yuear_lib._mx_rows((codes.expand(rows, 64), scales.expand(rows, 4)), -1, "mx_gemm")
+    with pytest.raises(ValueError, match="2.31"):
+        yuear_lib._mx_shape(torch.zeros(1, 32, dtype=torch.bfloat16).expand(rows, 32), "mx_quantize")

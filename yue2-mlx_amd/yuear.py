@@ -748,8 +748,10 @@ def paged_attention_decode(qkv, k_pages, v_pages, table, pos, cos, sin, q_norm=N
 # first in the low half), scales float8_e8m0fnu [rows, k / 32] ----
 
 _MX = ("block-scaled rows are (codes, scales) on one device: codes float8_e4m3fn [rows, k] or uint8 [rows, k / 2] "
-       "with whole rows, scales float8_e8m0fnu [rows, k / 32] with whole rows, k a multiple of 32 up to 2^20")
+       "with whole rows, scales float8_e8m0fnu [rows, k / 32] with whole rows, k a multiple of 32 up to 2^20, rows "
+       "below 2^31")
 _MX_K = 1 << 20
+_MX_ROWS = (1 << 31) - 1  # what the library's calls count in
 
 
 def _mx_rows(packed, index, name):
@@ -760,7 +762,8 @@ def _mx_rows(packed, index, name):
         dtype, k = codes.dtype, ss[1] * 32
         bits = 8 if dtype is _E4M3 and shape[1] == k else 4 if dtype is _UINT8 and 2 * shape[1] == k else 0
         rows = shape[0]
-        if bits and 0 < k <= _MX_K and ss[0] == rows and codes.get_device() == index and scales.get_device() == index:
+        if (bits and 0 < k <= _MX_K and ss[0] == rows <= _MX_ROWS and codes.get_device() == index
+                and scales.get_device() == index):
             stride, scale_stride = codes.stride(), scales.stride()
             if stride[1] == 1 and (scale_stride[1] == 1 or k == 32):
                 return (rows, k, bits, codes.data_ptr(), stride[0] if rows > 1 else shape[1], scales.data_ptr(),
@@ -799,8 +802,8 @@ def _mx_out(x, rows, k, bits, out, index, name):
 def _mx_shape(x, name):
     """(rows, k) of what is quantised."""
     shape = x.shape
-    if len(shape) != 2 or shape[1] % 32 or not 0 < shape[1] <= _MX_K:
-        _refuse(name, "x is bfloat16 [rows, k] with k a multiple of 32 up to 2^20")
+    if len(shape) != 2 or shape[1] % 32 or not 0 < shape[1] <= _MX_K or shape[0] > _MX_ROWS:
+        _refuse(name, "x is bfloat16 [rows, k] with k a multiple of 32 up to 2^20 and rows below 2^31")
     return shape
 
 
