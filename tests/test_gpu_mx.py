@@ -138,8 +138,9 @@ def test_dequantize_every_code_and_scale(torch, yuear_lib, bits):
 
 # ---- norm ----
 
-# Of y in 32 bits: the squares' sum (k / 256 additions in a lane, 8 across) and its root, quotient and two products,
-# each half a step of 2^-24 of the value, the sum's halved by the root: under (8192 / 256 * 8 + 24) * 2^-25 = 2^-16.9.
+# Wider than needed: what y has with all of it in 32 bits, the squares' sum (k / 256 additions in a lane, 8 across) and
+# its root, quotient and two products, each half a step of 2^-24 of the value, the sum's halved by the root: under
+# (8192 / 256 * 8 + 24) * 2^-25 = 2^-16.9. (The kernel's codes are those of 64 bits: the tests of every code below.)
 NORM_FINE = 2.0 ** -16
 
 
@@ -312,7 +313,7 @@ def forced(torch, yuear_lib, form, a, w, a_bits, out, residual=None, swiglu=Fals
 
 
 # tokens, features, K: one and two rounds of a ring, odd numbers of 128s and of 512s, tiles with one
-# row or column, more tiles than a workgroup's first (256 x 256: 300 x 35000 has 274 of them)
+# row or column; each workgroup has one tile (test_tiles_one_after_another has more of them)
 FORMS = [(1, 2, 128), (5, 40, 384), (16, 66, 640), (33, 34, 1152), (65, 130, 512), (130, 62, 1664), (257, 300, 896),
          (40, 514, 2304), (300, 130, 4224)]
 

@@ -53,7 +53,7 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_rsrc(const uint8_t *base,
 // |gate| 7.3e-8 of it, no more than half a step of gate, a 32-bit sum, does (|gate| 6e-8). A
 // quarter of the quotient's parts: 1 / (1 + e^-gate) itself would be subnormal, which the
 // reciprocal takes for zero, from gate = -87.3 on, where the result need not be. Eight operations a
-// value, two of them of quarter rate: with expf and a division they were a third of the SwiGLU
+// value and half a one for far gates, two of them of quarter rate: with expf and a division they were a third of the SwiGLU
 // tiles' time past the last product.
 __device__ __forceinline__ float silu_times(float gate, float up) {
   const float r = __builtin_amdgcn_rcpf(fmaf(__builtin_amdgcn_exp2f(gate * -1.44269502f), 0.25f, 0.25f));
@@ -203,7 +203,7 @@ __device__ __forceinline__ void finish32(const GemmArgs &p, int m, int n, int h,
 // MFMA operands: no barrier before the sums. (Operands loaded straight into registers
 // have neighbouring lanes in different rows: some 55 cycles a load instead of 16, and
 // 137 MB of weights in 35 to 45 us instead of 29.) Bound by a launch and one or two
-// trips to memory: 1 x 5120 x 3072 3.8 us, 8 x 16384 x 3072 (27 MB) 7.7 to 8.2, 24 x 5120 x 3072 by
+// trips to memory (here to the last-level cache): 1 x 5120 x 3072 3.8 us, 8 x 16384 x 3072 (27 MB) 7.7 to 8.2, 24 x 5120 x 3072 by
 // 32 x 32 4.7, 64 x 5120 x 3072 8.2.
 //
 // 16 x 16 x 128 MFMAs, lane l = 16 g + r: row r; W and 4-bit A k 32 g .. 32 g + 31 of the
@@ -447,7 +447,8 @@ __global__ __launch_bounds__(1024) void stream_kernel(GemmArgs p, int a_rows) {
 // the ring, a group in use and the one after it; a lane reads the bytes of its row
 // and step and shifts them so that k-block h of each 64 is at byte 0 or 2.
 //
-// us of stores:                 64x64  64x128  128x128  192x192  256x256
+// us of stores, operands from
+// the last-level cache:         64x64  64x128  128x128  192x192  256x256
 //   8 bits, 100 x 5120 x 3072      8.5    10.5     13.2
 //   8 bits, 300 x 5120 x 3072     15.8    11.6     14.1     24.5
 //   8 bits, 1000 x 5120 x 3072    36.6    29.1     25.5     26.0     33.7
@@ -455,7 +456,7 @@ __global__ __launch_bounds__(1024) void stream_kernel(GemmArgs p, int a_rows) {
 //   8 bits, 3000 x 16384 x 3072            207      149      141      117
 //   4 bits, 6001 x 12288 x 2048            165      124      104       95
 // The largest run at 2.6 PFLOP/s (8 bits, 2.9 at K 8192) and 3.4 (4 bits, 4.2): matrix
-// cores busy 61 and 36% of the cycles at the 2.0 GHz that the power limit leaves (operands of
+// cores busy 62 and 37% of the cycles at the 2.0 GHz that the power limit leaves (operands of
 // zeros run 27-30% faster), in 4 bits SwiGLU a sixth of the time (K 2048).
 // The smallest are bound by LDS: 64 x 64 tiles of 197 x 3072 x 8192 bring 768 KiB a CU at 70
 // KB/us of the 66 (rows of 64 bytes) to 120 (128) that loads into LDS reach, 15.6 us.
@@ -985,8 +986,9 @@ template <int ABITS> hipError_t launch(int form, const GemmArgs &p, hipStream_t 
 }
 
 // Estimated us of m x n x k by a form, infinite where it cannot run; fitted on MI355X to 4400
-// shapes in all forms (to 6000 tokens, 84000 features, K 128-8192; 6-13% rms where a form is
-// within 1.6 of the fastest). Over them what it picks takes 0.7% more than the fastest form.
+// shapes of stores in all forms (to 6000 tokens, 84000 features, K 128-8192; 6-13% rms where a form
+// is within 1.6 of the fastest). Over 450 other shapes what it picks takes 1.9% more than the
+// fastest form for stores and SwiGLU of 8-bit rows, 3.3% with a residual, 1.4 to 2.5% for 4-bit rows.
 double form_time(int form, int bits, int m, int n, int k, int cus) {
   const bool a8 = bits == 8;
   const double kk = k / 1024.0;

@@ -12,9 +12,10 @@
 //
 // All three are bound by memory: a lane moves 8 values, 16 bytes of bf16, so a
 // wave reads whole KiB, and four lanes share a scale (two DPP steps). MI355X, where a
-// plain copy reaches 4.7 TB/s: quantising 3000 x 8192 in 8 bits 13.5 us (5.5 TB/s), 16384 x 3072
-// in 4 bits 26 us, back 21; the norm of 3000 x 3072 with its residual 12.6 us (5.1 TB/s). One
-// row of 3072: 2.0 to 2.4 and 2.4 to 3.0 us, a launch.
+// plain copy reaches 4.7 TB/s, from memory (from the last-level cache): quantising 3000 x 8192
+// in 8 bits 17.9 us (13.5 to 15.2), 4.2 TB/s; 16384 x 3072 in 4 bits and back 52, 4.9 TB/s; the
+// norm of 3000 x 3072 with its residual 17.2 (12.6 to 14.4), 3.8 TB/s. One row of 3072: 1.8 and
+// 2.6 us, a launch.
 #include <algorithm>
 
 #include "kernels.h"
@@ -297,10 +298,10 @@ __global__ __launch_bounds__(1024) void norm_kernel(NormArgs p) {
 
 constexpr int kMaxNormK = 16384;
 
-// One chunk a lane and k / 512 waves are the quickest for few rows, two the quickest for
-// many long ones (us, with a residual; four waves for every row as before 3.0, 31.0):
-//    1 x 3072: 2.70, 2.87    8000 x 3072: 29.7, 29.0    8000 x 2048: 18.9, 18.6
-//    1 x 2048: 2.50, 2.82    3000 x 8192: 31.2, 29.3    8000 x 1024: 11.4, 10.8
+// One chunk a lane and k / 512 waves are the quickest for few rows, two no slower for many long
+// ones, whose workgroups they halve (us, with a residual, rows from memory):
+//    1 x 3072: 2.43, 2.62    8000 x 3072: 35.2, 35.0    8000 x 2048: 23.6, 24.5
+//    1 x 2048: 2.14, 2.52    3000 x 8192: 35.0, 35.0    8000 x 1024: 15.1, 14.8
 // The choice goes by k alone, so that a row's sum has one order however many rows there are.
 template <int BITS> hipError_t launch_norm(NormArgs p, hipStream_t s) {
   const int each = p.k <= 2048 ? 1 : 2, threads = (p.k / 8 + 64 * each - 1) / (64 * each) * 64;
