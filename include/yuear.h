@@ -522,11 +522,11 @@ int32_t yuear_op_mx_dequantize(const uint8_t *dev_codes, int64_t codes_stride,
 /* The residual addition and RMSNorm before a projection, with their output
  * quantised as above: sum = bf16(x + residual) (which may be the same memory as x
  * or residual, with the same stride), y = sum * gain / sqrt(mean(sum^2) + eps), codes
- * and scales of y: those of 64-bit arithmetic (a y within 2^-43 of it of the middle of
- * two codes or of a power of two is taken for that), where sum * gain, the root's argument
- * and y are 0 or within the exponents of 32 bits from 2^-122 on. A y past the largest
- * number of 32 bits is an infinity: its 32 values get scale 255. Null residual and sum: y
- * of x. k up to 16384, gain [k]. */
+ * and scales of y: those of 64-bit arithmetic (a y next to the middle of two codes or
+ * to a power of two, within 2^-43 of its size, may be taken for that), where sum * gain,
+ * the root's argument and y are 0 or within the exponents of 32 bits from 2^-122 on. A y
+ * past the largest number of 32 bits is an infinity: its 32 values get scale 255. Null
+ * residual and sum: y of x. k up to 16384, gain [k]. */
 int32_t yuear_op_mx_rms_norm(const uint16_t *dev_x, int64_t x_stride,
                              const uint16_t *dev_residual, int64_t residual_stride,
                              const uint16_t *dev_gain, float eps, int32_t rows, int32_t k,

@@ -205,7 +205,7 @@ __device__ __forceinline__ bool near_an_edge(const float (&p)[8], float scale) {
 // The same in 64 bits, scale with a Newton step (none where it is 0 or infinite): 1.5 times the
 // square of scale's 2.5 roundings of 2^-24 is left, 2^-44.7. Products may lie on an edge itself
 // though their factor is no float (rows of one magnitude: 3 gain / 3), so what is within 2^-43 of
-// one is taken for it; the rest is rounded to odd, towards zero and the last bit set, which keeps
+// one may be taken for it; the rest is rounded to odd, towards zero and the last bit set, which keeps
 // its side.
 __device__ __forceinline__ void settle8(const float (&p)[8], double mean, float scale, float (&y)[8]) {
   asm volatile("" : "+v"(scale));  // or the step is taken ahead of the branch
